@@ -46,7 +46,7 @@
 extern "C" {
 #endif
 
-#define PM_DELTA_ABI_VERSION 14
+#define PM_DELTA_ABI_VERSION 15
 
 /* element types */
 #define PM_DTYPE_F32 0
@@ -431,6 +431,113 @@ int pm_delta_bwd_noalloc(const void* q, const void* k, const void* v, const floa
                          const float* s0, const float* go, const float* gs, float* gq, float* gk,
                          float* gv, float* gbeta, float* gs0, int B, int T, int H, int D,
                          int in_dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The elementwise gated linear recurrence: for every sequence and channel
+ *     h_t = exp(g_t) h_{t-1} + x_t
+ * with log-gates g (exp(g) <= 1 keeps the state bounded; positive ones are
+ * accepted as long as products of up to a sequence's gates stay finite in
+ * fp32).  The vector-state sibling of the gated delta rule; no reference
+ * counterpart.
+ *
+ *   x, g   (n_seqs, T, C), or packed (T, C) with cu_seqlens: channels
+ *          contiguous, batch and token strides x_sb, x_st, g_sb, g_st in
+ *          elements (views of a wider projection run as they are); x fp32 or
+ *          bf16, g fp32 or (with bf16 x) bf16
+ *   h      x's shape, contiguous, h_dtype
+ *   s0     (n_seqs, C) fp32 or NULL (zeros); s_out (n_seqs, C) fp32, the
+ *          state after each sequence's last token (an empty sequence's is its
+ *          s0).  s0 may be s_out.
+ *   slots  NULL, or int32 (n_seqs): sequence i's state is row slots[i] of the
+ *          pool s0 == s_out of n_slots rows, read and written in place (no
+ *          slot twice).  A sequence whose slot is outside [0, n_slots) starts
+ *          from zero, its state is not stored, and *bad_slot (device int32,
+ *          may be NULL) becomes nonzero.
+ *   kept   NULL, or fp32 (n_seqs, ceil(T / PM_RECURRENCE_SPAN), C): the state
+ *          before each span of tokens, for the backward (fixed length only).
+ *   cu_seqlens  as in pm_delta_fwd_varlen (clamped into [0, T]; tokens that
+ *          no sequence covers are left unwritten).
+ * Sums and states are fp32 whatever the types; h is rounded once.
+ * workspace: pm_linear_recurrence_workspace_bytes (0 where none is needed).
+ */
+#define PM_RECURRENCE_SPAN 256
+int pm_linear_recurrence(const void* x, const void* g, const int32_t* cu_seqlens, const float* s0,
+                         const int32_t* slots, int n_slots, int32_t* bad_slot, void* h, float* s_out,
+                         float* kept, int n_seqs, int T, int C, int64_t x_sb, int64_t x_st, int64_t g_sb,
+                         int64_t g_st, int x_dtype, int g_dtype, int h_dtype, void* workspace,
+                         size_t ws_bytes, void* stream);
+/* Workspace bytes of pm_linear_recurrence (packed: whether cu_seqlens is given)
+ * and, with packed 0 and n_seqs = B, of pm_linear_recurrence_bwd. */
+size_t pm_linear_recurrence_workspace_bytes(int n_seqs, int T, int C, int packed, int x_dtype);
+
+/*
+ * Its reverse mode over (B, T, C): gh = dL/dh (contiguous, h_dtype, NULL for
+ * zeros), gs = dL/ds_out (fp32, NULL for zeros), `kept` from the forward.
+ *     d_t = gh_t + exp(g_{t+1}) d_{t+1},  gx_t = d_t,  gg_t = d_t exp(g_t) h_{t-1}
+ * gx and gg are contiguous, in x's and g's type; gs0 (B, C) fp32.  h is
+ * recomputed in fp32 from x and `kept`, so that gg does not depend on h's
+ * rounding.  Every output is written in full.
+ */
+int pm_linear_recurrence_bwd(const void* x, const void* g, const float* kept, const void* gh,
+                             const float* gs, void* gx, void* gg, float* gs0, int B, int T, int C,
+                             int64_t x_sb, int64_t x_st, int64_t g_sb, int64_t g_st, int x_dtype,
+                             int g_dtype, int h_dtype, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * One token for B rows, in place: s = exp(g) s + x, h = s.  x, g: (B, C) with
+ * row strides x_sb, g_sb; h contiguous (B, C).  slots as pm_delta_step_slots:
+ * a slot outside [0, n_slots) is padding (no state touched, its h row zero).
+ */
+int pm_linear_recurrence_step(float* s_inout, const int32_t* slots, int n_slots, const void* x,
+                              const void* g, void* h, int B, int C, int64_t x_sb, int64_t g_sb,
+                              int x_dtype, int g_dtype, int h_dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Norms of queries and keys for each head, with the position rotation in the
+ * same pass: what the delta rule's q and k go through on the way from their
+ * projection (the model's x / max(||x||, 1e-6), model/__init__.py:203-205, is
+ * PM_NORM_L2 without weights; the rotation has no reference counterpart).
+ * For one head of one token, u = r x with
+ *   PM_NORM_L2   r = 1 / max(||x||, eps)
+ *   PM_NORM_RMS  r = 1 / sqrt(mean x^2 + eps)
+ * y = u * weight, and the first R elements are turned in pairs (i, i + R / 2),
+ * or (2 i, 2 i + 1) with `interleaved`:
+ *   z1 = y1 cos - y2 sin,  z2 = y2 cos + y1 sin.
+ *
+ *   q, k       (B, T, Hq, D), (B, T, Hk, D), elements of a head contiguous;
+ *              strides: host array of q's batch, token and head strides, then
+ *              k's, in elements
+ *   q_out, k_out  contiguous, in dtype
+ *   *_weight   (D) in w_dtype, or NULL
+ *   table      fp32 (P, R): R / 2 cosines, then R / 2 sines, for each position
+ *   positions  int32 (or int64) (B, T) with batch stride pos_sb (0: one row for
+ *              all), tokens contiguous; NULL: 0, 1, 2, ...  A token whose
+ *              position is outside [0, P) comes out as NaN (and its gradients,
+ *              the weights' with it); nothing outside the table is read.
+ * D in [1, 256], R even, 0 (no rotation; table and positions unused) to D.
+ * fp32 arithmetic, one rounding.
+ */
+#define PM_NORM_L2 0
+#define PM_NORM_RMS 1
+int pm_norm_rotate(const void* q, const void* k, const float* table, const void* positions,
+                   const void* q_weight, const void* k_weight, void* q_out, void* k_out, int B, int T,
+                   int Hq, int Hk, int D, int R, int P, const int64_t* strides, int64_t pos_sb,
+                   int pos_is_int64, int norm, float eps, int interleaved, int dtype, int w_dtype,
+                   void* stream);
+
+/*
+ * Its reverse mode: gq_out, gk_out (contiguous, dtype, NULL for zeros) to gq,
+ * gk (contiguous, dtype) and, where asked for, the weights' gradients (D) fp32,
+ * summed over all rows in an order that does not change from run to run
+ * (they need the workspace; without them it may be NULL).
+ */
+int pm_norm_rotate_bwd(const void* q, const void* k, const float* table, const void* positions,
+                       const void* q_weight, const void* k_weight, const void* gq_out, const void* gk_out,
+                       void* gq, void* gk, float* gq_weight, float* gk_weight, int B, int T, int Hq, int Hk,
+                       int D, int R, int P, const int64_t* strides, int64_t pos_sb, int pos_is_int64, int norm,
+                       float eps, int interleaved, int dtype, int w_dtype, void* workspace, size_t ws_bytes,
+                       void* stream);
+size_t pm_norm_rotate_bwd_workspace_bytes(int B, int T, int Hq, int Hk, int D);
 
 /* Thread-local message for the last nonzero return on this thread. */
 const char* pm_last_error(void);

@@ -18,12 +18,16 @@ import torch  # noqa: F401  (see module docstring: must precede CDLL)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpmdelta.so")
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 MAX_D = 256
 MAX_D_BWD = 256
 NOALLOC_SCRATCH_BYTES = 64 << 20
+
+RECURRENCE_SPAN = 256
+NORM_L2 = 0
+NORM_RMS = 1
 
 E_NULL, E_SHAPE, E_DTYPE, E_ALIGN, E_WORKSPACE, E_UNSUPPORTED = -1, -2, -3, -4, -5, -6
 
@@ -60,6 +64,13 @@ EXPORTS = (
     "pm_kda_delta_step",
     "pm_kda_delta_bwd",
     "pm_kda_delta_bwd_workspace_bytes",
+    "pm_linear_recurrence",
+    "pm_linear_recurrence_workspace_bytes",
+    "pm_linear_recurrence_bwd",
+    "pm_linear_recurrence_step",
+    "pm_norm_rotate",
+    "pm_norm_rotate_bwd",
+    "pm_norm_rotate_bwd_workspace_bytes",
 )
 
 _lib = None
@@ -152,6 +163,22 @@ def lib() -> ctypes.CDLL:
         L.pm_kda_delta_bwd.restype = i
         L.pm_kda_delta_bwd_workspace_bytes.argtypes = [i] * 5
         L.pm_kda_delta_bwd_workspace_bytes.restype = sz
+        i64, f = ctypes.c_int64, ctypes.c_float
+        L.pm_linear_recurrence.argtypes = [vp] * 5 + [i] + [vp] * 4 + [i] * 3 + [i64] * 4 + [i] * 3 + [vp, sz, vp]
+        L.pm_linear_recurrence.restype = i
+        L.pm_linear_recurrence_workspace_bytes.argtypes = [i] * 5
+        L.pm_linear_recurrence_workspace_bytes.restype = sz
+        L.pm_linear_recurrence_bwd.argtypes = [vp] * 8 + [i] * 3 + [i64] * 4 + [i] * 3 + [vp, sz, vp]
+        L.pm_linear_recurrence_bwd.restype = i
+        L.pm_linear_recurrence_step.argtypes = [vp, vp, i] + [vp] * 3 + [i] * 2 + [i64] * 2 + [i] * 3 + [vp]
+        L.pm_linear_recurrence_step.restype = i
+        rot = [i] * 7 + [ctypes.POINTER(i64), i64, i, i, f, i, i, i]
+        L.pm_norm_rotate.argtypes = [vp] * 8 + rot + [vp]
+        L.pm_norm_rotate.restype = i
+        L.pm_norm_rotate_bwd.argtypes = [vp] * 12 + rot + [vp, sz, vp]
+        L.pm_norm_rotate_bwd.restype = i
+        L.pm_norm_rotate_bwd_workspace_bytes.argtypes = [i] * 5
+        L.pm_norm_rotate_bwd_workspace_bytes.restype = sz
         got = L.pm_abi_version()
         if got != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH}: ABI version {got}, expected {ABI_VERSION}")

@@ -13,6 +13,9 @@
 //   K10   decay_chunked_f32.hip     chunked reverse mode of the gated rules on fp32 MFMA, and
 //                                   their chunked forward for fp32 inputs (K10f)
 //   K11   norm_rows.hip             row normalisation of the model's backward and its reverse
+// (pm_layer_abi.hip holds the entry points of the operators beside the delta rule:
+//   K12   linear_recurrence.hip     elementwise gated linear recurrence
+//   K13   norm_rotate.hip           norms and position rotation of q's and k's heads)
 // Mirrors the checks of kernels/__init__.py:308-338 (shapes), :613-614 and
 // :676-677 (chunk >= 1); shapes arrive as integers, so the Python layer
 // (prometheus_amd/kernels) raises KernelError for the tensor-level checks
@@ -130,11 +133,10 @@ hipError_t launch_copy_f32(float* dst, const float* src, size_t n, hipStream_t s
 namespace {
 
 thread_local char g_err[512] = "";
-// Kernel-selection knobs (pm_delta_set_path / pm_delta_set_tile): per calling
-// thread, so that a workspace-size query and the call it sizes always see the
-// same setting, whatever other threads select meanwhile.
-thread_local int g_path = 0;
-thread_local int g_tile = 0;
+
+}  // namespace
+
+namespace pm {
 
 int fail(int code, const char* fmt, ...) {
     va_list ap;
@@ -143,6 +145,21 @@ int fail(int code, const char* fmt, ...) {
     va_end(ap);
     return code;
 }
+
+void clear_error() { g_err[0] = '\0'; }
+
+}  // namespace pm
+
+namespace {
+
+using pm::fail;
+
+// Kernel-selection knobs (pm_delta_set_path / pm_delta_set_tile): per calling
+// thread, so that a workspace-size query and the call it sizes always see the
+// same setting, whatever other threads select meanwhile.
+thread_local int g_path = 0;
+thread_local int g_tile = 0;
+
 
 // Scratch of pm_delta_bwd_noalloc: a file-scope device array, one copy per GPU,
 // held until the process ends.  Host code never uses `scratch` itself (its

@@ -252,4 +252,87 @@ hipError_t launch_varlen_check(const int32_t* cu, int n_seqs, int total, int32_t
 constexpr int kVarlenOrderMax = 8192;
 hipError_t launch_varlen_order(const int32_t* cu, int n_seqs, int total, int32_t* order, hipStream_t st);
 
+// The thread's error message (pm_last_error) set to `fmt`, and `code` returned; and cleared.
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+void clear_error();
+
+// The elementwise gated linear recurrence (linear_recurrence.hip): h_t = exp(g_t) h_{t-1} + x_t
+// for n_seqs sequences of C channels, (n_seqs, T, C) or, with cu_seqlens, packed (T, C) (offsets
+// clamped into [0, T]).  x and g have token and batch strides in elements; h is contiguous.
+// States: row i of s0 and s_out is sequence i's, or, with slots, row slots[i] is (s_out is
+// s0; a slot outside [0, n_slots) starts from zero, is not stored, and sets *bad).
+constexpr int kRecSpan = 256;  // tokens between the states kept for the backward
+struct RecurrenceArgs {
+    const void* x;
+    const void* g;
+    const int32_t* cu_seqlens;  // nullable
+    const float* s0;            // nullable
+    const int32_t* slots;       // nullable
+    int n_slots;
+    int32_t* bad;  // nullable
+    void* h;
+    float* s_out;
+    float* kept;  // nullable: (n_seqs, ceil(T / kRecSpan), C), the state before each span
+    int n_seqs, T, C;
+    int64_t x_sb, x_st, g_sb, g_st;
+    bool x_bf16, g_bf16, h_bf16;
+    void* workspace;
+};
+hipError_t launch_recurrence(const RecurrenceArgs& a, hipStream_t st);
+
+// Its gradients: d_t = gh_t + exp(g_{t+1}) d_{t+1}, gx_t = d_t, gg_t = d_t exp(g_t) h_{t-1}, with
+// h recomputed from x and the kept states.  gh, gx and gg are contiguous, in h's, x's and g's type.
+struct RecurrenceBwdArgs {
+    const void* x;
+    const void* g;
+    const float* kept;
+    const void* gh;   // nullable
+    const float* gs;  // nullable
+    void* gx;
+    void* gg;
+    float* gs0;
+    int B, T, C;
+    int64_t x_sb, x_st, g_sb, g_st;
+    bool x_bf16, g_bf16, h_bf16;
+    void* workspace;
+};
+hipError_t launch_recurrence_bwd(const RecurrenceBwdArgs& a, hipStream_t st);
+
+// One token: s = exp(g) s + x in place, h = s; row b's state is s[slots[b]], or s[b].
+struct RecurrenceStepArgs {
+    float* s;
+    const int32_t* slots;  // nullable
+    int n_slots;
+    const void* x;
+    const void* g;
+    void* h;
+    int B, C;
+    int64_t x_sb, g_sb;
+    bool x_bf16, g_bf16, h_bf16;
+};
+hipError_t launch_recurrence_step(const RecurrenceStepArgs& a, hipStream_t st);
+
+// Norms and position rotation of q's and k's heads (norm_rotate.hip).  Side 0 is q, side 1 k.
+struct NormRotateArgs {
+    const void* x[2];
+    const void* weight[2];  // nullable
+    void* y[2];
+    int H[2];
+    int64_t sb[2], st[2], sh[2];  // batch, token and head strides of x
+    const float* table;           // nullable: (P, R), R / 2 cosines, then R / 2 sines
+    const void* pos;              // nullable: 0, 1, 2, ... in every batch row
+    int64_t pos_sb;               // 0: one row of positions for every batch row
+    int B, T, D, R, P;
+    bool pos64, bf16, w_bf16, rms, interleaved;
+    float eps;
+    // backward: gradients of y (contiguous, nullable), of x (contiguous) and of the weights
+    const void* gy[2];
+    void* gx[2];
+    float* gw[2];  // nullable
+    void* workspace;
+};
+hipError_t launch_norm_rotate(const NormRotateArgs& a, hipStream_t st);
+hipError_t launch_norm_rotate_bwd(const NormRotateArgs& a, hipStream_t st);
+size_t norm_rotate_bwd_ws_bytes(int B, int T, int Hq, int Hk, int D);
+
 }  // namespace pm

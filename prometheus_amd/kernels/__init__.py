@@ -21,8 +21,10 @@ as the reference does (``kernels/__init__.py:344-347``), and runs the fp32
 per-token kernel.
 
 Beyond the reference surface: ``chunked_delta_rule_varlen`` (packed batch
-with ``cu_seqlens``), ``delta_rule_step`` (public single-token decode step)
-and the keyword ``out_dtype`` (bf16 output, opt-in; fp32 by default).
+with ``cu_seqlens``), ``delta_rule_step`` (public single-token decode step),
+the keyword ``out_dtype`` (bf16 output, opt-in; fp32 by default), and the operators
+beside the delta rule: ``linear_recurrence`` (``recurrence.py``) and ``norm_rotate``
+(``head_norm.py``).
 """
 
 from __future__ import annotations
@@ -833,6 +835,20 @@ def _gated_step(q, k, v, beta, g, state, per_channel):
     return call.out(o)
 
 
+from prometheus_amd.kernels.head_norm import (  # noqa: E402  (they use the helpers above)
+    norm_rotate,
+    norm_rotate_bwd,
+    norm_rotate_fwd,
+    rotation_table,
+)
+from prometheus_amd.kernels.recurrence import (  # noqa: E402
+    linear_recurrence,
+    linear_recurrence_bwd,
+    linear_recurrence_fwd,
+    linear_recurrence_step,
+    linear_recurrence_varlen,
+)
+
 __all__ = [
     "DEFAULT_CHUNK",
     "KernelError",
@@ -852,4 +868,13 @@ __all__ = [
     "chunked_gated_delta_rule_fwd",
     "chunked_gated_delta_rule_bwd",
     "gated_delta_rule_step",
+    "linear_recurrence",
+    "linear_recurrence_fwd",
+    "linear_recurrence_bwd",
+    "linear_recurrence_varlen",
+    "linear_recurrence_step",
+    "norm_rotate",
+    "norm_rotate_fwd",
+    "norm_rotate_bwd",
+    "rotation_table",
 ]

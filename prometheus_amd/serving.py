@@ -23,6 +23,10 @@ host memory. ``LinearStateCache`` is that pool on one GPU:
   between replays; slots outside ``[0, n_slots)`` are padding);
 * ``swap_out`` / ``swap_in``: park states in pinned host memory and restore
   them (the spec's tier-2 parking of long sessions).
+
+``RecurrenceStateCache`` is the same for layers of ``kernels.linear_recurrence``, whose state is
+a vector of C channels (``(n_layers, n_slots, C)`` fp32): its ``prefill`` reads and writes the
+slots in the kernel, without gathering them first.
 """
 
 from __future__ import annotations
@@ -32,22 +36,20 @@ import heapq
 import torch
 
 from prometheus_amd import _native, kernels
+from prometheus_amd.kernels import recurrence
 
-__all__ = ["LinearStateCache"]
+__all__ = ["LinearStateCache", "RecurrenceStateCache"]
 
 
-class LinearStateCache:
-    """Per-request recurrent states of ``n_layers`` linear-attention layers."""
+class _SlotPool:
+    """Slots of per-request states, each ``state`` fp32 per layer: bookkeeping and tiering."""
 
-    def __init__(self, n_layers: int, n_slots: int, heads: int, dim: int, device=None):
-        if n_layers < 1 or n_slots < 1 or heads < 1 or dim < 1:
-            raise ValueError("n_layers, n_slots, heads and dim must be >= 1")
+    def __init__(self, n_layers: int, n_slots: int, state: tuple, device):
         if device is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        self.n_layers, self.n_slots, self.heads, self.dim = n_layers, n_slots, heads, dim
+        self.n_layers, self.n_slots, self._state = n_layers, n_slots, state
         # one spare slot past the end: out-of-range device slot indices land there
-        self._pool = torch.zeros((n_layers, n_slots + 1, heads, dim, dim), dtype=torch.float32,
-                                 device=device)
+        self._pool = torch.zeros((n_layers, n_slots + 1, *state), dtype=torch.float32, device=device)
         self.pool = self._pool[:, :n_slots]
         self._bad_slot = torch.zeros(1, dtype=torch.int32, device=device)
         # a min-heap: alloc hands out the lowest free slots, so that a batch admitted in
@@ -82,28 +84,6 @@ class LinearStateCache:
         idx = self._index(slots)
         self._pool[:, idx] = 0.0
 
-    # ---- compute ----
-    def prefill(self, layer: int, slots, q, k, v, beta, cu_seqlens=None, config=None):
-        """Run prompts through the forward from the slots' states into them.
-
-        Fixed length: q, k, v ``(n, T, H, D)``, beta ``(n, T, H)``, one request per
-        row. Packed: q, k, v ``(1, N, H, D)`` with ``cu_seqlens`` ``(n + 1,)``.
-        Returns the output ``(.., H, D)`` fp32. ``slots`` may be a list of ints or a
-        GPU int tensor; with GPU ``slots`` and ``cu_seqlens`` nothing here waits for
-        the device (see ``check_slots`` and ``kernels.check_varlen``).
-        """
-        self._check_layer(layer)
-        idx = self._index(slots)
-        self._check_cuda(q, k, v, beta)
-        self._pool[layer, self.n_slots].zero_()  # the spare slot: a fresh state
-        s0 = self._pool[layer, idx]  # gathered copy (n, H, D, D)
-        if cu_seqlens is None:
-            o, s = kernels.chunked_delta_rule(q, k, v, beta, s0, config)
-        else:
-            o, s = kernels.chunked_delta_rule_varlen(q, k, v, beta, cu_seqlens, s0, config)
-        self._pool[layer, idx] = s
-        return o
-
     def check_slots(self) -> None:
         """Raise ``ValueError`` if a GPU slot tensor given to ``prefill`` or ``reset`` since
         the last check held an index outside ``[0, n_slots)`` (synchronises; clears)."""
@@ -111,49 +91,18 @@ class LinearStateCache:
             self._bad_slot.zero_()
             raise ValueError(f"a device slot index was outside [0, {self.n_slots})")
 
-    def decode(self, layer: int, slots: torch.Tensor, q, k, v, beta, out=None):
-        """One token per request: q, k, v ``(B, H, D)``, beta ``(B, H)``, ``slots``
-        an int32 GPU tensor ``(B,)``. Updates the states in place and returns
-        ``out`` ``(B, H, D)`` fp32 (allocated when None)."""
-        self._check_layer(layer)
-        self._check_cuda(q, k, v, beta, slots)
-        b = slots.shape[0] if slots.dim() == 1 else -1
-        if b < 0 or slots.dtype != torch.int32 or not slots.is_contiguous():
-            raise ValueError("slots must be a contiguous int32 tensor of shape (B,)")
-        want = (b, self.heads, self.dim)
-        for name, x in (("q", q), ("k", k), ("v", v)):
-            if tuple(x.shape) != want or not x.is_contiguous():
-                raise ValueError(f"{name} must be contiguous {want}, got {tuple(x.shape)}")
-        if q.dtype != k.dtype or q.dtype != v.dtype or q.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError("q, k, v must share one dtype, fp32 or bf16")
-        if tuple(beta.shape) != (b, self.heads) or beta.dtype != torch.float32 or not beta.is_contiguous():
-            raise ValueError(f"beta must be contiguous fp32 {(b, self.heads)}")
-        if out is None:
-            out = torch.empty(want, dtype=torch.float32, device=q.device)
-        elif tuple(out.shape) != want or out.dtype != torch.float32 or not out.is_contiguous():
-            raise ValueError(f"out must be contiguous fp32 {want}")
-        rc = _native.lib().pm_delta_step_slots(
-            self.pool[layer].data_ptr(), slots.data_ptr(), self.n_slots, q.data_ptr(), k.data_ptr(),
-            v.data_ptr(), beta.data_ptr(), out.data_ptr(), b, self.heads, self.dim,
-            _native.DTYPE_BF16 if q.dtype == torch.bfloat16 else _native.DTYPE_F32,
-            torch.cuda.current_stream(q.device).cuda_stream,
-        )
-        _native.check(rc)
-        return out
-
     # ---- tiering ----
     def swap_out(self, slots) -> torch.Tensor:
         """The slots' states of every layer, copied to pinned host memory:
-        ``(n_layers, n, H, D, D)``. The slots stay allocated."""
+        ``(n_layers, n, *state)``. The slots stay allocated."""
         idx = self._index(slots)
-        host = torch.empty((self.n_layers, len(idx), self.heads, self.dim, self.dim),
-                           dtype=torch.float32, pin_memory=True)
+        host = torch.empty((self.n_layers, len(idx), *self._state), dtype=torch.float32, pin_memory=True)
         host.copy_(self._pool[:, idx])
         return host
 
     def swap_in(self, slots, saved: torch.Tensor) -> None:
         idx = self._index(slots)
-        want = (self.n_layers, len(idx), self.heads, self.dim, self.dim)
+        want = (self.n_layers, len(idx), *self._state)
         if tuple(saved.shape) != want:
             raise ValueError(f"saved states {tuple(saved.shape)} != {want}")
         self._pool[:, idx] = saved.to(self._pool.device, dtype=torch.float32)
@@ -189,3 +138,150 @@ class LinearStateCache:
         for x in xs:
             if not (isinstance(x, torch.Tensor) and x.device == self.pool.device):
                 raise ValueError("inputs must be tensors on the pool's device")
+
+
+class LinearStateCache(_SlotPool):
+    """Per-request recurrent states of ``n_layers`` linear-attention layers."""
+
+    def __init__(self, n_layers: int, n_slots: int, heads: int, dim: int, device=None):
+        if n_layers < 1 or n_slots < 1 or heads < 1 or dim < 1:
+            raise ValueError("n_layers, n_slots, heads and dim must be >= 1")
+        super().__init__(n_layers, n_slots, (heads, dim, dim), device)
+        self.heads, self.dim = heads, dim
+
+    def prefill(self, layer: int, slots, q, k, v, beta, cu_seqlens=None, config=None):
+        """Run prompts through the forward from the slots' states into them.
+
+        Fixed length: q, k, v ``(n, T, H, D)``, beta ``(n, T, H)``, one request per
+        row. Packed: q, k, v ``(1, N, H, D)`` with ``cu_seqlens`` ``(n + 1,)``.
+        Returns the output ``(.., H, D)`` fp32. ``slots`` may be a list of ints or a
+        GPU int tensor; with GPU ``slots`` and ``cu_seqlens`` nothing here waits for
+        the device (see ``check_slots`` and ``kernels.check_varlen``).
+        """
+        self._check_layer(layer)
+        idx = self._index(slots)
+        self._check_cuda(q, k, v, beta)
+        self._pool[layer, self.n_slots].zero_()  # the spare slot: a fresh state
+        s0 = self._pool[layer, idx]  # gathered copy (n, H, D, D)
+        if cu_seqlens is None:
+            o, s = kernels.chunked_delta_rule(q, k, v, beta, s0, config)
+        else:
+            o, s = kernels.chunked_delta_rule_varlen(q, k, v, beta, cu_seqlens, s0, config)
+        self._pool[layer, idx] = s
+        return o
+
+    def decode(self, layer: int, slots: torch.Tensor, q, k, v, beta, out=None):
+        """One token per request: q, k, v ``(B, H, D)``, beta ``(B, H)``, ``slots``
+        an int32 GPU tensor ``(B,)``. Updates the states in place and returns
+        ``out`` ``(B, H, D)`` fp32 (allocated when None)."""
+        self._check_layer(layer)
+        self._check_cuda(q, k, v, beta, slots)
+        b = slots.shape[0] if slots.dim() == 1 else -1
+        if b < 0 or slots.dtype != torch.int32 or not slots.is_contiguous():
+            raise ValueError("slots must be a contiguous int32 tensor of shape (B,)")
+        want = (b, self.heads, self.dim)
+        for name, x in (("q", q), ("k", k), ("v", v)):
+            if tuple(x.shape) != want or not x.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {want}, got {tuple(x.shape)}")
+        if q.dtype != k.dtype or q.dtype != v.dtype or q.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("q, k, v must share one dtype, fp32 or bf16")
+        if tuple(beta.shape) != (b, self.heads) or beta.dtype != torch.float32 or not beta.is_contiguous():
+            raise ValueError(f"beta must be contiguous fp32 {(b, self.heads)}")
+        if out is None:
+            out = torch.empty(want, dtype=torch.float32, device=q.device)
+        elif tuple(out.shape) != want or out.dtype != torch.float32 or not out.is_contiguous():
+            raise ValueError(f"out must be contiguous fp32 {want}")
+        rc = _native.lib().pm_delta_step_slots(
+            self.pool[layer].data_ptr(), slots.data_ptr(), self.n_slots, q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), beta.data_ptr(), out.data_ptr(), b, self.heads, self.dim,
+            _native.DTYPE_BF16 if q.dtype == torch.bfloat16 else _native.DTYPE_F32,
+            torch.cuda.current_stream(q.device).cuda_stream,
+        )
+        _native.check(rc)
+        return out
+
+
+class RecurrenceStateCache(_SlotPool):
+    """Per-request states of ``n_layers`` layers of the elementwise linear recurrence."""
+
+    def __init__(self, n_layers: int, n_slots: int, channels: int, device=None):
+        if n_layers < 1 or n_slots < 1 or channels < 1:
+            raise ValueError("n_layers, n_slots and channels must be >= 1")
+        super().__init__(n_layers, n_slots, (channels,), device)
+        self.channels = channels
+
+    def prefill(self, layer: int, slots, x, g, cu_seqlens=None, *, out_dtype=None):
+        """Run prompts through the recurrence from the slots' states into them, in place.
+
+        Fixed length: x, g ``(n, T, C)``, one request per row. Packed: ``(N, C)`` or ``(1, N, C)``
+        with ``cu_seqlens`` ``(n + 1,)``. Returns h shaped like x. ``slots`` (each at most once)
+        may be a list of ints or a GPU int tensor; with GPU ``slots`` and ``cu_seqlens`` nothing
+        here waits for the device: a request whose slot is out of range starts from a zero state,
+        leaves the pool untouched and is reported by ``check_slots``.
+        """
+        self._check_layer(layer)
+        odt = kernels._out_dtype(out_dtype)
+        if isinstance(slots, torch.Tensor) and slots.device.type == "cuda":
+            if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
+                raise ValueError("a GPU slot tensor must be 1-D int32 or int64")
+            n = slots.shape[0]
+        else:
+            slots = self._ids(slots)
+            n = len(slots)
+            if len(set(slots)) != n:
+                raise ValueError("a slot may be given once")
+        if kernels._wants_grad(x, g):
+            raise ValueError("prefill is forward only: call it under torch.no_grad()")
+        if cu_seqlens is None:
+            _, seq, chan = recurrence._check(x, g, None, 3)
+            n_seqs, cu = x.shape[0], None
+        else:
+            seq, chan, n_seqs, cu = recurrence._packed(x, g, cu_seqlens)
+        if chan != self.channels:
+            raise ValueError(f"x has {chan} channels, the cache {self.channels}")
+        if n_seqs != n:
+            raise ValueError(f"{n} slots for {n_seqs} prompts")
+        self._check_cuda(x, g)
+        call = kernels._Call(x, g)
+        xt, gt = recurrence._types(x, g)
+        with torch.cuda.device(call.device):
+            if isinstance(slots, list):
+                slots = torch.tensor(slots, dtype=torch.int32, device=call.device)
+            elif slots.device != self._pool.device:
+                raise ValueError("slots must be on the pool's device")
+            elif slots.dtype == torch.int64:
+                # (clamped: an index past int32 must not come back into range)
+                slots = slots.clamp(-1, self.n_slots).to(torch.int32)
+            xd, gd = (t if t.dim() == 3 else t[None] for t in (recurrence._rows(call, x, xt),
+                                                               recurrence._rows(call, g, gt)))
+            if cu is not None:
+                cu = recurrence._offsets(call, cu, n_seqs, seq)
+            pool = self._pool[layer]
+            h, _ = recurrence._launch(call, xd, gd, cu, pool, slots.contiguous(), self.n_slots, self._bad_slot, pool,
+                                      n_seqs, seq, chan, odt, False)
+        return h.reshape(x.shape)
+
+    def decode(self, layer: int, slots: torch.Tensor, x, g, out=None, *, out_dtype=None):
+        """One token per request: x, g ``(B, C)``, ``slots`` an int32 GPU tensor ``(B,)``. Updates
+        the states in place and returns ``out`` ``(B, C)`` (allocated when None: fp32, or
+        ``out_dtype``). Slots outside ``[0, n_slots)`` are padding: no state is touched and their
+        rows are zero. Allocation-free with ``out=`` and x and g in a type the kernel takes."""
+        self._check_layer(layer)
+        self._check_cuda(x, g, slots)
+        if slots.dim() != 1 or slots.dtype != torch.int32 or not slots.is_contiguous():
+            raise ValueError("slots must be a contiguous int32 tensor of shape (B,)")
+        want = (slots.shape[0], self.channels)
+        if tuple(x.shape) != want or tuple(g.shape) != want:
+            raise ValueError(f"x and g must be {want}, got {tuple(x.shape)} and {tuple(g.shape)}")
+        if x.dtype not in (torch.float32, torch.bfloat16) or g.dtype not in (torch.float32, x.dtype):
+            raise ValueError("x must be fp32 or bf16, and g fp32 or x's type")
+        if want[1] > 1 and (x.stride(1) != 1 or g.stride(1) != 1):
+            raise ValueError("x and g must have contiguous channels")
+        if out is None:
+            out = torch.empty(want, dtype=kernels._out_dtype(out_dtype), device=x.device)
+        elif (tuple(out.shape) != want or out.dtype not in (torch.float32, torch.bfloat16)
+              or not out.is_contiguous() or out.device != x.device):
+            raise ValueError(f"out must be contiguous fp32 or bf16 {want} on the pool's device")
+        recurrence._step(self._pool[layer], slots, self.n_slots, x, g, out,
+                         torch.cuda.current_stream(x.device).cuda_stream)
+        return out
