@@ -279,6 +279,9 @@ struct RecurrenceArgs {
     void* workspace;
 };
 hipError_t launch_recurrence(const RecurrenceArgs& a, hipStream_t st);
+// Bytes of its workspace and of its backward's (0: none), and the number of its tiles.
+size_t recurrence_ws_bytes(int n_seqs, int T, int C, bool packed, bool x_bf16);
+int64_t recurrence_tiles(int n_seqs, int T, int C, bool packed, bool x_bf16);
 
 // Its gradients: d_t = gh_t + exp(g_{t+1}) d_{t+1}, gx_t = d_t, gg_t = d_t exp(g_t) h_{t-1}, with
 // h recomputed from x and the kept states.  gh, gx and gg are contiguous, in h's, x's and g's type.

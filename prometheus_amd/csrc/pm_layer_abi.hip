@@ -40,11 +40,17 @@ int check_stride(const char* name, int64_t s) {
     return 0;
 }
 
-int check_sizes(int n, int T, int C) {
-    if (n < 0 || T < 0 || C < 0) return fail(PM_E_SHAPE, "sizes must be >= 0 (got %d, %d, %d)", n, T, C);
-    if (static_cast<int64_t>(n) * C > kMaxElems || (T > 0 && static_cast<int64_t>(n) * C > kMaxElems / T))
-        return fail(PM_E_SHAPE, "problem too large");
-    return 0;
+bool sizes_fit(int n_seqs, int T, int C, bool packed, int x_dtype) {
+    if (static_cast<int64_t>(n_seqs) * C > kMaxElems || T > INT32_MAX - PM_RECURRENCE_SPAN) return false;
+    const int64_t rows = packed ? C : static_cast<int64_t>(n_seqs) * C;
+    if (T > 0 && rows > kMaxElems / T) return false;
+    // (the counter that hands out tiles has 32 bits)
+    return pm::recurrence_tiles(n_seqs, T, C, packed, x_dtype == PM_DTYPE_BF16) <= (int64_t(1) << 31);
+}
+
+int check_sizes(int n_seqs, int T, int C, bool packed, int x_dtype) {
+    if (n_seqs < 0 || T < 0 || C < 0) return fail(PM_E_SHAPE, "sizes must be >= 0 (got %d, %d, %d)", n_seqs, T, C);
+    return sizes_fit(n_seqs, T, C, packed, x_dtype) ? 0 : fail(PM_E_SHAPE, "problem too large");
 }
 
 }  // namespace
@@ -52,8 +58,8 @@ int check_sizes(int n, int T, int C) {
 extern "C" {
 
 size_t pm_linear_recurrence_workspace_bytes(int n_seqs, int T, int C, int packed, int x_dtype) {
-    (void)n_seqs, (void)T, (void)C, (void)packed, (void)x_dtype;
-    return 0;
+    if (!known(x_dtype) || n_seqs <= 0 || T <= 0 || C <= 0 || !sizes_fit(n_seqs, T, C, packed != 0, x_dtype)) return 0;
+    return pm::recurrence_ws_bytes(n_seqs, T, C, packed != 0, x_dtype == PM_DTYPE_BF16);
 }
 
 int pm_linear_recurrence(const void* x, const void* g, const int32_t* cu_seqlens, const float* s0,
@@ -62,9 +68,7 @@ int pm_linear_recurrence(const void* x, const void* g, const int32_t* cu_seqlens
                          int x_dtype, int g_dtype, int h_dtype, void* workspace, size_t ws_bytes, void* stream) {
     pm::clear_error();
     if (int rc = check_types(x_dtype, g_dtype, h_dtype)) return rc;
-    if (int rc = check_sizes(cu_seqlens ? 1 : n_seqs, T, C)) return rc;
-    if (n_seqs < 0 || static_cast<int64_t>(n_seqs) * C > kMaxElems)
-        return fail(PM_E_SHAPE, "n_seqs %d out of range", n_seqs);
+    if (int rc = check_sizes(n_seqs, T, C, cu_seqlens != nullptr, x_dtype)) return rc;
     if (int rc = check_stride("x_sb", x_sb)) return rc;
     if (int rc = check_stride("x_st", x_st)) return rc;
     if (int rc = check_stride("g_sb", g_sb)) return rc;
@@ -96,7 +100,7 @@ int pm_linear_recurrence_bwd(const void* x, const void* g, const float* kept, co
                              size_t ws_bytes, void* stream) {
     pm::clear_error();
     if (int rc = check_types(x_dtype, g_dtype, h_dtype)) return rc;
-    if (int rc = check_sizes(B, T, C)) return rc;
+    if (int rc = check_sizes(B, T, C, false, x_dtype)) return rc;
     if (int rc = check_stride("x_sb", x_sb)) return rc;
     if (int rc = check_stride("x_st", x_st)) return rc;
     if (int rc = check_stride("g_sb", g_sb)) return rc;
@@ -124,7 +128,7 @@ int pm_linear_recurrence_step(float* s_inout, const int32_t* slots, int n_slots,
                               void* stream) {
     pm::clear_error();
     if (int rc = check_types(x_dtype, g_dtype, h_dtype)) return rc;
-    if (int rc = check_sizes(B, 1, C)) return rc;
+    if (int rc = check_sizes(B, 1, C, false, x_dtype)) return rc;
     if (int rc = check_stride("x_sb", x_sb)) return rc;
     if (int rc = check_stride("g_sb", g_sb)) return rc;
     if (B == 0 || C == 0) return 0;
