@@ -149,6 +149,7 @@ __global__ __launch_bounds__(kThreads, PACKED ? 2 : 4) void recurrence_kernel(Re
     __shared__ float sA[TL][CW], sH[TL][CW];
     __shared__ Map<PACKED> total[PARTS][CW], lb[PARTS][CW];
     __shared__ int start[PACKED ? kTileT : 1], stop[PACKED ? kTileT : 1];
+    __shared__ float first[CW];
     __shared__ uint32_t slot;
     const int tid = threadIdx.x, lc = tid % kLanesC, tl = tid / kLanesC;
     const int ch = tid % CW, part = tid / CW;
@@ -168,6 +169,13 @@ __global__ __launch_bounds__(kThreads, PACKED ? 2 : 4) void recurrence_kernel(Re
             const int n = t0 + r < a.T ? nc : 0;
             xr[r].load(xp + r * a.x_st, n);
             gr[r].load(gp + r * a.g_st, n);
+        }
+        // the state before the sequence: read by its first tile only, before that tile's map is
+        // out, as the last tile may write the same row of the pool soon after
+        if (!PACKED && j == 0 && part == 0) {
+            const int64_t row = state_row(a.slots, a.n_slots, seq);
+            if (row < 0 && a.bad) atomicOr(a.bad, 1);
+            first[ch] = a.s0 && row >= 0 && cbase + ch < a.C ? a.s0[row * a.C + cbase + ch] : 0.f;
         }
         unsigned starts = 0, stops = 0;  // bit r: a sequence starts (ends) with token t0 + r
         if constexpr (PACKED) {
@@ -227,16 +235,12 @@ __global__ __launch_bounds__(kThreads, PACKED ? 2 : 4) void recurrence_kernel(Re
         }
         total[part][ch] = sum;
         __syncthreads();
+        float s = !PACKED && j == 0 ? first[ch] : 0.f;
         if (p.next && part == 0) {
 #pragma unroll
             for (int i = 1; i < PARTS; ++i) sum.then(total[i][ch]);
+            if (!PACKED && j == 0) sum = {0.f, sum.of(s)};  // the first tile's map yields its state
             publish(p.map + (col * p.tiles + j) * CW + ch, sum.word());
-        }
-        float s = 0.f;
-        if constexpr (!PACKED) {
-            const int64_t row = state_row(a.slots, a.n_slots, seq);
-            if (j == 0 && row < 0 && a.bad && tid == 0) atomicOr(a.bad, 1);
-            if (a.s0 && row >= 0 && j < kGroup && cbase + ch < a.C) s = a.s0[row * a.C + cbase + ch];
         }
         s = state_before<PACKED, CW, PARTS>(p, col, j, ch, part, s, lb);
         if (a.kept && part == 0 && cbase + ch < a.C) a.kept[(seq * p.tiles + j) * a.C + cbase + ch] = s;

@@ -341,6 +341,29 @@ def test_cache_prefill_and_decode(types):
     assert torch.equal(cache.pool[:, [7, 3]].cpu(), saved)
 
 
+@pytest.mark.parametrize("types", [TYPES[0], TYPES[3]])
+@pytest.mark.parametrize("T", [257, 3000, 9000])
+def test_cache_prefill_in_place_over_many_spans(T, types):
+    """The last span writes the row of the pool that the first has read: the same bits as a call
+    with states of its own, prompts of one length and packed."""
+    n, C = 3, 640
+    x, g, s0 = _inputs(n, T, C, types, seed=T, rate=1e-3)
+    want, end = kernels.linear_recurrence(x, g, s0, out_dtype=types[2])
+    cache = serving.RecurrenceStateCache(1, 5, C)
+    slots = torch.tensor([4, 0, 2], dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        cache.pool[0, slots.long()] = s0
+        h = cache.prefill(0, slots, x, g, out_dtype=types[2])
+        assert torch.equal(h, want) and torch.equal(cache.pool[0, slots.long()], end)
+    cu = torch.arange(0, (n + 1) * T, T, dtype=torch.int32, device="cuda")
+    flat = [t.reshape(n * T, C) for t in (x, g)]
+    want, end = kernels.linear_recurrence_varlen(*flat, cu, s0, out_dtype=types[2])
+    for _ in range(3):
+        cache.pool[0, slots.long()] = s0
+        h = cache.prefill(0, slots, *flat, cu, out_dtype=types[2])
+        assert torch.equal(h, want) and torch.equal(cache.pool[0, slots.long()], end)
+
+
 def test_cache_padding_and_bad_slots():
     C = 70
     cache = serving.RecurrenceStateCache(1, 4, C)
