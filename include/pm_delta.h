@@ -455,12 +455,12 @@ int pm_delta_bwd_noalloc(const void* q, const void* k, const void* v, const floa
  *          may be NULL) becomes nonzero.
  *   kept   NULL, or fp32 (n_seqs, ceil(T / PM_RECURRENCE_SPAN), C): the state
  *          before each span of tokens, for the backward (fixed length only).
- *   cu_seqlens  as in pm_delta_fwd_varlen (clamped into [0, T]; tokens that
- *          no sequence covers are left unwritten).
+ *   cu_seqlens  as in pm_delta_fwd_varlen (clamped into [0, T]; h of tokens
+ *          that no sequence covers is unspecified).
  * Sums and states are fp32 whatever the types; h is rounded once.
  * workspace: pm_linear_recurrence_workspace_bytes (0 where none is needed).
  */
-#define PM_RECURRENCE_SPAN 256
+#define PM_RECURRENCE_SPAN 128
 int pm_linear_recurrence(const void* x, const void* g, const int32_t* cu_seqlens, const float* s0,
                          const int32_t* slots, int n_slots, int32_t* bad_slot, void* h, float* s_out,
                          float* kept, int n_seqs, int T, int C, int64_t x_sb, int64_t x_st, int64_t g_sb,

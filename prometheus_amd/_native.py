@@ -25,7 +25,7 @@ MAX_D = 256
 MAX_D_BWD = 256
 NOALLOC_SCRATCH_BYTES = 64 << 20
 
-RECURRENCE_SPAN = 256
+RECURRENCE_SPAN = 128
 NORM_L2 = 0
 NORM_RMS = 1
 

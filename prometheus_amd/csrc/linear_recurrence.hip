@@ -5,36 +5,60 @@
 //   d_t = gh_t + exp(g_{t+1}) d_{t+1},  gx_t = d_t,  gg_t = d_t exp(g_t) h_{t-1}
 //
 // Bound by memory: one exponential and a few multiply-adds an element against 6 bytes (bf16
-// forward) or 10 (backward). So every element is read once and written once: a tile of 256 tokens
+// forward) or 10 (backward). So every element is read once and written once: a tile of 512 tokens
 // by one 128-byte line of channels stays in registers from its loads to its stores, and what
 // tokens need of each other goes as affine maps s -> A s + H of the spans between them.
-//   1. each thread folds its own 4 tokens of 8 (fp32: 4) channels into one map;
+//   1. each thread folds its own 8 tokens of 8 (fp32: 4) channels into one map;
 //   2. through LDS the tile's maps fold in a fixed tree: per part of the tile, then the tile;
 //   3. a tile that is not its sequence's first waits for the state before it (below);
 //   4. the state walks down the tree again and through each thread's tokens.
 // The backward is the same with the message c_t = exp(g_t) d_t, c_t = exp(g_t) (gh_t + c_{t+1}),
 // from the last tile to the first, on top of a forward inside the tile from the kept state.
 //
-// Between tiles (T > 256), in one pass: a tile publishes its map as soon as it is folded; the
-// state before tile j is the state at the start of j's group of 16 tiles, taken through the maps
-// of the group's tiles before j in order; the group's last tile publishes the next group's state.
-// The order of every product and sum is fixed by j, not by which tile is done first, so results
-// are the same bits every time; and the chain that cannot run in parallel is one hop in 16 tiles.
-// Words carry value and readiness together (relaxed 8-byte atomics of agent scope; the workspace
-// starts as all ones, which no value is), so no fences. Tiles are handed out by a counter in the
-// order in which they wait for each other: the tiles a tile waits for are held by workgroups that
-// run already, so every wait ends.
+// Between tiles, in one pass: a tile publishes its map as soon as it is folded; the state before
+// tile j is the state at the start of j's group of 16 tiles, taken through the maps of the group's
+// tiles before j in order; the group's last tile publishes the next group's state. The order of
+// every product and sum is fixed by j, not by which tile is done first, so results are the same
+// bits every time; and the chain that cannot run in parallel is one hop in 16 tiles. Words carry
+// value and readiness together (relaxed 8-byte atomics of agent scope; the workspace starts as all
+// ones, which no value is), so no fences. Tiles are handed out by a counter in the order in which
+// they wait for each other, and a workgroup finishes its tile before it folds its next: the first
+// tile that is not done is always somebody's to do, and waits for nothing, so every wait ends.
+//
+// Workgroups stay: while one waits and stores, its next tile's loads are under way (forward; the
+// backward's registers hold one tile). A tile is 196 kB of traffic to a compute unit, whose 512
+// threads hold its inputs as they are in memory and make gates and products again from them after
+// the wait (holding them as floats spilled, and halved the waves).
+//
+// Measured (a card that copies at 5.0 TB/s): forward 4 x 4096 tokens of 4096 bf16 channels 88 us
+// (4.6 TB/s; with 256-token tiles, a workgroup to each and the values held 121), backward 138 us
+// (4.9 TB/s; 226), 65521 tokens of 2048 channels 162 us (5.0 TB/s; 239). An elementwise pass over
+// the same lines takes 84: rows of 128 bytes are what bounds it (512 bytes: 69, but then tiles are
+// short, and four times the hops and words cost more than the rows gain: 92 to 97). Columns dealt
+// to XCDs in runs of neighbours were slower (96), stores that stay out of the caches 2% faster.
 
 #include "pm_internal.h"
 #include "pm_vec.h"
 
 namespace pm {
 
-constexpr int kTok = 4;                       // tokens to a thread
-constexpr int kTileT = kRecSpan;              // tokens to a tile
-constexpr int kLanesC = 8;                    // threads across the channels of a tile
-constexpr int kThreads = kTileT / kTok * kLanesC;
-constexpr int kGroup = 16;                    // tiles to a group
+constexpr int kLanesC = 8;  // threads across the channels of a tile: a 128-byte line of x
+constexpr int kGroup = 16;  // tiles to a group
+
+// The shape of a tile: `tok` tokens to a thread, `threads` to a workgroup. Long tiles fill a
+// compute unit with one workgroup and pass states on; of the others, which hold the whole of a
+// short sequence, two or four fit.
+template <int TOK, int THREADS, int BLOCKS, bool CHAINED>
+struct Shape {
+    static constexpr int tok = TOK, threads = THREADS, span = THREADS / kLanesC * TOK;
+    static constexpr int blocks = BLOCKS;                       // workgroups that the card holds at a time
+    static constexpr int waves = THREADS * BLOCKS / 256 / 256;  // to a SIMD
+    static constexpr bool chained = CHAINED;
+};
+typedef Shape<8, 512, 256, true> Long;
+typedef Shape<4, 512, 512, false> Middle;
+typedef Shape<4, 256, 1024, false> Short;
+static_assert(Long::span % kRecSpan == 0 && Middle::span % kRecSpan == 0 && Short::span == kRecSpan, "kept states start every tile");
 
 // The tiles of a call and the words through which they pass states (all null where each
 // sequence is one tile).
@@ -42,6 +66,7 @@ struct Tiles {
     int cgroups;     // channel groups
     int64_t cols;    // sequences x channel groups
     int64_t tiles;   // tiles along the tokens
+    int span;        // tokens to a tile: which Shape
     uint32_t* next;  // the counter that hands out tiles
     uint64_t* map;   // [col][tile][channel]: H below, A above
     uint64_t* state; // [col][group][channel]: the state before the group below, 0 above
@@ -53,27 +78,33 @@ __device__ __forceinline__ uint64_t word(uint32_t above, float below) {
 __device__ __forceinline__ void publish(uint64_t* p, uint64_t v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ uint64_t wait_word(uint64_t* p) {
-    for (;;) {
-        const uint64_t v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (static_cast<uint32_t>(v >> 32) != 0xffffffffu) return v;
+__device__ __forceinline__ uint64_t look(uint64_t* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// the word at p once it is there; v is what a look at it gave
+__device__ __forceinline__ uint64_t wait_word(uint64_t* p, uint64_t v) {
+    while (static_cast<uint32_t>(v >> 32) == 0xffffffffu) {
         __builtin_amdgcn_s_sleep(1);
+        v = look(p);
     }
+    return v;
 }
 __device__ __forceinline__ float low(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
 __device__ __forceinline__ float high(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
 
-// s -> A s + H. A negative A (PACKED only) is a map that a sequence starts in: its H is the state
-// whatever came before, infinities and NaN included.
+// s -> A s + H. An A whose sign bit is set (PACKED only) is a map that a sequence starts in: its H
+// is the state whatever came before, infinities and NaN included.
 template <bool PACKED>
 struct Map {
     float A, H;
+    __device__ __forceinline__ bool anew() const { return PACKED && static_cast<int>(__float_as_uint(A)) < 0; }
+    // a token's gate (which has no sign) and input; the sign of A stays
+    __device__ __forceinline__ void token(float a, float x) { H = fmaf(a, H, x), A *= a; }
     __device__ __forceinline__ void then(const Map& m) {
-        const bool anew = PACKED && m.A < 0.f;
-        H = anew ? m.H : fmaf(m.A, H, m.H);
-        A = anew ? m.A : (PACKED && A < 0.f ? A : A * m.A);
+        H = m.of(H);
+        A = m.anew() ? m.A : A * m.A;
     }
-    __device__ __forceinline__ float of(float s) const { return PACKED && A < 0.f ? H : fmaf(A, s, H); }
+    __device__ __forceinline__ float of(float s) const { return anew() ? H : fmaf(A, s, H); }
     __device__ __forceinline__ uint64_t word() const {
         const uint32_t a = __float_as_uint(A);
         return pm::word(a == 0xffffffffu ? 0x7fc00000u : a, H);  // (a NaN all of whose bits are set)
@@ -82,6 +113,8 @@ struct Map {
 };
 
 __device__ __forceinline__ float gate(float g) { return __builtin_amdgcn_exp2f(g * 1.44269504088896341f); }
+
+__host__ __device__ inline int64_t spans_of(int T) { return (static_cast<int64_t>(T) + kRecSpan - 1) / kRecSpan; }
 
 // Row of a sequence's state in s0 and s_out, or -1 (a slot outside the pool).
 __device__ __forceinline__ int64_t state_row(const int32_t* slots, int n_slots, int seq) {
@@ -93,24 +126,27 @@ __device__ __forceinline__ int64_t state_row(const int32_t* slots, int n_slots, 
 // Where the thread (ch, part) of a tile's fold stands in a group's chain, and the state it takes
 // from there. All threads of the workgroup call it; `lb` is LDS [PARTS][CW]. `j` counts tiles in
 // the order in which they wait for each other, `first` is the state before tile 0.
-template <bool PACKED, int CW, int PARTS>
+template <bool CHAINED, bool PACKED, int CW, int PARTS>
 __device__ __forceinline__ float state_before(const Tiles& p, int64_t col, int64_t j, int ch, int part, float first,
                                               Map<PACKED> (*lb)[CW]) {
-    if (!p.next || j == 0) return first;
+    if (!CHAINED || !p.next || j == 0) return first;
     constexpr int Q = (kGroup + PARTS - 1) / PARTS;  // tiles of the group to a part
-    const int64_t g0 = j / kGroup * kGroup;
+    const int64_t g0 = j / kGroup * kGroup, groups = (p.tiles + kGroup - 1) / kGroup;
     const int n = static_cast<int>(j - g0);
+    uint64_t* maps = p.map + (col * p.tiles + g0 + part * Q) * CW + ch;
+    uint64_t* state = p.state + (col * groups + j / kGroup) * CW + ch;
+    const bool chained = part == 0 && g0 > 0;
+    // every word is asked for before the first is waited for
+    uint64_t w[Q], from = 0;
+    if (chained) from = look(state);
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+        if (part * Q + i < n) w[i] = look(maps + static_cast<int64_t>(i) * CW);
     Map<PACKED> m{1.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < Q; ++i) {
-        const int q = part * Q + i;
-        if (q < n) m.then(Map<PACKED>::read(wait_word(p.map + (col * p.tiles + g0 + q) * CW + ch)));
-    }
-    if (part == 0) {
-        const int64_t groups = (p.tiles + kGroup - 1) / kGroup;
-        const float s = g0 == 0 ? first : low(wait_word(p.state + (col * groups + j / kGroup) * CW + ch));
-        m.H = m.of(s);
-    }
+    for (int i = 0; i < Q; ++i)
+        if (part * Q + i < n) m.then(Map<PACKED>::read(wait_word(maps + static_cast<int64_t>(i) * CW, w[i])));
+    if (part == 0) m.H = m.of(chained ? low(wait_word(state, from)) : first);
     lb[part][ch] = m;
     __syncthreads();
     float s = lb[0][ch].H;
@@ -127,49 +163,108 @@ __device__ __forceinline__ void publish_state(const Tiles& p, int64_t col, int64
     publish(p.state + (col * groups + j / kGroup + 1) * CW + ch, word(0, s));
 }
 
-// The next tile of a workgroup, or -1. `slot` is one LDS word.
-__device__ __forceinline__ int64_t next_tile(const Tiles& p, int64_t last, uint32_t* slot) {
-    const int64_t all = p.cols * p.tiles;
+// A workgroup's tiles: thread 0 asks for the next one early (ask), all threads have it after the
+// barrier that follows tell.
+struct Turns {
+    const Tiles& p;
+    uint32_t* slot;  // LDS
+    uint32_t got;
     int64_t id;
-    if (p.next) {
-        __syncthreads();  // the last tile's reads of LDS, this word's among them, are done
-        if (threadIdx.x == 0) *slot = __hip_atomic_fetch_add(p.next, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __device__ __forceinline__ Turns(const Tiles& tiles, uint32_t* lds) : p(tiles), slot(lds), got(0), id(blockIdx.x) {
+        if (!p.next) return;
+        ask();
+        tell();
         __syncthreads();
-        id = *slot;
-    } else {
-        if (last >= 0) __syncthreads();
-        id = last < 0 ? blockIdx.x : last + gridDim.x;
+        take();
+        __syncthreads();
     }
-    return id < all ? id : -1;
+    __device__ __forceinline__ bool done() const { return id >= p.cols * p.tiles; }
+    __device__ __forceinline__ void ask() {
+        if (p.next && threadIdx.x == 0) got = __hip_atomic_fetch_add(p.next, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __device__ __forceinline__ void tell() {
+        if (p.next && threadIdx.x == 0) *slot = got;
+    }
+    __device__ __forceinline__ void take() { id = p.next ? *slot : id + gridDim.x; }
+};
+
+template <bool PACKED, int CW>
+struct Place {
+    int64_t j, col;
+    int seq, cbase;
+    __device__ __forceinline__ Place(const Tiles& p, int64_t id) {
+        // (32 bits: the number of tiles is at most 2^31)
+        const uint32_t u = static_cast<uint32_t>(id), cols = static_cast<uint32_t>(p.cols), q = u / cols, c = u - q * cols;
+        j = q, col = c;
+        const uint32_t b = PACKED ? 0 : c / static_cast<uint32_t>(p.cgroups);
+        seq = static_cast<int>(b);
+        cbase = static_cast<int>(c - b * p.cgroups) * CW;
+    }
+};
+
+template <typename X, typename G, int V, int K>
+__device__ __forceinline__ void load_tile(const RecurrenceArgs& a, int seq, int t0, int c0, Row<X, V> (&xr)[K],
+                                          Row<G, V> (&gr)[K]) {
+    const X* xp = static_cast<const X*>(a.x) + seq * a.x_sb + t0 * a.x_st + c0;
+    const G* gp = static_cast<const G*>(a.g) + seq * a.g_sb + t0 * a.g_st + c0;
+#pragma unroll
+    for (int r = 0; r < K; ++r) {
+        const int n = t0 + r < a.T ? a.C - c0 : 0;
+        xr[r].load(xp + r * a.x_st, n);
+        gr[r].load(gp + r * a.g_st, n);
+    }
 }
 
-template <typename X, typename G, typename H, int V, bool PACKED>
-__global__ __launch_bounds__(kThreads, PACKED ? 2 : 4) void recurrence_kernel(RecurrenceArgs a, Tiles p) {
-    constexpr int CW = kLanesC * V, TL = kTileT / kTok, PARTS = kThreads / CW, PER = TL / PARTS;
+// Keeps the compiler from carrying values made from a row across this point in registers: they
+// are made again from the row, which costs less than the waves that the registers would.
+template <typename E, int V>
+__device__ __forceinline__ void forget(Row<E, V>& r) {
+#pragma unroll
+    for (uint32_t& w : r.raw) asm volatile("" : "+v"(w));
+}
+
+template <typename X, typename G, typename H, int V, typename S, bool PACKED>
+__global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(RecurrenceArgs a, Tiles p) {
+    constexpr int K = S::tok, CW = kLanesC * V, TL = S::span / K, PARTS = S::threads / CW, PER = TL / PARTS;
+    typedef Map<PACKED> M;
     __shared__ float sA[TL][CW], sH[TL][CW];
-    __shared__ Map<PACKED> total[PARTS][CW], lb[PARTS][CW];
-    __shared__ int start[PACKED ? kTileT : 1], stop[PACKED ? kTileT : 1];
+    __shared__ M total[PARTS][CW], lb[PARTS][CW];
+    // where a packed sequence starts or ends in the tile: which one, by token, and the tokens, a
+    // bit each, by thread (starts below, ends from bit K on)
+    __shared__ int start[PACKED ? S::span : 1], stop[PACKED ? S::span : 1];
+    __shared__ unsigned marks[PACKED ? TL : 1];
     __shared__ float first[CW];
     __shared__ uint32_t slot;
     const int tid = threadIdx.x, lc = tid % kLanesC, tl = tid / kLanesC;
     const int ch = tid % CW, part = tid / CW;
 
-    for (int64_t id = next_tile(p, -1, &slot); id >= 0; id = next_tile(p, id, &slot)) {
-        const int64_t j = id / p.cols, col = id - j * p.cols;
-        const int seq = PACKED ? 0 : static_cast<int>(col / p.cgroups);
-        const int cbase = static_cast<int>(PACKED ? col : col % p.cgroups) * CW;
+    // a sequence's offsets, clamped; the first S::threads sequences' stay in registers
+    auto offset = [&](int i) { return min(max(a.cu_seqlens[i], 0), a.T); };
+    int b0 = 0, e0 = 0;
+    if constexpr (PACKED) {
+        if (tid < a.n_seqs) b0 = offset(tid), e0 = offset(tid + 1);
+        if (tid < TL) marks[tid] = 0;
+        __syncthreads();
+    }
+
+    Turns turns(p, &slot);
+    Row<X, V> xn[K];
+    Row<G, V> gn[K];
+    if (!turns.done()) {
+        const Place<PACKED, CW> at(p, turns.id);
+        load_tile<X, G, V, K>(a, at.seq, static_cast<int>(at.j) * S::span + tl * K, at.cbase + lc * V, xn, gn);
+    }
+    while (!turns.done()) {
+        const Place<PACKED, CW> at(p, turns.id);
+        const int64_t j = at.j, col = at.col;
+        const int seq = at.seq, cbase = at.cbase;
         const int c0 = cbase + lc * V, nc = a.C - c0;  // this thread's channels, and how many are there
-        const int tile0 = static_cast<int>(j) * kTileT, t0 = tile0 + tl * kTok;
-        const X* xp = static_cast<const X*>(a.x) + seq * a.x_sb + t0 * a.x_st + c0;
-        const G* gp = static_cast<const G*>(a.g) + seq * a.g_sb + t0 * a.g_st + c0;
-        Row<X, V> xr[kTok];
-        Row<G, V> gr[kTok];
+        const int tile0 = static_cast<int>(j) * S::span, t0 = tile0 + tl * K;
+        Row<X, V> xr[K];
+        Row<G, V> gr[K];
 #pragma unroll
-        for (int r = 0; r < kTok; ++r) {
-            const int n = t0 + r < a.T ? nc : 0;
-            xr[r].load(xp + r * a.x_st, n);
-            gr[r].load(gp + r * a.g_st, n);
-        }
+        for (int r = 0; r < K; ++r) xr[r] = xn[r], gr[r] = gn[r];
+        turns.ask();
         // the state before the sequence: read by its first tile only, before that tile's map is
         // out, as the last tile may write the same row of the pool soon after
         if (!PACKED && j == 0 && part == 0) {
@@ -177,108 +272,134 @@ __global__ __launch_bounds__(kThreads, PACKED ? 2 : 4) void recurrence_kernel(Re
             if (row < 0 && a.bad) atomicOr(a.bad, 1);
             first[ch] = a.s0 && row >= 0 && cbase + ch < a.C ? a.s0[row * a.C + cbase + ch] : 0.f;
         }
-        unsigned starts = 0, stops = 0;  // bit r: a sequence starts (ends) with token t0 + r
+        H* hp = static_cast<H*>(a.h) + (static_cast<int64_t>(seq) * a.T + t0) * a.C + c0;
+        auto finish = [&](int r, const float(&h)[V], int ends) {
+            if (t0 + r < a.T) store_row<H, V>(hp + static_cast<int64_t>(r) * a.C, h, nc);
+            if (ends >= 0) {
+                const int64_t row = state_row(a.slots, a.n_slots, ends);
+                if (row >= 0) store_row<float, V>(a.s_out + row * a.C + c0, h, nc);
+            }
+        };
+        unsigned mark = 0;
+        auto boundaries = [&](int b, int e, int i) {  // of sequence i, as far as they are in this tile
+            const int u = b - tile0, w = e - 1 - tile0;
+            if (b < e && u >= 0 && u < S::span) start[u] = i, atomicOr(marks + u / K, 1u << u % K);
+            if (b < e && w >= 0 && w < S::span) stop[w] = i, atomicOr(marks + w / K, 1u << (K + w % K));
+        };
         if constexpr (PACKED) {
-            for (int i = tid; i < kTileT; i += kThreads) start[i] = stop[i] = -1;
+            boundaries(b0, e0, tid);
+            for (int i = tid + S::threads; i < a.n_seqs; i += S::threads) boundaries(offset(i), offset(i + 1), i);
             __syncthreads();
-            for (int i = tid; i < a.n_seqs; i += kThreads) {
-                const int b = min(max(a.cu_seqlens[i], 0), a.T), e = min(max(a.cu_seqlens[i + 1], b), a.T);
-                if (b == e) continue;
-                if (b >= tile0 && b < tile0 + kTileT) start[b - tile0] = i;
-                if (e > tile0 && e <= tile0 + kTileT) stop[e - 1 - tile0] = i;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < kTok; ++r) {
-                starts |= (start[tl * kTok + r] >= 0) << r;
-                stops |= (stop[tl * kTok + r] >= 0) << r;
-            }
+            mark = marks[tl];
         }
-        float av[kTok][V], xv[kTok][V];
-        Map<PACKED> m[V];
+        int known = K;  // tokens from here on follow a sequence's start in this thread
+        M m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = {1.f, 0.f};
+        // (tokens past the end are zeros: gates of one and nothing added)
+        if (!PACKED || !__any(mark != 0)) {
 #pragma unroll
-        for (int r = 0; r < kTok; ++r) {
+            for (int r = 0; r < K; ++r)
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                // (tokens past the end are zeros: gates of one and nothing added)
-                av[r][v] = gate(gr[r][v]);
-                xv[r][v] = xr[r][v];
-            }
-            if (PACKED && (starts >> r & 1)) {
-                // the start's state goes into x here, where it is read once: the sequence's last
-                // tile may write the same row of the pool as soon as this tile's map is out
-                const int64_t row = state_row(a.slots, a.n_slots, start[tl * kTok + r]);
-                if (row < 0 && a.bad) atomicOr(a.bad, 1);
-                Row<float, V> s;
-                s.load(a.s0 && row >= 0 ? a.s0 + row * a.C + c0 : nullptr, a.s0 && row >= 0 ? nc : 0);
+                for (int v = 0; v < V; ++v) m[v].token(gate(gr[r][v]), xr[r][v]);
+        } else {
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    xv[r][v] = fmaf(av[r][v], s[v], xv[r][v]);
-                    m[v] = {-1.f, xv[r][v]};
+            for (int r = 0; r < K; ++r) {
+                if (mark >> r & 1) {
+                    // the start's state is read here, once: the sequence's last tile may write the
+                    // same row of the pool as soon as this tile's map is out
+                    const int64_t row = state_row(a.slots, a.n_slots, start[tl * K + r]);
+                    if (row < 0 && a.bad) atomicOr(a.bad, 1);
+                    Row<float, V> s;
+                    s.load(a.s0 && row >= 0 ? a.s0 + row * a.C + c0 : nullptr, a.s0 && row >= 0 ? nc : 0);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) m[v] = {-1.f, s[v]};
+                    known = min(known, r);
                 }
-            } else {
 #pragma unroll
-                for (int v = 0; v < V; ++v) m[v].then({av[r][v], xv[r][v]});
+                for (int v = 0; v < V; ++v) m[v].token(gate(gr[r][v]), xr[r][v]);
+                if (known <= r) {
+                    // nothing before this thread's tokens matters any more: h is there
+                    float h[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) h[v] = m[v].H;
+                    finish(r, h, mark >> (K + r) & 1 ? stop[tl * K + r] : -1);
+                }
             }
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) sA[tl][lc * V + v] = m[v].A, sH[tl][lc * V + v] = m[v].H;
         __syncthreads();
 
-        Map<PACKED> mine[PER], sum{1.f, 0.f};
+        if (PACKED && tid < TL) marks[tid] = 0;  // (read above; the next tile's come after a barrier)
+        M mine[PER], sum{1.f, 0.f};
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             mine[i] = {sA[part * PER + i][ch], sH[part * PER + i][ch]};
             sum.then(mine[i]);
         }
         total[part][ch] = sum;
+        turns.tell();
         __syncthreads();
+        turns.take();
         float s = !PACKED && j == 0 ? first[ch] : 0.f;
-        if (p.next && part == 0) {
+        if (S::chained && p.next && part == 0) {
 #pragma unroll
             for (int i = 1; i < PARTS; ++i) sum.then(total[i][ch]);
             if (!PACKED && j == 0) sum = {0.f, sum.of(s)};  // the first tile's map yields its state
             publish(p.map + (col * p.tiles + j) * CW + ch, sum.word());
         }
-        s = state_before<PACKED, CW, PARTS>(p, col, j, ch, part, s, lb);
-        if (a.kept && part == 0 && cbase + ch < a.C) a.kept[(seq * p.tiles + j) * a.C + cbase + ch] = s;
+        if (!turns.done()) {
+            const Place<PACKED, CW> next(p, turns.id);
+            load_tile<X, G, V, K>(a, next.seq, static_cast<int>(next.j) * S::span + tl * K, next.cbase + lc * V, xn, gn);
+        }
+        s = state_before<S::chained, PACKED, CW, PARTS>(p, col, j, ch, part, s, lb);
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)
             if (i < part) s = total[i][ch].of(s);
+        const int from = tile0 + part * PER * K;  // this part's first token
+        if (!PACKED && a.kept && from % kRecSpan == 0 && from < a.T && cbase + ch < a.C)
+            a.kept[(seq * spans_of(a.T) + from / kRecSpan) * a.C + cbase + ch] = s;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             sH[part * PER + i][ch] = s;
             s = mine[i].of(s);
         }
-        if (part == PARTS - 1) publish_state<CW>(p, col, j, ch, s);
+        if (S::chained && part == PARTS - 1) publish_state<CW>(p, col, j, ch, s);
         __syncthreads();
 
         float h[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = sH[tl][lc * V + v];
-        H* hp = static_cast<H*>(a.h) + (static_cast<int64_t>(seq) * a.T + t0) * a.C + c0;
+        __syncthreads();  // (the next tile's maps go where these states were)
 #pragma unroll
-        for (int r = 0; r < kTok; ++r) {
-            const int t = t0 + r;
+        for (int r = 0; r < K; ++r) forget(xr[r]), forget(gr[r]);
+        auto walk = [&](int r) {
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                h[v] = PACKED && (starts >> r & 1) ? xv[r][v] : fmaf(av[r][v], h[v], xv[r][v]);
-            if (t < a.T) store_row<H, V>(hp + static_cast<int64_t>(r) * a.C, h, nc);
-            const int ends = PACKED ? (stops >> r & 1 ? stop[tl * kTok + r] : -1) : (t == a.T - 1 ? seq : -1);
-            if (ends >= 0) {
-                const int64_t row = state_row(a.slots, a.n_slots, ends);
-                if (row >= 0) store_row<float, V>(a.s_out + row * a.C + c0, h, nc);
+            for (int v = 0; v < V; ++v) h[v] = fmaf(gate(gr[r][v]), h[v], xr[r][v]);
+        };
+        if (!PACKED || !__any(mark != 0)) {
+#pragma unroll
+            for (int r = 0; r < K; ++r) {
+                walk(r);
+                finish(r, h, !PACKED && t0 + r == a.T - 1 ? seq : -1);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < K; ++r) {
+                if (known <= r) break;
+                walk(r);
+                finish(r, h, mark >> (K + r) & 1 ? stop[tl * K + r] : -1);
             }
         }
+        if constexpr (PACKED) __syncthreads();  // (and its boundaries where these are)
     }
 }
 
 // The gradients; tiles go from the last to the first, and c_t = exp(g_t) d_t is the state.
-template <typename X, typename G, typename H, int V>
-__global__ __launch_bounds__(kThreads, 4) void recurrence_bwd_kernel(RecurrenceBwdArgs a, Tiles p) {
-    constexpr int CW = kLanesC * V, TL = kTileT / kTok, PARTS = kThreads / CW, PER = TL / PARTS;
+template <typename X, typename G, typename H, int V, typename S>
+__global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(RecurrenceBwdArgs a, Tiles p) {
+    constexpr int K = S::tok, CW = kLanesC * V, TL = S::span / K, PARTS = S::threads / CW, PER = TL / PARTS;
     typedef Map<false> M;
     __shared__ float sA[TL][CW], sF[TL][CW], sB[TL][CW];
     __shared__ M fwd[PARTS][CW], bwd[PARTS][CW], lb[PARTS][CW];
@@ -286,42 +407,39 @@ __global__ __launch_bounds__(kThreads, 4) void recurrence_bwd_kernel(RecurrenceB
     const int tid = threadIdx.x, lc = tid % kLanesC, tl = tid / kLanesC;
     const int ch = tid % CW, part = tid / CW;
 
-    for (int64_t id = next_tile(p, -1, &slot); id >= 0; id = next_tile(p, id, &slot)) {
-        const int64_t j = id / p.cols, col = id - j * p.cols, tile = p.tiles - 1 - j;
-        const int b = static_cast<int>(col / p.cgroups), cbase = static_cast<int>(col % p.cgroups) * CW;
+    Turns turns(p, &slot);
+    while (!turns.done()) {
+        const Place<false, CW> at(p, turns.id);
+        const int64_t j = at.j, col = at.col, tile = p.tiles - 1 - j;
+        const int b = at.seq, cbase = at.cbase;
         const int c0 = cbase + lc * V, nc = a.C - c0;
-        const int t0 = static_cast<int>(tile) * kTileT + tl * kTok;
+        const int t0 = static_cast<int>(tile) * S::span + tl * K;
         const X* xp = static_cast<const X*>(a.x) + b * a.x_sb + t0 * a.x_st + c0;
         const G* gp = static_cast<const G*>(a.g) + b * a.g_sb + t0 * a.g_st + c0;
         const int64_t out = (static_cast<int64_t>(b) * a.T + t0) * a.C + c0;
-        Row<X, V> xr[kTok];
-        Row<G, V> gr[kTok];
-        Row<H, V> hr[kTok];
+        Row<X, V> xr[K];
+        Row<G, V> gr[K];
+        Row<H, V> hr[K];
 #pragma unroll
-        for (int r = 0; r < kTok; ++r) {
+        for (int r = 0; r < K; ++r) {
             const int n = t0 + r < a.T ? nc : 0;
             xr[r].load(xp + r * a.x_st, n);
             gr[r].load(gp + r * a.g_st, n);
             hr[r].load(static_cast<const H*>(a.gh) + out + static_cast<int64_t>(r) * a.C, a.gh ? n : 0);
         }
-        float av[kTok][V];
-        M f[V], w[V];  // the tokens' map of h, and of c
+        turns.ask();
+        const bool there = cbase + ch < a.C;
+        float h = there ? a.kept[(b * spans_of(a.T) + tile * (S::span / kRecSpan)) * a.C + cbase + ch] : 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) f[v] = w[v] = {1.f, 0.f};
+        for (int v = 0; v < V; ++v) {
+            M f{1.f, 0.f};  // the tokens' map of h
+            float w = 0.f;  // and of c, whose factor is the same
 #pragma unroll
-        for (int r = 0; r < kTok; ++r)
+            for (int r = 0; r < K; ++r) f.token(gate(gr[r][v]), xr[r][v]);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                av[r][v] = gate(gr[r][v]);
-                f[v].then({av[r][v], xr[r][v]});
-            }
-#pragma unroll
-        for (int r = kTok - 1; r >= 0; --r)
-#pragma unroll
-            for (int v = 0; v < V; ++v) w[v].H = av[r][v] * (w[v].H + hr[r][v]);
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            sA[tl][lc * V + v] = f[v].A, sF[tl][lc * V + v] = f[v].H, sB[tl][lc * V + v] = w[v].H;
+            for (int r = K - 1; r >= 0; --r) w = gate(gr[r][v]) * (w + hr[r][v]);
+            sA[tl][lc * V + v] = f.A, sF[tl][lc * V + v] = f.H, sB[tl][lc * V + v] = w;
+        }
         __syncthreads();
 
         float A[PER], F[PER], B[PER];
@@ -335,16 +453,16 @@ __global__ __launch_bounds__(kThreads, 4) void recurrence_bwd_kernel(RecurrenceB
         for (int i = PER - 1; i >= 0; --i) down.then({A[i], B[i]});
         fwd[part][ch] = up;
         bwd[part][ch] = down;
+        turns.tell();
         __syncthreads();
-        if (p.next && part == PARTS - 1) {
+        turns.take();
+        if (S::chained && p.next && part == PARTS - 1) {
 #pragma unroll
             for (int i = PARTS - 2; i >= 0; --i) down.then(bwd[i][ch]);
             publish(p.map + (col * p.tiles + j) * CW + ch, down.word());
         }
-        const bool there = cbase + ch < a.C;
         float c = a.gs && j < kGroup && there ? a.gs[static_cast<int64_t>(b) * a.C + cbase + ch] : 0.f;
-        float h = there ? a.kept[(b * p.tiles + tile) * a.C + cbase + ch] : 0.f;
-        c = state_before<false, CW, PARTS>(p, col, j, ch, part, c, lb);
+        c = state_before<S::chained, false, CW, PARTS>(p, col, j, ch, part, c, lb);
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)
             if (i < part) h = fwd[i][ch].of(h);
@@ -362,32 +480,37 @@ __global__ __launch_bounds__(kThreads, 4) void recurrence_bwd_kernel(RecurrenceB
             c = fmaf(A[i], c, B[i]);
         }
         if (part == 0) {
-            publish_state<CW>(p, col, j, ch, c);
+            if (S::chained) publish_state<CW>(p, col, j, ch, c);
             if (tile == 0 && there) a.gs0[static_cast<int64_t>(b) * a.C + cbase + ch] = c;
         }
         __syncthreads();
 
-        float hb[kTok][V], cv[V];  // the state before each token; c behind it
+        Row<X, V> gx[K];
+        Row<G, V> gg[K];
+#pragma unroll
+        for (int r = 0; r < K; ++r) forget(xr[r]), forget(gr[r]), forget(hr[r]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            hb[0][v] = sF[tl][lc * V + v], cv[v] = sB[tl][lc * V + v];
+            float hb[K];  // the state before each token
+            hb[0] = sF[tl][lc * V + v];
 #pragma unroll
-            for (int r = 1; r < kTok; ++r) hb[r][v] = fmaf(av[r - 1][v], hb[r - 1][v], xr[r - 1][v]);
-        }
+            for (int r = 1; r < K; ++r) hb[r] = fmaf(gate(gr[r - 1][v]), hb[r - 1], xr[r - 1][v]);
+            float cv = sB[tl][lc * V + v];
 #pragma unroll
-        for (int r = kTok - 1; r >= 0; --r) {
-            float gx[V], gg[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                gx[v] = hr[r][v] + cv[v];
-                cv[v] = av[r][v] * gx[v];
-                gg[v] = cv[v] * hb[r][v];
+            for (int r = K - 1; r >= 0; --r) {
+                const float d = hr[r][v] + cv;
+                cv = gate(gr[r][v]) * d;
+                gx[r].set(v, d);
+                gg[r].set(v, cv * hb[r]);
             }
+        }
+        __syncthreads();  // (the next tile's maps go where these states were)
+#pragma unroll
+        for (int r = 0; r < K; ++r)
             if (t0 + r < a.T) {
-                store_row<X, V>(static_cast<X*>(a.gx) + out + static_cast<int64_t>(r) * a.C, gx, nc);
-                store_row<G, V>(static_cast<G*>(a.gg) + out + static_cast<int64_t>(r) * a.C, gg, nc);
+                gx[r].store(static_cast<X*>(a.gx) + out + static_cast<int64_t>(r) * a.C, nc);
+                gg[r].store(static_cast<G*>(a.gg) + out + static_cast<int64_t>(r) * a.C, nc);
             }
-        }
     }
 }
 
@@ -450,7 +573,11 @@ static Tiles tiles_of(int n_seqs, int T, int C, bool packed, bool x_bf16, void* 
     Tiles p{};
     p.cgroups = (C + cw - 1) / cw;
     p.cols = static_cast<int64_t>(packed ? 1 : n_seqs) * p.cgroups;
-    p.tiles = (static_cast<int64_t>(T) + kTileT - 1) / kTileT;
+    // sequences that a short tile holds take it: as many bytes under way with fewer idle threads
+    // (64 x 128 tokens of 2048 channels forward 20 us, in long tiles 67; 16 x 256 of 4096 middle
+    // 19, long 34); longer ones never do (4 x 4096 of 4096: short 124, long 89)
+    p.span = T <= Short::span ? Short::span : T <= Middle::span ? Middle::span : Long::span;
+    p.tiles = (static_cast<int64_t>(T) + p.span - 1) / p.span;
     if (p.tiles > 1) {
         p.next = static_cast<uint32_t*>(workspace);
         p.map = static_cast<uint64_t*>(workspace) + 32;
@@ -472,8 +599,17 @@ size_t recurrence_ws_bytes(int n_seqs, int T, int C, bool packed, bool x_bf16) {
     return n ? static_cast<size_t>(n + 32) * 8 : 0;
 }
 
-// Workgroups of a launch: one to a tile, up to a bound from which each takes several in turn.
-static unsigned blocks_of(int64_t n) { return static_cast<unsigned>(n < (1 << 20) ? n : 1 << 20); }
+// f(Shape, grid) of a call
+template <typename F>
+static void by_shape(const Tiles& p, F f) {
+    const int64_t n = p.cols * p.tiles;
+    auto go = [&](auto shape) {
+        f(shape, dim3(static_cast<unsigned>(n < decltype(shape)::blocks ? n : decltype(shape)::blocks)));
+    };
+    if (p.span == Short::span) go(Short{});
+    else if (p.span == Middle::span) go(Middle{});
+    else go(Long{});
+}
 
 static hipError_t begin(const Tiles& p, int64_t words, const RecurrenceArgs& a, hipStream_t st) {
     int64_t blocks = (words + 2047) / 2048;  // eight words a thread
@@ -495,9 +631,11 @@ hipError_t launch_recurrence(const RecurrenceArgs& a, hipStream_t st) {
         typedef PM_ELEM(g) G;
         typedef PM_ELEM(h) H;
         constexpr int V = sizeof(X) == 2 ? 8 : 4;
-        const dim3 grid(blocks_of(p.cols * p.tiles));
-        if (packed) hipLaunchKernelGGL((recurrence_kernel<X, G, H, V, true>), grid, dim3(kThreads), 0, st, a, p);
-        else hipLaunchKernelGGL((recurrence_kernel<X, G, H, V, false>), grid, dim3(kThreads), 0, st, a, p);
+        by_shape(p, [&](auto shape, dim3 grid) {
+            typedef decltype(shape) S;
+            if (packed) hipLaunchKernelGGL((recurrence_kernel<X, G, H, V, S, true>), grid, dim3(S::threads), 0, st, a, p);
+            else hipLaunchKernelGGL((recurrence_kernel<X, G, H, V, S, false>), grid, dim3(S::threads), 0, st, a, p);
+        });
         e = hipGetLastError();
     });
     return e;
@@ -517,8 +655,10 @@ hipError_t launch_recurrence_bwd(const RecurrenceBwdArgs& a, hipStream_t st) {
         typedef PM_ELEM(g) G;
         typedef PM_ELEM(h) H;
         constexpr int V = sizeof(X) == 2 ? 8 : 4;
-        hipLaunchKernelGGL((recurrence_bwd_kernel<X, G, H, V>), dim3(blocks_of(p.cols * p.tiles)), dim3(kThreads), 0, st,
-                           a, p);
+        by_shape(p, [&](auto shape, dim3 grid) {
+            typedef decltype(shape) S;
+            hipLaunchKernelGGL((recurrence_bwd_kernel<X, G, H, V, S>), grid, dim3(S::threads), 0, st, a, p);
+        });
         e = hipGetLastError();
     });
     return e;

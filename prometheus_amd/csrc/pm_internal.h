@@ -261,7 +261,7 @@ void clear_error();
 // clamped into [0, T]).  x and g have token and batch strides in elements; h is contiguous.
 // States: row i of s0 and s_out is sequence i's, or, with slots, row slots[i] is (s_out is
 // s0; a slot outside [0, n_slots) starts from zero, is not stored, and sets *bad).
-constexpr int kRecSpan = 256;  // tokens between the states kept for the backward
+constexpr int kRecSpan = 128;  // tokens between the states kept for the backward
 struct RecurrenceArgs {
     const void* x;
     const void* g;

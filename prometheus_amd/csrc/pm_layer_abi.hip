@@ -41,7 +41,7 @@ int check_stride(const char* name, int64_t s) {
 }
 
 bool sizes_fit(int n_seqs, int T, int C, bool packed, int x_dtype) {
-    if (static_cast<int64_t>(n_seqs) * C > kMaxElems || T > INT32_MAX - PM_RECURRENCE_SPAN) return false;
+    if (static_cast<int64_t>(n_seqs) * C > kMaxElems || T > INT32_MAX - 1024) return false;
     const int64_t rows = packed ? C : static_cast<int64_t>(n_seqs) * C;
     if (T > 0 && rows > kMaxElems / T) return false;
     // (the counter that hands out tiles has 32 bits)

@@ -138,7 +138,7 @@ def linear_recurrence(x, g, state=None, *, out_dtype=None):
 
 def linear_recurrence_fwd(x, g, state=None, *, out_dtype=None):
     """Explicit forward of the VJP pair: ``((h, next_state), residual)`` for
-    ``linear_recurrence_bwd``. The residual keeps x, g and one state in every 256 tokens, not h."""
+    ``linear_recurrence_bwd``. The residual keeps x, g and one state in every 128 tokens, not h."""
     call, xd, gd, kept, h, s = _forward(x, g, state, out_dtype, keep=True)
     residual = _RecurrenceResidual(call.out(xd), call.out(gd), call.out(kept), h.dtype)
     return (call.out(h), call.out(s)), residual
