@@ -29,6 +29,7 @@ beside the delta rule: ``linear_recurrence`` (``recurrence.py``) and ``norm_rota
 
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass
 from typing import Any
 
@@ -136,22 +137,25 @@ class _Call:
     """Moves a call's arrays onto one GPU and remembers how to give results back."""
 
     def __init__(self, *xs):
-        tensors = [x for x in xs if isinstance(x, torch.Tensor)]
-        dev_tensors = [t for t in tensors if t.device.type == "cuda"]
+        device, tensors = None, False
+        for x in xs:
+            if isinstance(x, torch.Tensor):
+                tensors = True
+                if x.is_cuda:
+                    if device is None:
+                        device = x.device
+                    elif x.device != device:
+                        raise KernelError("all tensors must be on the same device")
         self.host_numpy = not tensors
-        self.host_torch = bool(tensors) and not dev_tensors
-        if dev_tensors:
-            self.device = dev_tensors[0].device
-            for t in dev_tensors:
-                if t.device != self.device:
-                    raise KernelError("all tensors must be on the same device")
-        else:
-            self.device = _device()
+        self.host_torch = tensors and device is None
+        self.device = _device() if device is None else device
 
     def dev(self, x, dtype=None):
         if x is None:
             return None
         if isinstance(x, torch.Tensor):
+            if x.is_cuda and x.device == self.device and (dtype is None or x.dtype == dtype) and x.is_contiguous():
+                return x
             t = x
         else:
             t = torch.from_numpy(np.ascontiguousarray(np.asarray(x, dtype=np.float32)))
@@ -175,6 +179,8 @@ def _qkv_dtype(q, k, v) -> torch.dtype:
 
 
 def _out_dtype(out_dtype) -> torch.dtype:
+    if out_dtype is torch.bfloat16:
+        return out_dtype
     if out_dtype is None or out_dtype in (torch.float32, np.float32, "fp32", "float32"):
         return torch.float32
     if out_dtype in (torch.bfloat16, "bf16", "bfloat16"):
@@ -194,8 +200,18 @@ def _aligned16(t):
     return t if t is None or t.numel() == 0 or t.data_ptr() % 16 == 0 else t.clone()
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """A context in which ``device`` is the current one (it mostly is)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # (torch.cuda.current_stream builds a Stream object around this number: 3 us, a quarter of a
+    # decode call)
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 # ---------------------------------------------------------------------------

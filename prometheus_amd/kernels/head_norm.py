@@ -10,6 +10,7 @@ and the weights have no reference counterpart.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Any
@@ -24,7 +25,12 @@ from prometheus_amd import kernels as _k
 __all__ = ["norm_rotate", "norm_rotate_fwd", "norm_rotate_bwd", "rotation_table"]
 
 _NORMS = {"l2": _native.NORM_L2, "rms": _native.NORM_RMS}
-_Strides = ctypes.c_int64 * 6
+
+
+@functools.lru_cache(maxsize=256)
+def _strides(*values):
+    """The host array of six strides that the kernels read (never written)."""
+    return (ctypes.c_int64 * 6)(*values)
 
 
 @dataclass(frozen=True)
@@ -99,8 +105,8 @@ def _check(q, k, table, positions, norm, q_weight, k_weight, eps) -> tuple:
 
 def _heads(call, x, dtype):
     """``x`` on the call's device in ``dtype``, the elements of a head contiguous."""
-    if isinstance(x, torch.Tensor) and x.device == call.device and x.dtype == dtype and (
-            x.shape[-1] <= 1 or x.stride(-1) == 1):
+    if isinstance(x, torch.Tensor) and x.dtype == dtype and x.device == call.device and (
+            x.stride(-1) == 1 or x.shape[-1] <= 1):
         return x
     return call.dev(x, dtype)
 
@@ -111,12 +117,9 @@ class _Plan:
     def __init__(self, q, k, table, positions, norm, q_weight, k_weight, eps, interleaved, *more):
         self.dims = _check(q, k, table, positions, norm, q_weight, k_weight, eps)
         self.call = call = _k._Call(q, k, table, positions, q_weight, k_weight, *more)
-        bf16 = all(isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16 for x in (q, k))
-        self.dtype = torch.bfloat16 if bf16 else torch.float32
-        ws = [w for w in (q_weight, k_weight) if w is not None]
-        w_bf16 = bool(ws) and all(isinstance(w, torch.Tensor) and w.dtype == torch.bfloat16 for w in ws)
-        w_dtype = torch.bfloat16 if w_bf16 else torch.float32
-        self.q, self.k = _heads(call, q, self.dtype), _heads(call, k, self.dtype)
+        self.dtype = dtype = _common_bf16(q, k)
+        w_dtype = _common_bf16(*(w for w in (q_weight, k_weight) if w is not None))
+        self.q, self.k = _heads(call, q, dtype), _heads(call, k, dtype)
         self.wq, self.wk = call.dev(q_weight, w_dtype), call.dev(k_weight, w_dtype)
         self.table = call.dev(table, torch.float32)
         self.pos, pos_sb, pos64 = None, 0, 0
@@ -124,31 +127,59 @@ class _Plan:
             p = positions if isinstance(positions, torch.Tensor) else torch.from_numpy(np.asarray(positions))
             if p.dtype not in (torch.int32, torch.int64):
                 p = p.to(torch.int64)
-            p = p.to(call.device)
+            if p.device != call.device:
+                p = p.to(call.device)
             if p.dim() == 2 and (p.shape[1] <= 1 or p.stride(1) == 1):
                 pos_sb = p.stride(0)
             else:
                 p = p.contiguous()
                 pos_sb = p.shape[1] if p.dim() == 2 else 0
             self.pos, pos64 = p, int(p.dtype == torch.int64)
-        strides = []
-        for x in (self.q, self.k):
-            st = x.stride()
-            strides += st[:3] if x.dim() == 4 else (0, st[0], st[1])
-        self.shared = (*self.dims, _Strides(*strides), pos_sb, pos64, _NORMS[norm], eps, int(interleaved),
-                       _k._code(self.dtype), _k._code(w_dtype))
-        self.inputs = tuple(_k._ptr(t) for t in (self.q, self.k, self.table, self.pos, self.wq, self.wk))
+        qs, ks = self.q.stride(), self.k.stride()
+        if len(qs) == 3:
+            qs, ks = (0, *qs), (0, *ks)
+        self.shared = (*self.dims, _strides(*qs[:3], *ks[:3]), pos_sb, pos64, _NORMS[norm], eps, int(interleaved),
+                       _k._code(dtype), _k._code(w_dtype))
+
+    def tensors(self):
+        return self.q, self.k, self.table, self.pos, self.wq, self.wk
+
+
+def _common_bf16(*xs) -> torch.dtype:
+    """bf16 if there are arrays and all are bf16 tensors, else fp32."""
+    for x in xs:
+        if not isinstance(x, torch.Tensor) or x.dtype != torch.bfloat16:
+            return torch.float32
+    return torch.bfloat16 if xs else torch.float32
 
 
 def _forward(q, k, table, positions, norm, q_weight, k_weight, eps, interleaved):
     # (the plan's shape checks come first; its _Call then finds the device)
     plan = _Plan(q, k, table, positions, norm, q_weight, k_weight, eps, interleaved)
-    dev = plan.call.device
-    with torch.cuda.device(dev):
-        qo = torch.empty(plan.q.shape, dtype=plan.dtype, device=dev)
-        ko = torch.empty(plan.k.shape, dtype=plan.dtype, device=dev)
-        _native.check(_native.lib().pm_norm_rotate(*plan.inputs, _k._ptr(qo), _k._ptr(ko), *plan.shared, _k._stream(dev)))
+    dev, ptr = plan.call.device, _k._ptr
+    with _k._on(dev):
+        qo = torch.empty_like(plan.q, memory_format=torch.contiguous_format)
+        ko = torch.empty_like(plan.k, memory_format=torch.contiguous_format)
+        _native.check(_native.lib().pm_norm_rotate(
+            ptr(plan.q), ptr(plan.k), ptr(plan.table), ptr(plan.pos), ptr(plan.wq), ptr(plan.wk), ptr(qo), ptr(ko),
+            *plan.shared, _k._stream(dev)))
     return plan, qo, ko
+
+
+def _launch_bwd(dev, tensors, shared, gqo, gko, want_weights):
+    """The backward on device tensors: ``(gq, gk, gq_weight, gk_weight)``."""
+    q, k, table, pos, wq, wk = tensors
+    L, ptr, f32 = _native.lib(), _k._ptr, torch.float32
+    gq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    gk = torch.empty_like(k, memory_format=torch.contiguous_format)
+    gwq, gwk = (torch.empty(w.shape, dtype=f32, device=dev) if w is not None and want else None
+                for w, want in zip((wq, wk), want_weights))
+    nbytes = L.pm_norm_rotate_bwd_workspace_bytes(*shared[:5]) if gwq is not None or gwk is not None else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _native.check(L.pm_norm_rotate_bwd(
+        ptr(q), ptr(k), ptr(table), ptr(pos), ptr(wq), ptr(wk), ptr(gqo), ptr(gko), ptr(gq), ptr(gk), ptr(gwq),
+        ptr(gwk), *shared, ptr(ws), nbytes, _k._stream(dev)))
+    return gq, gk, gwq, gwk
 
 
 class _NormRotate(torch.autograd.Function):
@@ -157,20 +188,31 @@ class _NormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, table, positions, norm, eps, interleaved):
         plan, qo, ko = _forward(q, k, table, positions, norm, q_weight, k_weight, eps, interleaved)
-        ctx.save_for_backward(plan.q, plan.k, plan.wq, plan.wk, plan.table, plan.pos)
+        tensors = plan.tensors()
+        ctx.save_for_backward(*tensors)
         ctx.options = norm, eps, interleaved
+        ctx.shared, ctx.strides = plan.shared, [None if t is None else t.stride() for t in tensors]
         ctx.set_materialize_grads(False)  # a missing gradient is None, not a tensor of zeros
-        ctx.like = [(t.dtype, t.device) if isinstance(t, torch.Tensor) else None for t in (q, k, q_weight, k_weight)]
+        # (the type and device of each input's gradient; None: as the backward gives it)
+        ctx.like = [(t.dtype, t.device) if isinstance(t, torch.Tensor) and t is not u else None
+                    for t, u in ((q, plan.q), (k, plan.k))]
+        ctx.like += [(t.dtype, t.device) if isinstance(t, torch.Tensor) and (t is not u or t.dtype != torch.float32)
+                     else None for t, u in ((q_weight, plan.wq), (k_weight, plan.wk))]
         return plan.call.out(qo), plan.call.out(ko)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, wq, wk, table, pos = ctx.saved_tensors
-        res = _NormRotateResidual(q, k, table, pos, wq, wk, *ctx.options)
-        need = ctx.needs_input_grad
-        grads = _backward(res, (gq, gk), (need[2], need[3]))
-        return (*(None if t is None or like is None or not n else t.to(device=like[1], dtype=like[0])
+        tensors, need = ctx.saved_tensors, ctx.needs_input_grad
+        want = (need[2], need[3])
+        if [None if t is None else t.stride() for t in tensors] == ctx.strides:
+            call = _k._Call(tensors[0])
+            with _k._on(call.device):
+                grads = _launch_bwd(call.device, tensors, ctx.shared, call.dev(gq), call.dev(gk), want)
+        else:  # (saved-tensor hooks may hand back another layout)
+            q, k, table, pos, wq, wk = tensors
+            grads = _backward(_NormRotateResidual(q, k, table, pos, wq, wk, *ctx.options), (gq, gk), want)
+        return (*((t if like is None else t.to(device=like[1], dtype=like[0])) if n and t is not None else None
                   for t, like, n in zip(grads, ctx.like, need)), None, None, None, None, None)
 
 
@@ -193,7 +235,6 @@ def norm_rotate(q, k, table=None, positions=None, *, norm="l2", q_weight=None, k
     the end. Differentiable in q, k and the weights.
     """
     if _k._wants_grad(q, k, q_weight, k_weight):
-        _check(q, k, table, positions, norm, q_weight, k_weight, eps)
         return _NormRotate.apply(q, k, q_weight, k_weight, table, positions, norm, eps, interleaved)
     plan, qo, ko = _forward(q, k, table, positions, norm, q_weight, k_weight, eps, interleaved)
     return plan.call.out(qo), plan.call.out(ko)
@@ -221,17 +262,8 @@ def _backward(res, grads, want_weights):
             raise _k.KernelError(f"grad of {name} shape {_k._shape(gx)} != {_k._shape(x)}")
     plan = _Plan(res.q, res.k, res.table, res.positions, res.norm, res.q_weight, res.k_weight, res.eps,
                  res.interleaved, *grads)
-    dev, call = plan.call.device, plan.call
-    L = _native.lib()
-    with torch.cuda.device(dev):
+    call = plan.call
+    with _k._on(call.device):
         gqo, gko = (call.dev(x, plan.dtype) for x in grads)
-        gq = torch.empty(plan.q.shape, dtype=plan.dtype, device=dev)
-        gk = torch.empty(plan.k.shape, dtype=plan.dtype, device=dev)
-        gwq, gwk = (torch.empty(w.shape, dtype=torch.float32, device=dev) if w is not None and want else None
-                    for w, want in zip((plan.wq, plan.wk), want_weights))
-        nbytes = L.pm_norm_rotate_bwd_workspace_bytes(*plan.dims[:5]) if gwq is not None or gwk is not None else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _native.check(L.pm_norm_rotate_bwd(
-            *plan.inputs, _k._ptr(gqo), _k._ptr(gko), _k._ptr(gq), _k._ptr(gk), _k._ptr(gwq), _k._ptr(gwk),
-            *plan.shared, _k._ptr(ws), nbytes, _k._stream(dev)))
-    return tuple(None if t is None else call.out(t) for t in (gq, gk, gwq, gwk))
+        out = _launch_bwd(call.device, plan.tensors(), plan.shared, gqo, gko, want_weights)
+    return tuple(None if t is None else call.out(t) for t in out)

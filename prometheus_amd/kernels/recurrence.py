@@ -53,8 +53,8 @@ def _types(x, g) -> tuple[torch.dtype, torch.dtype]:
 def _rows(call, x, dtype):
     """``x`` on the call's device in ``dtype``, its last dimension contiguous (no copy of a view
     that has it so)."""
-    if isinstance(x, torch.Tensor) and x.device == call.device and x.dtype == dtype and (
-            x.shape[-1] <= 1 or x.stride(-1) == 1):
+    if isinstance(x, torch.Tensor) and x.dtype == dtype and x.device == call.device and (
+            x.stride(-1) == 1 or x.shape[-1] <= 1):
         return x
     return call.dev(x, dtype)
 
@@ -74,7 +74,7 @@ def _launch(call, xd, gd, cu, s0, slots, n_slots, bad, s_out, n_seqs, T, C, out_
     """The forward on device tensors: ``(h, kept)``; ``s_out`` is written. xd and gd are
     (n_seqs, T, C), or packed (1, T, C) with ``cu``."""
     L = _native.lib()
-    h = torch.empty(xd.shape, dtype=out_dtype, device=call.device)
+    h = torch.empty_like(xd, dtype=out_dtype, memory_format=torch.contiguous_format)
     spans = -(-T // _native.RECURRENCE_SPAN)
     kept = torch.empty((n_seqs, spans, C), dtype=torch.float32, device=call.device) if keep else None
     xc, gc = _k._code(xd.dtype), _k._code(gd.dtype)
@@ -92,11 +92,29 @@ def _forward(x, g, state, out_dtype, keep=False):
     odt = _k._out_dtype(out_dtype)
     call = _k._Call(x, g, state)
     xt, gt = _types(x, g)
-    with torch.cuda.device(call.device):
+    with _k._on(call.device):
         xd, gd, sd = _rows(call, x, xt), _rows(call, g, gt), call.dev(state, torch.float32)
         s_out = torch.empty((batch, chan), dtype=torch.float32, device=call.device)
         h, kept = _launch(call, xd, gd, None, sd, None, 0, None, s_out, batch, seq, chan, odt, keep)
     return call, xd, gd, kept, h, s_out
+
+
+def _launch_bwd(call, xd, gd, kept, gh, gs, h_dtype):
+    """The backward on device tensors: ``(gx, gg, gs0)``."""
+    batch, seq, chan = xd.shape
+    L = _native.lib()
+    gx = torch.empty_like(xd, memory_format=torch.contiguous_format)
+    gg = torch.empty_like(gd, memory_format=torch.contiguous_format)
+    gs0 = torch.empty((batch, chan), dtype=torch.float32, device=call.device)
+    xc, gc = _k._code(xd.dtype), _k._code(gd.dtype)
+    nbytes = L.pm_linear_recurrence_workspace_bytes(batch, seq, chan, 0, xc)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=call.device) if nbytes else None
+    xs, gst = xd.stride(), gd.stride()
+    _native.check(L.pm_linear_recurrence_bwd(
+        _k._ptr(xd), _k._ptr(gd), _k._ptr(kept), _k._ptr(gh), _k._ptr(gs), _k._ptr(gx), _k._ptr(gg), _k._ptr(gs0),
+        batch, seq, chan, xs[0], xs[1], gst[0], gst[1], xc, gc, _k._code(h_dtype), _k._ptr(ws), nbytes,
+        _k._stream(call.device)))
+    return gx, gg, gs0
 
 
 class _LinearRecurrence(torch.autograd.Function):
@@ -108,16 +126,27 @@ class _LinearRecurrence(torch.autograd.Function):
         ctx.save_for_backward(xd, gd, kept)
         ctx.h_dtype = h.dtype
         ctx.set_materialize_grads(False)  # a missing gradient is None, not a tensor of zeros
-        ctx.like = [(t.dtype, t.device) if isinstance(t, torch.Tensor) else None for t in (x, g, state)]
+        # (the type and device of each input's gradient; None: as the backward gives it)
+        ctx.like = [(t.dtype, t.device) if isinstance(t, torch.Tensor) and u is not t else None
+                    for t, u in ((x, xd), (g, gd))]
+        if isinstance(state, torch.Tensor) and (state.dtype != torch.float32 or state.device != call.device):
+            ctx.like.append((state.dtype, state.device))
+        else:
+            ctx.like.append(None)
         return call.out(h), call.out(s)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gh, gs):
         xd, gd, kept = ctx.saved_tensors
-        grads = linear_recurrence_bwd(_RecurrenceResidual(xd, gd, kept, ctx.h_dtype), (gh, gs))
-        return (*(None if like is None or not need else t.to(device=like[1], dtype=like[0])
-                  for t, like, need in zip(grads, ctx.like, ctx.needs_input_grad)), None)
+        # (saved-tensor hooks may hand back another layout, but the same shapes)
+        call = _k._Call(xd)
+        with _k._on(call.device):
+            grads = _launch_bwd(call, _rows(call, xd, xd.dtype), _rows(call, gd, gd.dtype), call.dev(kept),
+                                call.dev(gh), call.dev(gs), ctx.h_dtype)
+        need = ctx.needs_input_grad
+        return (*((t if like is None else t.to(device=like[1], dtype=like[0])) if n else None
+                  for t, like, n in zip(grads, ctx.like, need)), None)
 
 
 def linear_recurrence(x, g, state=None, *, out_dtype=None):
@@ -130,7 +159,6 @@ def linear_recurrence(x, g, state=None, *, out_dtype=None):
     and a torch input requires grad, the backward is ``linear_recurrence_bwd``.
     """
     if _k._wants_grad(x, g, state):
-        _check(x, g, state, 3)
         return _LinearRecurrence.apply(x, g, state, out_dtype)
     call, _, _, _, h, s = _forward(x, g, state, out_dtype)
     return call.out(h), call.out(s)
@@ -161,21 +189,10 @@ def linear_recurrence_bwd(residual: _RecurrenceResidual, grads):
         raise _k.KernelError(f"grad of state shape {_k._shape(gs)} != {(batch, chan)}")
     call = _k._Call(x, g, kept, gh, gs)
     xt, gt = _types(x, g)
-    L = _native.lib()
-    with torch.cuda.device(call.device):
-        xd, gd = _rows(call, x, xt), _rows(call, g, gt)
-        kd, gsd = call.dev(kept, torch.float32), call.dev(gs, torch.float32)
-        ghd = call.dev(gh, residual.h_dtype)
-        gx = torch.empty(xd.shape, dtype=xt, device=call.device)
-        gg = torch.empty(xd.shape, dtype=gt, device=call.device)
-        gs0 = torch.empty((batch, chan), dtype=torch.float32, device=call.device)
-        nbytes = L.pm_linear_recurrence_workspace_bytes(batch, seq, chan, 0, _k._code(xt))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=call.device) if nbytes else None
-        _native.check(L.pm_linear_recurrence_bwd(
-            _k._ptr(xd), _k._ptr(gd), _k._ptr(kd), _k._ptr(ghd), _k._ptr(gsd), _k._ptr(gx), _k._ptr(gg),
-            _k._ptr(gs0), batch, seq, chan, xd.stride(0), xd.stride(1), gd.stride(0), gd.stride(1),
-            _k._code(xt), _k._code(gt), _k._code(residual.h_dtype), _k._ptr(ws), nbytes, _k._stream(call.device)))
-    return call.out(gx), call.out(gg), call.out(gs0)
+    with _k._on(call.device):
+        grads = _launch_bwd(call, _rows(call, x, xt), _rows(call, g, gt), call.dev(kept, torch.float32),
+                            call.dev(gh, residual.h_dtype), call.dev(gs, torch.float32), residual.h_dtype)
+    return tuple(call.out(t) for t in grads)
 
 
 def _packed(x, g, cu_seqlens):
@@ -227,7 +244,7 @@ def linear_recurrence_varlen(x, g, cu_seqlens, state=None, *, out_dtype=None):
     odt = _k._out_dtype(out_dtype)
     call = _k._Call(x, g, state, cu_seqlens)
     xt, gt = _types(x, g)
-    with torch.cuda.device(call.device):
+    with _k._on(call.device):
         xd, gd = (t if t.dim() == 3 else t[None] for t in (_rows(call, x, xt), _rows(call, g, gt)))
         sd = call.dev(state, torch.float32)
         s_out = torch.empty((n_seqs, chan), dtype=torch.float32, device=call.device)
@@ -251,11 +268,11 @@ def linear_recurrence_step(x, g, state, *, out_dtype=None):
     odt = _k._out_dtype(out_dtype)
     call = _k._Call(x, g, state)
     xt, gt = _types(x, g)
-    with torch.cuda.device(call.device):
+    with _k._on(call.device):
         xd, gd = _rows(call, x, xt), _rows(call, g, gt)
         sd = state if in_place else call.dev(state, torch.float32)
         h = torch.empty((batch, chan), dtype=odt, device=call.device)
-        _step(sd, None, 0, xd, gd, h, _k._stream(call.device))
+        _step(_k._ptr(sd), None, 0, xd, gd, h, _k._stream(call.device))
         if not in_place:
             host = sd.cpu()
             if isinstance(state, np.ndarray):
@@ -265,8 +282,9 @@ def linear_recurrence_step(x, g, state, *, out_dtype=None):
     return call.out(h)
 
 
-def _step(state, slots, n_slots, xd, gd, h, stream):
+def _step(state: int | None, slots, n_slots, xd, gd, h, stream):
+    """One token on device tensors; ``state`` is the states' address."""
     batch, chan = xd.shape
     _native.check(_native.lib().pm_linear_recurrence_step(
-        _k._ptr(state), _k._ptr(slots), n_slots, _k._ptr(xd), _k._ptr(gd), _k._ptr(h), batch, chan, xd.stride(0),
-        gd.stride(0), _k._code(xd.dtype), _k._code(gd.dtype), _k._code(h.dtype), stream))
+        state, _k._ptr(slots), n_slots, _k._ptr(xd), _k._ptr(gd), _k._ptr(h), batch, chan, xd.stride(0), gd.stride(0),
+        _k._code(xd.dtype), _k._code(gd.dtype), _k._code(h.dtype), stream))

@@ -135,8 +135,9 @@ class _SlotPool:
     def _check_cuda(self, *xs) -> None:
         if self.pool.device.type != "cuda":
             raise RuntimeError("the state cache computes on a HIP GPU; this pool is on the host")
+        device = self.pool.device
         for x in xs:
-            if not (isinstance(x, torch.Tensor) and x.device == self.pool.device):
+            if not (isinstance(x, torch.Tensor) and x.device == device):
                 raise ValueError("inputs must be tensors on the pool's device")
 
 
@@ -278,10 +279,10 @@ class RecurrenceStateCache(_SlotPool):
         if want[1] > 1 and (x.stride(1) != 1 or g.stride(1) != 1):
             raise ValueError("x and g must have contiguous channels")
         if out is None:
-            out = torch.empty(want, dtype=kernels._out_dtype(out_dtype), device=x.device)
+            out = torch.empty_like(x, dtype=kernels._out_dtype(out_dtype), memory_format=torch.contiguous_format)
         elif (tuple(out.shape) != want or out.dtype not in (torch.float32, torch.bfloat16)
               or not out.is_contiguous() or out.device != x.device):
             raise ValueError(f"out must be contiguous fp32 or bf16 {want} on the pool's device")
-        recurrence._step(self._pool[layer], slots, self.n_slots, x, g, out,
-                         torch.cuda.current_stream(x.device).cuda_stream)
+        recurrence._step(self._pool.data_ptr() + layer * self._pool.stride(0) * 4, slots, self.n_slots, x, g, out,
+                         kernels._stream(x.device))
         return out
