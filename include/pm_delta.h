@@ -466,6 +466,14 @@ int pm_linear_recurrence(const void* x, const void* g, const int32_t* cu_seqlens
                          float* kept, int n_seqs, int T, int C, int64_t x_sb, int64_t x_st, int64_t g_sb,
                          int64_t g_st, int x_dtype, int g_dtype, int h_dtype, void* workspace,
                          size_t ws_bytes, void* stream);
+/* The same with the check of the offsets on the way: where cu_seqlens is given
+ * and n_seqs and C are not 0, pm_varlen_check's bits are ORed into *cu_flag
+ * (device int32, may be NULL) without a launch of its own. */
+int pm_linear_recurrence_varlen(const void* x, const void* g, const int32_t* cu_seqlens, const float* s0,
+                                const int32_t* slots, int n_slots, int32_t* bad_slot, int32_t* cu_flag,
+                                void* h, float* s_out, float* kept, int n_seqs, int T, int C, int64_t x_sb,
+                                int64_t x_st, int64_t g_sb, int64_t g_st, int x_dtype, int g_dtype,
+                                int h_dtype, void* workspace, size_t ws_bytes, void* stream);
 /* Workspace bytes of pm_linear_recurrence (packed: whether cu_seqlens is given)
  * and, with packed 0 and n_seqs = B, of pm_linear_recurrence_bwd. */
 size_t pm_linear_recurrence_workspace_bytes(int n_seqs, int T, int C, int packed, int x_dtype);
@@ -476,7 +484,7 @@ size_t pm_linear_recurrence_workspace_bytes(int n_seqs, int T, int C, int packed
  *     d_t = gh_t + exp(g_{t+1}) d_{t+1},  gx_t = d_t,  gg_t = d_t exp(g_t) h_{t-1}
  * gx and gg are contiguous, in x's and g's type; gs0 (B, C) fp32.  h is
  * recomputed in fp32 from x and `kept`, so that gg does not depend on h's
- * rounding.  Every output is written in full.
+ * rounding.  Every output is written in full; none may overlap an input.
  */
 int pm_linear_recurrence_bwd(const void* x, const void* g, const float* kept, const void* gh,
                              const float* gs, void* gx, void* gg, float* gs0, int B, int T, int C,

@@ -65,6 +65,7 @@ EXPORTS = (
     "pm_kda_delta_bwd",
     "pm_kda_delta_bwd_workspace_bytes",
     "pm_linear_recurrence",
+    "pm_linear_recurrence_varlen",
     "pm_linear_recurrence_workspace_bytes",
     "pm_linear_recurrence_bwd",
     "pm_linear_recurrence_step",
@@ -166,6 +167,9 @@ def lib() -> ctypes.CDLL:
         i64, f = ctypes.c_int64, ctypes.c_float
         L.pm_linear_recurrence.argtypes = [vp] * 5 + [i] + [vp] * 4 + [i] * 3 + [i64] * 4 + [i] * 3 + [vp, sz, vp]
         L.pm_linear_recurrence.restype = i
+        L.pm_linear_recurrence_varlen.argtypes = ([vp] * 5 + [i] + [vp] * 5 + [i] * 3 + [i64] * 4 + [i] * 3
+                                                  + [vp, sz, vp])
+        L.pm_linear_recurrence_varlen.restype = i
         L.pm_linear_recurrence_workspace_bytes.argtypes = [i] * 5
         L.pm_linear_recurrence_workspace_bytes.restype = sz
         L.pm_linear_recurrence_bwd.argtypes = [vp] * 8 + [i] * 3 + [i64] * 4 + [i] * 3 + [vp, sz, vp]

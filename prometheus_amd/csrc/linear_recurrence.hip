@@ -514,14 +514,22 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
     }
 }
 
-// Before a call: `n` words of the workspace to all ones and the counter to zero; and the states
-// of sequences without tokens (all of them where T is 0), which pass through.
+// Before a call: `n` words of the workspace to all ones and the counter to zero; the check of a
+// packed call's offsets; and the states of sequences without tokens (all of them where T is 0),
+// which pass through.
 __global__ __launch_bounds__(256) void recurrence_begin_kernel(uint32_t* next, uint64_t* words, int64_t n,
                                                                RecurrenceArgs a) {
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
     if (next && at == 0) *next = 0;
     for (int64_t i = at; i < n; i += step) words[i] = ~uint64_t(0);
     for (int seq = blockIdx.x; seq < a.n_seqs; seq += gridDim.x) {
+        if (a.cu_seqlens && a.cu_flag && threadIdx.x == 0) {
+            const int b = a.cu_seqlens[seq], e = a.cu_seqlens[seq + 1];
+            const bool last = seq == a.n_seqs - 1;
+            const int bits = (seq == 0 && b != 0 ? 1 : 0) | (last && e != a.T ? 2 : 0) | (e < b ? 4 : 0) |
+                             (b < 0 || b > a.T || (last && (e < 0 || e > a.T)) ? 8 : 0);
+            if (bits) atomicOr(a.cu_flag, bits);
+        }
         if (a.T > 0) {
             if (!a.cu_seqlens) break;
             const int b = min(max(a.cu_seqlens[seq], 0), a.T), e = min(max(a.cu_seqlens[seq + 1], b), a.T);

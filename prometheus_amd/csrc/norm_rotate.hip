@@ -12,8 +12,13 @@
 // holds both members of its pairs: V elements (16 bytes) at i and V at i + R / 2 (neighbouring
 // pairs: 2 V in a row), so that the turn needs no other lane; the elements behind R are halved
 // the same way. L lanes, the next power of two, hold a head; sums over a head go through L lanes
-// by DPP. A group of L lanes takes NH heads of one token, whose angles and weights it reads once.
-// Any D up to 256, any strides and alignment.
+// by DPP. A group of L lanes takes NH heads of one token, whose angles it reads once (and, in a
+// backward with weights, as many tokens as 1024 workgroups leave it). Any D up to 256, any strides
+// and alignment.
+//
+// Measured at D = 128, bf16, on a card that copies at 5.0 TB/s: 16384 tokens of 16 + 16 heads
+// forward 49 us (5.5 TB/s; one wave to a head, element by element, 361), backward 80 (5.0 TB/s,
+// the weights' gradients among it).
 
 #include <type_traits>
 
@@ -24,7 +29,7 @@ namespace pm {
 
 constexpr int kRowMax = 256;  // largest D
 constexpr int kBlock = 256;
-constexpr int kHeads = 4;          // heads of a token to a group of lanes (few rows: 1)
+constexpr int kHeads = 2;          // heads of a token to a group of lanes (few rows: 1)
 constexpr int kBwdBlocks = 1024;   // workgroups of a backward that sums weights' gradients
 
 // Sum over groups of L lanes, every lane of a group with the same bits.
@@ -75,20 +80,21 @@ static int lanes_of(int D, int R, int V, bool contig) {
     return l;
 }
 
-// Item i of a side: head chunk i % chunks of token i / chunks.
+// Item i of a side: heads i % chunks + {0, chunks, 2 chunks, ..} of token i / chunks, so that
+// neighbouring groups of lanes read neighbouring heads.
 struct Item {
     int b, t, h;
 };
-__device__ __forceinline__ Item item_of(const NormRotateArgs& a, int64_t i, int64_t items, int chunks, int nh) {
+__device__ __forceinline__ Item item_of(const NormRotateArgs& a, int64_t i, int64_t items, int chunks) {
     Item w;
     if (items < (int64_t(1) << 32)) {  // (uniform: 32-bit divisions are a few instructions)
         const uint32_t u = static_cast<uint32_t>(i), tok = u / static_cast<uint32_t>(chunks);
-        w.h = static_cast<int>(u - tok * chunks) * nh;
+        w.h = static_cast<int>(u - tok * chunks);
         w.b = static_cast<int>(tok / static_cast<uint32_t>(a.T));
         w.t = static_cast<int>(tok - static_cast<uint32_t>(w.b) * a.T);
     } else {
         const int64_t tok = i / chunks;
-        w.h = static_cast<int>(i - tok * chunks) * nh;
+        w.h = static_cast<int>(i - tok * chunks);
         w.b = static_cast<int>(tok / a.T);
         w.t = static_cast<int>(tok - static_cast<int64_t>(w.b) * a.T);
     }
@@ -173,14 +179,14 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_kernel(NormRotateArgs a, i
 
     for (int64_t i = static_cast<int64_t>(blockIdx.x - (k ? q_blocks : 0)) * GROUPS + threadIdx.x / L; i < items;
          i += step) {
-        const Item at = item_of(a, i, items, chunks, NH);
+        const Item at = item_of(a, i, items, chunks);
         const E* x = static_cast<const E*>(a.x[k]) + at.b * a.sb[k] + at.t * a.st[k] + at.h * a.sh[k];
         Row<E, V> xa[NH], xb[NH];
 #pragma unroll
         for (int j = 0; j < NH; ++j) {
-            const bool there = at.h + j < H;
-            xa[j].load(x + j * a.sh[k] + w.a, there ? w.na : 0);
-            xb[j].load(x + j * a.sh[k] + w.b, there ? w.nb : 0);
+            const bool there = at.h + j * chunks < H;
+            xa[j].load(x + j * chunks * a.sh[k] + w.a, there ? w.na : 0);
+            xb[j].load(x + j * chunks * a.sh[k] + w.b, there ? w.nb : 0);
         }
         float c[V], s[V];
         const bool known = !a.table || load_angles<V>(a, w, at.b, at.t, c, s);
@@ -200,9 +206,9 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_kernel(NormRotateArgs a, i
                 for (int e = 0; e < V; ++e) ya[e] *= wa[e], yb[e] *= wb[e];
             }
             if (a.table) turn<V, CONTIG>(c, s, 1.f, ya, yb);
-            if (at.h + j < H) {
-                store_row<E, V>(y + j * a.D + w.a, ya, w.na);
-                store_row<E, V>(y + j * a.D + w.b, yb, w.nb);
+            if (at.h + j * chunks < H) {
+                store_row<E, V>(y + j * chunks * a.D + w.a, ya, w.na);
+                store_row<E, V>(y + j * chunks * a.D + w.b, yb, w.nb);
             }
         }
     }
@@ -226,18 +232,18 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_bwd_kernel(NormRotateArgs 
 
     for (int64_t i = static_cast<int64_t>(blockIdx.x - (k ? q_blocks : 0)) * GROUPS + threadIdx.x / L; i < items;
          i += step) {
-        const Item at = item_of(a, i, items, chunks, NH);
+        const Item at = item_of(a, i, items, chunks);
         const E* x = static_cast<const E*>(a.x[k]) + at.b * a.sb[k] + at.t * a.st[k] + at.h * a.sh[k];
         const int64_t out = ((static_cast<int64_t>(at.b) * a.T + at.t) * H + at.h) * a.D;
         const E* gz = static_cast<const E*>(a.gy[k]) + out;
         Row<E, V> xa[NH], xb[NH], za[NH], zb[NH];
 #pragma unroll
         for (int j = 0; j < NH; ++j) {
-            const bool there = at.h + j < H, any = there && a.gy[k];
-            xa[j].load(x + j * a.sh[k] + w.a, there ? w.na : 0);
-            xb[j].load(x + j * a.sh[k] + w.b, there ? w.nb : 0);
-            za[j].load(gz + j * a.D + w.a, any ? w.na : 0);
-            zb[j].load(gz + j * a.D + w.b, any ? w.nb : 0);
+            const bool there = at.h + j * chunks < H, any = there && a.gy[k];
+            xa[j].load(x + j * chunks * a.sh[k] + w.a, there ? w.na : 0);
+            xb[j].load(x + j * chunks * a.sh[k] + w.b, there ? w.nb : 0);
+            za[j].load(gz + j * chunks * a.D + w.a, any ? w.na : 0);
+            zb[j].load(gz + j * chunks * a.D + w.b, any ? w.nb : 0);
         }
         float c[V], s[V];
         const bool known = !a.table || load_angles<V>(a, w, at.b, at.t, c, s);
@@ -255,7 +261,7 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_bwd_kernel(NormRotateArgs 
             float scale = row_scale(a, group_sum<L>(ss), clipped);
             if (!known) scale = nan;
             if (a.weight[k]) {
-                if (at.h + j < H) {
+                if (at.h + j * chunks < H) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
                         ga[e] = fmaf(ya[e], xa[j][e] * scale, ga[e]);
@@ -276,9 +282,9 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_bwd_kernel(NormRotateArgs 
                 ya[e] = fmaf(xa[j][e] * scale, -dot, ya[e]) * scale;
                 yb[e] = fmaf(xb[j][e] * scale, -dot, yb[e]) * scale;
             }
-            if (at.h + j < H) {
-                store_row<E, V>(gx + j * a.D + w.a, ya, w.na);
-                store_row<E, V>(gx + j * a.D + w.b, yb, w.nb);
+            if (at.h + j * chunks < H) {
+                store_row<E, V>(gx + j * chunks * a.D + w.a, ya, w.na);
+                store_row<E, V>(gx + j * chunks * a.D + w.b, yb, w.nb);
             }
         }
     }
@@ -342,12 +348,17 @@ static void by_shape(const NormRotateArgs& a, int nh, F f) {
     }
 }
 
-// Heads to a group of lanes: 4 share a token's angles and keep 4 rows' loads in flight, as long as
-// there are enough groups to fill the card and most of the fours are whole.
+// Heads to a group of lanes. Two share a token's angles and keep two rows' loads under way, as long
+// as there are groups enough to fill the card, the twos are mostly whole, and a head is not so
+// small that it is one or two lanes. Measured one to two (us, bf16): 16384 tokens of 16 + 16 heads
+// of 128 forward 57 to 49, backward without weights 85 to 73, with them 83 to 80; 512 tokens of 32
+// + 32 backward 12.9 to 11.9; but 256 of 32 + 32 forward 4.5 to 4.9, 16384 of 3 + 3 backward 20.6
+// to 22.2, of 16 + 16 of 32 forward 17.4 to 20.9. Four: 51.5 and 76 of the first.
 static int heads_of(const NormRotateArgs& a, int lanes) {
     const int64_t tokens = static_cast<int64_t>(a.B) * a.T;
-    const int fours = (a.H[0] + kHeads - 1) / kHeads + (a.H[1] + kHeads - 1) / kHeads;
-    return tokens * fours * lanes >= 256 * 512 && 5 * (a.H[0] + a.H[1]) >= 3 * kHeads * fours ? kHeads : 1;
+    const int twos = (a.H[0] + kHeads - 1) / kHeads + (a.H[1] + kHeads - 1) / kHeads;
+    const bool fill = tokens * twos * lanes >= 256 * 512, whole = 5 * (a.H[0] + a.H[1]) >= 4 * kHeads * twos;
+    return fill && whole && lanes > 2 ? kHeads : 1;
 }
 
 // Workgroups of a side, at most `most`.

@@ -277,6 +277,7 @@ struct RecurrenceArgs {
     int64_t x_sb, x_st, g_sb, g_st;
     bool x_bf16, g_bf16, h_bf16;
     void* workspace;
+    int32_t* cu_flag;  // nullable: gets launch_varlen_check's bits, where cu_seqlens is given
 };
 hipError_t launch_recurrence(const RecurrenceArgs& a, hipStream_t st);
 // Bytes of its workspace and of its backward's (0: none), and the number of its tiles.

@@ -62,10 +62,11 @@ size_t pm_linear_recurrence_workspace_bytes(int n_seqs, int T, int C, int packed
     return pm::recurrence_ws_bytes(n_seqs, T, C, packed != 0, x_dtype == PM_DTYPE_BF16);
 }
 
-int pm_linear_recurrence(const void* x, const void* g, const int32_t* cu_seqlens, const float* s0,
-                         const int32_t* slots, int n_slots, int32_t* bad_slot, void* h, float* s_out, float* kept,
-                         int n_seqs, int T, int C, int64_t x_sb, int64_t x_st, int64_t g_sb, int64_t g_st,
-                         int x_dtype, int g_dtype, int h_dtype, void* workspace, size_t ws_bytes, void* stream) {
+int pm_linear_recurrence_varlen(const void* x, const void* g, const int32_t* cu_seqlens, const float* s0,
+                                const int32_t* slots, int n_slots, int32_t* bad_slot, int32_t* cu_flag, void* h,
+                                float* s_out, float* kept, int n_seqs, int T, int C, int64_t x_sb, int64_t x_st,
+                                int64_t g_sb, int64_t g_st, int x_dtype, int g_dtype, int h_dtype, void* workspace,
+                                size_t ws_bytes, void* stream) {
     pm::clear_error();
     if (int rc = check_types(x_dtype, g_dtype, h_dtype)) return rc;
     if (int rc = check_sizes(n_seqs, T, C, cu_seqlens != nullptr, x_dtype)) return rc;
@@ -81,7 +82,7 @@ int pm_linear_recurrence(const void* x, const void* g, const int32_t* cu_seqlens
     if (kept && cu_seqlens) return fail(PM_E_UNSUPPORTED, "states are kept for fixed-length batches only");
     if (!aligned(x, size_of(x_dtype)) || !aligned(g, size_of(g_dtype)) || !aligned(h, size_of(h_dtype)) ||
         !aligned(s0, 4) || !aligned(s_out, 4) || !aligned(kept, 4) || !aligned(cu_seqlens, 4) || !aligned(slots, 4) ||
-        !aligned(bad_slot, 4))
+        !aligned(bad_slot, 4) || !aligned(cu_flag, 4))
         return fail(PM_E_ALIGN, "every buffer must be aligned to its element size");
     const size_t need = pm_linear_recurrence_workspace_bytes(n_seqs, T, C, cu_seqlens != nullptr, x_dtype);
     if (need && (!workspace || ws_bytes < need || !aligned(workspace, 16)))
@@ -89,9 +90,18 @@ int pm_linear_recurrence(const void* x, const void* g, const int32_t* cu_seqlens
                     workspace ? ws_bytes : static_cast<size_t>(0));
     pm::RecurrenceArgs a{x, g, cu_seqlens, s0, slots, n_slots, bad_slot, h, s_out, kept, n_seqs, T, C, x_sb, x_st,
                          g_sb, g_st, x_dtype == PM_DTYPE_BF16, g_dtype == PM_DTYPE_BF16, h_dtype == PM_DTYPE_BF16,
-                         workspace};
+                         workspace, cu_flag};
     hipError_t e = pm::launch_recurrence(a, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? 0 : hip_fail(e, "linear recurrence launch");
+}
+
+int pm_linear_recurrence(const void* x, const void* g, const int32_t* cu_seqlens, const float* s0,
+                         const int32_t* slots, int n_slots, int32_t* bad_slot, void* h, float* s_out, float* kept,
+                         int n_seqs, int T, int C, int64_t x_sb, int64_t x_st, int64_t g_sb, int64_t g_st,
+                         int x_dtype, int g_dtype, int h_dtype, void* workspace, size_t ws_bytes, void* stream) {
+    return pm_linear_recurrence_varlen(x, g, cu_seqlens, s0, slots, n_slots, bad_slot, nullptr, h, s_out, kept, n_seqs,
+                                       T, C, x_sb, x_st, g_sb, g_st, x_dtype, g_dtype, h_dtype, workspace, ws_bytes,
+                                       stream);
 }
 
 int pm_linear_recurrence_bwd(const void* x, const void* g, const float* kept, const void* gh, const float* gs,

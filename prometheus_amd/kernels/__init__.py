@@ -193,7 +193,7 @@ def _code(dt: torch.dtype) -> int:
 
 
 def _ptr(t) -> int | None:
-    return None if t is None or t.numel() == 0 else t.data_ptr()
+    return None if t is None else t.data_ptr()  # (0, a null pointer, for an empty tensor)
 
 
 def _aligned16(t):

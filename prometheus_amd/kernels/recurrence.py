@@ -70,9 +70,9 @@ def _check(x, g, state, rank) -> tuple:
     return xs
 
 
-def _launch(call, xd, gd, cu, s0, slots, n_slots, bad, s_out, n_seqs, T, C, out_dtype, keep):
+def _launch(call, xd, gd, cu, s0, slots, n_slots, bad, s_out, n_seqs, T, C, out_dtype, keep, cu_flag=None):
     """The forward on device tensors: ``(h, kept)``; ``s_out`` is written. xd and gd are
-    (n_seqs, T, C), or packed (1, T, C) with ``cu``."""
+    (n_seqs, T, C), or packed (1, T, C) with ``cu``, whose check goes to ``cu_flag``."""
     L = _native.lib()
     h = torch.empty_like(xd, dtype=out_dtype, memory_format=torch.contiguous_format)
     spans = -(-T // _native.RECURRENCE_SPAN)
@@ -80,9 +80,9 @@ def _launch(call, xd, gd, cu, s0, slots, n_slots, bad, s_out, n_seqs, T, C, out_
     xc, gc = _k._code(xd.dtype), _k._code(gd.dtype)
     nbytes = L.pm_linear_recurrence_workspace_bytes(n_seqs, T, C, cu is not None, xc)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=call.device) if nbytes else None
-    _native.check(L.pm_linear_recurrence(
-        _k._ptr(xd), _k._ptr(gd), None if cu is None else cu.data_ptr(), _k._ptr(s0), _k._ptr(slots), n_slots,
-        _k._ptr(bad), _k._ptr(h), _k._ptr(s_out), _k._ptr(kept), n_seqs, T, C, xd.stride(0), xd.stride(1),
+    _native.check(L.pm_linear_recurrence_varlen(
+        _k._ptr(xd), _k._ptr(gd), _k._ptr(cu), _k._ptr(s0), _k._ptr(slots), n_slots,
+        _k._ptr(bad), _k._ptr(cu_flag), _k._ptr(h), _k._ptr(s_out), _k._ptr(kept), n_seqs, T, C, xd.stride(0), xd.stride(1),
         gd.stride(0), gd.stride(1), xc, gc, _k._code(out_dtype), _k._ptr(ws), nbytes, _k._stream(call.device)))
     return h, kept
 
@@ -218,14 +218,17 @@ def _packed(x, g, cu_seqlens):
     return n_tok, chan, host.size - 1, host
 
 
-def _offsets(call, cu, n_seqs, n_tok):
-    """int32 offsets on the device, those of a GPU tensor checked there (``check_varlen``)."""
+def _offsets(call, cu, n_seqs, n_tok, chan):
+    """int32 offsets on the device and, for those of a GPU tensor, the flag of ``check_varlen`` that
+    the launch is to set (a call that launches nothing is checked here)."""
     if isinstance(cu, np.ndarray):
-        return torch.from_numpy(cu.astype(np.int32)).to(call.device)
-    cu = cu.to(torch.int32).contiguous()
-    _native.check(_native.lib().pm_varlen_check(cu.data_ptr(), n_seqs, n_tok,
-                                                _k._varlen_flag(call.device).data_ptr(), _k._stream(call.device)))
-    return cu
+        return torch.from_numpy(cu.astype(np.int32)).to(call.device), None
+    cu, flag = cu.to(torch.int32).contiguous(), _k._varlen_flag(call.device)
+    if n_seqs == 0 or chan == 0:
+        _native.check(_native.lib().pm_varlen_check(cu.data_ptr(), n_seqs, n_tok, flag.data_ptr(),
+                                                    _k._stream(call.device)))
+        return cu, None
+    return cu, flag
 
 
 def linear_recurrence_varlen(x, g, cu_seqlens, state=None, *, out_dtype=None):
@@ -248,8 +251,8 @@ def linear_recurrence_varlen(x, g, cu_seqlens, state=None, *, out_dtype=None):
         xd, gd = (t if t.dim() == 3 else t[None] for t in (_rows(call, x, xt), _rows(call, g, gt)))
         sd = call.dev(state, torch.float32)
         s_out = torch.empty((n_seqs, chan), dtype=torch.float32, device=call.device)
-        h, _ = _launch(call, xd, gd, _offsets(call, cu, n_seqs, n_tok), sd, None, 0, None, s_out, n_seqs, n_tok,
-                       chan, odt, False)
+        cu, flag = _offsets(call, cu, n_seqs, n_tok, chan)
+        h, _ = _launch(call, xd, gd, cu, sd, None, 0, None, s_out, n_seqs, n_tok, chan, odt, False, flag)
     return call.out(h.reshape(_k._shape(x))), call.out(s_out)
 
 

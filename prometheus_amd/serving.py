@@ -255,11 +255,12 @@ class RecurrenceStateCache(_SlotPool):
                 slots = slots.clamp(-1, self.n_slots).to(torch.int32)
             xd, gd = (t if t.dim() == 3 else t[None] for t in (recurrence._rows(call, x, xt),
                                                                recurrence._rows(call, g, gt)))
+            flag = None
             if cu is not None:
-                cu = recurrence._offsets(call, cu, n_seqs, seq)
+                cu, flag = recurrence._offsets(call, cu, n_seqs, seq, chan)
             pool = self._pool[layer]
             h, _ = recurrence._launch(call, xd, gd, cu, pool, slots.contiguous(), self.n_slots, self._bad_slot, pool,
-                                      n_seqs, seq, chan, odt, False)
+                                      n_seqs, seq, chan, odt, False, flag)
         return h.reshape(x.shape)
 
     def decode(self, layer: int, slots: torch.Tensor, x, g, out=None, *, out_dtype=None):

@@ -1,5 +1,5 @@
 """GPU tests of the operators beside the delta rule where their kernels change course: tokens around
-the tiles' and groups' edges, more tiles than workgroups, many packed sequences, heads by fours,
+the tiles' and groups' edges, more tiles than workgroups, many packed sequences, heads in groups,
 strides past 32 bits, and both directions in a graph.
 
 Tolerances are the oracle's error bounds for fp32 arithmetic plus half a step of the output's type.
@@ -156,7 +156,7 @@ def test_both_directions_replayed_from_a_graph():
 @pytest.mark.parametrize("B,T,Hq,Hk,D,R,interleaved", [
     (2, 4100, 16, 4, 128, 128, False), (1, 2100, 7, 8, 256, 64, True), (3, 1500, 11, 12, 80, 40, False),
     (1, 9000, 8, 8, 33, 32, False), (2, 4500, 8, 4, 96, 0, False), (1, 30000, 4, 4, 16, 16, True)])
-def test_heads_by_fours(B, T, Hq, Hk, D, R, interleaved, dtype):
+def test_heads_in_groups(B, T, Hq, Hk, D, R, interleaved, dtype):
     gen = torch.Generator(device="cuda").manual_seed(D)
     q, k = (torch.randn(B, T, H, D, generator=gen, device="cuda").to(dtype) for H in (Hq, Hk))
     wq = 1 + 0.2 * torch.randn(D, generator=gen, device="cuda")
@@ -194,3 +194,18 @@ def test_heads_strides_past_32_bits():
         assert all(torch.equal(u, v) for u, v in zip(got, want))
         for u, v in zip(kernels.norm_rotate_bwd(res2, got)[:2], kernels.norm_rotate_bwd(res, got)[:2]):
             assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("N,C", [(400, 16), (3000, 8), (0, 8), (400, 0)])
+def test_malformed_device_offsets_are_named(N, C):
+    x = torch.randn(N, C, device="cuda")
+    kernels.check_varlen()
+    for cu, what in (([1, N], r"cu_seqlens\[0\]"), ([0, N + 1], r"cu_seqlens\[-1\].*outside"), ([0, N + 7, N], "outside"),
+                     ([0, 2, 1, N], "decreasing"), ([-1, N], r"cu_seqlens\[0\].*outside"), ([N + 1], r"cu_seqlens\[0\]"),
+                     ([0, N, N - 1], r"cu_seqlens\[-1\].*decreasing")):
+        kernels.linear_recurrence_varlen(x, -x.abs(), torch.tensor(cu, dtype=torch.int32, device="cuda"))
+        with pytest.raises(kernels.KernelError, match=what):
+            kernels.check_varlen()
+    for cu in ([0, N], [0, 0, N, N]):
+        kernels.linear_recurrence_varlen(x, -x.abs(), torch.tensor(cu, device="cuda"))
+        kernels.check_varlen()
