@@ -27,15 +27,17 @@
 //
 // Workgroups stay: while one waits and stores, its next tile's loads are under way (forward; the
 // backward's registers hold one tile). A tile is 196 kB of traffic to a compute unit, whose 512
-// threads hold its inputs as they are in memory and make gates and products again from them after
-// the wait (holding them as floats spilled, and halved the waves).
+// threads hold x and gh as they are in memory, and make what they need of them again after the
+// wait; the gates, of which an exponential is a quarter of a tile's arithmetic, are kept.
 //
-// Measured (a card that copies at 5.0 TB/s): forward 4 x 4096 tokens of 4096 bf16 channels 88 us
-// (4.6 TB/s; with 256-token tiles, a workgroup to each and the values held 121), backward 138 us
-// (4.9 TB/s; 226), 65521 tokens of 2048 channels 162 us (5.0 TB/s; 239). An elementwise pass over
-// the same lines takes 84: rows of 128 bytes are what bounds it (512 bytes: 69, but then tiles are
-// short, and four times the hops and words cost more than the rows gain: 92 to 97). Columns dealt
-// to XCDs in runs of neighbours were slower (96), stores that stay out of the caches 2% faster.
+// Measured (a card that copies at 5.0 TB/s): forward 4 x 4096 tokens of 4096 bf16 channels 82 us
+// (4.9 TB/s; with 256-token tiles, a workgroup to each and every value held 121; gates made twice
+// 88), backward 135 us (5.0 TB/s; 226; 140), 65521 tokens of 2048 channels 151 us (5.3 TB/s; 239;
+// 163). An elementwise pass over the same lines takes 84, over rows of 512 bytes 69; but wide tiles
+// are short, and four times the hops and words cost more than the rows gain (256 bytes: 87 and 133,
+// 157 for the long one; 512 bytes 89 where 128 take 84). Columns dealt to XCDs in runs of neighbours
+// were slower (96), stores that stay out of the caches 2% faster, and asking for the words before
+// the next tile's loads no faster (82, 134, 154).
 
 #include "pm_internal.h"
 #include "pm_vec.h"
@@ -293,6 +295,11 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
             mark = marks[tl];
         }
         int known = K;  // tokens from here on follow a sequence's start in this thread
+        float av[K][V];
+#pragma unroll
+        for (int r = 0; r < K; ++r)
+#pragma unroll
+            for (int v = 0; v < V; ++v) av[r][v] = gate(gr[r][v]);
         M m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = {1.f, 0.f};
@@ -301,7 +308,7 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
 #pragma unroll
             for (int r = 0; r < K; ++r)
 #pragma unroll
-                for (int v = 0; v < V; ++v) m[v].token(gate(gr[r][v]), xr[r][v]);
+                for (int v = 0; v < V; ++v) m[v].token(av[r][v], xr[r][v]);
         } else {
 #pragma unroll
             for (int r = 0; r < K; ++r) {
@@ -317,7 +324,7 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
                     known = min(known, r);
                 }
 #pragma unroll
-                for (int v = 0; v < V; ++v) m[v].token(gate(gr[r][v]), xr[r][v]);
+                for (int v = 0; v < V; ++v) m[v].token(av[r][v], xr[r][v]);
                 if (known <= r) {
                     // nothing before this thread's tokens matters any more: h is there
                     float h[V];
@@ -373,10 +380,10 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
         for (int v = 0; v < V; ++v) h[v] = sH[tl][lc * V + v];
         __syncthreads();  // (the next tile's maps go where these states were)
 #pragma unroll
-        for (int r = 0; r < K; ++r) forget(xr[r]), forget(gr[r]);
+        for (int r = 0; r < K; ++r) forget(xr[r]);
         auto walk = [&](int r) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = fmaf(gate(gr[r][v]), h[v], xr[r][v]);
+            for (int v = 0; v < V; ++v) h[v] = fmaf(av[r][v], h[v], xr[r][v]);
         };
         if (!PACKED || !__any(mark != 0)) {
 #pragma unroll
@@ -430,14 +437,28 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
         turns.ask();
         const bool there = cbase + ch < a.C;
         float h = there ? a.kept[(b * spans_of(a.T) + tile * (S::span / kRecSpan)) * a.C + cbase + ch] : 0.f;
+        // (bf16 rows leave registers for the gates; beside fp32 rows they are made again: 132 us at 4 x
+        // 4096 tokens of 2048 channels, kept 146)
+        constexpr bool KEEP = sizeof(X) == 2;
+        float av[KEEP ? K : 1][KEEP ? V : 1];
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int r = 0; r < K; ++r)
+#pragma unroll
+                for (int v = 0; v < V; ++v) av[r][v] = gate(gr[r][v]);
+        }
+        auto gate_at = [&](int r, int v) {
+            if constexpr (KEEP) return av[r][v];
+            else return gate(gr[r][v]);
+        };
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             M f{1.f, 0.f};  // the tokens' map of h
             float w = 0.f;  // and of c, whose factor is the same
 #pragma unroll
-            for (int r = 0; r < K; ++r) f.token(gate(gr[r][v]), xr[r][v]);
+            for (int r = 0; r < K; ++r) f.token(gate_at(r, v), xr[r][v]);
 #pragma unroll
-            for (int r = K - 1; r >= 0; --r) w = gate(gr[r][v]) * (w + hr[r][v]);
+            for (int r = K - 1; r >= 0; --r) w = gate_at(r, v) * (w + hr[r][v]);
             sA[tl][lc * V + v] = f.A, sF[tl][lc * V + v] = f.H, sB[tl][lc * V + v] = w;
         }
         __syncthreads();
@@ -488,18 +509,21 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
         Row<X, V> gx[K];
         Row<G, V> gg[K];
 #pragma unroll
-        for (int r = 0; r < K; ++r) forget(xr[r]), forget(gr[r]), forget(hr[r]);
+        for (int r = 0; r < K; ++r) {
+            forget(xr[r]), forget(hr[r]);
+            if constexpr (!KEEP) forget(gr[r]);
+        }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float hb[K];  // the state before each token
             hb[0] = sF[tl][lc * V + v];
 #pragma unroll
-            for (int r = 1; r < K; ++r) hb[r] = fmaf(gate(gr[r - 1][v]), hb[r - 1], xr[r - 1][v]);
+            for (int r = 1; r < K; ++r) hb[r] = fmaf(gate_at(r - 1, v), hb[r - 1], xr[r - 1][v]);
             float cv = sB[tl][lc * V + v];
 #pragma unroll
             for (int r = K - 1; r >= 0; --r) {
                 const float d = hr[r][v] + cv;
-                cv = gate(gr[r][v]) * d;
+                cv = gate_at(r, v) * d;
                 gx[r].set(v, d);
                 gg[r].set(v, cv * hb[r]);
             }

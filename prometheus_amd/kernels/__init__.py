@@ -200,6 +200,17 @@ def _aligned16(t):
     return t if t is None or t.numel() == 0 or t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _once(backward):
+    """``once_differentiable`` for a backward that launches kernels: refuses to be differentiated
+    itself, and costs nothing where no graph of it is asked for."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
 _HERE = contextlib.nullcontext()
 
 
@@ -247,7 +258,11 @@ def _forward(q, k, v, beta, state, chunk: int, out_dtype):
 
 
 def _wants_grad(*xs) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in xs)
+    if torch.is_grad_enabled():
+        for x in xs:
+            if isinstance(x, torch.Tensor) and x.requires_grad:
+                return True
+    return False
 
 
 class _ChunkedDeltaRule(torch.autograd.Function):

@@ -17,7 +17,6 @@ from typing import Any
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from prometheus_amd import _native
 from prometheus_amd import kernels as _k
@@ -111,6 +110,11 @@ def _heads(call, x, dtype):
     return call.dev(x, dtype)
 
 
+@functools.lru_cache(maxsize=1024)
+def _ws_bytes(B, T, Hq, Hk, D) -> int:
+    return _native.lib().pm_norm_rotate_bwd_workspace_bytes(B, T, Hq, Hk, D)
+
+
 class _Plan:
     """One call's device tensors and the arguments both directions share."""
 
@@ -174,7 +178,7 @@ def _launch_bwd(dev, tensors, shared, gqo, gko, want_weights):
     gk = torch.empty_like(k, memory_format=torch.contiguous_format)
     gwq, gwk = (torch.empty(w.shape, dtype=f32, device=dev) if w is not None and want else None
                 for w, want in zip((wq, wk), want_weights))
-    nbytes = L.pm_norm_rotate_bwd_workspace_bytes(*shared[:5]) if gwq is not None or gwk is not None else 0
+    nbytes = _ws_bytes(*shared[:5]) if gwq is not None or gwk is not None else 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _native.check(L.pm_norm_rotate_bwd(
         ptr(q), ptr(k), ptr(table), ptr(pos), ptr(wq), ptr(wk), ptr(gqo), ptr(gko), ptr(gq), ptr(gk), ptr(gwq),
@@ -190,30 +194,32 @@ class _NormRotate(torch.autograd.Function):
         plan, qo, ko = _forward(q, k, table, positions, norm, q_weight, k_weight, eps, interleaved)
         tensors = plan.tensors()
         ctx.save_for_backward(*tensors)
-        ctx.options = norm, eps, interleaved
+        ctx.call, ctx.options = plan.call, (norm, eps, interleaved)
         ctx.shared, ctx.strides = plan.shared, [None if t is None else t.stride() for t in tensors]
         ctx.set_materialize_grads(False)  # a missing gradient is None, not a tensor of zeros
-        # (the type and device of each input's gradient; None: as the backward gives it)
-        ctx.like = [(t.dtype, t.device) if isinstance(t, torch.Tensor) and t is not u else None
-                    for t, u in ((q, plan.q), (k, plan.k))]
-        ctx.like += [(t.dtype, t.device) if isinstance(t, torch.Tensor) and (t is not u or t.dtype != torch.float32)
-                     else None for t, u in ((q_weight, plan.wq), (k_weight, plan.wk))]
+        # (the type and device of each input's gradient, where it is not as the backward gives it)
+        as_given = q is plan.q and k is plan.k and all(
+            w is None or (w is u and w.dtype == torch.float32) for w, u in ((q_weight, plan.wq), (k_weight, plan.wk)))
+        ctx.like = None if as_given else [(t.dtype, t.device) if isinstance(t, torch.Tensor) else None
+                                          for t in (q, k, q_weight, k_weight)]
         return plan.call.out(qo), plan.call.out(ko)
 
     @staticmethod
-    @once_differentiable
+    @_k._once
     def backward(ctx, gq, gk):
         tensors, need = ctx.saved_tensors, ctx.needs_input_grad
         want = (need[2], need[3])
         if [None if t is None else t.stride() for t in tensors] == ctx.strides:
-            call = _k._Call(tensors[0])
+            call = ctx.call
             with _k._on(call.device):
                 grads = _launch_bwd(call.device, tensors, ctx.shared, call.dev(gq), call.dev(gk), want)
         else:  # (saved-tensor hooks may hand back another layout)
             q, k, table, pos, wq, wk = tensors
             grads = _backward(_NormRotateResidual(q, k, table, pos, wq, wk, *ctx.options), (gq, gk), want)
-        return (*((t if like is None else t.to(device=like[1], dtype=like[0])) if n and t is not None else None
-                  for t, like, n in zip(grads, ctx.like, need)), None, None, None, None, None)
+        if ctx.like is not None:
+            grads = [t if t is None or like is None else t.to(device=like[1], dtype=like[0])
+                     for t, like in zip(grads, ctx.like)]
+        return (*[t if n else None for t, n in zip(grads, need)], None, None, None, None, None)
 
 
 def norm_rotate(q, k, table=None, positions=None, *, norm="l2", q_weight=None, k_weight=None, eps=1e-6,

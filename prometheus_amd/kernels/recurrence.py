@@ -14,11 +14,11 @@ and sums are fp32 always.
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from prometheus_amd import _native
 from prometheus_amd import kernels as _k
@@ -61,29 +61,35 @@ def _rows(call, x, dtype):
 
 def _check(x, g, state, rank) -> tuple:
     xs, gs = _k._shape(x), _k._shape(g)
-    names = {3: "(B, T, C)", 2: "(B, C)"}[rank]
     if len(xs) != rank or gs != xs:
+        names = {3: "(B, T, C)", 2: "(B, C)"}[rank]
         raise _k.KernelError(f"x and g must both have shape {names}; got {xs} and {gs}")
-    want = (xs[0], xs[-1])
-    if state is not None and _k._shape(state) != want:
-        raise _k.KernelError(f"state shape {_k._shape(state)} != {want}")
+    if state is not None and _k._shape(state) != (xs[0], xs[-1]):
+        raise _k.KernelError(f"state shape {_k._shape(state)} != {(xs[0], xs[-1])}")
     return xs
+
+
+@functools.lru_cache(maxsize=1024)
+def _ws_bytes(n_seqs, T, C, packed, x_code) -> int:
+    """Bytes of the forward's workspace and (packed False) of the backward's."""
+    return _native.lib().pm_linear_recurrence_workspace_bytes(n_seqs, T, C, packed, x_code)
 
 
 def _launch(call, xd, gd, cu, s0, slots, n_slots, bad, s_out, n_seqs, T, C, out_dtype, keep, cu_flag=None):
     """The forward on device tensors: ``(h, kept)``; ``s_out`` is written. xd and gd are
     (n_seqs, T, C), or packed (1, T, C) with ``cu``, whose check goes to ``cu_flag``."""
-    L = _native.lib()
+    ptr = _k._ptr
     h = torch.empty_like(xd, dtype=out_dtype, memory_format=torch.contiguous_format)
     spans = -(-T // _native.RECURRENCE_SPAN)
     kept = torch.empty((n_seqs, spans, C), dtype=torch.float32, device=call.device) if keep else None
     xc, gc = _k._code(xd.dtype), _k._code(gd.dtype)
-    nbytes = L.pm_linear_recurrence_workspace_bytes(n_seqs, T, C, cu is not None, xc)
+    nbytes = _ws_bytes(n_seqs, T, C, cu is not None, xc)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=call.device) if nbytes else None
-    _native.check(L.pm_linear_recurrence_varlen(
-        _k._ptr(xd), _k._ptr(gd), _k._ptr(cu), _k._ptr(s0), _k._ptr(slots), n_slots,
-        _k._ptr(bad), _k._ptr(cu_flag), _k._ptr(h), _k._ptr(s_out), _k._ptr(kept), n_seqs, T, C, xd.stride(0), xd.stride(1),
-        gd.stride(0), gd.stride(1), xc, gc, _k._code(out_dtype), _k._ptr(ws), nbytes, _k._stream(call.device)))
+    (x_sb, x_st, _), (g_sb, g_st, _) = xd.stride(), gd.stride()
+    _native.check(_native.lib().pm_linear_recurrence_varlen(
+        xd.data_ptr(), gd.data_ptr(), ptr(cu), ptr(s0), ptr(slots), n_slots, ptr(bad), ptr(cu_flag), h.data_ptr(),
+        s_out.data_ptr(), ptr(kept), n_seqs, T, C, x_sb, x_st, g_sb, g_st, xc, gc, _k._code(out_dtype), ptr(ws), nbytes,
+        _k._stream(call.device)))
     return h, kept
 
 
@@ -102,18 +108,17 @@ def _forward(x, g, state, out_dtype, keep=False):
 def _launch_bwd(call, xd, gd, kept, gh, gs, h_dtype):
     """The backward on device tensors: ``(gx, gg, gs0)``."""
     batch, seq, chan = xd.shape
-    L = _native.lib()
+    ptr = _k._ptr
     gx = torch.empty_like(xd, memory_format=torch.contiguous_format)
     gg = torch.empty_like(gd, memory_format=torch.contiguous_format)
     gs0 = torch.empty((batch, chan), dtype=torch.float32, device=call.device)
     xc, gc = _k._code(xd.dtype), _k._code(gd.dtype)
-    nbytes = L.pm_linear_recurrence_workspace_bytes(batch, seq, chan, 0, xc)
+    nbytes = _ws_bytes(batch, seq, chan, False, xc)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=call.device) if nbytes else None
-    xs, gst = xd.stride(), gd.stride()
-    _native.check(L.pm_linear_recurrence_bwd(
-        _k._ptr(xd), _k._ptr(gd), _k._ptr(kept), _k._ptr(gh), _k._ptr(gs), _k._ptr(gx), _k._ptr(gg), _k._ptr(gs0),
-        batch, seq, chan, xs[0], xs[1], gst[0], gst[1], xc, gc, _k._code(h_dtype), _k._ptr(ws), nbytes,
-        _k._stream(call.device)))
+    (x_sb, x_st, _), (g_sb, g_st, _) = xd.stride(), gd.stride()
+    _native.check(_native.lib().pm_linear_recurrence_bwd(
+        xd.data_ptr(), gd.data_ptr(), ptr(kept), ptr(gh), ptr(gs), gx.data_ptr(), gg.data_ptr(), gs0.data_ptr(), batch,
+        seq, chan, x_sb, x_st, g_sb, g_st, xc, gc, _k._code(h_dtype), ptr(ws), nbytes, _k._stream(call.device)))
     return gx, gg, gs0
 
 
@@ -124,29 +129,28 @@ class _LinearRecurrence(torch.autograd.Function):
     def forward(ctx, x, g, state, out_dtype):
         call, xd, gd, kept, h, s = _forward(x, g, state, out_dtype, keep=True)
         ctx.save_for_backward(xd, gd, kept)
-        ctx.h_dtype = h.dtype
+        ctx.call, ctx.h_dtype = call, h.dtype
         ctx.set_materialize_grads(False)  # a missing gradient is None, not a tensor of zeros
-        # (the type and device of each input's gradient; None: as the backward gives it)
-        ctx.like = [(t.dtype, t.device) if isinstance(t, torch.Tensor) and u is not t else None
-                    for t, u in ((x, xd), (g, gd))]
-        if isinstance(state, torch.Tensor) and (state.dtype != torch.float32 or state.device != call.device):
-            ctx.like.append((state.dtype, state.device))
-        else:
-            ctx.like.append(None)
+        # (the type and device of each input's gradient, where it is not as the backward gives it)
+        as_given = xd is x and gd is g and (state is None or (
+            isinstance(state, torch.Tensor) and state.dtype == torch.float32 and state.device == call.device))
+        ctx.like = None if as_given else [(t.dtype, t.device) if isinstance(t, torch.Tensor) else None
+                                          for t in (x, g, state)]
         return call.out(h), call.out(s)
 
     @staticmethod
-    @once_differentiable
+    @_k._once
     def backward(ctx, gh, gs):
         xd, gd, kept = ctx.saved_tensors
         # (saved-tensor hooks may hand back another layout, but the same shapes)
-        call = _k._Call(xd)
+        call = ctx.call
         with _k._on(call.device):
             grads = _launch_bwd(call, _rows(call, xd, xd.dtype), _rows(call, gd, gd.dtype), call.dev(kept),
                                 call.dev(gh), call.dev(gs), ctx.h_dtype)
-        need = ctx.needs_input_grad
-        return (*((t if like is None else t.to(device=like[1], dtype=like[0])) if n else None
-                  for t, like, n in zip(grads, ctx.like, need)), None)
+        if ctx.like is not None:
+            grads = [t if like is None else t.to(device=like[1], dtype=like[0]) for t, like in zip(grads, ctx.like)]
+        x, g, state, _ = ctx.needs_input_grad
+        return grads[0] if x else None, grads[1] if g else None, grads[2] if state else None, None
 
 
 def linear_recurrence(x, g, state=None, *, out_dtype=None):

@@ -209,3 +209,34 @@ def test_malformed_device_offsets_are_named(N, C):
     for cu in ([0, N], [0, 0, N, N]):
         kernels.linear_recurrence_varlen(x, -x.abs(), torch.tensor(cu, device="cuda"))
         kernels.check_varlen()
+
+
+def test_gradients_of_gradients_are_refused():
+    x = torch.randn(1, 9, 4, device="cuda", requires_grad=True)
+    h, _ = kernels.linear_recurrence(x, -x.abs())
+    (gx,) = torch.autograd.grad(h.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|differentiate twice"):
+        gx.sum().backward()
+    q = torch.randn(1, 5, 2, 8, device="cuda", requires_grad=True)
+    zq, _ = kernels.norm_rotate(q, q)
+    (gq,) = torch.autograd.grad(zq.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|differentiate twice"):
+        gq.sum().backward()
+
+
+@pytest.mark.parametrize("where", ["input", "gate", "state"])
+def test_gradients_come_in_each_input_s_type_and_place(where):
+    """Inputs on the host, of another type or not contiguous, and tensors that hooks pack."""
+    base = {"input": torch.randn(2, 300, 7), "gate": -torch.rand(2, 300, 7), "state": torch.randn(2, 7)}
+    want = [t.cuda().requires_grad_(True) for t in base.values()]
+    h, s = kernels.linear_recurrence(*want)
+    grads = torch.autograd.grad(h.square().sum() + s.sum(), want)
+    for change in (lambda t: t.double(), lambda t: t.cpu(), lambda t: t.transpose(0, -1).contiguous().transpose(0, -1)):
+        args = [change(t.cuda()) if n == where else t.cuda() for n, t in base.items()]
+        args = [t.detach().requires_grad_(True) for t in args]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+            h, s = kernels.linear_recurrence(*args)
+        got = torch.autograd.grad(h.square().sum() + s.sum(), args)
+        for g, a, w in zip(got, args, grads):
+            assert g.dtype == a.dtype and g.device == a.device
+            assert torch.equal(g.cuda().float(), w)
