@@ -606,8 +606,8 @@ static Tiles tiles_of(int n_seqs, int T, int C, bool packed, bool x_bf16, void* 
     p.cgroups = (C + cw - 1) / cw;
     p.cols = static_cast<int64_t>(packed ? 1 : n_seqs) * p.cgroups;
     // sequences that a short tile holds take it: as many bytes under way with fewer idle threads
-    // (64 x 128 tokens of 2048 channels forward 20 us, in long tiles 67; 16 x 256 of 4096 middle
-    // 19, long 34); longer ones never do (4 x 4096 of 4096: short 124, long 89)
+    // (64 x 128 tokens of 2048 channels forward 18 us, in long tiles 67; 16 x 256 of 4096 middle
+    // 17.5, long 34); longer ones never do (4 x 4096 of 4096: short 124, long 89)
     p.span = T <= Short::span ? Short::span : T <= Middle::span ? Middle::span : Long::span;
     p.tiles = (static_cast<int64_t>(T) + p.span - 1) / p.span;
     if (p.tiles > 1) {

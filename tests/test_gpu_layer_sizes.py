@@ -240,3 +240,26 @@ def test_gradients_come_in_each_input_s_type_and_place(where):
         for g, a, w in zip(got, args, grads):
             assert g.dtype == a.dtype and g.device == a.device
             assert torch.equal(g.cuda().float(), w)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_packed_sequences_do_not_reach_each_other(dtype):
+    """NaN and infinities of a sequence, in its state, tokens or gates, leave the others' bits alone."""
+    lens = [3, 509, 1, 4, 700, 8, 2, 100, 1500, 37]
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    C, n = 72, len(lens)
+    x, g = _inputs((int(cu[-1]), C), dtype, 11, 0.05)
+    s0 = torch.randn(n, C, device="cuda")
+    want, end = kernels.linear_recurrence_varlen(x, g, cu, s0, out_dtype=dtype)
+    for i, value in ((0, torch.nan), (1, torch.inf), (4, -torch.inf), (7, torch.nan), (8, torch.inf)):
+        y, gate, s = x.clone(), g.clone(), s0.clone()
+        y[cu[i]:cu[i + 1], ::3] = value
+        gate[cu[i]:cu[i + 1], 1::3] = value
+        s[i, 2::3] = value
+        h, last = kernels.linear_recurrence_varlen(y, gate, cu, s, out_dtype=dtype)
+        others = torch.ones(int(cu[-1]), dtype=torch.bool, device="cuda")
+        others[cu[i]:cu[i + 1]] = False
+        assert torch.equal(h[others], want[others])
+        keep = torch.arange(n, device="cuda") != i
+        assert torch.equal(last[keep], end[keep])
+        assert not torch.isfinite(h[cu[i]:cu[i + 1], ::3]).any() and not torch.isfinite(last[i, ::3]).any()
