@@ -25,19 +25,19 @@
 // they wait for each other, and a workgroup finishes its tile before it folds its next: the first
 // tile that is not done is always somebody's to do, and waits for nothing, so every wait ends.
 //
-// Workgroups stay: while one waits and stores, its next tile's loads are under way (forward; the
+// Workgroups stay: while one walks and stores, its next tile's loads are under way (forward; the
 // backward's registers hold one tile). A tile is 196 kB of traffic to a compute unit, whose 512
 // threads hold x and gh as they are in memory, and make what they need of them again after the
 // wait; the gates, of which an exponential is a quarter of a tile's arithmetic, are kept.
 //
-// Measured (a card that copies at 5.0 TB/s): forward 4 x 4096 tokens of 4096 bf16 channels 82 us
-// (4.9 TB/s; with 256-token tiles, a workgroup to each and every value held 121; gates made twice
-// 88), backward 135 us (5.0 TB/s; 226; 140), 65521 tokens of 2048 channels 151 us (5.3 TB/s; 239;
-// 163). An elementwise pass over the same lines takes 84, over rows of 512 bytes 69; but wide tiles
-// are short, and four times the hops and words cost more than the rows gain (256 bytes: 87 and 133,
-// 157 for the long one; 512 bytes 89 where 128 take 84). Columns dealt to XCDs in runs of neighbours
-// were slower (96), stores that stay out of the caches 2% faster, and asking for the words before
-// the next tile's loads no faster (82, 134, 154).
+// Measured (a card that copies at 5.0 TB/s): forward 4 x 4096 tokens of 4096 bf16 channels 79 us
+// (5.1 TB/s), backward 131 (5.1 TB/s), 65521 tokens of 2048 channels 146 (5.5 TB/s). On the way:
+// 256-token tiles, a workgroup to each and every value held 121, 226 and 239; as here but gates made
+// twice 88, 140 and 163; a branch at every row and words asked for after the tile's loads 82, 135
+// and 151. An elementwise pass over the same lines takes 84, over rows of 512 bytes 69; but wide
+// tiles are short, and four times the hops and words cost more than the rows gain (256 bytes, two
+// workgroups to a compute unit: 151 for the long one; 512 bytes: 183). Columns dealt to XCDs in runs
+// of neighbours were slower (96 of 88), stores that stay out of the caches 2% faster.
 
 #include "pm_internal.h"
 #include "pm_vec.h"
@@ -80,17 +80,10 @@ __device__ __forceinline__ uint64_t word(uint32_t above, float below) {
 __device__ __forceinline__ void publish(uint64_t* p, uint64_t v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ uint64_t look(uint64_t* p) {
+__device__ __forceinline__ uint64_t load_word(uint64_t* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// the word at p once it is there; v is what a look at it gave
-__device__ __forceinline__ uint64_t wait_word(uint64_t* p, uint64_t v) {
-    while (static_cast<uint32_t>(v >> 32) == 0xffffffffu) {
-        __builtin_amdgcn_s_sleep(1);
-        v = look(p);
-    }
-    return v;
-}
+__device__ __forceinline__ bool missing(uint64_t v) { return static_cast<uint32_t>(v >> 32) == 0xffffffffu; }
 __device__ __forceinline__ float low(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
 __device__ __forceinline__ float high(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
 
@@ -125,38 +118,72 @@ __device__ __forceinline__ int64_t state_row(const int32_t* slots, int n_slots, 
     return r >= 0 && r < n_slots ? r : -1;
 }
 
-// Where the thread (ch, part) of a tile's fold stands in a group's chain, and the state it takes
-// from there. All threads of the workgroup call it; `lb` is LDS [PARTS][CW]. `j` counts tiles in
-// the order in which they wait for each other, `first` is the state before tile 0.
+// Waits for all of the wave's loads. Where a branch may have left some under way, the compiler
+// holds up the next use of their registers until every load before is back, the tile's own too.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
+// What the thread (ch, part) of a tile's fold takes from the tiles before: some of the group's maps
+// and, in part 0, the state at the group's start. `j` counts tiles in the order in which they wait
+// for each other. All threads of a workgroup call all three.
 template <bool CHAINED, bool PACKED, int CW, int PARTS>
-__device__ __forceinline__ float state_before(const Tiles& p, int64_t col, int64_t j, int ch, int part, float first,
-                                              Map<PACKED> (*lb)[CW]) {
-    if (!CHAINED || !p.next || j == 0) return first;
-    constexpr int Q = (kGroup + PARTS - 1) / PARTS;  // tiles of the group to a part
-    const int64_t g0 = j / kGroup * kGroup, groups = (p.tiles + kGroup - 1) / kGroup;
-    const int n = static_cast<int>(j - g0);
-    uint64_t* maps = p.map + (col * p.tiles + g0 + part * Q) * CW + ch;
-    uint64_t* state = p.state + (col * groups + j / kGroup) * CW + ch;
-    const bool chained = part == 0 && g0 > 0;
-    // every word is asked for before the first is waited for
-    uint64_t w[Q], from = 0;
-    if (chained) from = look(state);
+struct Before {
+    static constexpr int Q = (kGroup + PARTS - 1) / PARTS;  // tiles of the group to a part
+    uint64_t* maps;
+    uint64_t* from;
+    uint64_t w[Q], s;
+    int n;      // maps to read
+    bool deep;  // whether to read the state
+
+    // Asks for every word.
+    __device__ __forceinline__ void look(const Tiles& p, int64_t col, int64_t j, int ch, int part) {
+        if (!CHAINED || !p.next) return;
+        const int64_t g0 = j / kGroup * kGroup, groups = (p.tiles + kGroup - 1) / kGroup;
+        n = static_cast<int>(j - g0) - part * Q;
+        deep = part == 0 && g0 > 0;
+        maps = p.map + (col * p.tiles + g0 + part * Q) * CW + ch;
+        from = p.state + (col * groups + j / kGroup) * CW + ch;
+        if (deep) s = load_word(from);
 #pragma unroll
-    for (int i = 0; i < Q; ++i)
-        if (part * Q + i < n) w[i] = look(maps + static_cast<int64_t>(i) * CW);
-    Map<PACKED> m{1.f, 0.f};
+        for (int i = 0; i < Q; ++i)
+            if (i < n) w[i] = load_word(maps + static_cast<int64_t>(i) * CW);
+    }
+    // Waits for them. Loads come back in the order they were asked for, so this is done before the
+    // next tile's are, which would have to come back first.
+    __device__ __forceinline__ void wait(const Tiles& p) {
+        if (!CHAINED || !p.next) return;
+        for (;;) {  // (again for all that are missing at a time)
+            const bool s_missing = deep && missing(s);
+            bool any = s_missing, w_missing[Q];
 #pragma unroll
-    for (int i = 0; i < Q; ++i)
-        if (part * Q + i < n) m.then(Map<PACKED>::read(wait_word(maps + static_cast<int64_t>(i) * CW, w[i])));
-    if (part == 0) m.H = m.of(chained ? low(wait_word(state, from)) : first);
-    lb[part][ch] = m;
-    __syncthreads();
-    float s = lb[0][ch].H;
+            for (int i = 0; i < Q; ++i) w_missing[i] = i < n && missing(w[i]), any |= w_missing[i];
+            if (!any) break;
+            __builtin_amdgcn_s_sleep(1);
+            if (s_missing) s = load_word(from);
 #pragma unroll
-    for (int i = 1; i < PARTS; ++i)
-        if (i * Q < n) s = lb[i][ch].of(s);
-    return s;
-}
+            for (int i = 0; i < Q; ++i)
+                if (w_missing[i]) w[i] = load_word(maps + static_cast<int64_t>(i) * CW);
+        }
+        loads_done();
+    }
+    // The state before tile j; `first` is that before tile 0, `lb` is LDS [PARTS][CW].
+    __device__ __forceinline__ float state(const Tiles& p, int64_t j, int ch, int part, float first,
+                                           Map<PACKED> (*lb)[CW]) {
+        if (!CHAINED || !p.next || j == 0) return first;
+        Map<PACKED> m{1.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+            if (i < n) m.then(Map<PACKED>::read(w[i]));
+        if (part == 0) m.H = m.of(deep ? low(s) : first);
+        lb[part][ch] = m;
+        __syncthreads();
+        float before = lb[0][ch].H;
+        const int all = static_cast<int>(j % kGroup);
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i)
+            if (i * Q < all) before = lb[i][ch].of(before);
+        return before;
+    }
+};
 
 template <int CW>
 __device__ __forceinline__ void publish_state(const Tiles& p, int64_t col, int64_t j, int ch, float s) {
@@ -204,17 +231,22 @@ struct Place {
     }
 };
 
-template <typename X, typename G, int V, int K>
-__device__ __forceinline__ void load_tile(const RecurrenceArgs& a, int seq, int t0, int c0, Row<X, V> (&xr)[K],
-                                          Row<G, V> (&gr)[K]) {
-    const X* xp = static_cast<const X*>(a.x) + seq * a.x_sb + t0 * a.x_st + c0;
-    const G* gp = static_cast<const G*>(a.g) + seq * a.g_sb + t0 * a.g_st + c0;
+// A thread's rows of a tensor: token r at p + r st; those of `tokens` and `nc` channels that there
+// are, zeros for the others.
+template <typename E, int V, int K>
+__device__ __forceinline__ void load_rows(Row<E, V> (&rows)[K], const E* p, int64_t st) {
 #pragma unroll
-    for (int r = 0; r < K; ++r) {
-        const int n = t0 + r < a.T ? a.C - c0 : 0;
-        xr[r].load(xp + r * a.x_st, n);
-        gr[r].load(gp + r * a.g_st, n);
-    }
+    for (int r = 0; r < K; ++r) rows[r].load(p + r * st);
+}
+template <typename E, int V, int K>
+__device__ __forceinline__ void load_rows(Row<E, V> (&rows)[K], const E* p, int64_t st, int tokens, int nc) {
+#pragma unroll
+    for (int r = 0; r < K; ++r) rows[r].load(p + r * st, r < tokens ? nc : 0);
+}
+// Whether every token and channel of the tile is there.
+template <typename S, int CW>
+__device__ __forceinline__ bool tile_full(int T, int C, int64_t tile, int cbase) {
+    return (tile + 1) * S::span <= T && cbase + CW <= C;
 }
 
 // Keeps the compiler from carrying values made from a row across this point in registers: they
@@ -249,24 +281,40 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
         __syncthreads();
     }
 
+    Before<S::chained, PACKED, CW, PARTS> before;
     Turns turns(p, &slot);
     Row<X, V> xn[K];
     Row<G, V> gn[K];
-    if (!turns.done()) {
+    auto load_next = [&] {
+        if (turns.done()) return;
         const Place<PACKED, CW> at(p, turns.id);
-        load_tile<X, G, V, K>(a, at.seq, static_cast<int>(at.j) * S::span + tl * K, at.cbase + lc * V, xn, gn);
-    }
+        const int t0 = static_cast<int>(at.j) * S::span + tl * K, c0 = at.cbase + lc * V;
+        const bool full = tile_full<S, CW>(a.T, a.C, at.j, at.cbase);
+        const X* xp = static_cast<const X*>(a.x) + at.seq * a.x_sb + t0 * a.x_st + c0;
+        const G* gp = static_cast<const G*>(a.g) + at.seq * a.g_sb + t0 * a.g_st + c0;
+        if (full) {
+            load_rows(xn, xp, a.x_st);
+            load_rows(gn, gp, a.g_st);
+        } else {
+            load_rows(xn, xp, a.x_st, a.T - t0, a.C - c0);
+            load_rows(gn, gp, a.g_st, a.T - t0, a.C - c0);
+            loads_done();
+        }
+    };
+    load_next();
     while (!turns.done()) {
         const Place<PACKED, CW> at(p, turns.id);
         const int64_t j = at.j, col = at.col;
         const int seq = at.seq, cbase = at.cbase;
         const int c0 = cbase + lc * V, nc = a.C - c0;  // this thread's channels, and how many are there
         const int tile0 = static_cast<int>(j) * S::span, t0 = tile0 + tl * K;
+        const bool full = tile_full<S, CW>(a.T, a.C, j, cbase);
         Row<X, V> xr[K];
         Row<G, V> gr[K];
 #pragma unroll
         for (int r = 0; r < K; ++r) xr[r] = xn[r], gr[r] = gn[r];
         turns.ask();
+        before.look(p, col, j, ch, part);
         // the state before the sequence: read by its first tile only, before that tile's map is
         // out, as the last tile may write the same row of the pool soon after
         if (!PACKED && j == 0 && part == 0) {
@@ -356,11 +404,9 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
             if (!PACKED && j == 0) sum = {0.f, sum.of(s)};  // the first tile's map yields its state
             publish(p.map + (col * p.tiles + j) * CW + ch, sum.word());
         }
-        if (!turns.done()) {
-            const Place<PACKED, CW> next(p, turns.id);
-            load_tile<X, G, V, K>(a, next.seq, static_cast<int>(next.j) * S::span + tl * K, next.cbase + lc * V, xn, gn);
-        }
-        s = state_before<S::chained, PACKED, CW, PARTS>(p, col, j, ch, part, s, lb);
+        before.wait(p);
+        load_next();
+        s = before.state(p, j, ch, part, s, lb);
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)
             if (i < part) s = total[i][ch].of(s);
@@ -385,11 +431,21 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = fmaf(av[r][v], h[v], xr[r][v]);
         };
-        if (!PACKED || !__any(mark != 0)) {
+        if (full && (!PACKED || !__any(mark != 0))) {
 #pragma unroll
             for (int r = 0; r < K; ++r) {
                 walk(r);
-                finish(r, h, !PACKED && t0 + r == a.T - 1 ? seq : -1);
+                Row<H, V> out;
+#pragma unroll
+                for (int v = 0; v < V; ++v) out.set(v, h[v]);
+                out.store(hp + static_cast<int64_t>(r) * a.C);
+            }
+            if (!PACKED && t0 + K == a.T) finish(K, h, seq);  // (token K is none of the tile's: the state alone)
+        } else if (!PACKED) {
+#pragma unroll
+            for (int r = 0; r < K; ++r) {
+                walk(r);
+                finish(r, h, t0 + r == a.T - 1 ? seq : -1);
             }
         } else {
 #pragma unroll
@@ -414,6 +470,7 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
     const int tid = threadIdx.x, lc = tid % kLanesC, tl = tid / kLanesC;
     const int ch = tid % CW, part = tid / CW;
 
+    Before<S::chained, false, CW, PARTS> before;
     Turns turns(p, &slot);
     while (!turns.done()) {
         const Place<false, CW> at(p, turns.id);
@@ -421,20 +478,26 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
         const int b = at.seq, cbase = at.cbase;
         const int c0 = cbase + lc * V, nc = a.C - c0;
         const int t0 = static_cast<int>(tile) * S::span + tl * K;
-        const X* xp = static_cast<const X*>(a.x) + b * a.x_sb + t0 * a.x_st + c0;
-        const G* gp = static_cast<const G*>(a.g) + b * a.g_sb + t0 * a.g_st + c0;
         const int64_t out = (static_cast<int64_t>(b) * a.T + t0) * a.C + c0;
+        const bool full = tile_full<S, CW>(a.T, a.C, tile, cbase);
         Row<X, V> xr[K];
         Row<G, V> gr[K];
         Row<H, V> hr[K];
-#pragma unroll
-        for (int r = 0; r < K; ++r) {
-            const int n = t0 + r < a.T ? nc : 0;
-            xr[r].load(xp + r * a.x_st, n);
-            gr[r].load(gp + r * a.g_st, n);
-            hr[r].load(static_cast<const H*>(a.gh) + out + static_cast<int64_t>(r) * a.C, a.gh ? n : 0);
+        const X* xp = static_cast<const X*>(a.x) + b * a.x_sb + t0 * a.x_st + c0;
+        const G* gp = static_cast<const G*>(a.g) + b * a.g_sb + t0 * a.g_st + c0;
+        const H* hp = static_cast<const H*>(a.gh) + out;
+        if (full && a.gh) {
+            load_rows(xr, xp, a.x_st);
+            load_rows(gr, gp, a.g_st);
+            load_rows(hr, hp, a.C);
+        } else {
+            load_rows(xr, xp, a.x_st, a.T - t0, nc);
+            load_rows(gr, gp, a.g_st, a.T - t0, nc);
+            load_rows(hr, hp, a.C, a.gh ? a.T - t0 : 0, nc);
+            loads_done();
         }
         turns.ask();
+        before.look(p, col, j, ch, part);
         const bool there = cbase + ch < a.C;
         float h = there ? a.kept[(b * spans_of(a.T) + tile * (S::span / kRecSpan)) * a.C + cbase + ch] : 0.f;
         // (bf16 rows leave registers for the gates; beside fp32 rows they are made again: 132 us at 4 x
@@ -483,7 +546,8 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
             publish(p.map + (col * p.tiles + j) * CW + ch, down.word());
         }
         float c = a.gs && j < kGroup && there ? a.gs[static_cast<int64_t>(b) * a.C + cbase + ch] : 0.f;
-        c = state_before<S::chained, false, CW, PARTS>(p, col, j, ch, part, c, lb);
+        before.wait(p);
+        c = before.state(p, j, ch, part, c, lb);
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)
             if (i < part) h = fwd[i][ch].of(h);
@@ -529,12 +593,16 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
             }
         }
         __syncthreads();  // (the next tile's maps go where these states were)
+        X* gxp = static_cast<X*>(a.gx) + out;
+        G* ggp = static_cast<G*>(a.gg) + out;
+        if (full) {
 #pragma unroll
-        for (int r = 0; r < K; ++r)
-            if (t0 + r < a.T) {
-                gx[r].store(static_cast<X*>(a.gx) + out + static_cast<int64_t>(r) * a.C, nc);
-                gg[r].store(static_cast<G*>(a.gg) + out + static_cast<int64_t>(r) * a.C, nc);
-            }
+            for (int r = 0; r < K; ++r) gx[r].store(gxp + static_cast<int64_t>(r) * a.C), gg[r].store(ggp + static_cast<int64_t>(r) * a.C);
+        } else {
+#pragma unroll
+            for (int r = 0; r < K; ++r)
+                if (t0 + r < a.T) gx[r].store(gxp + static_cast<int64_t>(r) * a.C, nc), gg[r].store(ggp + static_cast<int64_t>(r) * a.C, nc);
+        }
     }
 }
 

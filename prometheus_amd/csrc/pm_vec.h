@@ -18,10 +18,11 @@ template <typename E, int V>
 struct Row {
     uint32_t raw[V * sizeof(E) / 4];
 
+    __device__ __forceinline__ void load(const E* p) { __builtin_memcpy(raw, p, sizeof raw); }
     // elements [0, n) of p, zeros beyond
     __device__ __forceinline__ void load(const E* p, int n) {
         if (n >= V) {
-            __builtin_memcpy(raw, p, sizeof raw);
+            load(p);
             return;
         }
 #pragma unroll
@@ -48,14 +49,17 @@ struct Row {
             raw[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, bf16_pair));
         }
     }
+    __device__ __forceinline__ void store(E* p) const {
+        // (outputs are not read again here: they go past the caches)
+        typedef uint32_t vec __attribute__((ext_vector_type(V * sizeof(E) / 4), aligned(sizeof(E))));
+        vec v;
+        __builtin_memcpy(&v, raw, sizeof raw);
+        __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
+    }
     // the first n elements to p
     __device__ __forceinline__ void store(E* p, int n) const {
         if (n >= V) {
-            // (outputs are not read again here: they go past the caches)
-            typedef uint32_t vec __attribute__((ext_vector_type(V * sizeof(E) / 4), aligned(sizeof(E))));
-            vec v;
-            __builtin_memcpy(&v, raw, sizeof raw);
-            __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
+            store(p);
             return;
         }
 #pragma unroll
