@@ -60,7 +60,8 @@ struct Shape {
 typedef Shape<8, 512, 256, true> Long;
 typedef Shape<4, 512, 512, false> Middle;
 typedef Shape<4, 256, 1024, false> Short;
-static_assert(Long::span % kRecSpan == 0 && Middle::span % kRecSpan == 0 && Short::span == kRecSpan, "kept states start every tile");
+static_assert(Long::span % kRecSpan == 0 && Middle::span % kRecSpan == 0 && Short::span == kRecSpan,
+              "kept states start every tile");
 
 // The tiles of a call and the words through which they pass states (all null where each
 // sequence is one tile).
@@ -209,7 +210,8 @@ struct Turns {
     }
     __device__ __forceinline__ bool done() const { return id >= p.cols * p.tiles; }
     __device__ __forceinline__ void ask() {
-        if (p.next && threadIdx.x == 0) got = __hip_atomic_fetch_add(p.next, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (p.next && threadIdx.x == 0)
+            got = __hip_atomic_fetch_add(p.next, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __device__ __forceinline__ void tell() {
         if (p.next && threadIdx.x == 0) *slot = got;
@@ -223,7 +225,8 @@ struct Place {
     int seq, cbase;
     __device__ __forceinline__ Place(const Tiles& p, int64_t id) {
         // (32 bits: the number of tiles is at most 2^31)
-        const uint32_t u = static_cast<uint32_t>(id), cols = static_cast<uint32_t>(p.cols), q = u / cols, c = u - q * cols;
+        const uint32_t u = static_cast<uint32_t>(id), cols = static_cast<uint32_t>(p.cols);
+        const uint32_t q = u / cols, c = u - q * cols;
         j = q, col = c;
         const uint32_t b = PACKED ? 0 : c / static_cast<uint32_t>(p.cgroups);
         seq = static_cast<int>(b);
@@ -597,11 +600,17 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
         G* ggp = static_cast<G*>(a.gg) + out;
         if (full) {
 #pragma unroll
-            for (int r = 0; r < K; ++r) gx[r].store(gxp + static_cast<int64_t>(r) * a.C), gg[r].store(ggp + static_cast<int64_t>(r) * a.C);
+            for (int r = 0; r < K; ++r) {
+                gx[r].store(gxp + static_cast<int64_t>(r) * a.C);
+                gg[r].store(ggp + static_cast<int64_t>(r) * a.C);
+            }
         } else {
 #pragma unroll
             for (int r = 0; r < K; ++r)
-                if (t0 + r < a.T) gx[r].store(gxp + static_cast<int64_t>(r) * a.C, nc), gg[r].store(ggp + static_cast<int64_t>(r) * a.C, nc);
+                if (t0 + r < a.T) {
+                    gx[r].store(gxp + static_cast<int64_t>(r) * a.C, nc);
+                    gg[r].store(ggp + static_cast<int64_t>(r) * a.C, nc);
+                }
         }
     }
 }
@@ -611,7 +620,8 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
 // which pass through.
 __global__ __launch_bounds__(256) void recurrence_begin_kernel(uint32_t* next, uint64_t* words, int64_t n,
                                                                RecurrenceArgs a) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
     if (next && at == 0) *next = 0;
     for (int64_t i = at; i < n; i += step) words[i] = ~uint64_t(0);
     for (int seq = blockIdx.x; seq < a.n_seqs; seq += gridDim.x) {
@@ -733,8 +743,9 @@ hipError_t launch_recurrence(const RecurrenceArgs& a, hipStream_t st) {
         constexpr int V = sizeof(X) == 2 ? 8 : 4;
         by_shape(p, [&](auto shape, dim3 grid) {
             typedef decltype(shape) S;
-            if (packed) hipLaunchKernelGGL((recurrence_kernel<X, G, H, V, S, true>), grid, dim3(S::threads), 0, st, a, p);
-            else hipLaunchKernelGGL((recurrence_kernel<X, G, H, V, S, false>), grid, dim3(S::threads), 0, st, a, p);
+            const dim3 block(S::threads);
+            if (packed) hipLaunchKernelGGL((recurrence_kernel<X, G, H, V, S, true>), grid, block, 0, st, a, p);
+            else hipLaunchKernelGGL((recurrence_kernel<X, G, H, V, S, false>), grid, block, 0, st, a, p);
         });
         e = hipGetLastError();
     });

@@ -145,7 +145,8 @@ __device__ __forceinline__ bool load_angles(const NormRotateArgs& a, const Part&
 
 // The lane's pairs turned by their angles (dir 1) or back (-1).
 template <int V, bool CONTIG>
-__device__ __forceinline__ void turn(const float (&c)[V], const float (&s)[V], float dir, float (&ya)[V], float (&yb)[V]) {
+__device__ __forceinline__ void turn(const float (&c)[V], const float (&s)[V], float dir, float (&ya)[V],
+                                     float (&yb)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         float& y1 = !CONTIG ? ya[i] : i < V / 2 ? ya[2 * i % V] : yb[2 * i % V];
