@@ -263,3 +263,39 @@ def test_packed_sequences_do_not_reach_each_other(dtype):
         keep = torch.arange(n, device="cuda") != i
         assert torch.equal(last[keep], end[keep])
         assert not torch.isfinite(h[cu[i]:cu[i + 1], ::3]).any() and not torch.isfinite(last[i, ::3]).any()
+
+
+@pytest.mark.parametrize("T", [100, 900, 9000])
+def test_backward_again_and_in_a_graph(T):
+    """A second backward of the same graph, and one that a captured graph replays, set up their own."""
+    x, g = _inputs((2, T, 136), BF16, T, 1e-2)
+    x, g = x.requires_grad_(True), g.requires_grad_(True)
+    gh = torch.randn(2, T, 136, device="cuda").to(BF16)
+    _, res = kernels.linear_recurrence_fwd(x.detach(), g.detach(), out_dtype=BF16)
+    want = kernels.linear_recurrence_bwd(res, (gh, None))[:2]
+
+    def check(got, want):
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+    h, _ = kernels.linear_recurrence(x, g, out_dtype=BF16)
+    for _ in range(3):
+        check(torch.autograd.grad(h, (x, g), gh, retain_graph=True), want)
+    with pytest.raises(RuntimeError, match="second time|already been freed"):
+        torch.autograd.grad(h, (x, g), gh)
+        torch.autograd.grad(h, (x, g), gh)
+    # the explicit pair in a graph, replayed with other gradients
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kernels.linear_recurrence_bwd(res, (gh, None))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = kernels.linear_recurrence_bwd(res, (gh, None))
+    for _ in range(3):
+        gh.copy_(torch.randn(2, T, 136, device="cuda"))
+        want = kernels.linear_recurrence_bwd(res, (gh, None))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check(outs, want)
