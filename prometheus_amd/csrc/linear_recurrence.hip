@@ -304,8 +304,10 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
             loads_done();
         }
     };
-    load_next();
+    // (short tiles have other workgroups of their compute unit to read meanwhile, and spilled)
+    if constexpr (S::chained) load_next();
     while (!turns.done()) {
+        if constexpr (!S::chained) load_next();
         const Place<PACKED, CW> at(p, turns.id);
         const int64_t j = at.j, col = at.col;
         const int seq = at.seq, cbase = at.cbase;
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
             publish(p.map + (col * p.tiles + j) * CW + ch, sum.word());
         }
         before.wait(p);
-        load_next();
+        if constexpr (S::chained) load_next();
         s = before.state(p, j, ch, part, s, lb);
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)
