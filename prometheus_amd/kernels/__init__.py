@@ -154,7 +154,7 @@ class _Call:
         if x is None:
             return None
         if isinstance(x, torch.Tensor):
-            if x.is_cuda and x.device == self.device and (dtype is None or x.dtype == dtype) and x.is_contiguous():
+            if (dtype is None or x.dtype == dtype) and x.get_device() == self.device.index and x.is_contiguous():
                 return x
             t = x
         else:

@@ -86,15 +86,15 @@ def _check(q, k, table, positions, norm, q_weight, k_weight, eps) -> tuple:
             raise _k.KernelError("positions need a table")
         if _k._shape(positions) not in ((seq,), qs[:-2]):
             raise _k.KernelError(f"positions shape {_k._shape(positions)} is neither {(seq,)} nor {qs[:-2]}")
-        host = positions.numpy() if isinstance(positions, torch.Tensor) and positions.device.type == "cpu" else positions
-        if not isinstance(host, torch.Tensor):
-            host = np.asarray(host)
-            if not np.issubdtype(host.dtype, np.integer):
-                raise _k.KernelError(f"positions must be integers, got {host.dtype}")
-            if host.size and (host.min() < 0 or host.max() >= rows):
-                raise _k.KernelError(f"positions {host.min()}..{host.max()} outside the table's {rows} rows")
-        elif positions.dtype not in (torch.int32, torch.int64):
-            raise _k.KernelError(f"positions must be int32 or int64, got {positions.dtype}")
+        if isinstance(positions, torch.Tensor) and positions.is_cuda:
+            if positions.dtype not in (torch.int32, torch.int64):
+                raise _k.KernelError(f"positions must be int32 or int64, got {positions.dtype}")
+            return batch, seq, qs[-2], ks[-2], dim, rot, rows
+        host = np.asarray(positions)
+        if not np.issubdtype(host.dtype, np.integer):
+            raise _k.KernelError(f"positions must be integers, got {host.dtype}")
+        if host.size and (host.min() < 0 or host.max() >= rows):
+            raise _k.KernelError(f"positions {host.min()}..{host.max()} outside the table's {rows} rows")
     elif rot and len(qs) == 3:
         raise _k.KernelError("q and k of shape (N, H, D) need positions")
     elif rot and seq > rows:
@@ -104,7 +104,7 @@ def _check(q, k, table, positions, norm, q_weight, k_weight, eps) -> tuple:
 
 def _heads(call, x, dtype):
     """``x`` on the call's device in ``dtype``, the elements of a head contiguous."""
-    if isinstance(x, torch.Tensor) and x.dtype == dtype and x.device == call.device and (
+    if isinstance(x, torch.Tensor) and x.dtype == dtype and x.get_device() == call.device.index and (
             x.stride(-1) == 1 or x.shape[-1] <= 1):
         return x
     return call.dev(x, dtype)
@@ -131,11 +131,11 @@ class _Plan:
             p = positions if isinstance(positions, torch.Tensor) else torch.from_numpy(np.asarray(positions))
             if p.dtype not in (torch.int32, torch.int64):
                 p = p.to(torch.int64)
-            if p.device != call.device:
+            if not p.is_cuda:
                 p = p.to(call.device)
             if p.dim() == 2 and (p.shape[1] <= 1 or p.stride(1) == 1):
                 pos_sb = p.stride(0)
-            else:
+            elif not p.is_contiguous():
                 p = p.contiguous()
                 pos_sb = p.shape[1] if p.dim() == 2 else 0
             self.pos, pos64 = p, int(p.dtype == torch.int64)

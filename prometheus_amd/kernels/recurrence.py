@@ -53,7 +53,7 @@ def _types(x, g) -> tuple[torch.dtype, torch.dtype]:
 def _rows(call, x, dtype):
     """``x`` on the call's device in ``dtype``, its last dimension contiguous (no copy of a view
     that has it so)."""
-    if isinstance(x, torch.Tensor) and x.dtype == dtype and x.device == call.device and (
+    if isinstance(x, torch.Tensor) and x.dtype == dtype and x.get_device() == call.device.index and (
             x.stride(-1) == 1 or x.shape[-1] <= 1):
         return x
     return call.dev(x, dtype)
