@@ -172,6 +172,7 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_kernel(NormRotateArgs a, i
     const float nan = __uint_as_float(0x7fc00000u);
     const bool k = static_cast<int>(blockIdx.x) >= q_blocks;
     const int H = a.H[k], chunks = (H + NH - 1) / NH;
+    const int64_t far = static_cast<int64_t>(chunks) * a.D;  // from one of a group's heads to its next
     const int64_t items = static_cast<int64_t>(a.B) * a.T * chunks;
     const int64_t step = static_cast<int64_t>(k ? gridDim.x - q_blocks : q_blocks) * GROUPS;
     const Part w = part_of<V, CONTIG>(a, threadIdx.x % L);
@@ -208,8 +209,8 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_kernel(NormRotateArgs a, i
             }
             if (a.table) turn<V, CONTIG>(c, s, 1.f, ya, yb);
             if (at.h + j * chunks < H) {
-                store_row<E, V>(y + j * chunks * a.D + w.a, ya, w.na);
-                store_row<E, V>(y + j * chunks * a.D + w.b, yb, w.nb);
+                store_row<E, V>(y + j * far + w.a, ya, w.na);
+                store_row<E, V>(y + j * far + w.b, yb, w.nb);
             }
         }
     }
@@ -225,6 +226,7 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_bwd_kernel(NormRotateArgs 
     const float nan = __uint_as_float(0x7fc00000u);
     const bool k = static_cast<int>(blockIdx.x) >= q_blocks;
     const int H = a.H[k], chunks = (H + NH - 1) / NH;
+    const int64_t far = static_cast<int64_t>(chunks) * a.D;  // from one of a group's heads to its next
     const int64_t items = static_cast<int64_t>(a.B) * a.T * chunks;
     const int64_t step = static_cast<int64_t>(k ? gridDim.x - q_blocks : q_blocks) * GROUPS;
     const Part w = part_of<V, CONTIG>(a, threadIdx.x % L);
@@ -243,8 +245,8 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_bwd_kernel(NormRotateArgs 
             const bool there = at.h + j * chunks < H, any = there && a.gy[k];
             xa[j].load(x + j * chunks * a.sh[k] + w.a, there ? w.na : 0);
             xb[j].load(x + j * chunks * a.sh[k] + w.b, there ? w.nb : 0);
-            za[j].load(gz + j * chunks * a.D + w.a, any ? w.na : 0);
-            zb[j].load(gz + j * chunks * a.D + w.b, any ? w.nb : 0);
+            za[j].load(gz + j * far + w.a, any ? w.na : 0);
+            zb[j].load(gz + j * far + w.b, any ? w.nb : 0);
         }
         float c[V], s[V];
         const bool known = !a.table || load_angles<V>(a, w, at.b, at.t, c, s);
@@ -284,8 +286,8 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_bwd_kernel(NormRotateArgs 
                 yb[e] = fmaf(xb[j][e] * scale, -dot, yb[e]) * scale;
             }
             if (at.h + j * chunks < H) {
-                store_row<E, V>(gx + j * chunks * a.D + w.a, ya, w.na);
-                store_row<E, V>(gx + j * chunks * a.D + w.b, yb, w.nb);
+                store_row<E, V>(gx + j * far + w.a, ya, w.na);
+                store_row<E, V>(gx + j * far + w.b, yb, w.nb);
             }
         }
     }
