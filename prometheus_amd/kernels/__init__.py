@@ -211,6 +211,22 @@ def _once(backward):
     return run
 
 
+def _layout(tensors) -> list:
+    """Each tensor's device, type, shape and strides (None for None)."""
+    return [None if t is None else (t.get_device(), t.dtype, t.shape, t.stride()) for t in tensors]
+
+
+def _as_saved(tensors, layout) -> list:
+    """What a backward saved, with autograd's hooks having handed it back otherwise than ``layout``: on
+    the device and in the type it was saved with again, in any strides; another shape is refused."""
+    back = []
+    for t, like in zip(tensors, layout):
+        if t is not None and t.shape != like[2]:
+            raise KernelError(f"a saved tensor of shape {tuple(like[2])} came back as {tuple(t.shape)}")
+        back.append(t if t is None else t.to(device=torch.device("cuda", like[0]), dtype=like[1]))
+    return back
+
+
 _HERE = contextlib.nullcontext()
 
 

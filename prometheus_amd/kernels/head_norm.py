@@ -195,7 +195,7 @@ class _NormRotate(torch.autograd.Function):
         tensors = plan.tensors()
         ctx.save_for_backward(*tensors)
         ctx.call, ctx.options = plan.call, (norm, eps, interleaved)
-        ctx.shared, ctx.strides = plan.shared, [None if t is None else t.stride() for t in tensors]
+        ctx.shared, ctx.layout = plan.shared, _k._layout(tensors)
         ctx.set_materialize_grads(False)  # a missing gradient is None, not a tensor of zeros
         # (the type and device of each input's gradient, where it is not as the backward gives it)
         as_given = q is plan.q and k is plan.k and all(
@@ -209,13 +209,13 @@ class _NormRotate(torch.autograd.Function):
     def backward(ctx, gq, gk):
         tensors, need = ctx.saved_tensors, ctx.needs_input_grad
         want = (need[2], need[3])
-        if [None if t is None else t.stride() for t in tensors] == ctx.strides:
+        if _k._layout(tensors) == ctx.layout:
             call = ctx.call
             with _k._on(call.device):
                 grads = _launch_bwd(call.device, tensors, ctx.shared, call.dev(gq), call.dev(gk), want)
         else:  # (saved-tensor hooks may hand back another layout)
-            q, k, table, pos, wq, wk = tensors
-            grads = _backward(_NormRotateResidual(q, k, table, pos, wq, wk, *ctx.options), (gq, gk), want)
+            res = _NormRotateResidual(*_k._as_saved(tensors, ctx.layout), *ctx.options)
+            grads = _backward(res, (gq, gk), want)
         if ctx.like is not None:
             grads = [t if t is None or like is None else t.to(device=like[1], dtype=like[0])
                      for t, like in zip(grads, ctx.like)]

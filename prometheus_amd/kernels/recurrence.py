@@ -129,6 +129,7 @@ class _LinearRecurrence(torch.autograd.Function):
     def forward(ctx, x, g, state, out_dtype):
         call, xd, gd, kept, h, s = _forward(x, g, state, out_dtype, keep=True)
         ctx.save_for_backward(xd, gd, kept)
+        ctx.layout = _k._layout((xd, gd, kept))
         ctx.call, ctx.h_dtype = call, h.dtype
         ctx.set_materialize_grads(False)  # a missing gradient is None, not a tensor of zeros
         # (the type and device of each input's gradient, where it is not as the backward gives it)
@@ -141,12 +142,12 @@ class _LinearRecurrence(torch.autograd.Function):
     @staticmethod
     @_k._once
     def backward(ctx, gh, gs):
-        xd, gd, kept = ctx.saved_tensors
-        # (saved-tensor hooks may hand back another layout, but the same shapes)
-        call = ctx.call
+        call, (xd, gd, kept) = ctx.call, ctx.saved_tensors
         with _k._on(call.device):
-            grads = _launch_bwd(call, _rows(call, xd, xd.dtype), _rows(call, gd, gd.dtype), call.dev(kept),
-                                call.dev(gh), call.dev(gs), ctx.h_dtype)
+            if _k._layout((xd, gd, kept)) != ctx.layout:  # (saved-tensor hooks may hand back another)
+                xd, gd, kept = _k._as_saved((xd, gd, kept), ctx.layout)
+                xd, gd, kept = _rows(call, xd, xd.dtype), _rows(call, gd, gd.dtype), call.dev(kept)
+            grads = _launch_bwd(call, xd, gd, kept, call.dev(gh), call.dev(gs), ctx.h_dtype)
         if ctx.like is not None:
             grads = [t if like is None else t.to(device=like[1], dtype=like[0]) for t, like in zip(grads, ctx.like)]
         x, g, state, _ = ctx.needs_input_grad

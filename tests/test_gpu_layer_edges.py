@@ -27,3 +27,42 @@ def test_the_most_heads():
         (want, _), res = kernels.norm_rotate_fwd(part, k)
         assert torch.equal(zq[:, a:a + cut], want), a
         assert torch.equal(gq[:, a:a + cut], kernels.norm_rotate_bwd(res, (want, None))[0]), a
+
+
+def _recurrence_step():
+    x, g = torch.randn(2, 300, 24, device="cuda").to(BF16), (-torch.rand(2, 300, 24, device="cuda")).to(BF16)
+    return kernels.linear_recurrence, [x, g, torch.randn(2, 24, device="cuda")]
+
+
+def _heads_step():
+    q, k = (torch.randn(2, 9, h, 64, device="cuda").to(BF16) for h in (4, 2))
+    table = kernels.rotation_table(9, 32)
+    w = 1 + 0.1 * torch.randn(64, device="cuda")
+    return lambda q, k, w: kernels.norm_rotate(q, k, table, torch.arange(9, device="cuda"), q_weight=w), [q, k, w]
+
+
+@pytest.mark.parametrize("step", [_recurrence_step, _heads_step])
+def test_saved_tensors_that_come_back_changed(step):
+    """On the host, in a wider type, with other strides, with fewer rows."""
+    f, args = step()
+    args = [t.requires_grad_(True) for t in args]
+
+    def grads(pack, unpack):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            a, b = f(*args)
+        return torch.autograd.grad(a.float().square().sum() + b.float().sum(), args)
+
+    def same(t):
+        return t
+
+    def wide(t):
+        return t.double() if t.is_floating_point() else t.int()
+
+    def turned(t):
+        return t.transpose(0, -1).contiguous().transpose(0, -1)
+
+    want = grads(same, same)
+    for pack, unpack in ((torch.Tensor.cpu, same), (wide, same), (turned, same), (lambda t: turned(wide(t)).cpu(), same)):
+        assert all(torch.equal(a, b) for a, b in zip(grads(pack, unpack), want))
+    with pytest.raises(kernels.KernelError):
+        grads(same, lambda t: t[:-1])
