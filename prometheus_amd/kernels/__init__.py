@@ -466,6 +466,14 @@ def _varlen_flag(device) -> torch.Tensor:
     return flag
 
 
+def _offsets_i32(cu: torch.Tensor, total: int) -> torch.Tensor:
+    """GPU offsets as contiguous int32. Those of a wider type are clamped first, to where the device's
+    check still finds them: an offset past int32 must not come back into range."""
+    if cu.dtype != torch.int32:
+        cu = cu.clamp(-1, min(total + 1, 2**31 - 1)).to(torch.int32)
+    return cu.contiguous()
+
+
 def check_varlen(device=None) -> None:
     """Surface what the device-side checks of ``chunked_delta_rule_varlen`` found.
 
@@ -557,7 +565,7 @@ def chunked_delta_rule_varlen(q, k, v, beta, cu_seqlens, state=None, config=None
         bd = call.dev(beta, torch.float32).reshape(n_tok, heads)
         sd = call.dev(state, torch.float32)
         if cu_on_dev:
-            cu = cu_seqlens.to(torch.int32).contiguous()
+            cu = _offsets_i32(cu_seqlens, n_tok)
             _native.check(_native.lib().pm_varlen_check(_ptr(cu), n_seqs, n_tok,
                                                         _varlen_flag(call.device).data_ptr(),
                                                         _stream(call.device)))

@@ -228,7 +228,7 @@ def _offsets(call, cu, n_seqs, n_tok, chan):
     the launch is to set (a call that launches nothing is checked here)."""
     if isinstance(cu, np.ndarray):
         return torch.from_numpy(cu.astype(np.int32)).to(call.device), None
-    cu, flag = cu.to(torch.int32).contiguous(), _k._varlen_flag(call.device)
+    cu, flag = _k._offsets_i32(cu, n_tok), _k._varlen_flag(call.device)
     if n_seqs == 0 or chan == 0:
         _native.check(_native.lib().pm_varlen_check(cu.data_ptr(), n_seqs, n_tok, flag.data_ptr(),
                                                     _k._stream(call.device)))

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from prometheus_amd import kernels
+from prometheus_amd import kernels, serving
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,30 @@ def test_saved_tensors_that_come_back_changed(step):
         assert all(torch.equal(a, b) for a, b in zip(grads(pack, unpack), want))
     with pytest.raises(kernels.KernelError):
         grads(same, lambda t: t[:-1])
+
+
+@pytest.mark.parametrize("cu", [[0, 2**32 + 100, 400], [2**32, 100, 400], [0, 100, 2**32 + 400], [0, 100 - 2**32, 400]])
+def test_wide_offsets_do_not_come_back_into_range(cu):
+    """64-bit offsets on the GPU whose lower halves are good ones."""
+    N, C = 400, 16
+    x, g = torch.randn(N, C, device="cuda"), -torch.rand(N, C, device="cuda")
+    offsets = torch.tensor(cu, device="cuda")
+    kernels.linear_recurrence_varlen(x, g, offsets)
+    with pytest.raises(kernels.KernelError):
+        kernels.check_varlen()
+    cache = serving.RecurrenceStateCache(1, 2, C)
+    cache.prefill(0, torch.tensor([0, 1], device="cuda"), x, g, offsets)
+    with pytest.raises(kernels.KernelError):
+        kernels.check_varlen()
+    kernels.linear_recurrence_varlen(x[:0], g[:0], offsets[:1])  # (launches nothing: checked apart)
+    if cu[0]:
+        with pytest.raises(kernels.KernelError):
+            kernels.check_varlen()
+    q, k, v = (torch.randn(N, 1, 64, device="cuda") for _ in range(3))
+    kernels.chunked_delta_rule_varlen(q, k, v, torch.rand(N, 1, device="cuda"), offsets)
+    with pytest.raises(kernels.KernelError):
+        kernels.check_varlen()
+    good = torch.tensor([0, 100, 400], device="cuda")
+    want = kernels.linear_recurrence_varlen(x, g, good.int())
+    assert all(torch.equal(a, b) for a, b in zip(kernels.linear_recurrence_varlen(x, g, good), want))
+    kernels.check_varlen()
