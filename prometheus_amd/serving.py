@@ -243,7 +243,7 @@ class RecurrenceStateCache(_SlotPool):
         if n_seqs != n:
             raise ValueError(f"{n} slots for {n_seqs} prompts")
         self._check_cuda(x, g)
-        call = kernels._Call(x, g)
+        call = kernels._Call(x, g, cu_seqlens)
         xt, gt = recurrence._types(x, g)
         with torch.cuda.device(call.device):
             if isinstance(slots, list):
