@@ -264,7 +264,9 @@ def linear_recurrence_varlen(x, g, cu_seqlens, state=None, *, out_dtype=None):
 def linear_recurrence_step(x, g, state, *, out_dtype=None):
     """One token: ``state = exp(g) state + x`` for (B, C) ``x`` and ``g``, ``state`` (B, C) fp32
     updated in place as in ``delta_rule_step``; returns h (B, C), the new state in fp32 or
-    ``out_dtype``."""
+    ``out_dtype``. Forward only, as ``linear_recurrence_varlen``."""
+    if _k._wants_grad(x, g, state):
+        raise _k.KernelError("linear_recurrence_step is forward only: call it under torch.no_grad()")
     batch, chan = _check(x, g, state, 2)
     if state is None:
         raise _k.KernelError(f"state shape None != {(batch, chan)}")

@@ -269,6 +269,8 @@ class RecurrenceStateCache(_SlotPool):
         ``out_dtype``). Slots outside ``[0, n_slots)`` are padding: no state is touched and their
         rows are zero. Allocation-free with ``out=`` and x and g in a type the kernel takes."""
         self._check_layer(layer)
+        if kernels._wants_grad(x, g):
+            raise ValueError("decode is forward only: call it under torch.no_grad()")
         self._check_cuda(x, g, slots)
         if slots.dim() != 1 or slots.dtype != torch.int32 or not slots.is_contiguous():
             raise ValueError("slots must be a contiguous int32 tensor of shape (B,)")

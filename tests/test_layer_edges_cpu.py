@@ -26,3 +26,20 @@ def test_cache_prefill_looks_at_the_offsets_device(monkeypatch):
     with pytest.raises(Compared):
         cache.prefill(0, [0, 1], x, x, cu)
     assert any(t is cu for t in seen)
+
+
+@pytest.mark.parametrize("who", [0, 1, 2])
+def test_steps_do_not_drop_gradients(who):
+    """A single token is forward only: while autograd records it is refused, not returned without a
+    graph. The states stay as they were."""
+    args = [torch.ones(2, 4), torch.zeros(2, 4), torch.ones(2, 4)]
+    args[who].requires_grad_(True)
+    with pytest.raises(kernels.KernelError, match="forward only"):
+        kernels.linear_recurrence_step(*args)
+    assert torch.equal(args[2], torch.ones(2, 4))
+    if who < 2:
+        cache = serving.RecurrenceStateCache(1, 2, 4, device="cpu")
+        with pytest.raises(ValueError, match="forward only"):
+            cache.decode(0, torch.zeros(2, dtype=torch.int32), *args[:2])
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # (the next check)
+            cache.decode(0, torch.zeros(2, dtype=torch.int32), *args[:2])
