@@ -238,8 +238,11 @@ def norm_rotate(q, k, table=None, positions=None, *, norm="l2", q_weight=None, k
     back, a token outside the table comes out as NaN and nothing outside the table is read.
 
     bf16 q and k give bf16 results, anything else fp32; arithmetic is fp32 with one rounding at
-    the end. Differentiable in q, k and the weights.
+    the end. Differentiable in q, k and the weights; a table that requires grad is refused while
+    autograd records.
     """
+    if _k._wants_grad(table):
+        raise _k.KernelError("norm_rotate has no gradient of the table: detach it")
     if _k._wants_grad(q, k, q_weight, k_weight):
         return _NormRotate.apply(q, k, q_weight, k_weight, table, positions, norm, eps, interleaved)
     plan, qo, ko = _forward(q, k, table, positions, norm, q_weight, k_weight, eps, interleaved)

@@ -43,3 +43,10 @@ def test_steps_do_not_drop_gradients(who):
             cache.decode(0, torch.zeros(2, dtype=torch.int32), *args[:2])
         with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # (the next check)
             cache.decode(0, torch.zeros(2, dtype=torch.int32), *args[:2])
+
+
+def test_a_table_s_gradient_is_not_dropped():
+    q = torch.ones(1, 3, 2, 4)
+    table = kernels.rotation_table(3, 4, device="cpu").requires_grad_(True)
+    with pytest.raises(kernels.KernelError, match="table"):
+        kernels.norm_rotate(q, q, table)
