@@ -518,6 +518,7 @@ int pm_linear_recurrence_step(float* s_inout, const int32_t* slots, int n_slots,
  *   q_out, k_out  contiguous, in dtype
  *   *_weight   (D) in w_dtype, or NULL
  *   table      fp32 (P, R): R / 2 cosines, then R / 2 sines, for each position
+ *              (not read, and may be NULL, where P is 0)
  *   positions  int32 (or int64) (B, T) with batch stride pos_sb (0: one row for
  *              all), tokens contiguous; NULL: 0, 1, 2, ...  A token whose
  *              position is outside [0, P) comes out as NaN (and its gradients,

@@ -191,7 +191,7 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_kernel(NormRotateArgs a, i
             xb[j].load(x + j * chunks * a.sh[k] + w.b, there ? w.nb : 0);
         }
         float c[V], s[V];
-        const bool known = !a.table || load_angles<V>(a, w, at.b, at.t, c, s);
+        const bool known = !a.R || load_angles<V>(a, w, at.b, at.t, c, s);
         E* y = static_cast<E*>(a.y[k]) + ((static_cast<int64_t>(at.b) * a.T + at.t) * H + at.h) * a.D;
 #pragma unroll
         for (int j = 0; j < NH; ++j) {
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_kernel(NormRotateArgs a, i
 #pragma unroll
                 for (int e = 0; e < V; ++e) ya[e] *= wa[e], yb[e] *= wb[e];
             }
-            if (a.table) turn<V, CONTIG>(c, s, 1.f, ya, yb);
+            if (a.R) turn<V, CONTIG>(c, s, 1.f, ya, yb);
             if (at.h + j * chunks < H) {
                 store_row<E, V>(y + j * far + w.a, ya, w.na);
                 store_row<E, V>(y + j * far + w.b, yb, w.nb);
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_bwd_kernel(NormRotateArgs 
             zb[j].load(gz + j * far + w.b, any ? w.nb : 0);
         }
         float c[V], s[V];
-        const bool known = !a.table || load_angles<V>(a, w, at.b, at.t, c, s);
+        const bool known = !a.R || load_angles<V>(a, w, at.b, at.t, c, s);
         E* gx = static_cast<E*>(a.gx[k]) + out;
 #pragma unroll
         for (int j = 0; j < NH; ++j) {
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_bwd_kernel(NormRotateArgs 
                 ss = fmaf(xa[j][e], xa[j][e], ss), ss = fmaf(xb[j][e], xb[j][e], ss);
                 ya[e] = za[j][e], yb[e] = zb[j][e];
             }
-            if (a.table) turn<V, CONTIG>(c, s, -1.f, ya, yb);
+            if (a.R) turn<V, CONTIG>(c, s, -1.f, ya, yb);
             bool clipped;
             float scale = row_scale(a, group_sum<L>(ss), clipped);
             if (!known) scale = nan;
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const float* part, in
 // f(null pointer of E, L, contig, NH) for a call
 template <typename E, typename F>
 static void by_shape(const NormRotateArgs& a, int nh, F f) {
-    const bool contig = a.interleaved || !a.table;
+    const bool contig = a.interleaved || !a.R;
     const int l = lanes_of(a.D, a.R, 16 / sizeof(E), contig);
     E* e = nullptr;
     auto with_lanes = [&](auto lanes) {
@@ -373,7 +373,7 @@ static int side_blocks(const NormRotateArgs& a, int side, int lanes, int nh, int
 
 template <typename E>
 static hipError_t forward(const NormRotateArgs& a, hipStream_t st) {
-    const int lanes = lanes_of(a.D, a.R, 16 / sizeof(E), a.interleaved || !a.table), nh = heads_of(a, lanes);
+    const int lanes = lanes_of(a.D, a.R, 16 / sizeof(E), a.interleaved || !a.R), nh = heads_of(a, lanes);
     const int q = side_blocks(a, 0, lanes, nh, 1 << 20), k = side_blocks(a, 1, lanes, nh, 1 << 20);
     by_shape<E>(a, nh, [&](auto e, auto l, auto contig, auto n) {
         hipLaunchKernelGGL((norm_rotate_kernel<std::remove_pointer_t<decltype(e)>, l(), contig(), n()>), dim3(q + k),
@@ -399,7 +399,7 @@ size_t norm_rotate_bwd_ws_bytes(int B, int T, int Hq, int Hk, int D) {
 template <typename E>
 static hipError_t backward(const NormRotateArgs& a, hipStream_t st) {
     const bool sums = a.gw[0] || a.gw[1];
-    const int lanes = lanes_of(a.D, a.R, 16 / sizeof(E), a.interleaved || !a.table), nh = heads_of(a, lanes);
+    const int lanes = lanes_of(a.D, a.R, 16 / sizeof(E), a.interleaved || !a.R), nh = heads_of(a, lanes);
     const int share = q_share(a.H[0], a.H[1]);
     const int q = side_blocks(a, 0, lanes, nh, sums ? share : 1 << 20);
     const int k = side_blocks(a, 1, lanes, nh, sums ? kBwdBlocks - share : 1 << 20);

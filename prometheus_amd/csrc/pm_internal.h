@@ -323,7 +323,7 @@ struct NormRotateArgs {
     void* y[2];
     int H[2];
     int64_t sb[2], st[2], sh[2];  // batch, token and head strides of x
-    const float* table;           // nullable: (P, R), R / 2 cosines, then R / 2 sines
+    const float* table;           // (P, R), R / 2 cosines, then R / 2 sines; not read where R or P is 0
     const void* pos;              // nullable: 0, 1, 2, ... in every batch row
     int64_t pos_sb;               // 0: one row of positions for every batch row
     int B, T, D, R, P;

@@ -173,7 +173,7 @@ int norm_rotate_args(pm::NormRotateArgs& a, const void* q, const void* k, const 
     const int64_t heads = static_cast<int64_t>(Hq) + Hk;
     if (heads > (1 << 24) || static_cast<int64_t>(B) * T > kMaxElems || static_cast<int64_t>(B) * T * heads > kMaxElems)
         return fail(PM_E_SHAPE, "problem too large");
-    if (R && !table) return fail(PM_E_NULL, "table is NULL");
+    if (R && P > 0 && !table) return fail(PM_E_NULL, "table is NULL");  // (without rows there is nothing to read)
     if (R && P < 0) return fail(PM_E_SHAPE, "P must be >= 0 (got %d)", P);
     if (!strides) return fail(PM_E_NULL, "strides is NULL");
     for (int i = 0; i < 6; ++i)

@@ -93,3 +93,20 @@ def test_wide_offsets_do_not_come_back_into_range(cu):
     want = kernels.linear_recurrence_varlen(x, g, good.int())
     assert all(torch.equal(a, b) for a, b in zip(kernels.linear_recurrence_varlen(x, g, good), want))
     kernels.check_varlen()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_a_table_without_rows(interleaved):
+    """No tokens need none of it; a token at any position is outside it, and comes out as NaN."""
+    table, w = kernels.rotation_table(0, 64), torch.ones(64, device="cuda")
+    assert table.shape == (0, 64)
+    q, k = torch.empty(2, 0, 4, 64, device="cuda"), torch.empty(2, 0, 2, 64, device="cuda")
+    (zq, zk), res = kernels.norm_rotate_fwd(q, k, table, q_weight=w, interleaved=interleaved)
+    gq, gk, gw, _ = kernels.norm_rotate_bwd(res, (zq, zk))
+    assert zq.shape == gq.shape == q.shape and zk.shape == gk.shape == k.shape and not gw.any()
+    q, k = torch.randn(3, 4, 64, device="cuda"), torch.randn(3, 2, 64, device="cuda")
+    outs, res = kernels.norm_rotate_fwd(q, k, table, torch.tensor([0, -1, 5], device="cuda"), interleaved=interleaved)
+    grads = kernels.norm_rotate_bwd(res, outs)[:2]
+    assert all(torch.isnan(t).all() for t in (*outs, *grads))
+    with pytest.raises(kernels.KernelError):
+        kernels.norm_rotate(q, k, table, [0, 1, 2], interleaved=interleaved)

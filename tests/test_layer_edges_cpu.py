@@ -2,10 +2,12 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
-from prometheus_amd import kernels, serving
+from prometheus_amd import _native, kernels, serving
 
 
 def test_cache_prefill_looks_at_the_offsets_device(monkeypatch):
@@ -50,3 +52,12 @@ def test_a_table_s_gradient_is_not_dropped():
     table = kernels.rotation_table(3, 4, device="cpu").requires_grad_(True)
     with pytest.raises(kernels.KernelError, match="table"):
         kernels.norm_rotate(q, q, table)
+
+
+def test_a_table_without_rows_is_no_null_pointer():
+    L, p = _native.lib(), ctypes.c_void_p(16)  # (never dereferenced: there are no tokens)
+    strides = (ctypes.c_int64 * 6)(0, 256, 64, 0, 256, 64)
+    for rows, want in ((0, 0), (1, _native.E_NULL)):
+        shared = (2, 0, 4, 4, 64, 64, rows, strides, 0, 0, 0, 1e-6, 0, 0, 0)
+        assert L.pm_norm_rotate(p, p, None, None, None, None, p, p, *shared, None) == want
+        assert L.pm_norm_rotate_bwd(p, p, None, None, None, None, p, p, p, p, None, None, *shared, None, 0, None) == want
