@@ -35,6 +35,7 @@ from typing import Any
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from prometheus_amd import _native
 
@@ -274,6 +275,12 @@ def _forward(q, k, v, beta, state, chunk: int, out_dtype):
 
 
 def _wants_grad(*xs) -> bool:
+    """Whether autograd records a call of ``xs``. Tangents (forward mode) are refused: the kernels
+    have none, and the results would come back without."""
+    if forward_ad._current_level >= 0:
+        for x in xs:
+            if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+                raise KernelError("forward-mode derivatives are not supported: pass tensors without tangents")
     if torch.is_grad_enabled():
         for x in xs:
             if isinstance(x, torch.Tensor) and x.requires_grad:

@@ -6,6 +6,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from prometheus_amd import _native, kernels, serving
 
@@ -61,3 +62,30 @@ def test_a_table_without_rows_is_no_null_pointer():
         shared = (2, 0, 4, 4, 64, 64, rows, strides, 0, 0, 0, 1e-6, 0, 0, 0)
         assert L.pm_norm_rotate(p, p, None, None, None, None, p, p, *shared, None) == want
         assert L.pm_norm_rotate_bwd(p, p, None, None, None, None, p, p, p, p, None, None, *shared, None, 0, None) == want
+
+
+def test_tangents_are_refused():
+    """A dual tensor's tangent is not passed by, with and without reverse mode beside it."""
+    x, q, s = torch.zeros(1, 3, 4), torch.ones(1, 3, 2, 4), torch.zeros(1, 4)
+    cache = serving.RecurrenceStateCache(1, 1, 4, device="cpu")
+    beta, one = torch.ones(1, 3, 2), torch.zeros(1, dtype=torch.int32)
+    with forward_ad.dual_level():
+        dual, heads = forward_ad.make_dual(x, x), forward_ad.make_dual(q, q)
+        calls = [
+            lambda: kernels.linear_recurrence(dual, x),
+            lambda: kernels.linear_recurrence(x, dual),
+            lambda: kernels.linear_recurrence(x, x, forward_ad.make_dual(s, s)),
+            lambda: kernels.linear_recurrence_varlen(dual, x, [0, 3]),
+            lambda: kernels.linear_recurrence_step(dual[:, 0], x[:, 0], s),
+            lambda: cache.prefill(0, [0], dual, x),
+            lambda: cache.decode(0, one, dual[:, 0], x[:, 0]),
+            lambda: kernels.norm_rotate(q, heads),
+            lambda: kernels.norm_rotate(q, q, q_weight=heads[0, 0, 0]),
+            lambda: kernels.chunked_delta_rule(q, heads, q, beta),
+        ]
+        for i, call in enumerate(calls):
+            with pytest.raises(kernels.KernelError, match="forward-mode"):
+                call()
+                pytest.fail(f"call {i} was not refused")
+            with torch.no_grad(), pytest.raises(kernels.KernelError, match="forward-mode"):
+                call()
