@@ -192,12 +192,13 @@ class LinearStateCache(_SlotPool):
             out = torch.empty(want, dtype=torch.float32, device=q.device)
         elif tuple(out.shape) != want or out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError(f"out must be contiguous fp32 {want}")
-        rc = _native.lib().pm_delta_step_slots(
-            self.pool[layer].data_ptr(), slots.data_ptr(), self.n_slots, q.data_ptr(), k.data_ptr(),
-            v.data_ptr(), beta.data_ptr(), out.data_ptr(), b, self.heads, self.dim,
-            _native.DTYPE_BF16 if q.dtype == torch.bfloat16 else _native.DTYPE_F32,
-            torch.cuda.current_stream(q.device).cuda_stream,
-        )
+        with kernels._on(q.device):
+            rc = _native.lib().pm_delta_step_slots(
+                self.pool[layer].data_ptr(), slots.data_ptr(), self.n_slots, q.data_ptr(), k.data_ptr(),
+                v.data_ptr(), beta.data_ptr(), out.data_ptr(), b, self.heads, self.dim,
+                _native.DTYPE_BF16 if q.dtype == torch.bfloat16 else _native.DTYPE_F32,
+                kernels._stream(q.device),
+            )
         _native.check(rc)
         return out
 
@@ -286,6 +287,7 @@ class RecurrenceStateCache(_SlotPool):
         elif (tuple(out.shape) != want or out.dtype not in (torch.float32, torch.bfloat16)
               or not out.is_contiguous() or out.device != x.device):
             raise ValueError(f"out must be contiguous fp32 or bf16 {want} on the pool's device")
-        recurrence._step(self._pool.data_ptr() + layer * self._pool.stride(0) * 4, slots, self.n_slots, x, g, out,
-                         kernels._stream(x.device))
+        with kernels._on(x.device):
+            recurrence._step(self._pool.data_ptr() + layer * self._pool.stride(0) * 4, slots, self.n_slots, x, g, out,
+                             kernels._stream(x.device))
         return out

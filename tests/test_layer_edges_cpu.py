@@ -2,7 +2,9 @@
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import types
 
 import pytest
 import torch
@@ -89,3 +91,35 @@ def test_tangents_are_refused():
                 pytest.fail(f"call {i} was not refused")
             with torch.no_grad(), pytest.raises(kernels.KernelError, match="forward-mode"):
                 call()
+
+
+def test_decode_runs_on_the_pool_s_device(monkeypatch):
+    """Both caches launch with the pool's device as the current one, whichever is current outside."""
+    inside = []
+
+    @contextlib.contextmanager
+    def on(device):
+        inside.append(device)
+        yield
+        inside.pop()
+
+    launched = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: launched.append((name, list(inside))) or 0
+
+    monkeypatch.setattr(kernels, "_on", on)
+    monkeypatch.setattr(kernels, "_stream", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=0))
+    monkeypatch.setattr(_native, "lib", Library)
+    slots = torch.zeros(2, dtype=torch.int32)
+    vectors = serving.RecurrenceStateCache(1, 2, 4, device="cpu")
+    matrices = serving.LinearStateCache(1, 2, 3, 4, device="cpu")
+    for cache in (vectors, matrices):
+        monkeypatch.setattr(cache, "_check_cuda", lambda *tensors: None)
+    vectors.decode(0, slots, torch.zeros(2, 4), torch.zeros(2, 4))
+    x = torch.zeros(2, 3, 4)
+    matrices.decode(0, slots, x, x, x, torch.zeros(2, 3))
+    cpu = torch.device("cpu")
+    assert launched == [("pm_linear_recurrence_step", [cpu]), ("pm_delta_step_slots", [cpu])]
