@@ -457,7 +457,10 @@ int pm_delta_bwd_noalloc(const void* q, const void* k, const void* v, const floa
  *          before each span of tokens, for the backward (fixed length only).
  *   cu_seqlens  as in pm_delta_fwd_varlen (clamped into [0, T]; h of tokens
  *          that no sequence covers is unspecified).
- * Sums and states are fp32 whatever the types; h is rounded once.
+ * Sums and states are fp32 whatever the types; h is rounded once.  A gate below
+ * 2^-126 (g < -87.3) counts as closed, as one of g = -inf: it leaves nothing of
+ * a finite state and makes NaN of an infinite one.  Through open gates, however
+ * many, an infinite state stays infinite.
  * workspace: pm_linear_recurrence_workspace_bytes (0 where none is needed).
  */
 #define PM_RECURRENCE_SPAN 128

@@ -88,6 +88,14 @@ __device__ __forceinline__ bool missing(uint64_t v) { return static_cast<uint32_
 __device__ __forceinline__ float low(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
 __device__ __forceinline__ float high(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
 
+// a b of factors of maps, which rounds to zero only where one of them is zero (a gate that is closed):
+// an infinite state stays one through however many gates, as it does token by token, and 0 x inf comes
+// of closed gates alone. (As bits: a factor is at least +0, but for a start's, of which the sign alone
+// counts. To a finite state's share this adds at most 2^-149 of the state.)
+__device__ __forceinline__ float product(float a, float b) {
+    return __uint_as_float(max(__float_as_uint(a * b), min(min(__float_as_uint(a), __float_as_uint(b)), 1u)));
+}
+
 // s -> A s + H. An A whose sign bit is set (PACKED only) is a map that a sequence starts in: its H
 // is the state whatever came before, infinities and NaN included.
 template <bool PACKED>
@@ -98,7 +106,7 @@ struct Map {
     __device__ __forceinline__ void token(float a, float x) { H = fmaf(a, H, x), A *= a; }
     __device__ __forceinline__ void then(const Map& m) {
         H = m.of(H);
-        A = m.anew() ? m.A : A * m.A;
+        A = m.anew() ? m.A : product(A, m.A);
     }
     __device__ __forceinline__ float of(float s) const { return anew() ? H : fmaf(A, s, H); }
     __device__ __forceinline__ uint64_t word() const {
@@ -108,6 +116,24 @@ struct Map {
     static __device__ __forceinline__ Map read(uint64_t v) { return {high(v), low(v)}; }
 };
 
+// A thread's factors m[v].A, as they are in p, after its K tokens with the gates gate(r, v): where plain
+// products have rounded to zero, which they hardly ever do, p gets what `product` says.
+template <int K, int V, bool PACKED, typename F>
+__device__ __forceinline__ void keep_open(float* p, const Map<PACKED> (&m)[V], F gate) {
+    uint32_t least = ~0u;
+#pragma unroll
+    for (int v = 0; v < V; ++v) least = min(least, __float_as_uint(m[v].A));
+    if (!__any(least == 0)) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        bool open = __float_as_uint(p[v]) == 0;  // (not a start's -0)
+#pragma unroll
+        for (int r = 0; r < K; ++r) open = open && gate(r, v) != 0.f;
+        if (open) p[v] = product(0x1p-100f, 0x1p-100f);
+    }
+}
+
+// (the hardware's exponential has no values below 2^-126: such a gate is zero)
 __device__ __forceinline__ float gate(float g) { return __builtin_amdgcn_exp2f(g * 1.44269504088896341f); }
 
 __host__ __device__ inline int64_t spans_of(int T) { return (static_cast<int64_t>(T) + kRecSpan - 1) / kRecSpan; }
@@ -389,6 +415,7 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_kernel(Recurr
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) sA[tl][lc * V + v] = m[v].A, sH[tl][lc * V + v] = m[v].H;
+        keep_open<K>(&sA[tl][lc * V], m, [&](int r, int v) { return av[r][v]; });
         __syncthreads();
 
         if (PACKED && tid < TL) marks[tid] = 0;  // (read above; the next tile's come after a barrier)
@@ -519,6 +546,7 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
             if constexpr (KEEP) return av[r][v];
             else return gate(gr[r][v]);
         };
+        M maps[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             M f{1.f, 0.f};  // the tokens' map of h
@@ -528,7 +556,9 @@ __global__ __launch_bounds__(S::threads, S::waves) void recurrence_bwd_kernel(Re
 #pragma unroll
             for (int r = K - 1; r >= 0; --r) w = gate_at(r, v) * (w + hr[r][v]);
             sA[tl][lc * V + v] = f.A, sF[tl][lc * V + v] = f.H, sB[tl][lc * V + v] = w;
+            maps[v].A = f.A;
         }
+        keep_open<K>(&sA[tl][lc * V], maps, gate_at);
         __syncthreads();
 
         float A[PER], F[PER], B[PER];

@@ -160,7 +160,8 @@ def linear_recurrence(x, g, state=None, *, out_dtype=None):
     state: (batch, channels) fp32 initial state, zeros if None. Returns ``(h, next_state)``: h
     shaped like x (fp32 unless ``out_dtype`` asks for bf16), next_state (batch, channels) fp32.
     Gates at or below zero keep the state bounded; positive ones are accepted as long as the
-    products of a sequence's gates stay finite in fp32. Differentiable: when autograd records
+    products of a sequence's gates stay finite in fp32. A gate below 2^-126 (g < -87.3) counts as
+    closed: it leaves nothing of the state before (NaN of an infinite one). Differentiable: when autograd records
     and a torch input requires grad, the backward is ``linear_recurrence_bwd``.
     """
     if _k._wants_grad(x, g, state):

@@ -110,3 +110,55 @@ def test_a_table_without_rows(interleaved):
     assert all(torch.isnan(t).all() for t in (*outs, *grads))
     with pytest.raises(kernels.KernelError):
         kernels.norm_rotate(q, k, table, [0, 1, 2], interleaved=interleaved)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [1, 100, 256, 700, 9000, 20000])
+def test_an_infinite_state_passes_open_gates(T, dtype):
+    """Gates of exp(-2), whose products over a span are zero in fp32: what is infinite stays so, from
+    the initial state, from a token, packed, and back from the last gradient."""
+    C = 70
+    x, g = torch.randn(2, T, C, device="cuda").to(dtype), torch.full((2, T, C), -2.0, dtype=dtype, device="cuda")
+    g[:, :, 1::4] = -40.0  # (the products of a few tokens are)
+    s0 = torch.randn(2, C, device="cuda")
+    inf, at = torch.inf, T // 3
+    hit = torch.zeros(2, T, C, device="cuda")
+    s0[0, 5], s0[1, 8] = inf, -inf
+    x[1, at, 13], x[0, at, 16] = inf, -inf
+    hit[0, :, 5], hit[1, :, 8], hit[1, at:, 13], hit[0, at:, 16] = inf, -inf, inf, -inf
+    still = hit == 0
+    end = hit[:, -1] != 0
+
+    def check(h, s):
+        assert torch.equal(h[~still].float(), hit[~still]) and torch.isfinite(h[still]).all()
+        assert torch.equal(s[end], hit[:, -1][end]) and torch.isfinite(s[~end]).all()
+
+    (h, s), res = kernels.linear_recurrence_fwd(x, g, s0, out_dtype=dtype)
+    check(h, s)
+    cu = torch.tensor([0, T, 2 * T], device="cuda")
+    h, s = kernels.linear_recurrence_varlen(x.reshape(2 * T, C), g.reshape(2 * T, C), cu, s0, out_dtype=dtype)
+    check(h.reshape(2, T, C), s)
+    clean = torch.randn(2, T, C, device="cuda").to(dtype), torch.randn(2, C, device="cuda")
+    _, res = kernels.linear_recurrence_fwd(clean[0], g, clean[1], out_dtype=dtype)
+    gh, gs = torch.randn(2, T, C, device="cuda").to(dtype), torch.randn(2, C, device="cuda")
+    gs[0, 5], gh[1, at, 9] = inf, -inf
+    gx, gg, gs0 = kernels.linear_recurrence_bwd(res, (gh, gs))
+    hit = torch.zeros(2, T, C, device="cuda")
+    hit[0, :, 5], hit[1, :at + 1, 9] = inf, -inf
+    still = hit == 0
+    assert torch.equal(gx[~still].float(), hit[~still]) and torch.isfinite(gx[still]).all()
+    assert gs0[0, 5] == inf and gs0[1, 9] == -inf and torch.isfinite(gg[still]).all()
+    assert torch.isinf(gg[~still]).all()  # (h before each token is not zero here)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [40, 700, 9000])
+def test_a_closed_gate_leaves_nothing(T, dtype):
+    """exp(-inf) is zero, whatever its neighbours: a finite state before it is gone to the last bit."""
+    x, g = torch.zeros(1, T, 66, dtype=dtype, device="cuda"), torch.full((1, T, 66), -3.0, dtype=dtype, device="cuda")
+    g[0, T // 2] = -torch.inf
+    s0 = torch.full((1, 66), 1e38, device="cuda")
+    (h, s), res = kernels.linear_recurrence_fwd(x, g, s0, out_dtype=dtype)
+    assert not h[0, T // 2:].any() and not s.any() and h[0, :T // 2].float()[:10].all()
+    gx, _, gs0 = kernels.linear_recurrence_bwd(res, (None, s0))
+    assert not gx[0, :T // 2].any() and not gs0.any()
