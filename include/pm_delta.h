@@ -541,7 +541,8 @@ int pm_norm_rotate(const void* q, const void* k, const float* table, const void*
  * Its reverse mode: gq_out, gk_out (contiguous, dtype, NULL for zeros) to gq,
  * gk (contiguous, dtype) and, where asked for, the weights' gradients (D) fp32,
  * summed over all rows in an order that does not change from run to run
- * (they need the workspace; without them it may be NULL).
+ * (they need the workspace; without them it may be NULL).  A weight that is
+ * NULL has none: PM_E_NULL.
  */
 int pm_norm_rotate_bwd(const void* q, const void* k, const float* table, const void* positions,
                        const void* q_weight, const void* k_weight, const void* gq_out, const void* gk_out,

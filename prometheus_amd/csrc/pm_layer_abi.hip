@@ -258,6 +258,8 @@ int pm_norm_rotate_bwd(const void* q, const void* k, const float* table, const v
     if ((gq_weight || gk_weight) && (!workspace || ws_bytes < need || !aligned(workspace, 16)))
         return fail(PM_E_WORKSPACE, "the weights' gradients need a 16-byte aligned workspace of %zu bytes (got %zu)",
                     need, workspace ? ws_bytes : static_cast<size_t>(0));
+    if ((gq_weight && !q_weight) || (gk_weight && !k_weight))
+        return fail(PM_E_NULL, "a weight's gradient needs the weight");
     a.gy[0] = gq_out, a.gy[1] = gk_out;
     a.gx[0] = gq, a.gx[1] = gk;
     a.gw[0] = gq_weight, a.gw[1] = gk_weight;

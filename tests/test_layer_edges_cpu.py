@@ -123,3 +123,14 @@ def test_decode_runs_on_the_pool_s_device(monkeypatch):
     matrices.decode(0, slots, x, x, x, torch.zeros(2, 3))
     cpu = torch.device("cpu")
     assert launched == [("pm_linear_recurrence_step", [cpu]), ("pm_delta_step_slots", [cpu])]
+
+
+def test_a_weight_that_is_not_there_has_no_gradient():
+    """The C entry used to write zeros where a NULL weight's gradient was asked for."""
+    L, p = _native.lib(), ctypes.c_void_p(16)  # never dereferenced: validation fails first
+    strides = (ctypes.c_int64 * 6)(120, 24, 6, 30, 6, 6)
+    need = L.pm_norm_rotate_bwd_workspace_bytes(2, 5, 4, 1, 6)
+    for wq, wk, gwq, gwk in ((None, p, p, None), (p, None, None, p), (None, None, p, p)):
+        rc = L.pm_norm_rotate_bwd(p, p, None, None, wq, wk, p, p, p, p, gwq, gwk, 2, 5, 4, 1, 6, 0, 0, strides, 0, 0, 0,
+                                  1e-6, 0, 0, 0, p, need, None)
+        assert rc == _native.E_NULL and b"weight" in L.pm_last_error()
