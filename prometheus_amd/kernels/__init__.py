@@ -212,20 +212,14 @@ def _once(backward):
     return run
 
 
-def _layout(tensors) -> list:
-    """Each tensor's device, type, shape and strides (None for None)."""
-    return [None if t is None else (t.get_device(), t.dtype, t.shape, t.stride()) for t in tensors]
-
-
-def _as_saved(tensors, layout) -> list:
-    """What a backward saved, with autograd's hooks having handed it back otherwise than ``layout``: on
-    the device and in the type it was saved with again, in any strides; another shape is refused."""
-    back = []
-    for t, like in zip(tensors, layout):
-        if t is not None and t.shape != like[2]:
-            raise KernelError(f"a saved tensor of shape {tuple(like[2])} came back as {tuple(t.shape)}")
-        back.append(t if t is None else t.to(device=torch.device("cuda", like[0]), dtype=like[1]))
-    return back
+def _as_saved(t, dtype, shape, device):
+    """``t``, as autograd's hooks handed it back, in the type and on the device it was saved with (None
+    for None); another shape is refused."""
+    if t is None:
+        return None
+    if t.shape != shape:
+        raise KernelError(f"a saved tensor of shape {tuple(shape)} came back as {tuple(t.shape)}")
+    return t.to(device=device, dtype=dtype)
 
 
 _HERE = contextlib.nullcontext()
@@ -233,7 +227,7 @@ _HERE = contextlib.nullcontext()
 
 def _on(device: torch.device):
     """A context in which ``device`` is the current one (it mostly is)."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _stream(device: torch.device) -> int:

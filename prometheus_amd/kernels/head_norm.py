@@ -195,7 +195,8 @@ class _NormRotate(torch.autograd.Function):
         tensors = plan.tensors()
         ctx.save_for_backward(*tensors)
         ctx.call, ctx.options = plan.call, (norm, eps, interleaved)
-        ctx.shared, ctx.layout = plan.shared, _k._layout(tensors)
+        ctx.shared = plan.shared
+        ctx.saved = [None if t is None else (t.dtype, t.shape, t.stride()) for t in tensors]
         ctx.set_materialize_grads(False)  # a missing gradient is None, not a tensor of zeros
         # (the type and device of each input's gradient, where it is not as the backward gives it)
         as_given = q is plan.q and k is plan.k and all(
@@ -209,13 +210,17 @@ class _NormRotate(torch.autograd.Function):
     def backward(ctx, gq, gk):
         tensors, need = ctx.saved_tensors, ctx.needs_input_grad
         want = (need[2], need[3])
-        if _k._layout(tensors) == ctx.layout:
-            call = ctx.call
+        call, gpu = ctx.call, ctx.call.device.index
+        for t, like in zip(tensors, ctx.saved):
+            if t is not None and not ((t.dtype, t.shape, t.stride()) == like and t.get_device() == gpu):
+                # (saved-tensor hooks may hand back another layout, or copies elsewhere or of another type)
+                tensors = [u if u is None else _k._as_saved(u, *like[:2], call.device)
+                           for u, like in zip(tensors, ctx.saved)]
+                grads = _backward(_NormRotateResidual(*tensors, *ctx.options), (gq, gk), want)
+                break
+        else:
             with _k._on(call.device):
                 grads = _launch_bwd(call.device, tensors, ctx.shared, call.dev(gq), call.dev(gk), want)
-        else:  # (saved-tensor hooks may hand back another layout)
-            res = _NormRotateResidual(*_k._as_saved(tensors, ctx.layout), *ctx.options)
-            grads = _backward(res, (gq, gk), want)
         if ctx.like is not None:
             grads = [t if t is None or like is None else t.to(device=like[1], dtype=like[0])
                      for t, like in zip(grads, ctx.like)]

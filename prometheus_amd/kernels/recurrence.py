@@ -129,7 +129,7 @@ class _LinearRecurrence(torch.autograd.Function):
     def forward(ctx, x, g, state, out_dtype):
         call, xd, gd, kept, h, s = _forward(x, g, state, out_dtype, keep=True)
         ctx.save_for_backward(xd, gd, kept)
-        ctx.layout = _k._layout((xd, gd, kept))
+        ctx.saved = (xd.dtype, gd.dtype, xd.shape, kept.shape)
         ctx.call, ctx.h_dtype = call, h.dtype
         ctx.set_materialize_grads(False)  # a missing gradient is None, not a tensor of zeros
         # (the type and device of each input's gradient, where it is not as the backward gives it)
@@ -143,10 +143,17 @@ class _LinearRecurrence(torch.autograd.Function):
     @_k._once
     def backward(ctx, gh, gs):
         call, (xd, gd, kept) = ctx.call, ctx.saved_tensors
+        xt, gt, shape, kept_shape = ctx.saved
+        gpu = call.device.index
         with _k._on(call.device):
-            if _k._layout((xd, gd, kept)) != ctx.layout:  # (saved-tensor hooks may hand back another)
-                xd, gd, kept = _k._as_saved((xd, gd, kept), ctx.layout)
-                xd, gd, kept = _rows(call, xd, xd.dtype), _rows(call, gd, gd.dtype), call.dev(kept)
+            if not (xd.dtype == xt and xd.shape == shape and xd.get_device() == gpu and gd.dtype == gt
+                    and gd.shape == shape and gd.get_device() == gpu and kept.dtype == torch.float32
+                    and kept.shape == kept_shape and kept.get_device() == gpu and kept.is_contiguous()
+                    and (shape[2] <= 1 or xd.stride(2) == gd.stride(2) == 1)):
+                # (saved-tensor hooks may hand back another layout, or copies elsewhere or of another type)
+                xd, gd, kept = (_k._as_saved(t, dtype, size, call.device) for t, dtype, size in (
+                    (xd, xt, shape), (gd, gt, shape), (kept, torch.float32, kept_shape)))
+                xd, gd, kept = _rows(call, xd, xt), _rows(call, gd, gt), kept.contiguous()
             grads = _launch_bwd(call, xd, gd, kept, call.dev(gh), call.dev(gs), ctx.h_dtype)
         if ctx.like is not None:
             grads = [t if like is None else t.to(device=like[1], dtype=like[0]) for t, like in zip(grads, ctx.like)]
@@ -297,5 +304,5 @@ def _step(state: int | None, slots, n_slots, xd, gd, h, stream):
     """One token on device tensors; ``state`` is the states' address."""
     batch, chan = xd.shape
     _native.check(_native.lib().pm_linear_recurrence_step(
-        state, _k._ptr(slots), n_slots, _k._ptr(xd), _k._ptr(gd), _k._ptr(h), batch, chan, xd.stride(0), gd.stride(0),
+        state, _k._ptr(slots), n_slots, xd.data_ptr(), gd.data_ptr(), h.data_ptr(), batch, chan, xd.stride(0), gd.stride(0),
         _k._code(xd.dtype), _k._code(gd.dtype), _k._code(h.dtype), stream))

@@ -51,6 +51,7 @@ class _SlotPool:
         # one spare slot past the end: out-of-range device slot indices land there
         self._pool = torch.zeros((n_layers, n_slots + 1, *state), dtype=torch.float32, device=device)
         self.pool = self._pool[:, :n_slots]
+        self._gpu = self._pool.get_device()  # (-1 on the host)
         self._bad_slot = torch.zeros(1, dtype=torch.int32, device=device)
         # a min-heap: alloc hands out the lowest free slots, so that a batch admitted in
         # order decodes through an increasing slot table, which walks the pool in address
@@ -133,11 +134,11 @@ class _SlotPool:
             raise ValueError(f"layer {layer} outside [0, {self.n_layers})")
 
     def _check_cuda(self, *xs) -> None:
-        if self.pool.device.type != "cuda":
+        gpu = self._gpu
+        if gpu < 0:
             raise RuntimeError("the state cache computes on a HIP GPU; this pool is on the host")
-        device = self.pool.device
         for x in xs:
-            if not (isinstance(x, torch.Tensor) and x.device == device):
+            if not (isinstance(x, torch.Tensor) and x.get_device() == gpu):
                 raise ValueError("inputs must be tensors on the pool's device")
 
 
@@ -276,7 +277,7 @@ class RecurrenceStateCache(_SlotPool):
         if slots.dim() != 1 or slots.dtype != torch.int32 or not slots.is_contiguous():
             raise ValueError("slots must be a contiguous int32 tensor of shape (B,)")
         want = (slots.shape[0], self.channels)
-        if tuple(x.shape) != want or tuple(g.shape) != want:
+        if x.shape != want or g.shape != want:
             raise ValueError(f"x and g must be {want}, got {tuple(x.shape)} and {tuple(g.shape)}")
         if x.dtype not in (torch.float32, torch.bfloat16) or g.dtype not in (torch.float32, x.dtype):
             raise ValueError("x must be fp32 or bf16, and g fp32 or x's type")
