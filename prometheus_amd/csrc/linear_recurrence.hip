@@ -30,14 +30,15 @@
 // threads hold x and gh as they are in memory, and make what they need of them again after the
 // wait; the gates, of which an exponential is a quarter of a tile's arithmetic, are kept.
 //
-// Measured (a card that copies at 5.0 TB/s): forward 4 x 4096 tokens of 4096 bf16 channels 79 us
-// (5.1 TB/s), backward 131 (5.1 TB/s), 65521 tokens of 2048 channels 146 (5.5 TB/s). On the way:
-// 256-token tiles, a workgroup to each and every value held 121, 226 and 239; as here but gates made
-// twice 88, 140 and 163; a branch at every row and words asked for after the tile's loads 82, 135
-// and 151. An elementwise pass over the same lines takes 84, over rows of 512 bytes 69; but wide
-// tiles are short, and four times the hops and words cost more than the rows gain (256 bytes, two
-// workgroups to a compute unit: 151 for the long one; 512 bytes: 183). Columns dealt to XCDs in runs
-// of neighbours were slower (96 of 88), stores that stay out of the caches 2% faster.
+// Measured (calls among others, their begin kernels with them, on a card that copies at 5.0 TB/s):
+// forward 4 x 4096 tokens of 4096 bf16 channels 71 us (5.6 TB/s), backward 134 (5.0 TB/s), 65521
+// tokens of 2048 channels 144 (5.6 TB/s). On the way, when this form took 79, 131 and 146: 256-token
+// tiles, a workgroup to each and every value held 121, 226 and 239; as here but gates made twice 88,
+// 140 and 163; a branch at every row and words asked for after the tile's loads 82, 135 and 151. An
+// elementwise pass over the same lines takes 84, over rows of 512 bytes 69; but wide tiles are short,
+// and four times the hops and words cost more than the rows gain (256 bytes, two workgroups to a
+// compute unit: 151 for the long one; 512 bytes: 183). Columns dealt to XCDs in runs of neighbours
+// were slower (96 of 88), stores that stay out of the caches 2% faster.
 
 #include "pm_internal.h"
 #include "pm_vec.h"

@@ -16,9 +16,9 @@
 // backward with weights, as many tokens as 1024 workgroups leave it). Any D up to 256, any strides
 // and alignment.
 //
-// Measured at D = 128, bf16, on a card that copies at 5.0 TB/s: 16384 tokens of 16 + 16 heads
-// forward 49 us (5.5 TB/s; one wave to a head, element by element, 361), backward 80 (5.0 TB/s,
-// the weights' gradients among it).
+// Measured at D = 128, bf16, calls among others on a card that copies at 5.0 TB/s: 16384 tokens of
+// 16 + 16 heads forward 46 us (5.8 TB/s; one wave to a head, element by element, 361), backward 72
+// (5.6 TB/s, the weights' gradients among it).
 
 #include <type_traits>
 
