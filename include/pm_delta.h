@@ -46,7 +46,7 @@
 extern "C" {
 #endif
 
-#define PM_DELTA_ABI_VERSION 15
+#define PM_DELTA_ABI_VERSION 16
 
 /* element types */
 #define PM_DTYPE_F32 0
@@ -551,6 +551,131 @@ int pm_norm_rotate_bwd(const void* q, const void* k, const float* table, const v
                        float eps, int interleaved, int dtype, int w_dtype, void* workspace, size_t ws_bytes,
                        void* stream);
 size_t pm_norm_rotate_bwd_workspace_bytes(int B, int T, int Hq, int Hk, int D);
+
+/* ------------------------------------------------------------------------
+ * Linear attention with a decay for each head, without the delta rule's
+ * correction (no reference counterpart): for every sequence and key head
+ *     S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t
+ * with log-decays g; a group of Hq / H query heads shares each key head's
+ * state (query head h reads key head h / (Hq / H)).
+ *
+ *   q        (n_seqs, T, Hq, D), k, v (n_seqs, T, H, D), or packed (T, heads,
+ *            D) with cu_seqlens: fp32 or bf16, the elements of a head
+ *            contiguous; strides: host array of q's batch, token and head
+ *            strides, then k's, then v's, in elements (views of a projection
+ *            run as they are)
+ *   g        fp32, heads contiguous, batch and token strides g_sb, g_st; both 0:
+ *            one constant a head
+ *   o        contiguous (n_seqs, T, Hq, D), out_dtype
+ *   s0       (n_seqs, H, D, D) fp32 or NULL (zeros); s_out the same, the state
+ *            after each sequence's last token (an empty sequence's is its s0).
+ *            s0 may be s_out.
+ *   slots    NULL, or int32 (n_seqs): sequence i's states are row slots[i] of
+ *            the pool s0 == s_out (n_slots, H, D, D), as in
+ *            pm_linear_recurrence (no slot twice; one outside the pool starts
+ *            from zero, is not stored and makes *bad_slot nonzero)
+ *   cu_seqlens, cu_flag  as in pm_linear_recurrence_varlen
+ * D in [1, 256].  States and sums are fp32; products run on bf16 MFMA over
+ * enough bf16 parts of each factor for a relative error of about 2^-17 (bf16
+ * inputs, before o's rounding) or 2^-24 (fp32 inputs).  A log-decay below -138
+ * counts as closed and one above 138 as infinite; an infinity may come out as
+ * NaN, and either reaches the other tokens of its chunk of 64 (fp32 inputs: 32).
+ * workspace: pm_decay_attention_workspace_bytes (in_place: s0 is s_out and not
+ * NULL; 0 where none is needed).
+ */
+int pm_decay_attention(const void* q, const void* k, const void* v, const float* g,
+                       const int32_t* cu_seqlens, const float* s0, const int32_t* slots, int n_slots,
+                       int32_t* bad_slot, int32_t* cu_flag, void* o, float* s_out, int n_seqs, int T,
+                       int Hq, int H, int D, const int64_t* strides, int64_t g_sb, int64_t g_st,
+                       int dtype, int out_dtype, float scale, void* workspace, size_t ws_bytes,
+                       void* stream);
+size_t pm_decay_attention_workspace_bytes(int n_seqs, int T, int Hq, int H, int D, int in_place);
+
+/*
+ * Its reverse mode over (B, T): go = dL/do contiguous in dtype, gs = dL/ds_out
+ * (fp32, NULL for zeros).  gq, gk, gv contiguous in dtype; gs0 (B, H, D, D) fp32,
+ * NULL: not wanted; gg fp32: (B, T, H), or (H), summed over all tokens in an order that does not
+ * change, where both of g's strides are 0; NULL: not wanted.  Every output is
+ * written in full; none may overlap an input.  workspace:
+ * pm_decay_attention_bwd_workspace_bytes (gates: gg is wanted).
+ */
+int pm_decay_attention_bwd(const void* q, const void* k, const void* v, const float* g, const float* s0,
+                           const void* go, const float* gs, void* gq, void* gk, void* gv, float* gg,
+                           float* gs0, int B, int T, int Hq, int H, int D, const int64_t* strides,
+                           int64_t g_sb, int64_t g_st, int dtype, float scale, void* workspace,
+                           size_t ws_bytes, void* stream);
+size_t pm_decay_attention_bwd_workspace_bytes(int B, int T, int Hq, int H, int D, int gates);
+
+/*
+ * One token for B rows, the states (B, H, D, D), or the pool's slots, updated in
+ * place: q (B, Hq, D), k, v (B, H, D), strides: host array of q's batch and head
+ * strides, then k's, then v's; g (B, H) with row stride g_sb (0: one constant a
+ * head); o contiguous (B, Hq, D).  slots as pm_delta_step_slots.  fp32 arithmetic.
+ */
+int pm_decay_attention_step(float* s_inout, const int32_t* slots, int n_slots, const void* q,
+                            const void* k, const void* v, const float* g, void* o, int B, int Hq, int H,
+                            int D, const int64_t* strides, int64_t g_sb, int dtype, int out_dtype,
+                            float scale, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The norm of a layer's output with its gate, before the output projection (no
+ * reference counterpart): for rows of C elements, with act(z) = z sigmoid(z)
+ * (PM_ACT_SILU) or sigmoid(z) (PM_ACT_SIGMOID),
+ *     y = r x weight act(gate),             r = 1 / sqrt(mean x^2 + eps)
+ * or, with gate_first,
+ *     y = r u weight, u = x act(gate),      r = 1 / sqrt(mean u^2 + eps).
+ *
+ *   x, gate  `rows` rows of C in [1, PM_NORM_MAX_ROW] contiguous elements; row i
+ *            starts at (i / inner) so + (i % inner) si; strides: host array of
+ *            x's so and si, then the gate's, in elements
+ *   weight   (C) or NULL (ones);  y contiguous (rows, C)
+ * fp32 arithmetic, one rounding.
+ */
+#define PM_NORM_MAX_ROW 16384
+#define PM_ACT_SILU 0
+#define PM_ACT_SIGMOID 1
+int pm_gated_norm(const void* x, const void* gate, const void* weight, void* y, int64_t rows, int inner,
+                  int C, const int64_t* strides, int activation, int gate_first, float eps, int x_dtype,
+                  int gate_dtype, int y_dtype, int w_dtype, void* stream);
+
+/*
+ * Its reverse mode: gy (contiguous, y_dtype) to gx and g_gate (contiguous, in x's
+ * and the gate's type) and, where asked for, the weight's gradient (C) fp32,
+ * summed in an order that does not change (it needs the workspace; without it
+ * that may be NULL).
+ */
+int pm_gated_norm_bwd(const void* x, const void* gate, const void* weight, const void* gy, void* gx,
+                      void* g_gate, float* g_weight, int64_t rows, int inner, int C,
+                      const int64_t* strides, int activation, int gate_first, float eps, int x_dtype,
+                      int gate_dtype, int y_dtype, int w_dtype, void* workspace, size_t ws_bytes,
+                      void* stream);
+size_t pm_gated_norm_bwd_workspace_bytes(int64_t rows, int C);
+
+/* ------------------------------------------------------------------------
+ * Between two blocks (no reference counterpart): the norm of a block's output
+ * (where post_weight is given), its sum with the residual and the norm before
+ * the next block:
+ *     h = residual + scale b,  b = x, or x post_weight / sqrt(mean x^2 + eps)
+ *     y = h weight / sqrt(mean h^2 + eps)      (h before its rounding)
+ * x and residual: rows of C in [1, PM_NORM_MAX_ROW] contiguous elements, x_st and
+ * r_st elements apart, in dtype and r_dtype; y (dtype) and h (r_dtype) contiguous;
+ * weight (C) or NULL (ones), post_weight (C) or NULL.  fp32 arithmetic, one rounding.
+ */
+int pm_residual_norm(const void* x, const void* residual, const void* weight, const void* post_weight,
+                     void* y, void* h, int64_t rows, int C, int64_t x_st, int64_t r_st, float scale,
+                     float eps, int dtype, int r_dtype, int w_dtype, int post_w_dtype, void* stream);
+
+/*
+ * Its reverse mode: gy, gh (contiguous, in y's and h's types, NULL for zeros) to
+ * gx and g_residual (contiguous, in x's and the residual's types) and, where asked
+ * for, the weights' gradients (C) fp32, as pm_gated_norm_bwd's.
+ */
+int pm_residual_norm_bwd(const void* x, const void* residual, const void* weight,
+                         const void* post_weight, const void* gy, const void* gh, void* gx,
+                         void* g_residual, float* g_weight, float* g_post_weight, int64_t rows, int C,
+                         int64_t x_st, int64_t r_st, float scale, float eps, int dtype, int r_dtype,
+                         int w_dtype, int post_w_dtype, void* workspace, size_t ws_bytes, void* stream);
+size_t pm_residual_norm_bwd_workspace_bytes(int64_t rows, int C);
 
 /* Thread-local message for the last nonzero return on this thread. */
 const char* pm_last_error(void);

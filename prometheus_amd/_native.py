@@ -18,7 +18,7 @@ import torch  # noqa: F401  (see module docstring: must precede CDLL)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpmdelta.so")
 
-ABI_VERSION = 15
+ABI_VERSION = 16
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 MAX_D = 256
@@ -28,6 +28,9 @@ NOALLOC_SCRATCH_BYTES = 64 << 20
 RECURRENCE_SPAN = 128
 NORM_L2 = 0
 NORM_RMS = 1
+NORM_MAX_ROW = 16384
+ACT_SILU = 0
+ACT_SIGMOID = 1
 
 E_NULL, E_SHAPE, E_DTYPE, E_ALIGN, E_WORKSPACE, E_UNSUPPORTED = -1, -2, -3, -4, -5, -6
 
@@ -72,6 +75,17 @@ EXPORTS = (
     "pm_norm_rotate",
     "pm_norm_rotate_bwd",
     "pm_norm_rotate_bwd_workspace_bytes",
+    "pm_decay_attention",
+    "pm_decay_attention_workspace_bytes",
+    "pm_decay_attention_bwd",
+    "pm_decay_attention_bwd_workspace_bytes",
+    "pm_decay_attention_step",
+    "pm_gated_norm",
+    "pm_gated_norm_bwd",
+    "pm_gated_norm_bwd_workspace_bytes",
+    "pm_residual_norm",
+    "pm_residual_norm_bwd",
+    "pm_residual_norm_bwd_workspace_bytes",
 )
 
 _lib = None
@@ -183,6 +197,32 @@ def lib() -> ctypes.CDLL:
         L.pm_norm_rotate_bwd.restype = i
         L.pm_norm_rotate_bwd_workspace_bytes.argtypes = [i] * 5
         L.pm_norm_rotate_bwd_workspace_bytes.restype = sz
+        pi64 = ctypes.POINTER(i64)
+        L.pm_decay_attention.argtypes = ([vp] * 7 + [i] + [vp] * 4 + [i] * 5 + [pi64, i64, i64, i, i, f]
+                                         + [vp, sz, vp])
+        L.pm_decay_attention.restype = i
+        L.pm_decay_attention_workspace_bytes.argtypes = [i] * 6
+        L.pm_decay_attention_workspace_bytes.restype = sz
+        L.pm_decay_attention_bwd.argtypes = [vp] * 12 + [i] * 5 + [pi64, i64, i64, i, f] + [vp, sz, vp]
+        L.pm_decay_attention_bwd.restype = i
+        L.pm_decay_attention_bwd_workspace_bytes.argtypes = [i] * 6
+        L.pm_decay_attention_bwd_workspace_bytes.restype = sz
+        L.pm_decay_attention_step.argtypes = [vp, vp, i] + [vp] * 5 + [i] * 4 + [pi64, i64, i, i, f, vp]
+        L.pm_decay_attention_step.restype = i
+        gated = [i64, i, i, pi64, i, i, f] + [i] * 4
+        L.pm_gated_norm.argtypes = [vp] * 4 + gated + [vp]
+        L.pm_gated_norm.restype = i
+        L.pm_gated_norm_bwd.argtypes = [vp] * 7 + gated + [vp, sz, vp]
+        L.pm_gated_norm_bwd.restype = i
+        L.pm_gated_norm_bwd_workspace_bytes.argtypes = [i64, i]
+        L.pm_gated_norm_bwd_workspace_bytes.restype = sz
+        res = [i64, i, i64, i64, f, f] + [i] * 4
+        L.pm_residual_norm.argtypes = [vp] * 6 + res + [vp]
+        L.pm_residual_norm.restype = i
+        L.pm_residual_norm_bwd.argtypes = [vp] * 10 + res + [vp, sz, vp]
+        L.pm_residual_norm_bwd.restype = i
+        L.pm_residual_norm_bwd_workspace_bytes.argtypes = [i64, i]
+        L.pm_residual_norm_bwd_workspace_bytes.restype = sz
         got = L.pm_abi_version()
         if got != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH}: ABI version {got}, expected {ABI_VERSION}")

@@ -1,0 +1,70 @@
+// pm_decay_args.h — what the kernels of K14 (pm_decay.h) take, for them and their callers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace pm {
+
+constexpr int kDecayKeep = 256;  // tokens between the states kept for the gates' gradient
+
+// One pass over n_seqs sequences (roles as in pm_decay.h).  Strides are in elements; the elements of
+// a head are contiguous.  HO heads of Q and O, HK of K and V, HS = min(HO, HK) states.
+struct DecayPass {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+    const float* g;  // [b][t][HS], heads contiguous; both strides 0: one constant a head
+    int64_t g_sb, g_st;
+    const int32_t* cu;  // nullable: packed (T tokens, n_seqs + 1 offsets, clamped into [0, T])
+    const float* s0;    // nullable: zeros
+    float* s_out;       // nullable
+    int64_t s_row, s_col;  // strides of a state's rows (K's dimension) and columns (V's)
+    const int32_t* slots;  // nullable: sequence i's state is row slots[i] of the pool s0, s_out
+    int n_slots;
+    int32_t* bad_slot;  // nullable
+    bool s0_gathered;   // s0 holds the sequences' states in order, whatever the slots
+    void* o;            // contiguous (.., HO, D)
+    bool out_bf16, reverse;
+    int n_seqs, T, HO, HK, HS, D;
+    int n_tiles;        // ceil(D / 64): column tiles
+    int span, n_spans;  // tokens a workgroup walks through, and workgroups along the longest sequence
+    float* span_state;  // [state][span][tile] accumulators: each span's own share of the state
+    double* span_log;   // [state][span] sum of its log-decays, in units of log 2
+    float a_scale, into_scale, out_scale;  // of A, of the state's part of O, of what enters the state
+    // for the gates' gradient
+    const void* aux;    // q (gq's pass), k (gk's)
+    int64_t x_sb, x_st, x_sh;
+    float* part;        // [tile][row][HO]
+    int64_t n_rows;
+    float* kept;        // [state][keep][tile] accumulators
+    float* cross;       // [state][keep][tile]
+    int keep, n_keep;   // chunks between kept states, and their number
+};
+
+struct DecayGateGrad {
+    const void* q;
+    const void* k;
+    const void* v;
+    const void* go;
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, go_sb, go_st, go_sh;
+    const float* g;
+    int64_t g_sb, g_st;
+    const float* r_part;
+    const float* c_part;
+    const float* cross;
+    float* gg;       // nullable: (B, T, H)
+    float* gg_part;  // nullable: (B, n_keep, H)
+    int64_t n_rows;
+    int B, T, Hq, H, D, n_tiles, n_keep;
+    float scale;
+};
+
+// kind: 0 outputs and state only, 1 gq's pass with its share of the gates' gradient, 2 gk's.
+hipError_t decay_pass_bf16(const DecayPass& a, int kind, hipStream_t st);
+hipError_t decay_pass_f32(const DecayPass& a, int kind, hipStream_t st);
+hipError_t decay_gate_grad_bf16(const DecayGateGrad& a, hipStream_t st);
+hipError_t decay_gate_grad_f32(const DecayGateGrad& a, hipStream_t st);
+
+}  // namespace pm

@@ -339,4 +339,127 @@ hipError_t launch_norm_rotate(const NormRotateArgs& a, hipStream_t st);
 hipError_t launch_norm_rotate_bwd(const NormRotateArgs& a, hipStream_t st);
 size_t norm_rotate_bwd_ws_bytes(int B, int T, int Hq, int Hk, int D);
 
+// Linear attention with a decay for each head (decay_attention.hip): S = e^g S + k v^T, o = scale S^T q.
+// q (n_seqs, T, Hq, D), k and v (.., H, D) with batch, token and head strides in elements (strides:
+// q's, k's, v's), or packed (T, heads, D) with cu; g fp32 [b][t][H] (both strides 0: one constant a
+// head).  States (.., H, D, D) fp32; slots and s0 == s_out as in RecurrenceArgs.
+struct DecayAttnArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    const int64_t* strides;
+    const float* g;
+    int64_t g_sb, g_st;
+    const int32_t* cu;     // nullable
+    int32_t* cu_flag;      // nullable: gets launch_varlen_check's bits
+    const float* s0;       // nullable
+    float* s_out;
+    const int32_t* slots;  // nullable
+    int n_slots;
+    int32_t* bad_slot;  // nullable
+    void* o;
+    int n_seqs, T, Hq, H, D;
+    bool bf16, out_bf16;
+    float scale;
+    void* workspace;
+};
+hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st);
+size_t decay_attn_ws_bytes(int n_seqs, int T, int Hq, int H, int D, bool in_place);
+// Workgroups along the grid's x, and spans along its y.
+int64_t decay_attn_groups(int n_seqs, int T, int Hq, int D);
+int decay_attn_spans(int n_seqs, int T, int Hq, int D);
+
+// Its gradients; go contiguous in q's type, gq, gk, gv contiguous in it; gg (B, T, H), or (H) where
+// both of g's strides are 0 (nullable: not wanted).
+struct DecayAttnBwdArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    const int64_t* strides;
+    const float* g;
+    int64_t g_sb, g_st;
+    const float* s0;  // nullable
+    const void* go;
+    const float* gs;  // nullable
+    void* gq;
+    void* gk;
+    void* gv;
+    float* gg;
+    float* gs0;  // nullable: not wanted
+    int B, T, Hq, H, D;
+    bool bf16;
+    float scale;
+    void* workspace;
+};
+hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st);
+size_t decay_attn_bwd_ws_bytes(int B, int T, int Hq, int H, int D, bool gates);
+
+// One token for B rows, in place; strides: q's batch and head, k's, v's.
+struct DecayAttnStepArgs {
+    float* s;
+    const int32_t* slots;  // nullable
+    int n_slots;
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t strides[6];
+    const float* g;
+    int64_t g_sb;
+    void* o;
+    int B, Hq, H, D;
+    bool bf16, out_bf16;
+    float scale;
+};
+hipError_t launch_decay_attn_step(const DecayAttnStepArgs& a, hipStream_t st);
+
+constexpr int kMaxRow = 16384;  // elements of a row of the two norms below
+
+// The norm of rows with weight and gate (gated_norm.hip).  Row i of x and z starts at
+// (i / inner) so + (i % inner) si; y, gy, gx, gz are contiguous.
+struct GatedNormArgs {
+    const void* x;
+    const void* z;
+    const void* w;  // nullable
+    void* y;
+    int64_t rows, x_so, x_si, z_so, z_si;
+    int inner, C;
+    bool x_bf16, z_bf16, y_bf16, w_bf16, silu, first;
+    float eps;
+    // backward
+    const void* gy;
+    void* gx;
+    void* gz;
+    float* gw;    // nullable
+    float* part;  // (gated_norm_groups, C), where gw is given
+};
+hipError_t launch_gated_norm(const GatedNormArgs& a, hipStream_t st);
+hipError_t launch_gated_norm_bwd(const GatedNormArgs& a, hipStream_t st);
+int64_t gated_norm_groups(int64_t rows, int C);
+
+// The norm after a block, the sum with the residual and the norm before the next (residual_norm.hip).
+// Rows of x and the residual are x_st and r_st elements apart; all else is contiguous.
+struct ResidualNormArgs {
+    const void* x;
+    const void* res;
+    const void* w;   // nullable
+    const void* wp;  // nullable: no norm of x
+    void* y;         // x's type
+    void* h;         // the residual's
+    int64_t rows, x_st, r_st;
+    int C;
+    bool x_bf16, r_bf16, w_bf16, wp_bf16;
+    float eps, scale;
+    // backward
+    const void* gy;  // nullable
+    const void* gh;  // nullable
+    void* gx;
+    void* gres;
+    float* gw;    // nullable
+    float* gwp;   // nullable
+    float* part;  // (2, residual_norm_groups, C), where either is given
+};
+hipError_t launch_residual_norm(const ResidualNormArgs& a, hipStream_t st);
+hipError_t launch_residual_norm_bwd(const ResidualNormArgs& a, hipStream_t st);
+int64_t residual_norm_groups(int64_t rows, int C);
+
 }  // namespace pm

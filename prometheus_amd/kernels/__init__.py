@@ -23,8 +23,9 @@ per-token kernel.
 Beyond the reference surface: ``chunked_delta_rule_varlen`` (packed batch
 with ``cu_seqlens``), ``delta_rule_step`` (public single-token decode step),
 the keyword ``out_dtype`` (bf16 output, opt-in; fp32 by default), and the operators
-beside the delta rule: ``linear_recurrence`` (``recurrence.py``) and ``norm_rotate``
-(``head_norm.py``).
+beside the delta rule: ``linear_recurrence`` (``recurrence.py``), ``norm_rotate``
+(``head_norm.py``), ``decay_attention`` (``decay.py``), ``gated_norm`` and
+``residual_norm`` (``row_norms.py``).
 """
 
 from __future__ import annotations
@@ -891,7 +892,14 @@ def _gated_step(q, k, v, beta, g, state, per_channel):
     return call.out(o)
 
 
-from prometheus_amd.kernels.head_norm import (  # noqa: E402  (they use the helpers above)
+from prometheus_amd.kernels.decay import (  # noqa: E402  (they use the helpers above)
+    decay_attention,
+    decay_attention_bwd,
+    decay_attention_fwd,
+    decay_attention_step,
+    decay_attention_varlen,
+)
+from prometheus_amd.kernels.head_norm import (  # noqa: E402
     norm_rotate,
     norm_rotate_bwd,
     norm_rotate_fwd,
@@ -903,6 +911,14 @@ from prometheus_amd.kernels.recurrence import (  # noqa: E402
     linear_recurrence_fwd,
     linear_recurrence_step,
     linear_recurrence_varlen,
+)
+from prometheus_amd.kernels.row_norms import (  # noqa: E402
+    gated_norm,
+    gated_norm_bwd,
+    gated_norm_fwd,
+    residual_norm,
+    residual_norm_bwd,
+    residual_norm_fwd,
 )
 
 __all__ = [
@@ -933,4 +949,15 @@ __all__ = [
     "norm_rotate_fwd",
     "norm_rotate_bwd",
     "rotation_table",
+    "decay_attention",
+    "decay_attention_fwd",
+    "decay_attention_bwd",
+    "decay_attention_varlen",
+    "decay_attention_step",
+    "gated_norm",
+    "gated_norm_fwd",
+    "gated_norm_bwd",
+    "residual_norm",
+    "residual_norm_fwd",
+    "residual_norm_bwd",
 ]

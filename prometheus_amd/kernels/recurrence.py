@@ -215,6 +215,11 @@ def _packed(x, g, cu_seqlens):
     if _k._shape(g) != xs or len(xs) not in (2, 3) or (len(xs) == 3 and xs[0] != 1):
         raise _k.KernelError(f"packed x and g must both be (N, C) or (1, N, C); got {xs} and {_k._shape(g)}")
     n_tok, chan = xs[-2:]
+    return n_tok, chan, *_cu(cu_seqlens, n_tok)
+
+
+def _cu(cu_seqlens, n_tok):
+    """``(n_seqs, offsets)`` of a packed call of ``n_tok`` tokens, as ``_packed`` gives them."""
     if n_tok >= 2**31:
         raise _k.KernelError("cu_seqlens exceeds int32")
     if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.device.type == "cuda":
@@ -222,13 +227,13 @@ def _packed(x, g, cu_seqlens):
             raise _k.KernelError("cu_seqlens must be a 1-D array of n_seqs + 1 offsets")
         if cu_seqlens.dtype not in (torch.int32, torch.int64):
             raise _k.KernelError(f"cu_seqlens must be an integer array, got {cu_seqlens.dtype}")
-        return n_tok, chan, cu_seqlens.numel() - 1, cu_seqlens
+        return cu_seqlens.numel() - 1, cu_seqlens
     host = cu_seqlens.detach().numpy() if isinstance(cu_seqlens, torch.Tensor) else np.asarray(cu_seqlens)
     if not np.issubdtype(host.dtype, np.integer):
         raise _k.KernelError(f"cu_seqlens must be an integer array, got {host.dtype}")
     host = host.astype(np.int64)
     _k._validate_cu(host, n_tok)
-    return n_tok, chan, host.size - 1, host
+    return host.size - 1, host
 
 
 def _offsets(call, cu, n_seqs, n_tok, chan):

@@ -26,7 +26,8 @@ host memory. ``LinearStateCache`` is that pool on one GPU:
 
 ``RecurrenceStateCache`` is the same for layers of ``kernels.linear_recurrence``, whose state is
 a vector of C channels (``(n_layers, n_slots, C)`` fp32): its ``prefill`` reads and writes the
-slots in the kernel, without gathering them first.
+slots in the kernel, without gathering them first. ``DecayStateCache`` is the same for layers of
+``kernels.decay_attention``, whose state is a matrix per key head (``(n_layers, n_slots, H, D, D)``).
 """
 
 from __future__ import annotations
@@ -36,9 +37,9 @@ import heapq
 import torch
 
 from prometheus_amd import _native, kernels
-from prometheus_amd.kernels import recurrence
+from prometheus_amd.kernels import decay, recurrence
 
-__all__ = ["LinearStateCache", "RecurrenceStateCache"]
+__all__ = ["LinearStateCache", "RecurrenceStateCache", "DecayStateCache"]
 
 
 class _SlotPool:
@@ -291,4 +292,100 @@ class RecurrenceStateCache(_SlotPool):
         with kernels._on(x.device):
             recurrence._step(self._pool.data_ptr() + layer * self._pool.stride(0) * 4, slots, self.n_slots, x, g, out,
                              kernels._stream(x.device))
+        return out
+
+
+class DecayStateCache(_SlotPool):
+    """Per-request states of ``n_layers`` layers of linear attention with a decay for each head."""
+
+    def __init__(self, n_layers: int, n_slots: int, heads: int, dim: int, device=None):
+        if n_layers < 1 or n_slots < 1 or heads < 1 or dim < 1:
+            raise ValueError("n_layers, n_slots, heads and dim must be >= 1")
+        super().__init__(n_layers, n_slots, (heads, dim, dim), device)
+        self.heads, self.dim = heads, dim
+
+    def prefill(self, layer: int, slots, q, k, v, g, cu_seqlens=None, *, scale=1.0, out_dtype=None):
+        """Run prompts through ``decay_attention`` from the slots' states into them, in place.
+
+        Fixed length: q ``(n, T, Hq, D)``, k, v ``(n, T, H, D)``, g ``(n, T, H)`` or ``(H,)``, one
+        request per row. Packed: ``(N, ..)`` or ``(1, N, ..)`` with ``cu_seqlens`` ``(n + 1,)``. Returns
+        o shaped like q. ``slots`` (each at most once) may be a list of ints or a GPU int tensor; with GPU
+        ``slots`` and ``cu_seqlens`` nothing here waits for the device: a request whose slot is out of
+        range starts from a zero state, leaves the pool untouched and is reported by ``check_slots``.
+        """
+        self._check_layer(layer)
+        if isinstance(slots, torch.Tensor) and slots.device.type == "cuda":
+            if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
+                raise ValueError("a GPU slot tensor must be 1-D int32 or int64")
+            n = slots.shape[0]
+        else:
+            slots = self._ids(slots)
+            n = len(slots)
+            if len(set(slots)) != n:
+                raise ValueError("a slot may be given once")
+        if kernels._wants_grad(q, k, v, g):
+            raise ValueError("prefill is forward only: call it under torch.no_grad()")
+        shape = kernels._shape(q)
+        if cu_seqlens is None:
+            (n_seqs, seq), _, heads, dim = decay._check(q, k, v, g, 4, scale)
+            cu = None
+        else:
+            seq, _, heads, dim, n_seqs, cu, (q, k, v, g) = decay._packed(q, k, v, g, cu_seqlens, scale)
+        if (heads, dim) != (self.heads, self.dim):
+            raise ValueError(f"k has {heads} heads of {dim}, the cache {self.heads} of {self.dim}")
+        if n_seqs != n:
+            raise ValueError(f"{n} slots for {n_seqs} prompts")
+        self._check_cuda(q, k, v, g)
+        call = kernels._Call(q, k, v, g, cu_seqlens)
+        dtype = kernels._qkv_dtype(q, k, v)
+        with kernels._on(call.device):
+            if isinstance(slots, list):
+                slots = torch.tensor(slots, dtype=torch.int32, device=call.device)
+            elif slots.device != self._pool.device:
+                raise ValueError("slots must be on the pool's device")
+            elif slots.dtype == torch.int64:
+                # (clamped: an index past int32 must not come back into range)
+                slots = slots.clamp(-1, self.n_slots).to(torch.int32)
+            qd, kd, vd = (decay._heads(call, x, dtype) for x in (q, k, v))
+            gd, g_strides = decay._decays(call, g)
+            flag = None
+            if cu is not None:
+                cu, flag = recurrence._offsets(call, cu, n_seqs, seq, 1)
+            o = torch.empty(shape, dtype=decay._out_dtype(out_dtype, dtype), device=call.device)
+            pool = self._pool[layer]
+            decay._launch(call, qd, kd, vd, gd, g_strides, cu, flag, pool, slots.contiguous(), self.n_slots,
+                          self._bad_slot, pool, o, n_seqs, seq, scale)
+        return o
+
+    def decode(self, layer: int, slots: torch.Tensor, q, k, v, g, out=None, *, scale=1.0, out_dtype=None):
+        """One token per request: q ``(B, Hq, D)``, k, v ``(B, H, D)``, g ``(B, H)`` or ``(H,)`` fp32,
+        ``slots`` an int32 GPU tensor ``(B,)``. Updates the states in place and returns ``out``
+        ``(B, Hq, D)`` (allocated when None: q's type, or ``out_dtype``). Slots outside
+        ``[0, n_slots)`` are padding: no state is touched and their rows are zero. Allocation-free with
+        ``out=``."""
+        self._check_layer(layer)
+        if kernels._wants_grad(q, k, v, g):
+            raise ValueError("decode is forward only: call it under torch.no_grad()")
+        self._check_cuda(q, k, v, g, slots)
+        if slots.dim() != 1 or slots.dtype != torch.int32 or not slots.is_contiguous():
+            raise ValueError("slots must be a contiguous int32 tensor of shape (B,)")
+        (batch,), _, heads, dim = decay._check(q, k, v, g, 3, scale)
+        if batch != slots.shape[0] or (heads, dim) != (self.heads, self.dim):
+            raise ValueError(f"k must be {(slots.shape[0], self.heads, self.dim)}, got {tuple(k.shape)}")
+        if q.dtype != k.dtype or q.dtype != v.dtype or q.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("q, k, v must share one dtype, fp32 or bf16")
+        if g.dtype != torch.float32:
+            raise ValueError("g must be fp32")
+        if dim > 1 and not q.stride(2) == k.stride(2) == v.stride(2) == 1:
+            raise ValueError("q, k and v must have the elements of a head contiguous")
+        if heads > 1 and g.stride(-1) != 1:
+            raise ValueError("g must have contiguous heads")
+        if out is None:
+            out = torch.empty(q.shape, dtype=decay._out_dtype(out_dtype, q.dtype), device=q.device)
+        elif (out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16) or not out.is_contiguous()
+              or out.device != q.device):
+            raise ValueError(f"out must be contiguous fp32 or bf16 {tuple(q.shape)} on the pool's device")
+        with kernels._on(q.device):
+            decay._step(self._pool.data_ptr() + layer * self._pool.stride(0) * 4, slots, self.n_slots, q, k, v, g,
+                        g.stride(0) if g.dim() == 2 else 0, out, scale, kernels._stream(q.device))
         return out
