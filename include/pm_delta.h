@@ -580,8 +580,8 @@ size_t pm_norm_rotate_bwd_workspace_bytes(int B, int T, int Hq, int Hk, int D);
  * inputs, before o's rounding) or 2^-24 (fp32 inputs).  A log-decay below -138
  * counts as closed and one above 138 as infinite; an infinity may come out as
  * NaN, and either reaches the other tokens of its chunk of 64 (fp32 inputs: 32).
- * workspace: pm_decay_attention_workspace_bytes (in_place: s0 is s_out and not
- * NULL; 0 where none is needed).
+ * workspace: pm_decay_attention_workspace_bytes (packed: cu_seqlens is given,
+ * in_place: s0 is s_out and not NULL; 0 where none is needed).
  */
 int pm_decay_attention(const void* q, const void* k, const void* v, const float* g,
                        const int32_t* cu_seqlens, const float* s0, const int32_t* slots, int n_slots,
@@ -589,7 +589,8 @@ int pm_decay_attention(const void* q, const void* k, const void* v, const float*
                        int Hq, int H, int D, const int64_t* strides, int64_t g_sb, int64_t g_st,
                        int dtype, int out_dtype, float scale, void* workspace, size_t ws_bytes,
                        void* stream);
-size_t pm_decay_attention_workspace_bytes(int n_seqs, int T, int Hq, int H, int D, int in_place);
+size_t pm_decay_attention_workspace_bytes(int n_seqs, int T, int Hq, int H, int D, int packed,
+                                          int in_place);
 
 /*
  * Its reverse mode over (B, T): go = dL/do contiguous in dtype, gs = dL/ds_out

@@ -201,7 +201,7 @@ def lib() -> ctypes.CDLL:
         L.pm_decay_attention.argtypes = ([vp] * 7 + [i] + [vp] * 4 + [i] * 5 + [pi64, i64, i64, i, i, f]
                                          + [vp, sz, vp])
         L.pm_decay_attention.restype = i
-        L.pm_decay_attention_workspace_bytes.argtypes = [i] * 6
+        L.pm_decay_attention_workspace_bytes.argtypes = [i] * 7
         L.pm_decay_attention_workspace_bytes.restype = sz
         L.pm_decay_attention_bwd.argtypes = [vp] * 12 + [i] * 5 + [pi64, i64, i64, i, f] + [vp, sz, vp]
         L.pm_decay_attention_bwd.restype = i

@@ -2,7 +2,7 @@
 // (pm_decay.h has their mathematics), the single token, and how calls are cut into workgroups.
 
 #include <algorithm>
-#include <type_traits>
+#include <utility>
 
 #include "pm_decay.h"
 #include "pm_internal.h"
@@ -38,43 +38,138 @@ __global__ __launch_bounds__(256) void sum_gate_parts(const float* part, float* 
     if (threadIdx.x == 0) gg[blockIdx.x] = static_cast<float>(s[0]);
 }
 
+// Packed calls: which sequence and span of it each slot of the grid is, each sequence's first slot, and
+// the check of the offsets (launch_varlen_check's bits).  One workgroup; every thread counts the spans of
+// its own run of sequences, then writes their slots.  Slots past the last are (-1, 0); where malformed
+// offsets overlap, those that would not fit are left out.
+__global__ __launch_bounds__(1024) void assign_slots(const int32_t* cu, int n_seqs, int T, int span, int n_slots,
+                                                     int2* table, int* first_slot, int32_t* flag) {
+    __shared__ int sums[1024];
+    const int t = threadIdx.x, per = (n_seqs + 1023) / 1024, i0 = min(t * per, n_seqs), i1 = min(i0 + per, n_seqs);
+    auto spans = [&](int i) {
+        const int z0 = min(max(cu[i], 0), T), z1 = min(max(cu[i + 1], 0), T);
+        return max((z1 - z0 + span - 1) / span, 1);
+    };
+    int n = 0, bits = 0;
+    for (int i = i0; i < i1; ++i) {
+        n = min(n + spans(i), n_slots);
+        if (cu[i + 1] < cu[i]) bits |= 4;
+        if (cu[i + 1] < 0 || cu[i + 1] > T) bits |= 8;
+    }
+    if (t == 0 && cu[0] != 0) bits |= cu[0] < 0 || cu[0] > T ? 9 : 1;
+    if (t == 0 && cu[n_seqs] != T) bits |= 2;
+    if (bits && flag) atomicOr(flag, bits);
+    sums[t] = n;
+    for (int m = 1; m < 1024; m <<= 1) {
+        __syncthreads();
+        const int x = t >= m ? sums[t - m] : 0;
+        __syncthreads();
+        sums[t] = min(sums[t] + x, n_slots);
+    }
+    __syncthreads();
+    int at = t > 0 ? sums[t - 1] : 0;
+    for (int i = i0; i < i1; ++i) {
+        const int k = spans(i);
+        first_slot[i] = at;
+        for (int j = 0; j < k && at < n_slots; ++j, ++at) table[at] = make_int2(i, j);
+    }
+    for (int j = sums[1023] + t; j < n_slots; j += 1024) table[j] = make_int2(-1, 0);
+}
+
+// States before the spans from each span's own share: S = e^G S + U, span after span, one thread per
+// element of a state.  The shares do not wait for each other: eight are asked for ahead.
+__global__ __launch_bounds__(256) void scan_spans(DecayPass a, const int* first_slot) {
+    const int64_t pair = blockIdx.y + static_cast<int64_t>(blockIdx.z) * 65535;
+    if (pair >= static_cast<int64_t>(a.n_seqs) * a.HS) return;
+    const int seq = static_cast<int>(pair / a.HS), h = static_cast<int>(pair % a.HS);
+    const int size = a.D * a.D, e = blockIdx.x * 256 + threadIdx.x;
+    if (e >= size) return;
+    int len = a.T, slot = seq * a.n_spans;
+    if (a.cu) {
+        len = max(min(max(a.cu[seq + 1], 0), a.T) - min(max(a.cu[seq], 0), a.T), 0);
+        slot = first_slot[seq];
+    }
+    const int n = min(max((len + a.span - 1) / a.span, 1), a.n_slots_grid - slot);
+    float S = 0.f;
+    if (a.s0) {
+        int64_t from = seq;
+        bool there = true;
+        if (a.slots && !a.s0_gathered) {
+            from = a.slots[seq];
+            there = from >= 0 && from < a.n_slots;
+        }
+        if (there) S = a.s0[(from * a.HS + h) * size + e];
+    }
+    float* u = a.span_state + (static_cast<int64_t>(slot) * a.HS + h) * size + e;
+    const double* log = a.span_log + static_cast<int64_t>(slot) * a.HS + h;
+    const int64_t step = static_cast<int64_t>(a.HS) * size;
+    if (n > 0) u[0] = S;
+    for (int i = 1; i < n; i += 8) {
+        float x[8], g[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j < n) x[j] = u[(i + j) * step], g[j] = exp2_f64(log[static_cast<int64_t>(i + j) * a.HS]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j < n) {
+                S = g[j] * S + x[j];
+                u[(i + j) * step] = S;
+            }
+    }
+}
+
 struct Plan {
-    int n_tiles, span, n_spans;
+    int n_tiles, n_dst, span, n_spans, n_slots;
+    bool split;
 };
 
-// Workgroups: one per sequence, output head and 64 columns of the state, or, where these are fewer
-// than two for every CU, as many again along the sequence as make it two (spans of at least 512
-// tokens: a span costs a state written and read, as much as 128 tokens' q, k, v and o).
-Plan plan(int n_seqs, int T, int HO, int D) {
-    Plan p{(D + kDecayCols - 1) / kDecayCols, max(T, 1), 1};
-    const int64_t groups = static_cast<int64_t>(n_seqs) * HO * p.n_tiles;
-    const int64_t want = groups > 0 ? (512 + groups - 1) / groups : 1;
-    if (want > 1 && T > 512) {
-        const int64_t per = std::max<int64_t>((T + want - 1) / want, 512);
-        p.span = static_cast<int>((per + kDecayKeep - 1) / kDecayKeep * kDecayKeep);
+// How a pass is cut into workgroups: one per sequence, state and column tile, or, where that leaves
+// CUs without two, as many again along the sequence (spans of at least 128 tokens; calls of up to 512
+// tokens stay whole, since the states' own pass costs as much as they take).  The query heads of a
+// group go one after another through one workgroup, which reads their keys once, where there is work
+// enough for every CU without them.
+Plan plan(int n_seqs, int T, int HO, int HS, int D, bool packed) {
+    Plan p{(D + decay_cols(D) - 1) / decay_cols(D), 1, max(T, 1), 1, n_seqs, false};
+    const int64_t tokens = packed ? T : static_cast<int64_t>(n_seqs) * T, want = 512;
+    if (HO > HS && tokens * HS * p.n_tiles >= want * 256) p.n_dst = HO / HS;
+    const int64_t groups = static_cast<int64_t>(HO / p.n_dst) * p.n_tiles;
+    if (T > 512 && n_seqs * groups < want) {
+        const int64_t span = std::max<int64_t>((tokens * groups + want - 1) / want, 128);
+        const int64_t n = (T + span - 1) / span;
+        p.span = static_cast<int>(((T + n - 1) / n + 63) / 64 * 64);
         p.n_spans = (T + p.span - 1) / p.span;
+        p.n_slots = packed ? T / p.span + n_seqs : n_seqs * p.n_spans;
+        p.split = p.n_spans > 1;
     }
     return p;
 }
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
-int padded(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-// Bytes of one state's accumulators: n_tiles workgroups of (padded D) x 64 floats.
-size_t frag_bytes(const Plan& p, int D) { return static_cast<size_t>(p.n_tiles) * padded(D) * kDecayCols * 4; }
 
-struct FwdWs {
-    size_t gathered, span_state, span_log, bytes;
+struct Layout {
+    size_t bytes = 0;
+    size_t take(size_t n) {
+        const size_t at = bytes;
+        bytes += up(n);
+        return at;
+    }
 };
-FwdWs fwd_ws(int n_seqs, int T, int Hq, int H, int D, bool in_place) {
-    const Plan p = plan(n_seqs, T, Hq, D);
-    const size_t states = static_cast<size_t>(n_seqs) * H;
+struct FwdWs {
+    size_t gathered, span_state, span_log, table, first_slot, bytes;
+};
+// Whether several workgroups read a first state that another one of them may already have replaced.
+bool shares_states(const Plan& p, int HO, int HS) { return !p.split && HO / p.n_dst > HS; }
+FwdWs fwd_ws(int n_seqs, int T, int Hq, int H, int D, bool packed, bool in_place) {
+    const Plan p = plan(n_seqs, T, Hq, H, D, packed);
+    const size_t state = static_cast<size_t>(H) * D * D * 4;
+    Layout l;
     FwdWs w{};
-    // several workgroups read a first state that another one may already have replaced
-    if (in_place && (p.n_spans > 1 || Hq > H)) w.bytes += up(states * D * D * 4);
-    w.span_state = w.bytes;
-    if (p.n_spans > 1) w.bytes += up(states * p.n_spans * frag_bytes(p, D));
-    w.span_log = w.bytes;
-    if (p.n_spans > 1) w.bytes += up(states * p.n_spans * 8);
+    w.gathered = l.take(in_place && shares_states(p, Hq, H) ? n_seqs * state : 0);
+    w.span_state = l.take(p.split ? p.n_slots * state : 0);
+    w.span_log = l.take(p.split ? static_cast<size_t>(p.n_slots) * H * 8 : 0);
+    w.table = l.take(packed ? static_cast<size_t>(p.n_slots) * 8 : 0);
+    w.first_slot = l.take(packed ? static_cast<size_t>(n_seqs) * 4 : 0);
+    w.bytes = l.bytes;
     return w;
 }
 
@@ -82,24 +177,23 @@ struct BwdWs {
     size_t span_state, span_log, kept, cross, r_part, c_part, gg_part, bytes;
 };
 BwdWs bwd_ws(int B, int T, int Hq, int H, int D, bool gates) {
-    const Plan pq = plan(B, T, Hq, D), pk = plan(B, T, H, D);
-    const size_t states = static_cast<size_t>(B) * H, spans = max(pq.n_spans, pk.n_spans);
-    const size_t keep = (T + kDecayKeep - 1) / kDecayKeep, rows = static_cast<size_t>(B) * T;
+    const Plan pq = plan(B, T, Hq, H, D, false), pk = plan(B, T, H, H, D, false);
+    const size_t slots = max(pq.split ? pq.n_slots : 0, pk.split ? pk.n_slots : 0);
+    const size_t states = static_cast<size_t>(B) * H, keep = (T + kDecayKeep - 1) / kDecayKeep;
+    const size_t rows = static_cast<size_t>(B) * T, tiles = pq.n_tiles;
+    Layout l;
     BwdWs w{};
-    auto take = [&](size_t n) {
-        const size_t at = w.bytes;
-        w.bytes += up(n);
-        return at;
-    };
-    w.span_state = take(spans > 1 ? states * spans * frag_bytes(pq, D) : 0);
-    w.span_log = take(spans > 1 ? states * spans * 8 : 0);
+    w.span_state = l.take(slots * H * D * D * 4);
+    w.span_log = l.take(slots * H * 8);
     if (gates) {
-        w.kept = take(states * keep * frag_bytes(pq, D));
-        w.cross = take(states * keep * pq.n_tiles * 4);
-        w.r_part = take(pq.n_tiles * rows * Hq * 4);
-        w.c_part = take(pq.n_tiles * rows * H * 4);
-        w.gg_part = take(states * keep * 4);
+        const int padded = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+        w.kept = l.take(states * keep * tiles * padded * decay_cols(D) * 4);
+        w.cross = l.take(states * keep * tiles * 4);
+        w.r_part = l.take(tiles * rows * Hq * 4);
+        w.c_part = l.take(tiles * rows * H * 4);
+        w.gg_part = l.take(states * keep * 4);
     }
+    w.bytes = l.bytes;
     return w;
 }
 
@@ -108,26 +202,45 @@ T* at(void* base, size_t off) {
     return reinterpret_cast<T*>(static_cast<char*>(base) + off);
 }
 
+hipError_t run_kind(const DecayPass& a, bool bf16, int kind, hipStream_t st) {
+    return bf16 ? decay_pass_bf16(a, kind, st) : decay_pass_f32(a, kind, st);
+}
+
+void apply(DecayPass& x, const Plan& p) {
+    x.n_tiles = p.n_tiles, x.n_dst = p.n_dst, x.span = p.span, x.n_spans = p.n_spans, x.n_slots_grid = p.n_slots;
+}
+
+// The states before the spans of x, from each span's own share.  The shares' pass takes K and V the
+// other way round: it stores a state's rows in 16-byte pieces.
+hipError_t span_states(DecayPass x, bool bf16, const int* first_slot, hipStream_t st) {
+    std::swap(x.k, x.v);
+    std::swap(x.k_sb, x.v_sb), std::swap(x.k_st, x.v_st), std::swap(x.k_sh, x.v_sh);
+    x.u_row = 1, x.u_col = x.D;
+    if (hipError_t e = run_kind(x, bf16, 3, st); e != hipSuccess) return e;
+    const int64_t pairs = static_cast<int64_t>(x.n_seqs) * x.HS;
+    const dim3 grid(static_cast<unsigned>((x.D * x.D + 255) / 256), static_cast<unsigned>(std::min<int64_t>(pairs, 65535)),
+                    static_cast<unsigned>((pairs + 65534) / 65535));
+    hipLaunchKernelGGL(scan_spans, grid, dim3(256), 0, st, x, first_slot);
+    return hipGetLastError();
+}
+
 }  // namespace
 
-size_t decay_attn_ws_bytes(int n_seqs, int T, int Hq, int H, int D, bool in_place) {
-    return fwd_ws(n_seqs, T, Hq, H, D, in_place).bytes;
+size_t decay_attn_ws_bytes(int n_seqs, int T, int Hq, int H, int D, bool packed, bool in_place) {
+    return fwd_ws(n_seqs, T, Hq, H, D, packed, in_place).bytes;
 }
 size_t decay_attn_bwd_ws_bytes(int B, int T, int Hq, int H, int D, bool gates) {
     return bwd_ws(B, T, Hq, H, D, gates).bytes;
 }
-int64_t decay_attn_groups(int n_seqs, int T, int Hq, int D) {
-    const Plan p = plan(n_seqs, T, Hq, D);
-    return (static_cast<int64_t>(n_seqs) * Hq + 7) / 8 * 8 * p.n_tiles;
+int64_t decay_attn_groups(int n_seqs, int T, int Hq, int H, int D, bool packed) {
+    const Plan p = plan(n_seqs, T, Hq, H, D, packed);
+    return (static_cast<int64_t>(p.n_slots) * (Hq / p.n_dst) + 7) / 8 * 8 * p.n_tiles;
 }
-int decay_attn_spans(int n_seqs, int T, int Hq, int D) { return plan(n_seqs, T, Hq, D).n_spans; }
 
 hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st) {
-    if (a.cu && a.cu_flag)
-        if (hipError_t e = launch_varlen_check(a.cu, a.n_seqs, a.T, a.cu_flag, st); e != hipSuccess) return e;
-    const Plan p = plan(a.n_seqs, a.T, a.Hq, a.D);
-    const bool in_place = a.s0 && a.s0 == a.s_out;
-    const FwdWs w = fwd_ws(a.n_seqs, a.T, a.Hq, a.H, a.D, in_place);
+    const bool packed = a.cu != nullptr, in_place = a.s0 && a.s0 == a.s_out;
+    const Plan p = plan(a.n_seqs, a.T, a.Hq, a.H, a.D, packed);
+    const FwdWs w = fwd_ws(a.n_seqs, a.T, a.Hq, a.H, a.D, packed, in_place);
     DecayPass x{};
     x.q = a.q, x.k = a.k, x.v = a.v;
     x.q_sb = a.strides[0], x.q_st = a.strides[1], x.q_sh = a.strides[2];
@@ -135,9 +248,22 @@ hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st) {
     x.v_sb = a.strides[6], x.v_st = a.strides[7], x.v_sh = a.strides[8];
     x.g = a.g, x.g_sb = a.g_sb, x.g_st = a.g_st;
     x.cu = a.cu;
-    x.s0 = a.s0, x.s_out = a.s_out, x.s_row = a.D, x.s_col = 1;
+    x.s0 = a.s0, x.s_out = a.s_out, x.s_row = x.u_row = a.D, x.s_col = x.u_col = 1;
     x.slots = a.slots, x.n_slots = a.n_slots, x.bad_slot = a.bad_slot;
-    if (in_place && (p.n_spans > 1 || a.Hq > a.H)) {
+    x.o = a.o, x.out_bf16 = a.out_bf16;
+    x.n_seqs = a.n_seqs, x.T = a.T, x.HO = a.Hq, x.HK = x.HS = a.H, x.D = a.D;
+    apply(x, p);
+    x.a_scale = x.into_scale = a.scale, x.out_scale = 1.f;
+    int* first_slot = nullptr;
+    if (packed) {
+        int2* table = at<int2>(a.workspace, w.table);
+        first_slot = at<int>(a.workspace, w.first_slot);
+        hipLaunchKernelGGL(assign_slots, dim3(1), dim3(1024), 0, st, a.cu, a.n_seqs, a.T, p.span, p.n_slots, table,
+                           first_slot, a.cu_flag);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        x.slot_table = table;
+    }
+    if (in_place && shares_states(p, a.Hq, a.H)) {
         const int64_t size = static_cast<int64_t>(a.H) * a.D * a.D;
         float* to = at<float>(a.workspace, w.gathered);
         for (int b0 = 0; b0 < a.n_seqs; b0 += 65535) {
@@ -150,18 +276,17 @@ hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st) {
         x.s0 = to;
         x.s0_gathered = true;
     }
-    x.o = a.o, x.out_bf16 = a.out_bf16;
-    x.n_seqs = a.n_seqs, x.T = a.T, x.HO = a.Hq, x.HK = x.HS = a.H, x.D = a.D;
-    x.n_tiles = p.n_tiles, x.span = p.span, x.n_spans = p.n_spans;
-    x.span_state = at<float>(a.workspace, w.span_state);
-    x.span_log = at<double>(a.workspace, w.span_log);
-    x.a_scale = x.into_scale = a.scale, x.out_scale = 1.f;
-    return a.bf16 ? decay_pass_bf16(x, 0, st) : decay_pass_f32(x, 0, st);
+    if (p.split) {
+        x.span_state = at<float>(a.workspace, w.span_state);
+        x.span_log = at<double>(a.workspace, w.span_log);
+        if (hipError_t e = span_states(x, a.bf16, first_slot, st); e != hipSuccess) return e;
+    }
+    return run_kind(x, a.bf16, 0, st);
 }
 
 hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
     const bool gates = a.gg != nullptr;
-    const Plan pq = plan(a.B, a.T, a.Hq, a.D), pk = plan(a.B, a.T, a.H, a.D);
+    const Plan pq = plan(a.B, a.T, a.Hq, a.H, a.D, false), pk = plan(a.B, a.T, a.H, a.H, a.D, false);
     const BwdWs w = bwd_ws(a.B, a.T, a.Hq, a.H, a.D, gates);
     struct Role {
         const void* p;
@@ -169,8 +294,8 @@ hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
     };
     const int64_t go_strides[3] = {static_cast<int64_t>(a.T) * a.Hq * a.D, static_cast<int64_t>(a.Hq) * a.D, a.D};
     const Role q{a.q, a.strides}, k{a.k, a.strides + 3}, v{a.v, a.strides + 6}, go{a.go, go_strides};
-    auto run = [&](Role Q, Role K, Role V, Role aux, int HO, int HK, const Plan& p, bool reverse, bool transposed,
-                   const float* s0, float* s_out, void* o, float* part, int kind) {
+    auto pass = [&](Role Q, Role K, Role V, Role aux, int HO, int HK, const Plan& p, bool reverse, bool transposed,
+                    const float* s0, float* s_out, void* o, float* part) {
         DecayPass x{};
         x.q = Q.p, x.q_sb = Q.s[0], x.q_st = Q.s[1], x.q_sh = Q.s[2];
         x.k = K.p, x.k_sb = K.s[0], x.k_st = K.s[1], x.k_sh = K.s[2];
@@ -178,29 +303,40 @@ hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
         x.aux = aux.p, x.x_sb = aux.s[0], x.x_st = aux.s[1], x.x_sh = aux.s[2];
         x.g = a.g, x.g_sb = a.g_sb, x.g_st = a.g_st;
         x.s0 = s0, x.s_out = s_out;
-        x.s_row = transposed ? 1 : a.D, x.s_col = transposed ? a.D : 1;
+        x.s_row = x.u_row = transposed ? 1 : a.D, x.s_col = x.u_col = transposed ? a.D : 1;
         x.o = o, x.out_bf16 = a.bf16, x.reverse = reverse;
         x.n_seqs = a.B, x.T = a.T, x.HO = HO, x.HK = HK, x.HS = a.H, x.D = a.D;
-        x.n_tiles = p.n_tiles, x.span = p.span, x.n_spans = p.n_spans;
-        x.span_state = at<float>(a.workspace, w.span_state);
-        x.span_log = at<double>(a.workspace, w.span_log);
+        apply(x, p);
+        if (p.split) {
+            x.span_state = at<float>(a.workspace, w.span_state);
+            x.span_log = at<double>(a.workspace, w.span_log);
+        }
         x.a_scale = a.scale, x.into_scale = reverse ? 1.f : a.scale, x.out_scale = reverse ? a.scale : 1.f;
         x.part = part;
         x.n_rows = static_cast<int64_t>(a.B) * a.T;
-        x.kept = at<float>(a.workspace, w.kept), x.cross = at<float>(a.workspace, w.cross);
-        x.keep = kDecayKeep / (a.bf16 ? 64 : 32), x.n_keep = (a.T + kDecayKeep - 1) / kDecayKeep;
-        return a.bf16 ? decay_pass_bf16(x, kind, st) : decay_pass_f32(x, kind, st);
+        if (gates) {
+            x.kept = at<float>(a.workspace, w.kept), x.cross = at<float>(a.workspace, w.cross);
+            x.keep = kDecayKeep / (a.bf16 ? 64 : 32), x.n_keep = (a.T + kDecayKeep - 1) / kDecayKeep;
+        }
+        return x;
     };
     float* r_part = at<float>(a.workspace, w.r_part);
     float* c_part = at<float>(a.workspace, w.c_part);
-    if (hipError_t e = run(go, v, k, q, a.Hq, a.H, pq, false, true, a.s0, nullptr, a.gq, r_part, gates ? 1 : 0);
-        e != hipSuccess)
-        return e;
-    if (hipError_t e = run(k, q, go, k, a.H, a.Hq, pk, true, false, a.gs, a.gs0, a.gv, nullptr, 0); e != hipSuccess)
-        return e;
-    if (hipError_t e = run(v, go, q, k, a.H, a.Hq, pk, true, true, a.gs, nullptr, a.gk, c_part, gates ? 2 : 0);
-        e != hipSuccess)
-        return e;
+    const DecayPass gq = pass(go, v, k, q, a.Hq, a.H, pq, false, true, a.s0, nullptr, a.gq, r_part);
+    const DecayPass gv = pass(k, q, go, k, a.H, a.Hq, pk, true, false, a.gs, a.gs0, a.gv, nullptr);
+    const DecayPass gk = pass(v, go, q, k, a.H, a.Hq, pk, true, true, a.gs, nullptr, a.gk, c_part);
+    if (pq.split) {
+        // (the states of q's gradient are the transposed ones, whose shares' pass runs the forward's way round)
+        DecayPass x = gq;
+        std::swap(x.k, x.v);
+        std::swap(x.k_sb, x.v_sb), std::swap(x.k_st, x.v_st), std::swap(x.k_sh, x.v_sh);
+        if (hipError_t e = span_states(x, a.bf16, nullptr, st); e != hipSuccess) return e;
+    }
+    if (hipError_t e = run_kind(gq, a.bf16, gates ? 1 : 0, st); e != hipSuccess) return e;
+    if (pk.split)  // (gk's and gv's states are the same, one transposed)
+        if (hipError_t e = span_states(gv, a.bf16, nullptr, st); e != hipSuccess) return e;
+    if (hipError_t e = run_kind(gv, a.bf16, 0, st); e != hipSuccess) return e;
+    if (hipError_t e = run_kind(gk, a.bf16, gates ? 2 : 0, st); e != hipSuccess) return e;
     if (!gates) return hipSuccess;
     const bool constant = a.g_sb == 0 && a.g_st == 0;
     if (a.T > 0) {

@@ -42,7 +42,6 @@ struct DecayShape {
     static constexpr int BLK = P == 1 ? 6 : 2;   // packed operand blocks of A (qblk)
 };
 
-constexpr int kDecayCols = 64;  // columns of the state per workgroup: 16 per wave
 constexpr double kLog2e = 1.4426950408889634;
 
 // ---- planes -----------------------------------------------------------------------------------
@@ -138,9 +137,13 @@ template <int DK>
 __device__ __forceinline__ u32x4_t op_row(const uint16_t* m, int row, int kb, int g) {
     return *reinterpret_cast<const u32x4_t*>(m + row * DK + 8 * ((4 * kb + g) ^ kf<DK>(row)));
 }
-// The V tile, 64 bf16 (8 chunks) a row: rows r and r + 1 lie in different halves of the banks, the
-// four pairs of rows r, r + 2, r + 4, r + 6 in different quarters of a half for any pair of chunks.
-__device__ __forceinline__ int vf(int r) { return 2 * ((r >> 1) & 3); }
+// The V tile, NT bf16 a row.  128: as K's.  64 (8 chunks): rows r and r + 1 lie in different halves of
+// the banks, the four pairs of rows r, r + 2, r + 4, r + 6 in different quarters of a half for any pair
+// of chunks.
+template <int NT>
+__device__ __forceinline__ int vf(int r) {
+    return NT == 64 ? 2 * ((r >> 1) & 3) : kq_f<128>(r);
+}
 
 // Transposed reads, waited for in the same block: N 8-byte reads from addr + the offsets.
 template <int O0, int O1>
@@ -156,18 +159,6 @@ __device__ __forceinline__ void tr4(unsigned addr, u32x2_t& a, u32x2_t& b, u32x2
                      "s_waitcnt lgkmcnt(0)"
                      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
                      : "v"(addr), "n"(O0), "n"(O1), "n"(O2), "n"(O3) : "memory");
-}
-template <int O0, int O1, int O2, int O3, int O4, int O5, int O6, int O7>
-__device__ __forceinline__ void tr8(unsigned addr, u32x2_t (&r)[8]) {
-    __asm__ volatile("ds_read_b64_tr_b16 %0, %8 offset:%9\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
-                     "ds_read_b64_tr_b16 %2, %8 offset:%11\n\tds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
-                     "ds_read_b64_tr_b16 %4, %8 offset:%13\n\tds_read_b64_tr_b16 %5, %8 offset:%14\n\t"
-                     "ds_read_b64_tr_b16 %6, %8 offset:%15\n\tds_read_b64_tr_b16 %7, %8 offset:%16\n\t"
-                     "s_waitcnt lgkmcnt(0)"
-                     : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]),
-                       "=&v"(r[7])
-                     : "v"(addr), "n"(O0), "n"(O1), "n"(O2), "n"(O3), "n"(O4), "n"(O5), "n"(O6), "n"(O7)
-                     : "memory");
 }
 __device__ __forceinline__ u32x4_t join(u32x2_t a, u32x2_t b) {
     const u32x4_t r = {a.x, a.y, b.x, b.y};
@@ -215,24 +206,39 @@ __device__ __forceinline__ void tri_tile(int x, int& i, int& j) {
 }
 
 // ---- the pass ---------------------------------------------------------------------------------
+//
+// A workgroup walks through one span of a sequence for one head (or a group of heads that share their
+// K and V, or their Q), NT = 64 CT columns of the state: wave w keeps 16 CT of them for all DK rows in
+// accumulators, 16 CT columns of O for the chunk, and a quarter of A's tiles, which the waves exchange
+// through LDS.  Two column tiles a wave (DK >= 128) halve the LDS reads of Q and K^T per product, which
+// bound the kernel with one (B4 T4096 H16 D128: 118 us with one, LDS at 220 KB a chunk and 64 columns).
+// The next chunk's rows are loaded into registers while this one's products run.
 
 // What a launch of decay_pass does besides its outputs.
 enum { kPassPlain = 0, kPassGq = 1, kPassGk = 2, kPassState = 3 };
 
+template <int DK>
+struct DecayTile {
+    static constexpr int CT = DK >= 128 ? 2 : 1, NT = 64 * CT;
+};
+
 template <int P, int DK, int KIND>
-__global__ __launch_bounds__(256, 1) void decay_pass(DecayPass a) {
+__global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void decay_pass(DecayPass a) {
     using Sh = DecayShape<P>;
     constexpr int C = Sh::C, PC = Sh::PC, MT = Sh::MT, KB = DK / 32, MD = DK / 16;
-    constexpr int UQ = C * DK / 8 / 256, UV = C * kDecayCols / 8 / 256;  // 8-element units per thread
+    constexpr int CT = DecayTile<DK>::CT, NT = DecayTile<DK>::NT;
+    constexpr int UQ = C * DK / 2048, UV = C * NT / 2048;  // 8-element units per thread
+    constexpr int RQ = 2048 / DK, RV = 2048 / NT;          // rows between a thread's units
     constexpr bool OUT = KIND != kPassState, AUX = KIND == kPassGq || KIND == kPassGk;
+    using E = typename std::conditional<P == 1, uint16_t, float>::type;
 
     __shared__ __attribute__((aligned(16))) uint16_t sq[OUT ? P * C * DK : 8];
     __shared__ __attribute__((aligned(16))) uint16_t sk[P * C * DK];
-    __shared__ __attribute__((aligned(16))) uint16_t sv[P * C * kDecayCols];
+    __shared__ __attribute__((aligned(16))) uint16_t sv[P * C * NT];
     __shared__ __attribute__((aligned(16))) uint16_t sa[OUT ? PC * Sh::BLK * 512 : 8];
-    __shared__ float2 sg[C];              // the sums G, split
-    __shared__ float s_into[C], s_out[C];  // e^{G_i} and e^{G_C - G_j}, with their scales
-    __shared__ double s_total;
+    __shared__ float2 sg[2][C];                  // the sums G, split
+    __shared__ float s_into[2][C], s_out[2][C];  // e^{G_i} and e^{G_C - G_j}, with their scales
+    __shared__ double s_total[2];
     __shared__ float s_part[AUX ? 4 : 1][AUX ? C : 1];
     __shared__ float s_dot[4];
 
@@ -241,67 +247,82 @@ __global__ __launch_bounds__(256, 1) void decay_pass(DecayPass a) {
     // workgroups of one head's column tiles are 8 apart: on one XCD, they share its L2's lines
     const unsigned id = blockIdx.x, rest = id >> 3;
     const int tile = static_cast<int>(rest % a.n_tiles);
-    const int64_t pair = static_cast<int64_t>(rest / a.n_tiles) * 8 + (id & 7);
-    const int HO = KIND == kPassState ? a.HS : a.HO;  // (the states' pass runs once per state)
-    if (pair >= static_cast<int64_t>(a.n_seqs) * HO) return;
-    const int seq = static_cast<int>(pair / HO), ho = static_cast<int>(pair % HO);
-    const int hs = ho / (HO / a.HS);                   // the state's head
-    const int n_src = a.HK / a.HS;
-    const int n0 = tile * kDecayCols;
+    const int64_t unit = static_cast<int64_t>(rest / a.n_tiles) * 8 + (id & 7);
+    const int groups = OUT ? a.HO / a.n_dst : a.HS;  // head groups (the states' pass: one per state)
+    if (unit >= static_cast<int64_t>(a.n_slots_grid) * groups) return;
+    const int slot_id = static_cast<int>(unit / groups), hg = static_cast<int>(unit % groups);
+    const int ho0 = OUT ? hg * a.n_dst : hg;
+    const int hs = OUT ? ho0 / (a.HO / a.HS) : hg;   // the state's head
+    const int n_src = a.HK / a.HS, n_dst = OUT ? a.n_dst : 1, n_m = n_src * n_dst;
+    const int n0 = tile * NT;
 
     // the sequence and this workgroup's span of it
+    int seq, order;
     int64_t start = 0, rows0 = 0;
     int len = a.T;
-    int64_t qb = 0, kb_ = 0, vb = 0, gb = 0, xb = 0;
+    const E *qp = static_cast<const E*>(a.q), *kp = static_cast<const E*>(a.k), *vp = static_cast<const E*>(a.v);
+    const E* xp = static_cast<const E*>(a.aux);
+    const float* gp = a.g + hs;
     if (a.cu) {
+        const int2 so = a.slot_table[slot_id];
+        seq = so.x, order = so.y;
+        if (seq < 0) return;
         const int z0 = min(max(a.cu[seq], 0), a.T), z1 = min(max(a.cu[seq + 1], 0), a.T);
-        start = z0;
+        start = rows0 = z0;
         len = max(z1 - z0, 0);
-        rows0 = z0;
     } else {
-        qb = seq * a.q_sb, kb_ = seq * a.k_sb, vb = seq * a.v_sb, gb = seq * a.g_sb, xb = seq * a.x_sb;
+        seq = slot_id / a.n_spans, order = slot_id % a.n_spans;
+        qp += seq * a.q_sb, kp += seq * a.k_sb, vp += seq * a.v_sb, gp += seq * a.g_sb, xp += seq * a.x_sb;
         rows0 = static_cast<int64_t>(seq) * a.T;
     }
-    const int n_spans = max((len + a.span - 1) / a.span, 1), order = blockIdx.y;
-    if (order >= n_spans || (KIND == kPassState && order + 1 >= n_spans)) return;
+    const int n_spans = max((len + a.span - 1) / a.span, 1);
+    if (!OUT && order + 1 >= n_spans) return;
     const int my_span = a.reverse ? n_spans - 1 - order : order;
-    const int c_begin = my_span * a.span;                    // first token, relative to the sequence
+    const int c_begin = my_span * a.span;  // first token, relative to the sequence
     const int c_end = min(c_begin + a.span, len);
     const int n_chunks = (c_end - c_begin + C - 1) / C;
-
     const int64_t state_pair = static_cast<int64_t>(seq) * a.HS + hs;
-    const int64_t frag = static_cast<int64_t>(MD) * 256;     // float4s of a workgroup's part of a state
-    // ---- the state before the span
-    f32x4_t S[MD];
+
+    // ---- the state before the span.  Tile ct of wave w: columns n(ct, l16), rows s_row_d(md, 4 lg + r);
+    // two tiles take turns every 4 columns, so that a lane's outputs of both are 8 columns in a row
+    int n_col[CT];
 #pragma unroll
-    for (int md = 0; md < MD; ++md) S[md] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const int n = n0 + 16 * w + l16;                         // this lane's column
+    for (int ct = 0; ct < CT; ++ct)
+        n_col[ct] = n0 + (CT == 1 ? 16 * w + l16 : 32 * w + 8 * (l16 >> 2) + 4 * ct + (l16 & 3));
+    f32x4_t S[CT][MD];
     int64_t slot_pair = state_pair;
     bool stored = true;
     if (a.slots) {
         const int slot = a.slots[seq];
         stored = slot >= 0 && slot < a.n_slots;
         slot_pair = static_cast<int64_t>(stored ? slot : 0) * a.HS + hs;
-        if (!stored && a.bad_slot && t == 0) *a.bad_slot = 1;
+        if (OUT && !stored && a.bad_slot && t == 0) *a.bad_slot = 1;
     }
-    if (KIND != kPassState) {
-        if (a.s0 && (stored || a.s0_gathered)) {
-            const float* s0 = a.s0 + (a.s0_gathered ? state_pair : slot_pair) * a.D * a.D;
+    {
+        const float* from = nullptr;
+        int64_t row = a.s_row, col = a.s_col;
+        if (OUT && a.span_state) {
+            from = a.span_state + (static_cast<int64_t>(slot_id) * a.HS + hs) * a.D * a.D;
+            row = a.u_row, col = a.u_col;
+        } else if (OUT && a.s0 && (stored || a.s0_gathered)) {
+            from = a.s0 + (a.s0_gathered ? state_pair : slot_pair) * a.D * a.D;
+        }
 #pragma unroll
-            for (int md = 0; md < MD; ++md)
+        for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = s_row_d(md, 4 * lg + r);
-                    if (d < a.D && n < a.D) S[md][r] = s0[static_cast<int64_t>(d) * a.s_row + static_cast<int64_t>(n) * a.s_col];
+            for (int md = 0; md < MD; ++md) {
+                S[ct][md] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                if (!from) continue;
+                const int d0 = s_row_d(md, 4 * lg);
+                const float* p = from + d0 * row + n_col[ct] * col;
+                if (row == 1 && a.D % 4 == 0) {
+                    if (d0 < a.D && n_col[ct] < a.D) __builtin_memcpy(&S[ct][md], p, 16);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (d0 + r < a.D && n_col[ct] < a.D) S[ct][md][r] = p[r * row];
                 }
-        }
-        for (int s = 0; s < order; ++s) {
-            const int64_t at = state_pair * a.n_spans + s;
-            const float e = exp2_f64(a.span_log[at]);
-            const f32x4_t* u = reinterpret_cast<const f32x4_t*>(a.span_state) + (at * a.n_tiles + tile) * frag;
-#pragma unroll
-            for (int md = 0; md < MD; ++md) S[md] = e * S[md] + u[(w * MD + md) * 64 + lane];
-        }
+            }
     }
 
     // halves of A's blocks that no tile covers
@@ -311,10 +332,22 @@ __global__ __launch_bounds__(256, 1) void decay_pass(DecayPass a) {
 #pragma unroll
             for (int i = 0; i < MT; i += 2) zero_upper_half(sa + p * Sh::BLK * 512, qblk(i, i >> 1), lane);
 
-    // ---- loads of one step (a chunk and one of its source heads) into registers
+    // ---- loads of one step (a chunk and one of its heads) into registers
+    const int64_t sgn = a.reverse ? -1 : 1;
+    const int64_t q_ds = sgn * a.q_st, k_ds = sgn * a.k_st, v_ds = sgn * a.v_st;
+    const int row_q = t / (DK / 8), col_q = 8 * (t % (DK / 8)), row_v = t / (NT / 8), col_v = n0 + 8 * (t % (NT / 8));
+    const int64_t q_off = row_q * q_ds + col_q, k_off = row_q * k_ds + col_q, v_off = row_v * v_ds + col_v;
+    const int left_q = a.D - col_q, left_v = a.D - col_v;
+    const bool even = a.D % 8 == 0;
     Raw8<P> rq[OUT ? UQ : 1], rk[UQ], rv[UV];
-    float rg = 0.f;
-    const int n_steps = n_chunks * n_src;
+#pragma unroll
+    for (int i = 0; i < UQ; ++i) {
+        rk[i].zero();
+        if (OUT) rq[i].zero();
+    }
+#pragma unroll
+    for (int i = 0; i < UV; ++i) rv[i].zero();
+    const int n_steps = n_chunks * n_m;
     auto chunk_at = [&](int c, int& first, int& cnt) {  // tokens relative to the sequence
         const int k = a.reverse ? n_chunks - 1 - c : c;
         first = c_begin + k * C;
@@ -322,88 +355,125 @@ __global__ __launch_bounds__(256, 1) void decay_pass(DecayPass a) {
     };
     auto fetch = [&](int step) {
         int first, cnt;
-        chunk_at(step / n_src, first, cnt);
-        const int m = step % n_src;
-        const int64_t kh = static_cast<int64_t>(hs) * (a.HK / a.HS) + m;  // the source head
+        chunk_at(step / n_m, first, cnt);
+        const int m = step % n_m;
+        const int64_t tok = start + (a.reverse ? first + cnt - 1 : first);  // row 0's token
+        const E* q0 = qp + tok * a.q_st + static_cast<int64_t>(ho0 + (n_dst > 1 ? m : 0)) * a.q_sh + q_off;
+        const int64_t kh = static_cast<int64_t>(hs) * n_src + (n_dst > 1 ? 0 : m);  // the source head
+        const E* k0 = kp + tok * a.k_st + kh * a.k_sh + k_off;
+        const E* v0 = vp + tok * a.v_st + kh * a.v_sh + v_off;
+        const bool do_q = OUT && (n_dst > 1 || m == 0), do_kv = n_dst == 1 || m == 0;
+        if (even && cnt == C) {  // whole rows: no tests but one for the columns past D
+            if (left_q > 0) {
+                if (do_q)
 #pragma unroll
-        for (int i = 0; i < UQ; ++i) {
-            const int u = t + 256 * i, row = u / (DK / 8), col = 8 * (u % (DK / 8));
-            const int64_t tok = start + (a.reverse ? first + cnt - 1 - row : first + row);
-            const bool in = row < cnt && col < a.D;
-            if (in) {
-                rk[i].load(a.k, kb_ + tok * a.k_st + kh * a.k_sh + col, a.D - col);
-                if (OUT) rq[i].load(a.q, qb + tok * a.q_st + static_cast<int64_t>(ho) * a.q_sh + col, a.D - col);
-            } else {
-                rk[i].zero();
-                if (OUT) rq[i].zero();
-            }
-        }
+                    for (int i = 0; i < UQ; ++i) rq[OUT ? i : 0].load(q0, i * RQ * q_ds, 8);
+                if (do_kv)
 #pragma unroll
-        for (int i = 0; i < UV; ++i) {
-            const int u = t + 256 * i, row = u >> 3, col = n0 + 8 * (u & 7);
-            const int64_t tok = start + (a.reverse ? first + cnt - 1 - row : first + row);
-            if (row < cnt && col < a.D) rv[i].load(a.v, vb + tok * a.v_st + kh * a.v_sh + col, a.D - col);
-            else rv[i].zero();
-        }
-        if (t < C && m == 0) {
-            rg = 0.f;
-            if (t < cnt) {
-                const int tok = a.reverse ? first + cnt - t : first + t;  // (backwards: the token after)
-                if (tok < len) rg = a.g[gb + (start + tok) * a.g_st + hs];
+                    for (int i = 0; i < UQ; ++i) rk[i].load(k0, i * RQ * k_ds, 8);
             }
+            if (left_v > 0 && do_kv)
+#pragma unroll
+                for (int i = 0; i < UV; ++i) rv[i].load(v0, i * RV * v_ds, 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < UQ; ++i) {
+                const bool in = row_q + i * RQ < cnt && left_q > 0;
+                if (do_q) {
+                    if (in) rq[OUT ? i : 0].load(q0, i * RQ * q_ds, left_q);
+                    else rq[OUT ? i : 0].zero();
+                }
+                if (do_kv) {
+                    if (in) rk[i].load(k0, i * RQ * k_ds, left_q);
+                    else rk[i].zero();
+                }
+            }
+            if (do_kv)
+#pragma unroll
+                for (int i = 0; i < UV; ++i) {
+                    if (row_v + i * RV < cnt && left_v > 0) rv[i].load(v0, i * RV * v_ds, left_v);
+                    else rv[i].zero();
+                }
         }
     };
-
-    f32x4_t O[MT];
-    double log_total = 0.0;
-    if (n_steps > 0) fetch(0);
-    for (int step = 0; step < n_steps; ++step) {
-        const int c = step / n_src, m = step % n_src;
+    // wave 0 has the log-decays: chunk c's are loaded while chunk c - 2 runs, and summed while c - 1 does
+    float rg = 0.f;
+    auto fetch_g = [&](int c) {
+        rg = 0.f;
+        if (t >= C || c >= n_chunks) return;
         int first, cnt;
         chunk_at(c, first, cnt);
+        const int tok = a.reverse ? first + cnt - t : first + t;  // (backwards: the token after)
+        if (t < cnt && tok < len) rg = gp[(start + tok) * a.g_st];
+    };
+    auto sum_g = [&](int buf) {
+        const double G = wave_prefix_f64(t < C ? log2_decay(rg) : 0.0);
+        const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(G), 63),
+                                             __builtin_amdgcn_readlane(__double2loint(G), 63));
+        if (t < C) {
+            sg[buf][t] = split_log(G);
+            s_into[buf][t] = exp2_f64(G) * a.into_scale;
+            s_out[buf][t] = exp2_f64(last - G) * a.out_scale;
+        }
+        if (t == 0) s_total[buf] = last;
+    };
+
+    f32x4_t O[CT][MT];
+    double log_total = 0.0;
+    if (n_steps > 0) fetch(0);
+    if (w == 0) {
+        fetch_g(0);
+        sum_g(0);
+        fetch_g(1);
+    }
+    for (int step = 0; step < n_steps; ++step) {
+        const int c = step / n_m, m = step % n_m, buf = c & 1;
+        const bool first_m = m == 0, last_m = m == n_m - 1, dst = n_dst > 1;
+        int first, cnt;
+        chunk_at(c, first, cnt);
+        const int ho = ho0 + (dst ? m : 0);
         // ---- registers to LDS
+        if (!dst || first_m) {
 #pragma unroll
-        for (int i = 0; i < UQ; ++i) {
-            const int u = t + 256 * i, row = u / (DK / 8), ch = (u % (DK / 8)) ^ kf<DK>(row);
-            u32x4_t p[P];
-            rk[i].planes(p);
+            for (int i = 0; i < UQ; ++i) {
+                const int row = row_q + i * RQ, ch = (t % (DK / 8)) ^ kf<DK>(row);
+                u32x4_t p[P];
+                rk[i].planes(p);
 #pragma unroll
-            for (int x = 0; x < P; ++x) *reinterpret_cast<u32x4_t*>(sk + x * C * DK + row * DK + 8 * ch) = p[x];
-            if (OUT) {
-                rq[i].planes(p);
+                for (int x = 0; x < P; ++x) *reinterpret_cast<u32x4_t*>(sk + x * C * DK + row * DK + 8 * ch) = p[x];
+            }
+#pragma unroll
+            for (int i = 0; i < UV; ++i) {
+                const int row = row_v + i * RV, ch = (t % (NT / 8)) ^ vf<NT>(row);
+                u32x4_t p[P];
+                rv[i].planes(p);
+#pragma unroll
+                for (int x = 0; x < P; ++x) *reinterpret_cast<u32x4_t*>(sv + x * C * NT + row * NT + 8 * ch) = p[x];
+            }
+        }
+        if (OUT && (dst || first_m))
+#pragma unroll
+            for (int i = 0; i < UQ; ++i) {
+                const int row = row_q + i * RQ, ch = (t % (DK / 8)) ^ kf<DK>(row);
+                u32x4_t p[P];
+                rq[OUT ? i : 0].planes(p);
 #pragma unroll
                 for (int x = 0; x < P; ++x) *reinterpret_cast<u32x4_t*>(sq + x * C * DK + row * DK + 8 * ch) = p[x];
             }
-        }
-#pragma unroll
-        for (int i = 0; i < UV; ++i) {
-            const int u = t + 256 * i, row = u >> 3, ch = (u & 7) ^ vf(row);
-            u32x4_t p[P];
-            rv[i].planes(p);
-#pragma unroll
-            for (int x = 0; x < P; ++x)
-                *reinterpret_cast<u32x4_t*>(sv + x * C * kDecayCols + row * kDecayCols + 8 * ch) = p[x];
-        }
-        if (w == 0 && m == 0) {
-            const double G = wave_prefix_f64(t < C ? log2_decay(rg) : 0.0);
-            const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(G), 63),
-                                                 __builtin_amdgcn_readlane(__double2loint(G), 63));
-            if (t < C) {
-                sg[t] = split_log(G);
-                s_into[t] = exp2_f64(G) * a.into_scale;
-                s_out[t] = exp2_f64(last - G) * a.out_scale;
-            }
-            if (t == 0) s_total = last;
-        }
         lds_barrier();
         if (step + 1 < n_steps) fetch(step + 1);
+        if (w == 0 && first_m) {
+            sum_g(buf ^ 1);
+            fetch_g(c + 2);
+        }
 
-        // ---- A, lower tiles, as packed operands
+        // ---- A, lower tiles, as packed operands; wave 0, which has the log-decays, takes the fewest
         if (OUT) {
-            for (int x = w; x < Sh::TRI; x += 4) {
+            const int x0 = C == 64 ? max(3 * w - 2, 0) : w - 1, x1 = C == 64 ? 3 * w + 1 : w;
+            for (int x = max(x0, 0); x < x1; ++x) {
                 int i, j;
                 tri_tile(x, i, j);
-                f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+                f32x4_t acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
                     u32x4_t ko[P], qo[P];
@@ -412,17 +482,18 @@ __global__ __launch_bounds__(256, 1) void decay_pass(DecayPass a) {
                         ko[p] = op_row<DK>(sk + p * C * DK, 16 * j + l16, kb, lg);
                         qo[p] = op_row<DK>(sq + p * C * DK, 16 * i + l16, kb, lg);
                     }
-                    acc = mfma_planes<P, P>(ko, qo, acc);
+                    acc[kb & 1] = mfma_planes<P, P>(ko, qo, acc[kb & 1]);
                 }
                 const int row = 16 * i + l16;
-                const float2 gi = sg[row];
+                const float2 gi = sg[buf][row];
+                f32x4_t A;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int col = 16 * j + 4 * lg + r;
-                    acc[r] = col <= row ? acc[r] * (exp2_diff(gi, sg[col]) * a.a_scale) : 0.f;
+                    A[r] = col <= row ? (acc[0][r] + acc[1][r]) * (exp2_diff(gi, sg[buf][col]) * a.a_scale) : 0.f;
                 }
                 u32x2_t ap[PC];
-                split4<PC>(acc, ap);
+                split4<PC>(A, ap);
 #pragma unroll
                 for (int p = 0; p < PC; ++p)
                     *reinterpret_cast<u32x2_t*>(sa + (p * Sh::BLK + qblk(i, j >> 1)) * 512 + lane * 8 + 4 * (j & 1)) =
@@ -431,194 +502,286 @@ __global__ __launch_bounds__(256, 1) void decay_pass(DecayPass a) {
             lds_barrier();
         }
 
-        const double chunk_log = s_total;
-        if (m == 0) {
-            // ---- the state's part of the outputs
+        const double chunk_log = s_total[buf];
+        if (dst || first_m) {
             if (OUT) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i) O[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    u32x4_t so[PC];
-                    const float s8[8] = {S[2 * kb][0], S[2 * kb][1], S[2 * kb][2], S[2 * kb][3],
-                                         S[2 * kb + 1][0], S[2 * kb + 1][1], S[2 * kb + 1][2], S[2 * kb + 1][3]};
-                    split8<PC>(s8, so);
+                // ---- the state's part of the outputs
+                constexpr int XN = 4 * CT;  // a lane's columns in a row
+                float aux[AUX ? MT : 1][XN];
+                if constexpr (AUX) {
+                    const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg);
+                    const int64_t tok = start + (a.reverse ? first + cnt - 1 : first);
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        u32x4_t qo[P];
+                        const int row = 16 * i + l16;
+                        const E* x = xp + (tok + sgn * row) * a.x_st + static_cast<int64_t>(ho) * a.x_sh + col;
+                        const int left = row < cnt ? a.D - col : 0;
+                        if (left >= XN) {
+                            if constexpr (P == 1) {
+                                uint32_t raw[XN / 2];
+                                __builtin_memcpy(raw, x, sizeof raw);
 #pragma unroll
-                        for (int p = 0; p < P; ++p) qo[p] = op_row<DK>(sq + p * C * DK, 16 * i + l16, kb, lg);
-                        O[i] = mfma_planes<PC, P>(so, qo, O[i]);
+                                for (int r = 0; r < XN; ++r)
+                                    aux[i][r] = __uint_as_float(r % 2 ? raw[r / 2] & 0xffff0000u : raw[r / 2] << 16);
+                            } else {
+                                __builtin_memcpy(aux[i], x, sizeof aux[i]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < XN; ++r) aux[i][r] = r < left ? to_f32(x[r]) : 0.f;
+                        }
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < MT; ++i) O[i] *= s_into[16 * i + l16];
-            }
-            if (KIND == kPassGq && (first / C) % a.keep == 0 && ho % (HO / a.HS) == 0) {
-                f32x4_t* kept = reinterpret_cast<f32x4_t*>(a.kept) +
-                                ((state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile) * frag;
+                for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                for (int md = 0; md < MD; ++md) kept[(w * MD + md) * 64 + lane] = S[md];
-            }
-            if constexpr (AUX) {
-                // each token's product of that part with the row of `aux` (q for gq, k for gk)
+                    for (int i = 0; i < MT; ++i) O[ct][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    u32x4_t so[CT][PC], qo[MT][P];
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int p = 0; p < P; ++p) qo[i][p] = op_row<DK>(sq + p * C * DK, 16 * i + l16, kb, lg);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        const f32x4_t s0 = S[ct][2 * kb], s1 = S[ct][2 * kb + 1];
+                        const float s8[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
+                        split8<PC>(s8, so[ct]);
+                    }
+#pragma unroll
+                    for (int x = PC - 1; x >= 0; --x)  // (the small products first, all tiles of one before the next)
+#pragma unroll
+                        for (int p = 0; p < P; ++p)
+                            if (x - p >= 0)
+#pragma unroll
+                                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                                    for (int i = 0; i < MT; ++i)
+                                        O[ct][i] = mfma32(__builtin_bit_cast(bf16x8_t, so[ct][x - p]),
+                                                          __builtin_bit_cast(bf16x8_t, qo[i][p]), O[ct][i]);
+                }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    const int row = 16 * i + l16, col = n0 + 16 * w + 4 * lg;
-                    float sum = 0.f;
-                    if (row < cnt) {
-                        const int64_t tok = start + (a.reverse ? first + cnt - 1 - row : first + row);
-                        const int64_t at = xb + tok * a.x_st + static_cast<int64_t>(ho) * a.x_sh + col;
+                    const float e = s_into[buf][16 * i + l16];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (col + r < a.D) {
-                                const float x = P == 1 ? bf16_to_f32(static_cast<const uint16_t*>(a.aux)[at + r])
-                                                       : static_cast<const float*>(a.aux)[at + r];
-                                sum += x * O[i][r];
-                            }
+                    for (int ct = 0; ct < CT; ++ct) O[ct][i] *= e;
+                }
+                if constexpr (AUX) {
+                    // each token's product of that part with the row of `aux` (q for gq, k for gk)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        float sum = 0.f;
+#pragma unroll
+                        for (int r = 0; r < XN; ++r) sum += aux[i][r] * O[r / 4][i][r % 4];
+                        sum += __shfl_xor(sum, 16);
+                        sum += __shfl_xor(sum, 32);
+                        if (lg == 0) s_part[w][16 * i + l16] = sum;
                     }
-                    sum += __shfl_xor(sum, 16);
-                    sum += __shfl_xor(sum, 32);
-                    if (lg == 0) s_part[w][row] = sum;
                 }
             }
+        }
+        if (first_m) {
+            if (KIND == kPassGq && (first / C) % a.keep == 0 && ho0 % (a.HO / a.HS) == 0) {
+                f32x4_t* kept = reinterpret_cast<f32x4_t*>(a.kept) +
+                                ((state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile) * (CT * MD * 256);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int md = 0; md < MD; ++md) kept[((w * CT + ct) * MD + md) * 64 + lane] = S[ct][md];
+            }
+            log_total += chunk_log;
+        }
+        const bool update = !dst || last_m;
+        if (dst ? last_m : first_m) {
             const float e = exp2_f64(chunk_log);
 #pragma unroll
-            for (int md = 0; md < MD; ++md) S[md] *= e;
-            log_total += chunk_log;
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int md = 0; md < MD; ++md) S[ct][md] *= e;
         }
         // ---- A V, and the state
 #pragma unroll
         for (int kb = 0; kb < MT / 2; ++kb) {
-            // V of tokens 32 kb + {4 lg + [0, 4), 16 + 4 lg + [0, 4)}, column 16 w + l16
+            // V of tokens 32 kb + {4 lg + [0, 4), 16 + 4 lg + [0, 4)}, columns n(ct, l16)
             const int j4 = (lane >> 2) & 3, cc = lane & 3, row = 4 * lg + j4;
-            const unsigned va = lds_addr(sv + (32 * kb + row) * kDecayCols +
-                                         8 * ((2 * w + (cc >> 1)) ^ vf(row)) + 4 * (cc & 1));
-            constexpr int R16 = 16 * kDecayCols * 2, VP = C * kDecayCols * 2;
-            u32x4_t vo[P];
-            f32x4_t x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
-            if constexpr (P == 1) {
-                u32x2_t lo, hi;
-                tr2<0, R16>(va, lo, hi);
-                vo[0] = join(lo, hi);
-                x0 = widen4(lo), x1 = widen4(hi);
-            } else {
-                u32x2_t lo[3], hi[3];
-                tr2<0, R16>(va, lo[0], hi[0]);
-                tr2<VP, VP + R16>(va, lo[1], hi[1]);
-                tr2<2 * VP, 2 * VP + R16>(va, lo[2], hi[2]);
+            const unsigned va = lds_addr(sv + (32 * kb + row) * NT +
+                                         (CT == 1 ? 8 * ((2 * w + (cc >> 1)) ^ vf<NT>(row)) + 4 * (cc & 1)
+                                                  : 8 * ((4 * w + cc) ^ vf<NT>(row))));
+            constexpr int R16 = 16 * NT * 2, VP = C * NT * 2;
+            u32x4_t vo[CT][P];
+            f32x4_t x0[CT], x1[CT];
 #pragma unroll
-                for (int p = 2; p >= 0; --p) {
-                    vo[p] = join(lo[p], hi[p]);
-                    x0 += widen4(lo[p]), x1 += widen4(hi[p]);
+            for (int ct = 0; ct < CT; ++ct) x0[ct] = x1[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            auto take = [&](int p, u32x2_t lo0, u32x2_t hi0, u32x2_t lo1, u32x2_t hi1) {
+                vo[0][p] = join(lo0, hi0);
+                x0[0] += widen4(lo0), x1[0] += widen4(hi0);
+                if (CT == 2) {
+                    vo[CT - 1][p] = join(lo1, hi1);
+                    x0[CT - 1] += widen4(lo1), x1[CT - 1] += widen4(hi1);
                 }
+            };
+            u32x2_t b0, b1, b2 = {0u, 0u}, b3 = {0u, 0u};
+            if constexpr (P == 3) {  // (the smallest parts first)
+                if constexpr (CT == 1) tr2<2 * VP, 2 * VP + R16>(va, b0, b1);
+                else tr4<2 * VP, 2 * VP + R16, 2 * VP + 8, 2 * VP + 8 + R16>(va, b0, b1, b2, b3);
+                take(2 % P, b0, b1, b2, b3);
+                if constexpr (CT == 1) tr2<VP, VP + R16>(va, b0, b1);
+                else tr4<VP, VP + R16, VP + 8, VP + 8 + R16>(va, b0, b1, b2, b3);
+                take(1 % P, b0, b1, b2, b3);
             }
+            if constexpr (CT == 1) tr2<0, R16>(va, b0, b1);
+            else tr4<0, R16, 8, 8 + R16>(va, b0, b1, b2, b3);
+            take(0, b0, b1, b2, b3);
             if (OUT) {
+                u32x4_t ao[MT][PC];
 #pragma unroll
-                for (int i = 2 * kb; i < MT; ++i) {
-                    u32x4_t ao[PC];
+                for (int i = 2 * kb; i < MT; ++i)
 #pragma unroll
                     for (int p = 0; p < PC; ++p)
-                        ao[p] = *reinterpret_cast<const u32x4_t*>(sa + (p * Sh::BLK + qblk(i, kb)) * 512 + lane * 8);
-                    O[i] = mfma_planes<P, PC>(vo, ao, O[i]);
-                }
-            }
-            float v8[8];
+                        ao[i][p] = *reinterpret_cast<const u32x4_t*>(sa + (p * Sh::BLK + qblk(i, kb)) * 512 + lane * 8);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                v8[r] = x0[r] * s_out[32 * kb + 4 * lg + r];
-                v8[4 + r] = x1[r] * s_out[32 * kb + 16 + 4 * lg + r];
+                for (int x = PC - 1; x >= 0; --x)
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+                        if (x - p >= 0)
+#pragma unroll
+                            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                                for (int i = 2 * kb; i < MT; ++i)
+                                    O[ct][i] = mfma32(__builtin_bit_cast(bf16x8_t, vo[ct][p]),
+                                                      __builtin_bit_cast(bf16x8_t, ao[i][x - p]), O[ct][i]);
             }
-            u32x4_t wo[PC];
-            split8<PC>(v8, wo);
+            if (!update) continue;
+            u32x4_t wo[CT][PC];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                float v8[8];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    v8[r] = x0[ct][r] * s_out[buf][32 * kb + 4 * lg + r];
+                    v8[4 + r] = x1[ct][r] * s_out[buf][32 * kb + 16 + 4 * lg + r];
+                }
+                split8<PC>(v8, wo[ct]);
+            }
 #pragma unroll
             for (int d32 = 0; d32 < KB; ++d32) {
                 // K^T: rows 32 d32 + 8 .. (s_row_d of tiles 2 d32 and 2 d32 + 1), the same tokens
                 const unsigned ka = lds_addr(sk + (32 * kb + row) * DK + 8 * ((4 * d32 + cc) ^ kf<DK>(row)));
                 constexpr int K16 = 16 * DK * 2, KP = C * DK * 2;
-                u32x4_t k0[P], k1[P];
-                u32x2_t a0, a1, b0, b1;
+                u32x4_t ko[2][P];
+                u32x2_t a0, a1;
                 tr4<0, K16, 8, 8 + K16>(ka, a0, a1, b0, b1);
-                k0[0] = join(a0, a1), k1[0] = join(b0, b1);
+                ko[0][0] = join(a0, a1), ko[1][0] = join(b0, b1);
                 if constexpr (P == 3) {
                     tr4<KP, KP + K16, KP + 8, KP + 8 + K16>(ka, a0, a1, b0, b1);
-                    k0[1] = join(a0, a1), k1[1] = join(b0, b1);
+                    ko[0][1] = join(a0, a1), ko[1][1] = join(b0, b1);
                     tr4<2 * KP, 2 * KP + K16, 2 * KP + 8, 2 * KP + 8 + K16>(ka, a0, a1, b0, b1);
-                    k0[2] = join(a0, a1), k1[2] = join(b0, b1);
+                    ko[0][2] = join(a0, a1), ko[1][2] = join(b0, b1);
                 }
-                S[2 * d32] = mfma_planes<P, PC>(k0, wo, S[2 * d32]);
-                S[2 * d32 + 1] = mfma_planes<P, PC>(k1, wo, S[2 * d32 + 1]);
+#pragma unroll
+                for (int x = PC - 1; x >= 0; --x)
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+                        if (x - p >= 0)
+#pragma unroll
+                            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    S[ct][2 * d32 + h] = mfma32(__builtin_bit_cast(bf16x8_t, ko[h][p]),
+                                                                __builtin_bit_cast(bf16x8_t, wo[ct][x - p]),
+                                                                S[ct][2 * d32 + h]);
             }
         }
         // ---- outputs
-        if (OUT && m == n_src - 1) {
+        if (OUT && (dst || last_m)) {
+            const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg), left = a.D - col;
+            const int64_t tok = rows0 + (a.reverse ? first + cnt - 1 : first);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const int row = 16 * i + l16, col = n0 + 16 * w + 4 * lg;
-                if (row >= cnt || col >= a.D) continue;
-                const int64_t tok = rows0 + (a.reverse ? first + cnt - 1 - row : first + row);
-                const int64_t at = (tok * HO + ho) * a.D + col;
-                const int left = a.D - col;
+                const int row = 16 * i + l16;
+                if (row >= cnt || left <= 0) continue;
+                const int64_t at = ((tok + sgn * row) * a.HO + ho) * a.D + col;
+                float v[4 * CT];
+#pragma unroll
+                for (int r = 0; r < 4 * CT; ++r) v[r] = O[r / 4][i][r % 4];
                 if (a.out_bf16) {
                     uint16_t* o = static_cast<uint16_t*>(a.o) + at;
-                    const u32x2_t v = cvt4(O[i]);
-                    if (left >= 4) __builtin_memcpy(o, &v, 8);
+                    uint32_t p[2 * CT];
+#pragma unroll
+                    for (int r = 0; r < 2 * CT; ++r) p[r] = pack2(v[2 * r], v[2 * r + 1]);
+                    if (left >= 4 * CT) __builtin_memcpy(o, p, sizeof p);
                     else
-                        for (int r = 0; r < left; ++r) o[r] = static_cast<uint16_t>((r < 2 ? v.x : v.y) >> (16 * (r & 1)));
+#pragma unroll
+                        for (int r = 0; r < 4 * CT; ++r)
+                            if (r < left) o[r] = static_cast<uint16_t>(p[r / 2] >> (16 * (r & 1)));
                 } else {
                     float* o = static_cast<float*>(a.o) + at;
-                    if (left >= 4) __builtin_memcpy(o, &O[i], 16);
+                    if (left >= 4 * CT) __builtin_memcpy(o, v, sizeof v);
                     else
-                        for (int r = 0; r < left; ++r) o[r] = O[i][r];
+#pragma unroll
+                        for (int r = 0; r < 4 * CT; ++r)
+                            if (r < left) o[r] = v[r];
                 }
             }
             if (KIND == kPassGk && (first / C) % a.keep == 0) {
                 // dL/dg of the chunk's first token: e^g <the state before it, the gradient after it>
                 const f32x4_t* kept = reinterpret_cast<const f32x4_t*>(a.kept) +
-                                      ((state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile) * frag;
+                                      ((state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile) * (CT * MD * 256);
                 float dot = 0.f;
 #pragma unroll
-                for (int md = 0; md < MD; ++md) {
-                    const f32x4_t x = kept[(w * MD + md) * 64 + lane] * S[md];
-                    dot += (x[0] + x[1]) + (x[2] + x[3]);
-                }
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int md = 0; md < MD; ++md) {
+                        const f32x4_t x = kept[((w * CT + ct) * MD + md) * 64 + lane] * S[ct][md];
+                        dot += (x[0] + x[1]) + (x[2] + x[3]);
+                    }
                 dot = wave_sum_row3(dot);
                 if (lane == 63) s_dot[w] = dot;
             }
         }
         lds_barrier();
         if constexpr (AUX)
-            if (m == 0 && t < cnt) {
+            if ((dst || first_m) && t < cnt) {
                 const int64_t tok = rows0 + (a.reverse ? first + cnt - 1 - t : first + t);
-                a.part[(static_cast<int64_t>(tile) * a.n_rows + tok) * HO + ho] =
+                a.part[(static_cast<int64_t>(tile) * a.n_rows + tok) * a.HO + ho] =
                     (s_part[0][t] + s_part[1][t]) + (s_part[2][t] + s_part[3][t]);
             }
-        if (KIND == kPassGk && m == n_src - 1 && t == 0 && (first / C) % a.keep == 0) {
-            const float e = exp2_f64(log2_decay(a.g[gb + (start + first) * a.g_st + hs]));
+        if (KIND == kPassGk && last_m && t == 0 && (first / C) % a.keep == 0) {
+            const float e = exp2_f64(log2_decay(gp[(start + first) * a.g_st]));
             a.cross[(state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile] =
                 e * ((s_dot[0] + s_dot[1]) + (s_dot[2] + s_dot[3]));
         }
     }
 
     // ---- the state after the span
-    if (KIND == kPassState) {
-        const int64_t at = state_pair * a.n_spans + order;
-        f32x4_t* u = reinterpret_cast<f32x4_t*>(a.span_state) + (at * a.n_tiles + tile) * frag;
-#pragma unroll
-        for (int md = 0; md < MD; ++md) u[(w * MD + md) * 64 + lane] = S[md];
-        if (tile == 0 && t == 0) a.span_log[at] = log_total;
-    } else if (a.s_out && order == n_spans - 1 && ho % (HO / a.HS) == 0 && stored) {
-        float e = 1.f;
-        if (a.reverse && len > 0) e = exp2_f64(log2_decay(a.g[gb + start * a.g_st + hs]));
-        float* so = a.s_out + slot_pair * a.D * a.D;
-#pragma unroll
-        for (int md = 0; md < MD; ++md)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = s_row_d(md, 4 * lg + r);
-                if (d < a.D && n < a.D) so[static_cast<int64_t>(d) * a.s_row + static_cast<int64_t>(n) * a.s_col] = e * S[md][r];
-            }
+    float* to = nullptr;
+    int64_t row = a.s_row, col = a.s_col;
+    float e = 1.f;
+    if (!OUT) {  // (the next span's place: the scan over spans turns shares into states)
+        to = a.span_state + (static_cast<int64_t>(slot_id + 1) * a.HS + hs) * a.D * a.D;
+        row = a.u_row, col = a.u_col;
+        if (tile == 0 && t == 0) a.span_log[static_cast<int64_t>(slot_id + 1) * a.HS + hs] = log_total;
+    } else if (a.s_out && order == n_spans - 1 && ho0 % (a.HO / a.HS) == 0 && stored) {
+        to = a.s_out + slot_pair * a.D * a.D;
+        if (a.reverse && len > 0) e = exp2_f64(log2_decay(gp[start * a.g_st]));
     }
+    if (to)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int md = 0; md < MD; ++md) {
+                const int d0 = s_row_d(md, 4 * lg);
+                float* p = to + d0 * row + n_col[ct] * col;
+                S[ct][md] *= e;
+                if (row == 1 && a.D % 4 == 0) {
+                    if (d0 < a.D && n_col[ct] < a.D) __builtin_memcpy(p, &S[ct][md], 16);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (d0 + r < a.D && n_col[ct] < a.D) p[r * row] = S[ct][md][r];
+                }
+            }
 }
 
 // ---- dL/dg ------------------------------------------------------------------------------------
@@ -750,10 +913,10 @@ __global__ __launch_bounds__(P == 1 ? 256 : 512) void decay_gate_grad(DecayGateG
 }
 
 template <int P, int DK>
-hipError_t launch_pass(const DecayPass& a, int kind, int n_spans, hipStream_t st) {
-    const int heads = kind == kPassState ? a.HS : a.HO;
-    const int64_t pairs = static_cast<int64_t>(a.n_seqs) * heads;
-    const dim3 grid(static_cast<unsigned>((pairs + 7) / 8 * 8 * a.n_tiles), static_cast<unsigned>(n_spans));
+hipError_t launch_pass(const DecayPass& a, int kind, hipStream_t st) {
+    const int groups = kind == kPassState ? a.HS : a.HO / a.n_dst;
+    const int64_t units = static_cast<int64_t>(a.n_slots_grid) * groups;
+    const dim3 grid(static_cast<unsigned>((units + 7) / 8 * 8 * a.n_tiles));
     switch (kind) {
         case kPassPlain: hipLaunchKernelGGL((decay_pass<P, DK, kPassPlain>), grid, dim3(256), 0, st, a); break;
         case kPassGq: hipLaunchKernelGGL((decay_pass<P, DK, kPassGq>), grid, dim3(256), 0, st, a); break;
@@ -763,17 +926,11 @@ hipError_t launch_pass(const DecayPass& a, int kind, int n_spans, hipStream_t st
     return hipGetLastError();
 }
 
-// One pass: the states of all spans but the last where there are several, then the outputs.
 template <int P>
 hipError_t run_pass(const DecayPass& a, int kind, hipStream_t st) {
-    auto go = [&](int what, int spans) {
-        if (a.D <= 64) return launch_pass<P, 64>(a, what, spans, st);
-        if (a.D <= 128) return launch_pass<P, 128>(a, what, spans, st);
-        return launch_pass<P, 256>(a, what, spans, st);
-    };
-    if (a.n_spans > 1)
-        if (hipError_t e = go(kPassState, a.n_spans - 1); e != hipSuccess) return e;
-    return go(kind, a.n_spans);
+    if (a.D <= 64) return launch_pass<P, 64>(a, kind, st);
+    if (a.D <= 128) return launch_pass<P, 128>(a, kind, st);
+    return launch_pass<P, 256>(a, kind, st);
 }
 
 template <int P>

@@ -40,7 +40,8 @@ bool decay_sizes_fit(int n, int T, int Hq, int H, int D) {
     const int64_t rows = static_cast<int64_t>(n) * std::max(T, 1);
     return rows <= kMaxElems / (static_cast<int64_t>(Hq) * D) &&
            static_cast<int64_t>(n) * H <= kMaxElems / (static_cast<int64_t>(D) * D) &&
-           pm::decay_attn_groups(n, T, Hq, D) <= INT32_MAX && static_cast<int64_t>(n) * H * (T / 256 + 1) <= INT32_MAX;
+           pm::decay_attn_groups(n, T, Hq, H, D, false) <= INT32_MAX &&
+           pm::decay_attn_groups(n, T, Hq, H, D, true) <= INT32_MAX && static_cast<int64_t>(n) * H * (T / 256 + 1) <= INT32_MAX;
 }
 
 // Sizes, types and strides that the calls of K14 share.
@@ -74,9 +75,10 @@ const char* const kAlign = "every buffer must be aligned to its element size";
 
 extern "C" {
 
-size_t pm_decay_attention_workspace_bytes(int n_seqs, int T, int Hq, int H, int D, int in_place) {
+size_t pm_decay_attention_workspace_bytes(int n_seqs, int T, int Hq, int H, int D, int packed,
+                                          int in_place) {
     if (!decay_sizes_fit(n_seqs, T, Hq, H, D)) return 0;
-    return pm::decay_attn_ws_bytes(n_seqs, T, Hq, H, D, in_place != 0);
+    return pm::decay_attn_ws_bytes(n_seqs, T, Hq, H, D, packed != 0, in_place != 0);
 }
 
 int pm_decay_attention(const void* q, const void* k, const void* v, const float* g, const int32_t* cu_seqlens,
@@ -96,7 +98,9 @@ int pm_decay_attention(const void* q, const void* k, const void* v, const float*
         !aligned(s0, 4) || !aligned(s_out, 4) || !aligned(cu_seqlens, 4) || !aligned(slots, 4) || !aligned(bad_slot, 4) ||
         !aligned(cu_flag, 4))
         return fail(PM_E_ALIGN, "%s", kAlign);
-    if (int rc = check_ws(pm::decay_attn_ws_bytes(n_seqs, T, Hq, H, D, s0 && s0 == s_out), workspace, ws_bytes)) return rc;
+    if (int rc = check_ws(pm::decay_attn_ws_bytes(n_seqs, T, Hq, H, D, cu_seqlens != nullptr, s0 && s0 == s_out),
+                          workspace, ws_bytes))
+        return rc;
     pm::DecayAttnArgs a{q, k, v, strides, g, g_sb, g_st, cu_seqlens, cu_flag, s0, s_out, slots, n_slots, bad_slot, o,
                         n_seqs, T, Hq, H, D, dtype == PM_DTYPE_BF16, out_dtype == PM_DTYPE_BF16, scale, workspace};
     hipError_t e = pm::launch_decay_attn(a, static_cast<hipStream_t>(stream));

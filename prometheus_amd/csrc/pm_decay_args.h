@@ -8,6 +8,9 @@ namespace pm {
 
 constexpr int kDecayKeep = 256;  // tokens between the states kept for the gates' gradient
 
+// Columns of the state that a workgroup keeps (pm_decay.h: DecayTile).
+constexpr int decay_cols(int D) { return D <= 64 ? 64 : 128; }
+
 // One pass over n_seqs sequences (roles as in pm_decay.h).  Strides are in elements; the elements of
 // a head are contiguous.  HO heads of Q and O, HK of K and V, HS = min(HO, HK) states.
 struct DecayPass {
@@ -18,7 +21,7 @@ struct DecayPass {
     const float* g;  // [b][t][HS], heads contiguous; both strides 0: one constant a head
     int64_t g_sb, g_st;
     const int32_t* cu;  // nullable: packed (T tokens, n_seqs + 1 offsets, clamped into [0, T])
-    const float* s0;    // nullable: zeros
+    const float* s0;    // nullable: zeros; not read where span_state is given
     float* s_out;       // nullable
     int64_t s_row, s_col;  // strides of a state's rows (K's dimension) and columns (V's)
     const int32_t* slots;  // nullable: sequence i's state is row slots[i] of the pool s0, s_out
@@ -28,10 +31,15 @@ struct DecayPass {
     void* o;            // contiguous (.., HO, D)
     bool out_bf16, reverse;
     int n_seqs, T, HO, HK, HS, D;
-    int n_tiles;        // ceil(D / 64): column tiles
-    int span, n_spans;  // tokens a workgroup walks through, and workgroups along the longest sequence
-    float* span_state;  // [state][span][tile] accumulators: each span's own share of the state
-    double* span_log;   // [state][span] sum of its log-decays, in units of log 2
+    int n_dst;          // output heads a workgroup takes, one after another (1 where HK > HO)
+    int n_tiles;        // column tiles of decay_cols(D)
+    // Spans: workgroups along a sequence.  Slot i is span i % n_spans of sequence i / n_spans, or
+    // (packed) slot_table[i] = (sequence, span), sequence -1: none; a sequence's slots are in a row.
+    int span, n_spans, n_slots_grid;
+    const int2* slot_table;
+    float* span_state;  // nullable: [slot][HS] states before the spans, (D, D) with strides u_row, u_col
+    int64_t u_row, u_col;
+    double* span_log;   // [slot][HS] the log-decay of the span before, in units of log 2
     float a_scale, into_scale, out_scale;  // of A, of the state's part of O, of what enters the state
     // for the gates' gradient
     const void* aux;    // q (gq's pass), k (gk's)
@@ -61,7 +69,8 @@ struct DecayGateGrad {
     float scale;
 };
 
-// kind: 0 outputs and state only, 1 gq's pass with its share of the gates' gradient, 2 gk's.
+// kind: 0 outputs and state only, 1 gq's pass with its share of the gates' gradient, 2 gk's,
+// 3 each span's own share of the state (from zeros) but the last one's, to the next slot of span_state.
 hipError_t decay_pass_bf16(const DecayPass& a, int kind, hipStream_t st);
 hipError_t decay_pass_f32(const DecayPass& a, int kind, hipStream_t st);
 hipError_t decay_gate_grad_bf16(const DecayGateGrad& a, hipStream_t st);

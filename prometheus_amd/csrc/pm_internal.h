@@ -364,10 +364,8 @@ struct DecayAttnArgs {
     void* workspace;
 };
 hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st);
-size_t decay_attn_ws_bytes(int n_seqs, int T, int Hq, int H, int D, bool in_place);
-// Workgroups along the grid's x, and spans along its y.
-int64_t decay_attn_groups(int n_seqs, int T, int Hq, int D);
-int decay_attn_spans(int n_seqs, int T, int Hq, int D);
+size_t decay_attn_ws_bytes(int n_seqs, int T, int Hq, int H, int D, bool packed, bool in_place);
+int64_t decay_attn_groups(int n_seqs, int T, int Hq, int H, int D, bool packed);  // workgroups of its grid
 
 // Its gradients; go contiguous in q's type, gq, gk, gv contiguous in it; gg (B, T, H), or (H) where
 // both of g's strides are 0 (nullable: not wanted).

@@ -114,19 +114,29 @@ __device__ __forceinline__ void store_part(const float (&g)[NV][8], float* lds, 
     }
 }
 
-// gw[c] = the sum over n parts, a wave for 16 columns, in an order that does not change
-__global__ __launch_bounds__(256) void sum_row_parts(const float* part, float* gw, int n, int C) {
-    __shared__ float s[16][17];
+// gw[c] = the sum over n parts, 64 threads for each of 16 columns, in an order that does not change; row
+// blockIdx.y is another weight's.
+struct RowParts {
+    float* gw[2];
+};
+__global__ __launch_bounds__(1024) void sum_row_parts(const float* part, RowParts to, int n, int C) {
+    __shared__ float s[64][17];
     const int col = blockIdx.x * 16 + threadIdx.x % 16, first = threadIdx.x / 16;
-    float x = 0.f;
+    float* gw = to.gw[blockIdx.y];
+    if (!gw) return;
+    const float* p = part + static_cast<int64_t>(blockIdx.y) * n * C;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};  // (four loads in flight)
     if (col < C)
-        for (int i = first; i < n; i += 16) x += part[static_cast<int64_t>(i) * C + col];
-    s[first][threadIdx.x % 16] = x;
+        for (int i = first; i < n; i += 256)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + 64 * j < n) x[j] += p[static_cast<int64_t>(i + 64 * j) * C + col];
+    s[first][threadIdx.x % 16] = (x[0] + x[1]) + (x[2] + x[3]);
     __syncthreads();
     if (threadIdx.x < 16 && col < C) {
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += s[i][threadIdx.x];
+        for (int i = 0; i < 64; ++i) sum += s[i][threadIdx.x];
         gw[col] = sum;
     }
 }

@@ -131,16 +131,10 @@ int64_t residual_norm_groups(int64_t rows, int C) { return row_groups(rows, C); 
 hipError_t launch_residual_norm(const ResidualNormArgs& a, hipStream_t st) { return by_types<false>(a, st); }
 
 hipError_t launch_residual_norm_bwd(const ResidualNormArgs& a, hipStream_t st) {
-    if (hipError_t e = by_types<true>(a, st); e != hipSuccess) return e;
-    const int n = static_cast<int>(residual_norm_groups(a.rows, a.C));
-    for (int s = 0; s < 2; ++s) {
-        float* gw = s ? a.gwp : a.gw;
-        if (!gw) continue;
-        hipLaunchKernelGGL(sum_row_parts, dim3(static_cast<unsigned>((a.C + 15) / 16)), dim3(256), 0, st,
-                           a.part + (s ? static_cast<int64_t>(n) * a.C : 0), gw, n, a.C);
-        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    }
-    return hipSuccess;
+    if (hipError_t e = by_types<true>(a, st); e != hipSuccess || !(a.gw || a.gwp)) return e;
+    hipLaunchKernelGGL(sum_row_parts, dim3(static_cast<unsigned>((a.C + 15) / 16), a.gwp ? 2 : 1), dim3(1024), 0, st, a.part,
+                       RowParts{{a.gw, a.gwp}}, static_cast<int>(residual_norm_groups(a.rows, a.C)), a.C);
+    return hipGetLastError();
 }
 
 }  // namespace pm

@@ -54,8 +54,8 @@ def _strides(*values):
 
 
 @functools.lru_cache(maxsize=1024)
-def _ws_bytes(n_seqs, T, Hq, H, D, in_place) -> int:
-    return _native.lib().pm_decay_attention_workspace_bytes(n_seqs, T, Hq, H, D, in_place)
+def _ws_bytes(n_seqs, T, Hq, H, D, packed, in_place) -> int:
+    return _native.lib().pm_decay_attention_workspace_bytes(n_seqs, T, Hq, H, D, packed, in_place)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -123,7 +123,7 @@ def _launch(call, qd, kd, vd, gd, g_strides, cu, flag, s0, slots, n_slots, bad, 
     ptr = _k._ptr
     Hq, H, D = qd.shape[2], kd.shape[2], qd.shape[3]
     in_place = s0 is not None and s0.data_ptr() == s_out.data_ptr()
-    nbytes = _ws_bytes(n_seqs, T, Hq, H, D, in_place)
+    nbytes = _ws_bytes(n_seqs, T, Hq, H, D, cu is not None, in_place)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=call.device) if nbytes else None
     _native.check(_native.lib().pm_decay_attention(
         ptr(qd), ptr(kd), ptr(vd), ptr(gd), ptr(cu), ptr(s0), ptr(slots), n_slots, ptr(bad), ptr(flag), ptr(o),
