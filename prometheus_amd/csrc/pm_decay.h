@@ -152,6 +152,18 @@ __device__ __forceinline__ void tr2(unsigned addr, u32x2_t& a, u32x2_t& b) {
                      "s_waitcnt lgkmcnt(0)"
                      : "=&v"(a), "=&v"(b) : "v"(addr), "n"(O0), "n"(O1) : "memory");
 }
+template <int O0, int O1, int O2, int O3, int O4, int O5, int O6, int O7>
+__device__ __forceinline__ void tr8(unsigned addr, u32x2_t (&r)[8]) {
+    __asm__ volatile("ds_read_b64_tr_b16 %0, %8 offset:%9\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+                     "ds_read_b64_tr_b16 %2, %8 offset:%11\n\tds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %4, %8 offset:%13\n\tds_read_b64_tr_b16 %5, %8 offset:%14\n\t"
+                     "ds_read_b64_tr_b16 %6, %8 offset:%15\n\tds_read_b64_tr_b16 %7, %8 offset:%16\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]),
+                       "=&v"(r[7])
+                     : "v"(addr), "n"(O0), "n"(O1), "n"(O2), "n"(O3), "n"(O4), "n"(O5), "n"(O6), "n"(O7)
+                     : "memory");
+}
 template <int O0, int O1, int O2, int O3>
 __device__ __forceinline__ void tr4(unsigned addr, u32x2_t& a, u32x2_t& b, u32x2_t& c, u32x2_t& d) {
     __asm__ volatile("ds_read_b64_tr_b16 %0, %4 offset:%5\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
@@ -490,7 +502,8 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int col = 16 * j + 4 * lg + r;
-                    A[r] = col <= row ? (acc[0][r] + acc[1][r]) * (exp2_diff(gi, sg[buf][col]) * a.a_scale) : 0.f;
+                    const float x = (acc[0][r] + acc[1][r]) * (exp2_diff(gi, sg[buf][col]) * a.a_scale);
+                    A[r] = col <= row ? x : 0.f;
                 }
                 u32x2_t ap[PC];
                 split4<PC>(A, ap);
@@ -499,7 +512,6 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                     *reinterpret_cast<u32x2_t*>(sa + (p * Sh::BLK + qblk(i, j >> 1)) * 512 + lane * 8 + 4 * (j & 1)) =
                         ap[p];
             }
-            lds_barrier();
         }
 
         const double chunk_log = s_total[buf];
@@ -507,28 +519,26 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
             if (OUT) {
                 // ---- the state's part of the outputs
                 constexpr int XN = 4 * CT;  // a lane's columns in a row
-                float aux[AUX ? MT : 1][XN];
+                uint32_t aux[AUX ? MT : 1][P == 1 ? XN / 2 : XN];  // as they are in memory
                 if constexpr (AUX) {
                     const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg);
                     const int64_t tok = start + (a.reverse ? first + cnt - 1 : first);
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        const int row = 16 * i + l16;
+                        const int row = 16 * i + l16, left = row < cnt ? a.D - col : 0;
                         const E* x = xp + (tok + sgn * row) * a.x_st + static_cast<int64_t>(ho) * a.x_sh + col;
-                        const int left = row < cnt ? a.D - col : 0;
                         if (left >= XN) {
-                            if constexpr (P == 1) {
-                                uint32_t raw[XN / 2];
-                                __builtin_memcpy(raw, x, sizeof raw);
-#pragma unroll
-                                for (int r = 0; r < XN; ++r)
-                                    aux[i][r] = __uint_as_float(r % 2 ? raw[r / 2] & 0xffff0000u : raw[r / 2] << 16);
-                            } else {
-                                __builtin_memcpy(aux[i], x, sizeof aux[i]);
-                            }
+                            __builtin_memcpy(aux[i], x, sizeof aux[i]);
                         } else {
 #pragma unroll
-                            for (int r = 0; r < XN; ++r) aux[i][r] = r < left ? to_f32(x[r]) : 0.f;
+                            for (int r = 0; r < XN; ++r) {
+                                if constexpr (P == 1) {
+                                    const uint32_t v = r < left ? x[r] : 0;
+                                    aux[i][r / 2] = r % 2 ? aux[i][r / 2] | v << 16 : v;
+                                } else {
+                                    aux[i][r] = r < left ? __float_as_uint(x[r]) : 0u;
+                                }
+                            }
                         }
                     }
                 }
@@ -573,7 +583,10 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                     for (int i = 0; i < MT; ++i) {
                         float sum = 0.f;
 #pragma unroll
-                        for (int r = 0; r < XN; ++r) sum += aux[i][r] * O[r / 4][i][r % 4];
+                        for (int r = 0; r < XN; ++r) {
+                            const uint32_t v = P == 1 ? (r % 2 ? aux[i][r / 2] & 0xffff0000u : aux[i][r / 2] << 16) : aux[i][r % (P == 1 ? 1 : XN)];
+                            sum += __uint_as_float(v) * O[r / 4][i][r % 4];
+                        }
                         sum += __shfl_xor(sum, 16);
                         sum += __shfl_xor(sum, 32);
                         if (lg == 0) s_part[w][16 * i + l16] = sum;
@@ -600,24 +613,24 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 #pragma unroll
                 for (int md = 0; md < MD; ++md) S[ct][md] *= e;
         }
-        // ---- A V, and the state
+        // ---- V, and the state
+        u32x4_t vo[MT / 2][CT][P];
+        const int j4 = (lane >> 2) & 3, cc = lane & 3, row_t = 4 * lg + j4;  // of the transposed reads
 #pragma unroll
         for (int kb = 0; kb < MT / 2; ++kb) {
             // V of tokens 32 kb + {4 lg + [0, 4), 16 + 4 lg + [0, 4)}, columns n(ct, l16)
-            const int j4 = (lane >> 2) & 3, cc = lane & 3, row = 4 * lg + j4;
-            const unsigned va = lds_addr(sv + (32 * kb + row) * NT +
-                                         (CT == 1 ? 8 * ((2 * w + (cc >> 1)) ^ vf<NT>(row)) + 4 * (cc & 1)
-                                                  : 8 * ((4 * w + cc) ^ vf<NT>(row))));
+            const unsigned va = lds_addr(sv + (32 * kb + row_t) * NT +
+                                         (CT == 1 ? 8 * ((2 * w + (cc >> 1)) ^ vf<NT>(row_t)) + 4 * (cc & 1)
+                                                  : 8 * ((4 * w + cc) ^ vf<NT>(row_t))));
             constexpr int R16 = 16 * NT * 2, VP = C * NT * 2;
-            u32x4_t vo[CT][P];
             f32x4_t x0[CT], x1[CT];
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) x0[ct] = x1[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
             auto take = [&](int p, u32x2_t lo0, u32x2_t hi0, u32x2_t lo1, u32x2_t hi1) {
-                vo[0][p] = join(lo0, hi0);
+                vo[kb][0][p] = join(lo0, hi0);
                 x0[0] += widen4(lo0), x1[0] += widen4(hi0);
                 if (CT == 2) {
-                    vo[CT - 1][p] = join(lo1, hi1);
+                    vo[kb][CT - 1][p] = join(lo1, hi1);
                     x0[CT - 1] += widen4(lo1), x1[CT - 1] += widen4(hi1);
                 }
             };
@@ -633,25 +646,6 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
             if constexpr (CT == 1) tr2<0, R16>(va, b0, b1);
             else tr4<0, R16, 8, 8 + R16>(va, b0, b1, b2, b3);
             take(0, b0, b1, b2, b3);
-            if (OUT) {
-                u32x4_t ao[MT][PC];
-#pragma unroll
-                for (int i = 2 * kb; i < MT; ++i)
-#pragma unroll
-                    for (int p = 0; p < PC; ++p)
-                        ao[i][p] = *reinterpret_cast<const u32x4_t*>(sa + (p * Sh::BLK + qblk(i, kb)) * 512 + lane * 8);
-#pragma unroll
-                for (int x = PC - 1; x >= 0; --x)
-#pragma unroll
-                    for (int p = 0; p < P; ++p)
-                        if (x - p >= 0)
-#pragma unroll
-                            for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                                for (int i = 2 * kb; i < MT; ++i)
-                                    O[ct][i] = mfma32(__builtin_bit_cast(bf16x8_t, vo[ct][p]),
-                                                      __builtin_bit_cast(bf16x8_t, ao[i][x - p]), O[ct][i]);
-            }
             if (!update) continue;
             u32x4_t wo[CT][PC];
 #pragma unroll
@@ -667,17 +661,17 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 #pragma unroll
             for (int d32 = 0; d32 < KB; ++d32) {
                 // K^T: rows 32 d32 + 8 .. (s_row_d of tiles 2 d32 and 2 d32 + 1), the same tokens
-                const unsigned ka = lds_addr(sk + (32 * kb + row) * DK + 8 * ((4 * d32 + cc) ^ kf<DK>(row)));
+                const unsigned ka = lds_addr(sk + (32 * kb + row_t) * DK + 8 * ((4 * d32 + cc) ^ kf<DK>(row_t)));
                 constexpr int K16 = 16 * DK * 2, KP = C * DK * 2;
                 u32x4_t ko[2][P];
                 u32x2_t a0, a1;
                 tr4<0, K16, 8, 8 + K16>(ka, a0, a1, b0, b1);
                 ko[0][0] = join(a0, a1), ko[1][0] = join(b0, b1);
                 if constexpr (P == 3) {
-                    tr4<KP, KP + K16, KP + 8, KP + 8 + K16>(ka, a0, a1, b0, b1);
-                    ko[0][1] = join(a0, a1), ko[1][1] = join(b0, b1);
-                    tr4<2 * KP, 2 * KP + K16, 2 * KP + 8, 2 * KP + 8 + K16>(ka, a0, a1, b0, b1);
-                    ko[0][2] = join(a0, a1), ko[1][2] = join(b0, b1);
+                    u32x2_t x[8];
+                    tr8<KP, KP + K16, KP + 8, KP + 8 + K16, 2 * KP, 2 * KP + K16, 2 * KP + 8, 2 * KP + 8 + K16>(ka, x);
+                    ko[0][1] = join(x[0], x[1]), ko[1][1] = join(x[2], x[3]);
+                    ko[0][2] = join(x[4], x[5]), ko[1][2] = join(x[6], x[7]);
                 }
 #pragma unroll
                 for (int x = PC - 1; x >= 0; --x)
@@ -693,6 +687,46 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                                                                 S[ct][2 * d32 + h]);
             }
         }
+        if (KIND == kPassGk && last_m && (first / C) % a.keep == 0) {
+            // dL/dg of the chunk's first token: e^g <the state before it, the gradient after it>
+            const f32x4_t* kept = reinterpret_cast<const f32x4_t*>(a.kept) +
+                                  ((state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile) * (CT * MD * 256);
+            float dot = 0.f;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int md = 0; md < MD; ++md) {
+                    const f32x4_t x = kept[((w * CT + ct) * MD + md) * 64 + lane] * S[ct][md];
+                    dot += (x[0] + x[1]) + (x[2] + x[3]);
+                }
+            dot = wave_sum_row3(dot);
+            if (lane == 63) s_dot[w] = dot;
+        }
+        // (from here on nothing reads the chunk's rows or log-decays: the next ones may come in; A is
+        // written again only after the barrier that follows them)
+        lds_barrier();
+        // ---- A V
+        if (OUT)
+#pragma unroll
+            for (int kb = 0; kb < MT / 2; ++kb) {
+                u32x4_t ao[MT][PC];
+#pragma unroll
+                for (int i = 2 * kb; i < MT; ++i)
+#pragma unroll
+                    for (int p = 0; p < PC; ++p)
+                        ao[i][p] = *reinterpret_cast<const u32x4_t*>(sa + (p * Sh::BLK + qblk(i, kb)) * 512 + lane * 8);
+#pragma unroll
+                for (int x = PC - 1; x >= 0; --x)
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+                        if (x - p >= 0)
+#pragma unroll
+                            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                                for (int i = 2 * kb; i < MT; ++i)
+                                    O[ct][i] = mfma32(__builtin_bit_cast(bf16x8_t, vo[kb][ct][p]),
+                                                      __builtin_bit_cast(bf16x8_t, ao[i][x - p]), O[ct][i]);
+            }
         // ---- outputs
         if (OUT && (dst || last_m)) {
             const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg), left = a.D - col;
@@ -724,23 +758,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                             if (r < left) o[r] = v[r];
                 }
             }
-            if (KIND == kPassGk && (first / C) % a.keep == 0) {
-                // dL/dg of the chunk's first token: e^g <the state before it, the gradient after it>
-                const f32x4_t* kept = reinterpret_cast<const f32x4_t*>(a.kept) +
-                                      ((state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile) * (CT * MD * 256);
-                float dot = 0.f;
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                    for (int md = 0; md < MD; ++md) {
-                        const f32x4_t x = kept[((w * CT + ct) * MD + md) * 64 + lane] * S[ct][md];
-                        dot += (x[0] + x[1]) + (x[2] + x[3]);
-                    }
-                dot = wave_sum_row3(dot);
-                if (lane == 63) s_dot[w] = dot;
-            }
         }
-        lds_barrier();
         if constexpr (AUX)
             if ((dst || first_m) && t < cnt) {
                 const int64_t tok = rows0 + (a.reverse ? first + cnt - 1 - t : first + t);
