@@ -563,7 +563,7 @@ size_t pm_norm_rotate_bwd_workspace_bytes(int B, int T, int Hq, int Hk, int D);
  *            D) with cu_seqlens: fp32 or bf16, the elements of a head
  *            contiguous; strides: host array of q's batch, token and head
  *            strides, then k's, then v's, in elements (views of a projection
- *            run as they are)
+ *            run as they are), tokens at most 2^23 elements apart
  *   g        fp32, heads contiguous, batch and token strides g_sb, g_st; both 0:
  *            one constant a head
  *   o        contiguous (n_seqs, T, Hq, D), out_dtype

@@ -89,19 +89,22 @@ __device__ __forceinline__ f32x4_t mfma_planes(const u32x4_t (&x)[NX], const u32
 
 // ---- loads from global memory -----------------------------------------------------------------
 
-// Eight elements of a row as they are in memory (P 1: bf16, P 3: fp32), zeros past `n` of them.
+// Eight elements of a row as they are in memory (P 1: bf16, P 3: fp32).
 template <int P>
 struct Raw8 {
-    uint32_t w[P == 1 ? 4 : 8];
+    static constexpr int W = P == 1 ? 4 : 8;
+    using E = typename std::conditional<P == 1, uint16_t, float>::type;
+    uint32_t w[W];
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < (P == 1 ? 4 : 8); ++i) w[i] = 0;
+        for (int i = 0; i < W; ++i) w[i] = 0;
     }
-    __device__ __forceinline__ void load(const void* base, int64_t at, int n) {
-        using E = typename std::conditional<P == 1, uint16_t, float>::type;
-        const E* p = static_cast<const E*>(base) + at;
+    // all eight, at any alignment of the elements
+    __device__ __forceinline__ void load(const void* p) { __builtin_memcpy(w, p, sizeof w); }
+    // the first n (at most 8) of p, zeros behind them
+    __device__ __forceinline__ void load(const E* p, int n) {
         if (n >= 8) {
-            __builtin_memcpy(w, p, sizeof w);  // (any alignment of the elements)
+            load(p);
             return;
         }
         zero();
@@ -111,6 +114,19 @@ struct Raw8 {
                 if constexpr (P == 1) w[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i % 2));
                 else w[i] = __float_as_uint(p[i]);
             }
+    }
+    // elements n.. moved to the front, zeros behind them
+    __device__ __forceinline__ void drop(int n) {
+        if (n >= 8) zero();
+#pragma unroll
+        for (int s = 1; s < 8; s *= 2)
+            if (n & s)
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const int by = P == 1 ? s / 2 : s;
+                    if (P == 1 && s == 1) w[i] = w[i] >> 16 | (i + 1 < W ? w[i + 1 < W ? i + 1 : 0] << 16 : 0u);
+                    else w[i] = i + by < W ? w[i + by < W ? i + by : 0] : 0u;
+                }
     }
     __device__ __forceinline__ void planes(u32x4_t (&p)[P]) const {
         if constexpr (P == 1) {
@@ -211,12 +227,6 @@ __device__ __forceinline__ float exp2_f64(double x) {
     return exp2_hw(static_cast<float>(x));
 }
 
-// (i, j) of lower tile number x: 0 (0,0), 1 (1,0), 2 (1,1), 3 (2,0), ...
-__device__ __forceinline__ void tri_tile(int x, int& i, int& j) {
-    i = x >= 6 ? 3 : x >= 3 ? 2 : x >= 1 ? 1 : 0;
-    j = x - i * (i + 1) / 2;
-}
-
 // ---- the pass ---------------------------------------------------------------------------------
 //
 // A workgroup walks through one span of a sequence for one head (or a group of heads that share their
@@ -254,7 +264,8 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
     __shared__ float s_part[AUX ? 4 : 1][AUX ? C : 1];
     __shared__ float s_dot[4];
 
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6, l16 = lane & 15, lg = lane >> 4;
+    const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, lg = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
 
     // workgroups of one head's column tiles are 8 apart: on one XCD, they share its L2's lines
     const unsigned id = blockIdx.x, rest = id >> 3;
@@ -344,82 +355,79 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 #pragma unroll
             for (int i = 0; i < MT; i += 2) zero_upper_half(sa + p * Sh::BLK * 512, qblk(i, i >> 1), lane);
 
-    // ---- loads of one step (a chunk and one of its heads) into registers
-    const int64_t sgn = a.reverse ? -1 : 1;
-    const int64_t q_ds = sgn * a.q_st, k_ds = sgn * a.k_st, v_ds = sgn * a.v_st;
+    // ---- loads of one step (a chunk and one of its heads) into registers.  Every lane loads, from a row
+    // and columns that are there, and what is not to be seen is cut off on the way to LDS: with branches
+    // around the loads the compiler merges registers behind them, and so waits for what was to arrive
+    // while the products run (22,000 cycles a chunk instead of 13,000).
     const int row_q = t / (DK / 8), col_q = 8 * (t % (DK / 8)), row_v = t / (NT / 8), col_v = n0 + 8 * (t % (NT / 8));
-    const int64_t q_off = row_q * q_ds + col_q, k_off = row_q * k_ds + col_q, v_off = row_v * v_ds + col_v;
-    const int left_q = a.D - col_q, left_v = a.D - col_v;
-    const bool even = a.D % 8 == 0;
+    const int at_q = max(min(col_q, a.D - 8), 0), at_v = max(min(col_v, a.D - 8), 0);
+    const uint32_t q_sb = a.q_st * sizeof(E), k_sb = a.k_st * sizeof(E), v_sb = a.v_st * sizeof(E);  // (64 of them fit)
+    const bool tiny = a.D < 8;  // (rows too short for such a load: element by element, later)
     Raw8<P> rq[OUT ? UQ : 1], rk[UQ], rv[UV];
-#pragma unroll
-    for (int i = 0; i < UQ; ++i) {
-        rk[i].zero();
-        if (OUT) rq[i].zero();
-    }
-#pragma unroll
-    for (int i = 0; i < UV; ++i) rv[i].zero();
     const int n_steps = n_chunks * n_m;
     auto chunk_at = [&](int c, int& first, int& cnt) {  // tokens relative to the sequence
         const int k = a.reverse ? n_chunks - 1 - c : c;
         first = c_begin + k * C;
         cnt = min(C, c_end - first);
     };
+    struct Src {
+        const E *q, *k, *v;  // the chunk's first token in memory
+    };
+    qp += start * a.q_st + ho0 * a.q_sh;
+    kp += start * a.k_st + static_cast<int64_t>(hs) * n_src * a.k_sh;
+    vp += start * a.v_st + static_cast<int64_t>(hs) * n_src * a.v_sh;
+    auto source = [&](int first, int m) {
+        const int mq = n_dst > 1 ? m : 0, mk = n_dst > 1 ? 0 : m;
+        return Src{qp + first * a.q_st + mq * a.q_sh, kp + first * a.k_st + mk * a.k_sh,
+                   vp + first * a.v_st + mk * a.v_sh};
+    };
+    auto token_of = [&](int row, int cnt) { return a.reverse ? cnt - 1 - row : row; };
     auto fetch = [&](int step) {
+        if (tiny) return;
         int first, cnt;
         chunk_at(step / n_m, first, cnt);
         const int m = step % n_m;
-        const int64_t tok = start + (a.reverse ? first + cnt - 1 : first);  // row 0's token
-        const E* q0 = qp + tok * a.q_st + static_cast<int64_t>(ho0 + (n_dst > 1 ? m : 0)) * a.q_sh + q_off;
-        const int64_t kh = static_cast<int64_t>(hs) * n_src + (n_dst > 1 ? 0 : m);  // the source head
-        const E* k0 = kp + tok * a.k_st + kh * a.k_sh + k_off;
-        const E* v0 = vp + tok * a.v_st + kh * a.v_sh + v_off;
-        const bool do_q = OUT && (n_dst > 1 || m == 0), do_kv = n_dst == 1 || m == 0;
-        if (even && cnt == C) {  // whole rows: no tests but one for the columns past D
-            if (left_q > 0) {
-                if (do_q)
-#pragma unroll
-                    for (int i = 0; i < UQ; ++i) rq[OUT ? i : 0].load(q0, i * RQ * q_ds, 8);
-                if (do_kv)
-#pragma unroll
-                    for (int i = 0; i < UQ; ++i) rk[i].load(k0, i * RQ * k_ds, 8);
-            }
-            if (left_v > 0 && do_kv)
-#pragma unroll
-                for (int i = 0; i < UV; ++i) rv[i].load(v0, i * RV * v_ds, 8);
-        } else {
+        const Src src = source(first, m);
+        if (n_dst == 1 || m == 0) {
 #pragma unroll
             for (int i = 0; i < UQ; ++i) {
-                const bool in = row_q + i * RQ < cnt && left_q > 0;
-                if (do_q) {
-                    if (in) rq[OUT ? i : 0].load(q0, i * RQ * q_ds, left_q);
-                    else rq[OUT ? i : 0].zero();
-                }
-                if (do_kv) {
-                    if (in) rk[i].load(k0, i * RQ * k_ds, left_q);
-                    else rk[i].zero();
-                }
+                const uint32_t tok = token_of(min(row_q + i * RQ, cnt - 1), cnt);
+                rk[i].load(reinterpret_cast<const char*>(src.k) + (tok * k_sb + static_cast<uint32_t>(at_q * sizeof(E))));
             }
-            if (do_kv)
 #pragma unroll
-                for (int i = 0; i < UV; ++i) {
-                    if (row_v + i * RV < cnt && left_v > 0) rv[i].load(v0, i * RV * v_ds, left_v);
-                    else rv[i].zero();
-                }
+            for (int i = 0; i < UV; ++i) {
+                const uint32_t tok = token_of(min(row_v + i * RV, cnt - 1), cnt);
+                rv[i].load(reinterpret_cast<const char*>(src.v) + (tok * v_sb + static_cast<uint32_t>(at_v * sizeof(E))));
+            }
         }
+        if (OUT && (n_dst > 1 || m == 0))
+#pragma unroll
+            for (int i = 0; i < UQ; ++i) {
+                const uint32_t tok = token_of(min(row_q + i * RQ, cnt - 1), cnt);
+                rq[OUT ? i : 0].load(reinterpret_cast<const char*>(src.q) +
+                                     (tok * q_sb + static_cast<uint32_t>(at_q * sizeof(E))));
+            }
+    };
+    // one of them on its way to LDS
+    auto cut = [&](Raw8<P>& x, int row, int cnt, int col, int at, const E* p, int64_t st) {
+        if (tiny && row < cnt) x.load(p + token_of(row, cnt) * st + col, a.D - col);
+        if (row >= cnt || col >= a.D) x.zero();
+        else if (!tiny && col != at) x.drop(col - at);
     };
     // wave 0 has the log-decays: chunk c's are loaded while chunk c - 2 runs, and summed while c - 1 does
     float rg = 0.f;
-    auto fetch_g = [&](int c) {
-        rg = 0.f;
-        if (t >= C || c >= n_chunks) return;
+    auto fetch_g = [&](int c) {  // (loads a value that is there; sum_g takes it for what it is)
         int first, cnt;
-        chunk_at(c, first, cnt);
+        chunk_at(min(c, n_chunks - 1), first, cnt);
         const int tok = a.reverse ? first + cnt - t : first + t;  // (backwards: the token after)
-        if (t < cnt && tok < len) rg = gp[(start + tok) * a.g_st];
+        rg = gp[(start + max(min(tok, len - 1), 0)) * a.g_st];
     };
-    auto sum_g = [&](int buf) {
-        const double G = wave_prefix_f64(t < C ? log2_decay(rg) : 0.0);
+    auto sum_g = [&](int c) {
+        int first, cnt;
+        chunk_at(min(c, n_chunks - 1), first, cnt);
+        const int buf = c & 1;
+        const bool there = t < cnt && (a.reverse ? first + cnt - t : first + t) < len;
+        const double G = wave_prefix_f64(there ? log2_decay(rg) : 0.0);
         const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(G), 63),
                                              __builtin_amdgcn_readlane(__double2loint(G), 63));
         if (t < C) {
@@ -433,7 +441,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
     f32x4_t O[CT][MT];
     double log_total = 0.0;
     if (n_steps > 0) fetch(0);
-    if (w == 0) {
+    if (w == 0 && n_steps > 0) {
         fetch_g(0);
         sum_g(0);
         fetch_g(1);
@@ -445,10 +453,14 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
         chunk_at(c, first, cnt);
         const int ho = ho0 + (dst ? m : 0);
         // ---- registers to LDS
+        const bool whole = cnt == C && a.D == DK;
+        Src src{};
+        if (!whole) src = source(first, m);
         if (!dst || first_m) {
 #pragma unroll
             for (int i = 0; i < UQ; ++i) {
                 const int row = row_q + i * RQ, ch = (t % (DK / 8)) ^ kf<DK>(row);
+                if (!whole) cut(rk[i], row, cnt, col_q, at_q, src.k, a.k_st);
                 u32x4_t p[P];
                 rk[i].planes(p);
 #pragma unroll
@@ -457,6 +469,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 #pragma unroll
             for (int i = 0; i < UV; ++i) {
                 const int row = row_v + i * RV, ch = (t % (NT / 8)) ^ vf<NT>(row);
+                if (!whole) cut(rv[i], row, cnt, col_v, at_v, src.v, a.v_st);
                 u32x4_t p[P];
                 rv[i].planes(p);
 #pragma unroll
@@ -467,6 +480,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 #pragma unroll
             for (int i = 0; i < UQ; ++i) {
                 const int row = row_q + i * RQ, ch = (t % (DK / 8)) ^ kf<DK>(row);
+                if (!whole) cut(rq[OUT ? i : 0], row, cnt, col_q, at_q, src.q, a.q_st);
                 u32x4_t p[P];
                 rq[OUT ? i : 0].planes(p);
 #pragma unroll
@@ -475,90 +489,62 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
         lds_barrier();
         if (step + 1 < n_steps) fetch(step + 1);
         if (w == 0 && first_m) {
-            sum_g(buf ^ 1);
+            sum_g(c + 1);
             fetch_g(c + 2);
         }
 
-        // ---- A, lower tiles, as packed operands; wave 0, which has the log-decays, takes the fewest
-        if (OUT) {
-            const int x0 = C == 64 ? max(3 * w - 2, 0) : w - 1, x1 = C == 64 ? 3 * w + 1 : w;
-            for (int x = max(x0, 0); x < x1; ++x) {
-                int i, j;
-                tri_tile(x, i, j);
-                f32x4_t acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    u32x4_t ko[P], qo[P];
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        ko[p] = op_row<DK>(sk + p * C * DK, 16 * j + l16, kb, lg);
-                        qo[p] = op_row<DK>(sq + p * C * DK, 16 * i + l16, kb, lg);
-                    }
-                    acc[kb & 1] = mfma_planes<P, P>(ko, qo, acc[kb & 1]);
-                }
-                const int row = 16 * i + l16;
-                const float2 gi = sg[buf][row];
-                f32x4_t A;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int col = 16 * j + 4 * lg + r;
-                    const float x = (acc[0][r] + acc[1][r]) * (exp2_diff(gi, sg[buf][col]) * a.a_scale);
-                    A[r] = col <= row ? x : 0.f;
-                }
-                u32x2_t ap[PC];
-                split4<PC>(A, ap);
-#pragma unroll
-                for (int p = 0; p < PC; ++p)
-                    *reinterpret_cast<u32x2_t*>(sa + (p * Sh::BLK + qblk(i, j >> 1)) * 512 + lane * 8 + 4 * (j & 1)) =
-                        ap[p];
-            }
-        }
-
         const double chunk_log = s_total[buf];
+        // ---- A's tiles of the wave's 16 source tokens and, from the same rows of Q, the state's part of
+        // the outputs (in a chunk's later heads of a group with shared Q: A alone)
+        f32x4_t A[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) A[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         if (dst || first_m) {
             if (OUT) {
-                // ---- the state's part of the outputs
                 constexpr int XN = 4 * CT;  // a lane's columns in a row
                 uint32_t aux[AUX ? MT : 1][P == 1 ? XN / 2 : XN];  // as they are in memory
-                if constexpr (AUX) {
-                    const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg);
-                    const int64_t tok = start + (a.reverse ? first + cnt - 1 : first);
+                const int x_col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg);
+                const bool x_wide = a.D % XN == 0;
+                const E* x_p = xp + (start + first) * a.x_st + static_cast<int64_t>(ho) * a.x_sh;
+                if (AUX && x_wide)
+                    // (rows and columns that are not there: some that are, since their O is 0)
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        const int row = 16 * i + l16, left = row < cnt ? a.D - col : 0;
-                        const E* x = xp + (tok + sgn * row) * a.x_st + static_cast<int64_t>(ho) * a.x_sh + col;
-                        if (left >= XN) {
-                            __builtin_memcpy(aux[i], x, sizeof aux[i]);
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < XN; ++r) {
-                                if constexpr (P == 1) {
-                                    const uint32_t v = r < left ? x[r] : 0;
-                                    aux[i][r / 2] = r % 2 ? aux[i][r / 2] | v << 16 : v;
-                                } else {
-                                    aux[i][r] = r < left ? __float_as_uint(x[r]) : 0u;
-                                }
-                            }
-                        }
+                        const uint32_t tok = token_of(min(16 * i + l16, cnt - 1), cnt);
+                        __builtin_memcpy(aux[AUX ? i : 0],
+                                         reinterpret_cast<const char*>(x_p) +
+                                             (tok * static_cast<uint32_t>(a.x_st * sizeof(E)) +
+                                              static_cast<uint32_t>(min(x_col, a.D - XN) * sizeof(E))),
+                                         sizeof aux[0]);
                     }
-                }
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
                     for (int i = 0; i < MT; ++i) O[ct][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
-                    u32x4_t so[CT][PC], qo[MT][P];
+                    u32x4_t so[CT][PC], qo[MT][P], ko[P];
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
                         for (int p = 0; p < P; ++p) qo[i][p] = op_row<DK>(sq + p * C * DK, 16 * i + l16, kb, lg);
+#pragma unroll
+                    for (int p = 0; p < P; ++p) ko[p] = op_row<DK>(sk + p * C * DK, 16 * (w % MT) + l16, kb, lg);
 #pragma unroll
                     for (int ct = 0; ct < CT; ++ct) {
                         const f32x4_t s0 = S[ct][2 * kb], s1 = S[ct][2 * kb + 1];
                         const float s8[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
                         split8<PC>(s8, so[ct]);
                     }
+#pragma unroll
+                    for (int x = P - 1; x >= 0; --x)
+#pragma unroll
+                        for (int p = 0; p < P; ++p)
+                            if (x - p >= 0)
+#pragma unroll
+                                for (int i = 0; i < MT; ++i)
+                                    A[i] = mfma32(__builtin_bit_cast(bf16x8_t, ko[x - p]),
+                                                  __builtin_bit_cast(bf16x8_t, qo[i][p]), A[i]);
 #pragma unroll
                     for (int x = PC - 1; x >= 0; --x)  // (the small products first, all tiles of one before the next)
 #pragma unroll
@@ -577,6 +563,21 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 #pragma unroll
                     for (int ct = 0; ct < CT; ++ct) O[ct][i] *= e;
                 }
+                if (AUX && !x_wide)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const int row = 16 * i + l16, left = row < cnt ? a.D - x_col : 0;
+                        const E* x = x_p + token_of(min(row, cnt - 1), cnt) * a.x_st + x_col;
+#pragma unroll
+                        for (int r = 0; r < XN; ++r) {
+                            if constexpr (P == 1) {
+                                const uint32_t v = r < left ? x[r] : 0;
+                                aux[AUX ? i : 0][r / 2] = r % 2 ? aux[AUX ? i : 0][r / 2] | v << 16 : v;
+                            } else {
+                                aux[AUX ? i : 0][r] = r < left ? __float_as_uint(x[r]) : 0u;
+                            }
+                        }
+                    }
                 if constexpr (AUX) {
                     // each token's product of that part with the row of `aux` (q for gq, k for gk)
 #pragma unroll
@@ -592,6 +593,49 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                         if (lg == 0) s_part[w][16 * i + l16] = sum;
                     }
                 }
+            }
+        }
+        if (OUT) {
+            if (!dst && !first_m)
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    u32x4_t qo[MT][P], ko[P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        ko[p] = op_row<DK>(sk + p * C * DK, 16 * (w % MT) + l16, kb, lg);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) qo[i][p] = op_row<DK>(sq + p * C * DK, 16 * i + l16, kb, lg);
+                    }
+#pragma unroll
+                    for (int x = P - 1; x >= 0; --x)
+#pragma unroll
+                        for (int p = 0; p < P; ++p)
+                            if (x - p >= 0)
+#pragma unroll
+                                for (int i = 0; i < MT; ++i)
+                                    A[i] = mfma32(__builtin_bit_cast(bf16x8_t, ko[x - p]),
+                                                  __builtin_bit_cast(bf16x8_t, qo[i][p]), A[i]);
+                }
+            // as packed operands: lane (lg, l16) has A[16 i + l16][16 w + 4 lg + r]
+            float2 gj[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) gj[r] = sg[buf][16 * (w % MT) + 4 * lg + r];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                if (i < w) continue;  // (above the diagonal)
+                const float2 gi = sg[buf][16 * i + l16];
+                f32x4_t x;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = A[i][r] * (exp2_diff(gi, gj[r]) * a.a_scale);
+                    if (i == w && 4 * lg + r > l16) x[r] = 0.f;
+                }
+                u32x2_t ap[PC];
+                split4<PC>(x, ap);
+                const int blk = i < 2 ? i : 2 * i - 2 + (w >> 1);  // (qblk)
+#pragma unroll
+                for (int p = 0; p < PC; ++p)
+                    *reinterpret_cast<u32x2_t*>(sa + (p * Sh::BLK + blk) * 512 + lane * 8 + 4 * (w & 1)) = ap[p];
             }
         }
         if (first_m) {
@@ -730,12 +774,11 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
         // ---- outputs
         if (OUT && (dst || last_m)) {
             const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg), left = a.D - col;
-            const int64_t tok = rows0 + (a.reverse ? first + cnt - 1 : first);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const int row = 16 * i + l16;
                 if (row >= cnt || left <= 0) continue;
-                const int64_t at = ((tok + sgn * row) * a.HO + ho) * a.D + col;
+                const int64_t at = ((rows0 + first + token_of(row, cnt)) * a.HO + ho) * a.D + col;
                 float v[4 * CT];
 #pragma unroll
                 for (int r = 0; r < 4 * CT; ++r) v[r] = O[r / 4][i][r % 4];
@@ -843,7 +886,9 @@ __global__ __launch_bounds__(P == 1 ? 256 : 512) void decay_gate_grad(DecayGateG
                 for (int i = 0; i < MT; ++i) {
                     Raw8<P> r;
                     const int row = 16 * i + l16;
-                    if (row < cnt && col < a.D) r.load(p, b * sb + (first + row) * st + head * sh + col, a.D - col);
+                    if (row < cnt && col < a.D)
+                        r.load(static_cast<const typename Raw8<P>::E*>(p) + (b * sb + (first + row) * st + head * sh + col),
+                               a.D - col);
                     else r.zero();
                     r.planes(op[i]);
                 }

@@ -29,6 +29,8 @@ size_t size_of(int dtype) { return dtype == PM_DTYPE_BF16 ? 2 : 4; }
 constexpr int64_t kMaxElems = int64_t(1) << 40;
 constexpr int64_t kMaxStride = int64_t(1) << 40;
 
+constexpr int64_t kMaxTokenStride = int64_t(1) << 23;  // (64 tokens are reached with 32-bit offsets)
+
 int check_stride(const char* name, int64_t s) {
     if (s < 0 || s > kMaxStride) return fail(PM_E_SHAPE, "%s %lld out of range", name, static_cast<long long>(s));
     return 0;
@@ -36,7 +38,7 @@ int check_stride(const char* name, int64_t s) {
 
 bool decay_sizes_fit(int n, int T, int Hq, int H, int D) {
     if (n < 0 || T < 0 || Hq < 1 || H < 1 || Hq % H || D < 1 || D > PM_DELTA_MAX_D) return false;
-    if (T > INT32_MAX - 1024 || Hq > (1 << 20)) return false;
+    if (T > INT32_MAX - 1024 || static_cast<int64_t>(Hq) * D > kMaxTokenStride) return false;
     const int64_t rows = static_cast<int64_t>(n) * std::max(T, 1);
     return rows <= kMaxElems / (static_cast<int64_t>(Hq) * D) &&
            static_cast<int64_t>(n) * H <= kMaxElems / (static_cast<int64_t>(D) * D) &&
@@ -56,6 +58,11 @@ int check_decay(int n, int T, int Hq, int H, int D, int dtype, int out_dtype, co
     if (!strides) return fail(PM_E_NULL, "strides is NULL");
     for (int i = 0; i < n_strides; ++i)
         if (int rc = check_stride("a stride", strides[i])) return rc;
+    if (n_strides == 9)
+        for (int i = 1; i < 9; i += 3)
+            if (T > 1 && strides[i] > kMaxTokenStride)
+                return fail(PM_E_SHAPE, "token strides of at most %lld elements (got %lld)",
+                            static_cast<long long>(kMaxTokenStride), static_cast<long long>(strides[i]));
     if (int rc = check_stride("g_sb", g_sb)) return rc;
     if (int rc = check_stride("g_st", g_st)) return rc;
     if (!std::isfinite(scale)) return fail(PM_E_SHAPE, "scale must be finite");

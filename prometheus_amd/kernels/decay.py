@@ -35,6 +35,9 @@ __all__ = [
 ]
 
 
+_MAX_TOKEN_STRIDE = 1 << 23  # elements
+
+
 @dataclass(frozen=True)
 class _DecayResidual:
     """Residual of ``decay_attention_fwd``: the arrays the kernel consumed (not copied) and the scale."""
@@ -93,11 +96,11 @@ def _out_dtype(out_dtype, dtype):
 
 def _heads(call, x, dtype):
     """``x`` on the call's device in ``dtype``, the elements of a head contiguous (no copy of a view
-    that has them so)."""
+    that has them so, and its tokens no further apart than the kernels reach)."""
     if isinstance(x, torch.Tensor) and x.dtype == dtype and x.get_device() == call.device.index and (
-            x.stride(-1) == 1 or x.shape[-1] <= 1):
+            x.stride(-1) == 1 or x.shape[-1] <= 1) and x.stride(-3) <= _MAX_TOKEN_STRIDE:
         return x
-    return call.dev(x, dtype)
+    return call.dev(x, dtype).contiguous()
 
 
 def _decays(call, g):
