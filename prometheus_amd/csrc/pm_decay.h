@@ -36,7 +36,8 @@ namespace {
 template <int P>
 struct DecayShape {
     static constexpr int C = P == 1 ? 64 : 32;   // tokens of a chunk (three planes of 64 would not fit LDS)
-    static constexpr int PC = P == 1 ? 2 : 3;    // planes of computed operands
+    static constexpr int PC = P == 1 ? 2 : 3;    // planes of what sums into states and gates' gradients
+    static constexpr int PA = P;                 // planes of what sums into outputs of q's type alone
     static constexpr int MT = C / 16;            // 16-token tiles
     static constexpr int TRI = MT * (MT + 1) / 2;  // lower 16x16 tiles of A
     static constexpr int BLK = P == 1 ? 6 : 2;   // packed operand blocks of A (qblk)
@@ -247,17 +248,18 @@ struct DecayTile {
 template <int P, int DK, int KIND>
 __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void decay_pass(DecayPass a) {
     using Sh = DecayShape<P>;
-    constexpr int C = Sh::C, PC = Sh::PC, MT = Sh::MT, KB = DK / 32, MD = DK / 16;
+    constexpr int C = Sh::C, PC = Sh::PC, PA = Sh::PA, MT = Sh::MT, KB = DK / 32, MD = DK / 16;
     constexpr int CT = DecayTile<DK>::CT, NT = DecayTile<DK>::NT;
     constexpr int UQ = C * DK / 2048, UV = C * NT / 2048;  // 8-element units per thread
     constexpr int RQ = 2048 / DK, RV = 2048 / NT;          // rows between a thread's units
     constexpr bool OUT = KIND != kPassState, AUX = KIND == kPassGq || KIND == kPassGk;
+    constexpr int PS = AUX ? PC : PA;  // planes of the state in the outputs' part
     using E = typename std::conditional<P == 1, uint16_t, float>::type;
 
     __shared__ __attribute__((aligned(16))) uint16_t sq[OUT ? P * C * DK : 8];
     __shared__ __attribute__((aligned(16))) uint16_t sk[P * C * DK];
     __shared__ __attribute__((aligned(16))) uint16_t sv[P * C * NT];
-    __shared__ __attribute__((aligned(16))) uint16_t sa[OUT ? PC * Sh::BLK * 512 : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t sa[OUT ? PA * Sh::BLK * 512 : 8];
     __shared__ float2 sg[2][C];                  // the sums G, split
     __shared__ float s_into[2][C], s_out[2][C];  // e^{G_i} and e^{G_C - G_j}, with their scales
     __shared__ double s_total[2];
@@ -351,7 +353,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
     // halves of A's blocks that no tile covers
     if (OUT && w == 0)
 #pragma unroll
-        for (int p = 0; p < PC; ++p)
+        for (int p = 0; p < PA; ++p)
 #pragma unroll
             for (int i = 0; i < MT; i += 2) zero_upper_half(sa + p * Sh::BLK * 512, qblk(i, i >> 1), lane);
 
@@ -364,7 +366,6 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
     const uint32_t q_sb = a.q_st * sizeof(E), k_sb = a.k_st * sizeof(E), v_sb = a.v_st * sizeof(E);  // (64 of them fit)
     const bool tiny = a.D < 8;  // (rows too short for such a load: element by element, later)
     Raw8<P> rq[OUT ? UQ : 1], rk[UQ], rv[UV];
-    const int n_steps = n_chunks * n_m;
     auto chunk_at = [&](int c, int& first, int& cnt) {  // tokens relative to the sequence
         const int k = a.reverse ? n_chunks - 1 - c : c;
         first = c_begin + k * C;
@@ -382,11 +383,10 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                    vp + first * a.v_st + mk * a.v_sh};
     };
     auto token_of = [&](int row, int cnt) { return a.reverse ? cnt - 1 - row : row; };
-    auto fetch = [&](int step) {
+    auto fetch = [&](int c, int m) {
         if (tiny) return;
         int first, cnt;
-        chunk_at(step / n_m, first, cnt);
-        const int m = step % n_m;
+        chunk_at(c, first, cnt);
         const Src src = source(first, m);
         if (n_dst == 1 || m == 0) {
 #pragma unroll
@@ -440,14 +440,14 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 
     f32x4_t O[CT][MT];
     double log_total = 0.0;
-    if (n_steps > 0) fetch(0);
-    if (w == 0 && n_steps > 0) {
+    if (n_chunks > 0) fetch(0, 0);
+    if (w == 0 && n_chunks > 0) {
         fetch_g(0);
         sum_g(0);
         fetch_g(1);
     }
-    for (int step = 0; step < n_steps; ++step) {
-        const int c = step / n_m, m = step % n_m, buf = c & 1;
+    for (int c = 0, m = 0; c < n_chunks;) {
+        const int buf = c & 1, m_next = m + 1 < n_m ? m + 1 : 0, c_next = m_next ? c : c + 1;
         const bool first_m = m == 0, last_m = m == n_m - 1, dst = n_dst > 1;
         int first, cnt;
         chunk_at(c, first, cnt);
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                 for (int x = 0; x < P; ++x) *reinterpret_cast<u32x4_t*>(sq + x * C * DK + row * DK + 8 * ch) = p[x];
             }
         lds_barrier();
-        if (step + 1 < n_steps) fetch(step + 1);
+        if (c_next < n_chunks) fetch(c_next, m_next);
         if (w == 0 && first_m) {
             sum_g(c + 1);
             fetch_g(c + 2);
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                     for (int i = 0; i < MT; ++i) O[ct][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
-                    u32x4_t so[CT][PC], qo[MT][P], ko[P];
+                    u32x4_t so[CT][PS], qo[MT][P], ko[P];
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -534,7 +534,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                     for (int ct = 0; ct < CT; ++ct) {
                         const f32x4_t s0 = S[ct][2 * kb], s1 = S[ct][2 * kb + 1];
                         const float s8[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
-                        split8<PC>(s8, so[ct]);
+                        split8<PS>(s8, so[ct]);
                     }
 #pragma unroll
                     for (int x = P - 1; x >= 0; --x)
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                                     A[i] = mfma32(__builtin_bit_cast(bf16x8_t, ko[x - p]),
                                                   __builtin_bit_cast(bf16x8_t, qo[i][p]), A[i]);
 #pragma unroll
-                    for (int x = PC - 1; x >= 0; --x)  // (the small products first, all tiles of one before the next)
+                    for (int x = PS - 1; x >= 0; --x)  // (the small products first, all tiles of one before the next)
 #pragma unroll
                         for (int p = 0; p < P; ++p)
                             if (x - p >= 0)
@@ -630,11 +630,11 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                     x[r] = A[i][r] * (exp2_diff(gi, gj[r]) * a.a_scale);
                     if (i == w && 4 * lg + r > l16) x[r] = 0.f;
                 }
-                u32x2_t ap[PC];
-                split4<PC>(x, ap);
+                u32x2_t ap[PA];
+                split4<PA>(x, ap);
                 const int blk = i < 2 ? i : 2 * i - 2 + (w >> 1);  // (qblk)
 #pragma unroll
-                for (int p = 0; p < PC; ++p)
+                for (int p = 0; p < PA; ++p)
                     *reinterpret_cast<u32x2_t*>(sa + (p * Sh::BLK + blk) * 512 + lane * 8 + 4 * (w & 1)) = ap[p];
             }
         }
@@ -668,14 +668,14 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                                                   : 8 * ((4 * w + cc) ^ vf<NT>(row_t))));
             constexpr int R16 = 16 * NT * 2, VP = C * NT * 2;
             f32x4_t x0[CT], x1[CT];
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) x0[ct] = x1[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
             auto take = [&](int p, u32x2_t lo0, u32x2_t hi0, u32x2_t lo1, u32x2_t hi1) {
                 vo[kb][0][p] = join(lo0, hi0);
-                x0[0] += widen4(lo0), x1[0] += widen4(hi0);
+                x0[0] = p == P - 1 ? widen4(lo0) : x0[0] + widen4(lo0);
+                x1[0] = p == P - 1 ? widen4(hi0) : x1[0] + widen4(hi0);
                 if (CT == 2) {
                     vo[kb][CT - 1][p] = join(lo1, hi1);
-                    x0[CT - 1] += widen4(lo1), x1[CT - 1] += widen4(hi1);
+                    x0[CT - 1] = p == P - 1 ? widen4(lo1) : x0[CT - 1] + widen4(lo1);
+                    x1[CT - 1] = p == P - 1 ? widen4(hi1) : x1[CT - 1] + widen4(hi1);
                 }
             };
             u32x2_t b0, b1, b2 = {0u, 0u}, b3 = {0u, 0u};
@@ -753,14 +753,14 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
         if (OUT)
 #pragma unroll
             for (int kb = 0; kb < MT / 2; ++kb) {
-                u32x4_t ao[MT][PC];
+                u32x4_t ao[MT][PA];
 #pragma unroll
                 for (int i = 2 * kb; i < MT; ++i)
 #pragma unroll
-                    for (int p = 0; p < PC; ++p)
+                    for (int p = 0; p < PA; ++p)
                         ao[i][p] = *reinterpret_cast<const u32x4_t*>(sa + (p * Sh::BLK + qblk(i, kb)) * 512 + lane * 8);
 #pragma unroll
-                for (int x = PC - 1; x >= 0; --x)
+                for (int x = PA - 1; x >= 0; --x)
 #pragma unroll
                     for (int p = 0; p < P; ++p)
                         if (x - p >= 0)
@@ -813,6 +813,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
             a.cross[(state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile] =
                 e * ((s_dot[0] + s_dot[1]) + (s_dot[2] + s_dot[3]));
         }
+        c = c_next, m = m_next;
     }
 
     // ---- the state after the span
