@@ -10,7 +10,7 @@
 
 namespace pm {
 
-hipError_t decay_pass_bf16(const DecayPass& a, int kind, hipStream_t st) { return run_pass<1>(a, kind, st); }
+hipError_t decay_pass_bf16(const DecayPasses& a, int kind, hipStream_t st) { return run_pass<1>(a, kind, st); }
 hipError_t decay_gate_grad_bf16(const DecayGateGrad& a, hipStream_t st) { return run_gate_grad<1>(a, st); }
 
 namespace {
@@ -78,8 +78,9 @@ __global__ __launch_bounds__(1024) void assign_slots(const int32_t* cu, int n_se
 
 // States before the spans from each span's own share: S = e^G S + U, span after span, one thread per
 // element of a state.  The shares do not wait for each other: eight are asked for ahead.
-__global__ __launch_bounds__(256) void scan_spans(DecayPass a, const int* first_slot) {
-    const int64_t pair = blockIdx.y + static_cast<int64_t>(blockIdx.z) * 65535;
+__global__ __launch_bounds__(256) void scan_spans(DecayPasses passes, const int* first_slot) {
+    const DecayPass& a = passes.pass[blockIdx.z % passes.n];
+    const int64_t pair = blockIdx.y + static_cast<int64_t>(blockIdx.z / passes.n) * 65535;
     if (pair >= static_cast<int64_t>(a.n_seqs) * a.HS) return;
     const int seq = static_cast<int>(pair / a.HS), h = static_cast<int>(pair % a.HS);
     const int size = a.D * a.D, e = blockIdx.x * 256 + threadIdx.x;
@@ -118,13 +119,15 @@ __global__ __launch_bounds__(256) void scan_spans(DecayPass a, const int* first_
     }
 }
 
+constexpr int kMinSpan = 128;
+
 struct Plan {
     int n_tiles, n_dst, span, n_spans, n_slots;
     bool split;
 };
 
 // How a pass is cut into workgroups: one per sequence, state and column tile, or, where that leaves
-// CUs without two, as many again along the sequence (spans of at least 128 tokens; calls of up to 512
+// CUs without two, as many again along the sequence (spans of at least kMinSpan tokens; calls of up to 512
 // tokens stay whole, since the states' own pass costs as much as they take).  The query heads of a
 // group go one after another through one workgroup, which reads their keys once, where there is work
 // enough for every CU without them.
@@ -134,7 +137,7 @@ Plan plan(int n_seqs, int T, int HO, int HS, int D, bool packed) {
     if (HO > HS && tokens * HS * p.n_tiles >= want * 256) p.n_dst = HO / HS;
     const int64_t groups = static_cast<int64_t>(HO / p.n_dst) * p.n_tiles;
     if (T > 512 && n_seqs * groups < want) {
-        const int64_t span = std::max<int64_t>((tokens * groups + want - 1) / want, 128);
+        const int64_t span = std::max<int64_t>((tokens * groups + want - 1) / want, kMinSpan);
         const int64_t n = (T + span - 1) / span;
         p.span = static_cast<int>(((T + n - 1) / n + 63) / 64 * 64);
         p.n_spans = (T + p.span - 1) / p.span;
@@ -173,25 +176,51 @@ FwdWs fwd_ws(int n_seqs, int T, int Hq, int H, int D, bool packed, bool in_place
     return w;
 }
 
+// The backward's passes: one cut for all three, which run as one launch.  Where the gates' gradient is
+// wanted, spans of at most kDecayGateSpan tokens.
+struct BwdPlan {
+    Plan q, k;  // gq's pass, and gk's and gv's
+};
+BwdPlan plan_bwd(int B, int T, int Hq, int H, int D, bool gates) {
+    BwdPlan p;
+    p.k = Plan{(D + decay_cols(D) - 1) / decay_cols(D), 1, max(T, 1), 1, B, false};
+    const int64_t tokens = static_cast<int64_t>(B) * T, want = 512;
+    int n_dst = 1;
+    if (Hq > H && tokens * H * p.k.n_tiles >= want * 256) n_dst = Hq / H;
+    const int64_t groups = static_cast<int64_t>(Hq / n_dst + 2 * H) * p.k.n_tiles;
+    int64_t span = p.k.span;
+    if (B * groups < want) span = std::max<int64_t>((tokens * groups + want - 1) / want, kMinSpan);
+    if (gates) span = std::min<int64_t>(span, kDecayGateSpan);
+    if (T > 512 && span < T) {
+        const int64_t n = (T + span - 1) / span;
+        p.k.span = static_cast<int>(((T + n - 1) / n + 63) / 64 * 64);
+        p.k.n_spans = (T + p.k.span - 1) / p.k.span;
+        p.k.n_slots = B * p.k.n_spans;
+        p.k.split = p.k.n_spans > 1;
+    }
+    p.q = p.k;
+    p.q.n_dst = n_dst;
+    return p;
+}
+
 struct BwdWs {
-    size_t span_state, span_log, kept, cross, r_part, c_part, gg_part, bytes;
+    size_t ahead, back, ahead_log, back_log, gs0, r_part, c_part, gg_part, bytes;
 };
 BwdWs bwd_ws(int B, int T, int Hq, int H, int D, bool gates) {
-    const Plan pq = plan(B, T, Hq, H, D, false), pk = plan(B, T, H, H, D, false);
-    const size_t slots = max(pq.split ? pq.n_slots : 0, pk.split ? pk.n_slots : 0);
-    const size_t states = static_cast<size_t>(B) * H, keep = (T + kDecayKeep - 1) / kDecayKeep;
-    const size_t rows = static_cast<size_t>(B) * T, tiles = pq.n_tiles;
+    const Plan p = plan_bwd(B, T, Hq, H, D, gates).k;
+    const size_t state = static_cast<size_t>(H) * D * D * 4, rows = static_cast<size_t>(B) * T;
+    const size_t slots = p.split ? p.n_slots : 0, tiles = p.n_tiles;
     Layout l;
     BwdWs w{};
-    w.span_state = l.take(slots * H * D * D * 4);
-    w.span_log = l.take(slots * H * 8);
+    w.ahead = l.take(slots * state);
+    w.back = l.take(slots * state);
+    w.ahead_log = l.take(slots * H * 8);
+    w.back_log = l.take(slots * H * 8);
     if (gates) {
-        const int padded = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-        w.kept = l.take(states * keep * tiles * padded * decay_cols(D) * 4);
-        w.cross = l.take(states * keep * tiles * 4);
+        w.gs0 = l.take(B * state);
         w.r_part = l.take(tiles * rows * Hq * 4);
         w.c_part = l.take(tiles * rows * H * 4);
-        w.gg_part = l.take(states * keep * 4);
+        w.gg_part = l.take(static_cast<size_t>(p.n_slots) * H * 4);
     }
     w.bytes = l.bytes;
     return w;
@@ -202,7 +231,7 @@ T* at(void* base, size_t off) {
     return reinterpret_cast<T*>(static_cast<char*>(base) + off);
 }
 
-hipError_t run_kind(const DecayPass& a, bool bf16, int kind, hipStream_t st) {
+hipError_t run_kind(const DecayPasses& a, bool bf16, int kind, hipStream_t st) {
     return bf16 ? decay_pass_bf16(a, kind, st) : decay_pass_f32(a, kind, st);
 }
 
@@ -210,16 +239,23 @@ void apply(DecayPass& x, const Plan& p) {
     x.n_tiles = p.n_tiles, x.n_dst = p.n_dst, x.span = p.span, x.n_spans = p.n_spans, x.n_slots_grid = p.n_slots;
 }
 
-// The states before the spans of x, from each span's own share.  The shares' pass takes K and V the
-// other way round: it stores a state's rows in 16-byte pieces.
-hipError_t span_states(DecayPass x, bool bf16, const int* first_slot, hipStream_t st) {
+// K and V change places, and with them a state's rows and columns.
+DecayPass turned(DecayPass x) {
     std::swap(x.k, x.v);
     std::swap(x.k_sb, x.v_sb), std::swap(x.k_st, x.v_st), std::swap(x.k_sh, x.v_sh);
-    x.u_row = 1, x.u_col = x.D;
-    if (hipError_t e = run_kind(x, bf16, 3, st); e != hipSuccess) return e;
-    const int64_t pairs = static_cast<int64_t>(x.n_seqs) * x.HS;
-    const dim3 grid(static_cast<unsigned>((x.D * x.D + 255) / 256), static_cast<unsigned>(std::min<int64_t>(pairs, 65535)),
-                    static_cast<unsigned>((pairs + 65534) / 65535));
+    std::swap(x.s_row, x.s_col), std::swap(x.u_row, x.u_col);
+    return x;
+}
+
+// The states before the spans of each pass, from each span's own share.
+hipError_t span_states(DecayPasses x, bool bf16, const int* first_slot, hipStream_t st) {
+    for (int i = 0; i < x.n; ++i)  // (the way round that stores a state's rows in 16-byte pieces)
+        if (x.pass[i].u_row != 1) x.pass[i] = turned(x.pass[i]);
+    if (hipError_t e = run_kind(x, bf16, 2, st); e != hipSuccess) return e;
+    const DecayPass& a = x.pass[0];
+    const int64_t pairs = static_cast<int64_t>(a.n_seqs) * a.HS;
+    const dim3 grid(static_cast<unsigned>((a.D * a.D + 255) / 256), static_cast<unsigned>(std::min<int64_t>(pairs, 65535)),
+                    static_cast<unsigned>((pairs + 65534) / 65535 * x.n));
     hipLaunchKernelGGL(scan_spans, grid, dim3(256), 0, st, x, first_slot);
     return hipGetLastError();
 }
@@ -279,14 +315,14 @@ hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st) {
     if (p.split) {
         x.span_state = at<float>(a.workspace, w.span_state);
         x.span_log = at<double>(a.workspace, w.span_log);
-        if (hipError_t e = span_states(x, a.bf16, first_slot, st); e != hipSuccess) return e;
+        if (hipError_t e = span_states({{x}, 1}, a.bf16, first_slot, st); e != hipSuccess) return e;
     }
-    return run_kind(x, a.bf16, 0, st);
+    return run_kind({{x}, 1}, a.bf16, 0, st);
 }
 
 hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
     const bool gates = a.gg != nullptr;
-    const Plan pq = plan(a.B, a.T, a.Hq, a.H, a.D, false), pk = plan(a.B, a.T, a.H, a.H, a.D, false);
+    const BwdPlan p = plan_bwd(a.B, a.T, a.Hq, a.H, a.D, gates);
     const BwdWs w = bwd_ws(a.B, a.T, a.Hq, a.H, a.D, gates);
     struct Role {
         const void* p;
@@ -294,8 +330,8 @@ hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
     };
     const int64_t go_strides[3] = {static_cast<int64_t>(a.T) * a.Hq * a.D, static_cast<int64_t>(a.Hq) * a.D, a.D};
     const Role q{a.q, a.strides}, k{a.k, a.strides + 3}, v{a.v, a.strides + 6}, go{a.go, go_strides};
-    auto pass = [&](Role Q, Role K, Role V, Role aux, int HO, int HK, const Plan& p, bool reverse, bool transposed,
-                    const float* s0, float* s_out, void* o, float* part) {
+    auto pass = [&](Role Q, Role K, Role V, Role aux, int HO, int HK, const Plan& cut, bool reverse, bool transposed,
+                    const float* s0, float* s_out, void* o, bool part) {
         DecayPass x{};
         x.q = Q.p, x.q_sb = Q.s[0], x.q_st = Q.s[1], x.q_sh = Q.s[2];
         x.k = K.p, x.k_sb = K.s[0], x.k_st = K.s[1], x.k_sh = K.s[2];
@@ -306,37 +342,23 @@ hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
         x.s_row = x.u_row = transposed ? 1 : a.D, x.s_col = x.u_col = transposed ? a.D : 1;
         x.o = o, x.out_bf16 = a.bf16, x.reverse = reverse;
         x.n_seqs = a.B, x.T = a.T, x.HO = HO, x.HK = HK, x.HS = a.H, x.D = a.D;
-        apply(x, p);
-        if (p.split) {
-            x.span_state = at<float>(a.workspace, w.span_state);
-            x.span_log = at<double>(a.workspace, w.span_log);
+        apply(x, cut);
+        if (cut.split) {
+            x.span_state = at<float>(a.workspace, reverse ? w.back : w.ahead);
+            x.span_log = at<double>(a.workspace, reverse ? w.back_log : w.ahead_log);
         }
         x.a_scale = a.scale, x.into_scale = reverse ? 1.f : a.scale, x.out_scale = reverse ? a.scale : 1.f;
-        x.part = part;
+        if (gates && part) x.part = at<float>(a.workspace, reverse ? w.c_part : w.r_part);
         x.n_rows = static_cast<int64_t>(a.B) * a.T;
-        if (gates) {
-            x.kept = at<float>(a.workspace, w.kept), x.cross = at<float>(a.workspace, w.cross);
-            x.keep = kDecayKeep / (a.bf16 ? 64 : 32), x.n_keep = (a.T + kDecayKeep - 1) / kDecayKeep;
-        }
         return x;
     };
-    float* r_part = at<float>(a.workspace, w.r_part);
-    float* c_part = at<float>(a.workspace, w.c_part);
-    const DecayPass gq = pass(go, v, k, q, a.Hq, a.H, pq, false, true, a.s0, nullptr, a.gq, r_part);
-    const DecayPass gv = pass(k, q, go, k, a.H, a.Hq, pk, true, false, a.gs, a.gs0, a.gv, nullptr);
-    const DecayPass gk = pass(v, go, q, k, a.H, a.Hq, pk, true, true, a.gs, nullptr, a.gk, c_part);
-    if (pq.split) {
-        // (the states of q's gradient are the transposed ones, whose shares' pass runs the forward's way round)
-        DecayPass x = gq;
-        std::swap(x.k, x.v);
-        std::swap(x.k_sb, x.v_sb), std::swap(x.k_st, x.v_st), std::swap(x.k_sh, x.v_sh);
-        if (hipError_t e = span_states(x, a.bf16, nullptr, st); e != hipSuccess) return e;
-    }
-    if (hipError_t e = run_kind(gq, a.bf16, gates ? 1 : 0, st); e != hipSuccess) return e;
-    if (pk.split)  // (gk's and gv's states are the same, one transposed)
-        if (hipError_t e = span_states(gv, a.bf16, nullptr, st); e != hipSuccess) return e;
-    if (hipError_t e = run_kind(gv, a.bf16, 0, st); e != hipSuccess) return e;
-    if (hipError_t e = run_kind(gk, a.bf16, gates ? 2 : 0, st); e != hipSuccess) return e;
+    float* gs0 = a.gs0 ? a.gs0 : gates && a.s0 ? at<float>(a.workspace, w.gs0) : nullptr;
+    const DecayPass gq = pass(go, v, k, q, a.Hq, a.H, p.q, false, true, a.s0, nullptr, a.gq, true);
+    const DecayPass gv = pass(k, q, go, k, a.H, a.Hq, p.k, true, false, a.gs, gs0, a.gv, false);
+    const DecayPass gk = pass(v, go, q, k, a.H, a.Hq, p.k, true, true, a.gs, nullptr, a.gk, true);
+    if (p.k.split)  // (gk's and gv's states are the same, one transposed)
+        if (hipError_t e = span_states({{gq, gk}, 2}, a.bf16, nullptr, st); e != hipSuccess) return e;
+    if (hipError_t e = run_kind({{gq, gv, gk}, 3}, a.bf16, gates ? 1 : 0, st); e != hipSuccess) return e;
     if (!gates) return hipSuccess;
     const bool constant = a.g_sb == 0 && a.g_st == 0;
     if (a.T > 0) {
@@ -346,18 +368,18 @@ hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
         x.v = v.p, x.v_sb = v.s[0], x.v_st = v.s[1], x.v_sh = v.s[2];
         x.go = go.p, x.go_sb = go.s[0], x.go_st = go.s[1], x.go_sh = go.s[2];
         x.g = a.g, x.g_sb = a.g_sb, x.g_st = a.g_st;
-        x.r_part = r_part, x.c_part = c_part, x.cross = at<float>(a.workspace, w.cross);
+        x.r_part = gq.part, x.c_part = gk.part;
+        x.ahead = gq.span_state, x.back = gk.span_state, x.s0 = a.s0, x.gs0 = gs0;
         x.gg = constant ? nullptr : a.gg, x.gg_part = constant ? at<float>(a.workspace, w.gg_part) : nullptr;
         x.n_rows = static_cast<int64_t>(a.B) * a.T;
         x.B = a.B, x.T = a.T, x.Hq = a.Hq, x.H = a.H, x.D = a.D;
-        x.n_tiles = pq.n_tiles, x.n_keep = (a.T + kDecayKeep - 1) / kDecayKeep;
+        x.n_tiles = p.k.n_tiles, x.span = p.k.span, x.n_spans = p.k.n_spans;
         x.scale = a.scale;
         if (hipError_t e = a.bf16 ? decay_gate_grad_bf16(x, st) : decay_gate_grad_f32(x, st); e != hipSuccess) return e;
     }
     if (constant) {
-        const int64_t n = static_cast<int64_t>(a.B) * ((a.T + kDecayKeep - 1) / kDecayKeep);
         hipLaunchKernelGGL(sum_gate_parts, dim3(static_cast<unsigned>(a.H)), dim3(256), 0, st,
-                           at<float>(a.workspace, w.gg_part), a.gg, n, a.H);
+                           at<float>(a.workspace, w.gg_part), a.gg, a.T > 0 ? static_cast<int64_t>(p.k.n_slots) : 0, a.H);
         return hipGetLastError();
     }
     return hipSuccess;

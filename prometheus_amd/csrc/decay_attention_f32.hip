@@ -4,7 +4,7 @@
 
 namespace pm {
 
-hipError_t decay_pass_f32(const DecayPass& a, int kind, hipStream_t st) { return run_pass<3>(a, kind, st); }
+hipError_t decay_pass_f32(const DecayPasses& a, int kind, hipStream_t st) { return run_pass<3>(a, kind, st); }
 hipError_t decay_gate_grad_f32(const DecayGateGrad& a, hipStream_t st) { return run_gate_grad<3>(a, st); }
 
 }  // namespace pm

@@ -25,6 +25,7 @@
 // difference G_i - G_j has fp32's relative error also where both are large (behind a closed gate).
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "pm_cdna4.h"
@@ -238,7 +239,7 @@ __device__ __forceinline__ float exp2_f64(double x) {
 // The next chunk's rows are loaded into registers while this one's products run.
 
 // What a launch of decay_pass does besides its outputs.
-enum { kPassPlain = 0, kPassGq = 1, kPassGk = 2, kPassState = 3 };
+enum { kPassPlain = 0, kPassPart = 1, kPassState = 2 };
 
 template <int DK>
 struct DecayTile {
@@ -246,13 +247,13 @@ struct DecayTile {
 };
 
 template <int P, int DK, int KIND>
-__global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void decay_pass(DecayPass a) {
+__global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void decay_pass(DecayPasses passes) {
     using Sh = DecayShape<P>;
     constexpr int C = Sh::C, PC = Sh::PC, PA = Sh::PA, MT = Sh::MT, KB = DK / 32, MD = DK / 16;
     constexpr int CT = DecayTile<DK>::CT, NT = DecayTile<DK>::NT;
     constexpr int UQ = C * DK / 2048, UV = C * NT / 2048;  // 8-element units per thread
     constexpr int RQ = 2048 / DK, RV = 2048 / NT;          // rows between a thread's units
-    constexpr bool OUT = KIND != kPassState, AUX = KIND == kPassGq || KIND == kPassGk;
+    constexpr bool OUT = KIND != kPassState, AUX = KIND == kPassPart;
     constexpr int PS = AUX ? PC : PA;  // planes of the state in the outputs' part
     using E = typename std::conditional<P == 1, uint16_t, float>::type;
 
@@ -264,15 +265,15 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
     __shared__ float s_into[2][C], s_out[2][C];  // e^{G_i} and e^{G_C - G_j}, with their scales
     __shared__ double s_total[2];
     __shared__ float s_part[AUX ? 4 : 1][AUX ? C : 1];
-    __shared__ float s_dot[4];
 
     const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, lg = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
 
-    // workgroups of one head's column tiles are 8 apart: on one XCD, they share its L2's lines
-    const unsigned id = blockIdx.x, rest = id >> 3;
-    const int tile = static_cast<int>(rest % a.n_tiles);
-    const int64_t unit = static_cast<int64_t>(rest / a.n_tiles) * 8 + (id & 7);
+    // workgroups of one head's passes and column tiles are 8 apart: on one XCD, they share its L2's lines
+    const unsigned id = blockIdx.x, rest = id >> 3, n_tiles = passes.pass[0].n_tiles;
+    const DecayPass& a = passes.pass[rest % passes.n];
+    const int tile = static_cast<int>(rest / passes.n % n_tiles);
+    const int64_t unit = static_cast<int64_t>(rest / passes.n / n_tiles) * 8 + (id & 7);
     const int groups = OUT ? a.HO / a.n_dst : a.HS;  // head groups (the states' pass: one per state)
     if (unit >= static_cast<int64_t>(a.n_slots_grid) * groups) return;
     const int slot_id = static_cast<int>(unit / groups), hg = static_cast<int>(unit % groups);
@@ -384,7 +385,18 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
     };
     auto token_of = [&](int row, int cnt) { return a.reverse ? cnt - 1 - row : row; };
     auto fetch = [&](int c, int m) {
-        if (tiny) return;
+        // (registers that a step does not load are cleared, so that none is kept from step to step)
+        if (tiny || c >= n_chunks || (n_dst > 1 && m > 0)) {
+#pragma unroll
+            for (int i = 0; i < UQ; ++i) rk[i].zero();
+#pragma unroll
+            for (int i = 0; i < UV; ++i) rv[i].zero();
+        }
+        if (!OUT || tiny || c >= n_chunks || (n_dst == 1 && m > 0)) {
+#pragma unroll
+            for (int i = 0; i < UQ; ++i) rq[OUT ? i : 0].zero();
+        }
+        if (tiny || c >= n_chunks) return;
         int first, cnt;
         chunk_at(c, first, cnt);
         const Src src = source(first, m);
@@ -440,7 +452,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 
     f32x4_t O[CT][MT];
     double log_total = 0.0;
-    if (n_chunks > 0) fetch(0, 0);
+    fetch(0, 0);
     if (w == 0 && n_chunks > 0) {
         fetch_g(0);
         sum_g(0);
@@ -487,7 +499,6 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                 for (int x = 0; x < P; ++x) *reinterpret_cast<u32x4_t*>(sq + x * C * DK + row * DK + 8 * ch) = p[x];
             }
         lds_barrier();
-        if (c_next < n_chunks) fetch(c_next, m_next);
         if (w == 0 && first_m) {
             sum_g(c + 1);
             fetch_g(c + 2);
@@ -506,7 +517,8 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                 const int x_col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg);
                 const bool x_wide = a.D % XN == 0;
                 const E* x_p = xp + (start + first) * a.x_st + static_cast<int64_t>(ho) * a.x_sh;
-                if (AUX && x_wide)
+                const bool parts = AUX && a.part;
+                if (parts && x_wide)
                     // (rows and columns that are not there: some that are, since their O is 0)
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
@@ -549,7 +561,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                     for (int x = PS - 1; x >= 0; --x)  // (the small products first, all tiles of one before the next)
 #pragma unroll
                         for (int p = 0; p < P; ++p)
-                            if (x - p >= 0)
+                            if (x - p >= 0 && (x < PA || parts))
 #pragma unroll
                                 for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -563,7 +575,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 #pragma unroll
                     for (int ct = 0; ct < CT; ++ct) O[ct][i] *= e;
                 }
-                if (AUX && !x_wide)
+                if (parts && !x_wide)
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
                         const int row = 16 * i + l16, left = row < cnt ? a.D - x_col : 0;
@@ -578,19 +590,19 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                             }
                         }
                     }
-                if constexpr (AUX) {
+                if (parts) {
                     // each token's product of that part with the row of `aux` (q for gq, k for gk)
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
                         float sum = 0.f;
 #pragma unroll
                         for (int r = 0; r < XN; ++r) {
-                            const uint32_t v = P == 1 ? (r % 2 ? aux[i][r / 2] & 0xffff0000u : aux[i][r / 2] << 16) : aux[i][r % (P == 1 ? 1 : XN)];
+                            const uint32_t v = P == 1 ? (r % 2 ? aux[AUX ? i : 0][r / 2] & 0xffff0000u : aux[AUX ? i : 0][r / 2] << 16) : aux[AUX ? i : 0][r % (P == 1 ? 1 : XN)];
                             sum += __uint_as_float(v) * O[r / 4][i][r % 4];
                         }
                         sum += __shfl_xor(sum, 16);
                         sum += __shfl_xor(sum, 32);
-                        if (lg == 0) s_part[w][16 * i + l16] = sum;
+                        if (lg == 0) s_part[AUX ? w : 0][AUX ? 16 * i + l16 : 0] = sum;
                     }
                 }
             }
@@ -639,14 +651,6 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
             }
         }
         if (first_m) {
-            if (KIND == kPassGq && (first / C) % a.keep == 0 && ho0 % (a.HO / a.HS) == 0) {
-                f32x4_t* kept = reinterpret_cast<f32x4_t*>(a.kept) +
-                                ((state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile) * (CT * MD * 256);
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                    for (int md = 0; md < MD; ++md) kept[((w * CT + ct) * MD + md) * 64 + lane] = S[ct][md];
-            }
             log_total += chunk_log;
         }
         const bool update = !dst || last_m;
@@ -731,21 +735,6 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                                                                 S[ct][2 * d32 + h]);
             }
         }
-        if (KIND == kPassGk && last_m && (first / C) % a.keep == 0) {
-            // dL/dg of the chunk's first token: e^g <the state before it, the gradient after it>
-            const f32x4_t* kept = reinterpret_cast<const f32x4_t*>(a.kept) +
-                                  ((state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile) * (CT * MD * 256);
-            float dot = 0.f;
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                for (int md = 0; md < MD; ++md) {
-                    const f32x4_t x = kept[((w * CT + ct) * MD + md) * 64 + lane] * S[ct][md];
-                    dot += (x[0] + x[1]) + (x[2] + x[3]);
-                }
-            dot = wave_sum_row3(dot);
-            if (lane == 63) s_dot[w] = dot;
-        }
         // (from here on nothing reads the chunk's rows or log-decays: the next ones may come in; A is
         // written again only after the barrier that follows them)
         lds_barrier();
@@ -771,6 +760,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                                     O[ct][i] = mfma32(__builtin_bit_cast(bf16x8_t, vo[kb][ct][p]),
                                                       __builtin_bit_cast(bf16x8_t, ao[i][x - p]), O[ct][i]);
             }
+        fetch(c_next, m_next);
         // ---- outputs
         if (OUT && (dst || last_m)) {
             const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg), left = a.D - col;
@@ -803,16 +793,11 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
             }
         }
         if constexpr (AUX)
-            if ((dst || first_m) && t < cnt) {
+            if (a.part && (dst || first_m) && t < cnt) {
                 const int64_t tok = rows0 + (a.reverse ? first + cnt - 1 - t : first + t);
                 a.part[(static_cast<int64_t>(tile) * a.n_rows + tok) * a.HO + ho] =
                     (s_part[0][t] + s_part[1][t]) + (s_part[2][t] + s_part[3][t]);
             }
-        if (KIND == kPassGk && last_m && t == 0 && (first / C) % a.keep == 0) {
-            const float e = exp2_f64(log2_decay(gp[(start + first) * a.g_st]));
-            a.cross[(state_pair * a.n_keep + first / C / a.keep) * a.n_tiles + tile] =
-                e * ((s_dot[0] + s_dot[1]) + (s_dot[2] + s_dot[3]));
-        }
         c = c_next, m = m_next;
     }
 
@@ -851,156 +836,191 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 // dL/dg_t sums, over all pairs of a token j < t and a token i >= t, what j contributes through i
 // (and what the first state and the last state's gradient add).  Per chunk: pairs inside it from
 // the products (q_i . k_j)(go_i . v_j) e^{G_i - G_j}; pairs with j before it or i behind it from the
-// two passes' products r_i, c_j; pairs around the whole chunk from the directly computed gradient at
-// every `keep` chunks' first token.  No sum is taken as a difference of others over more than those
-// 256 tokens.  One wave a chunk, one workgroup `keep` chunks (256 tokens).
+// two passes' products r_i, c_j; pairs around the whole chunk from the gradient at its span's first
+// token, e^g <the state before it, the gradient of the state behind it>, which is handed on from chunk
+// to chunk: no sum is taken as a difference of others over more than a span's 512 tokens.
+//
+// A workgroup takes a span, each of its four waves a chunk at a time.
 template <int P>
-__global__ __launch_bounds__(P == 1 ? 256 : 512) void decay_gate_grad(DecayGateGrad a) {
+__global__ __launch_bounds__(256) void decay_gate_grad(DecayGateGrad a) {
     using Sh = DecayShape<P>;
-    constexpr int C = Sh::C, MT = Sh::MT, W = 256 / C;  // (W: chunks, waves)
+    constexpr int C = Sh::C, MT = Sh::MT, W = 4;
     __shared__ float sp[W][C][C + 1];
     __shared__ float2 sg[W][C];
     __shared__ float s_r[W][C], s_c[W][C + 1], s_sum[W];
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6, l16 = lane & 15, lg = lane >> 4;
+    const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, lg = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int G = a.Hq / a.H;
     const int64_t id = blockIdx.x;
     const int h = static_cast<int>(id % a.H);
-    const int ks = static_cast<int>(id / a.H % a.n_keep);
-    const int64_t b = id / a.H / a.n_keep, pair = b * a.H + h;
-    const int first = (ks * W + w) * C, cnt = min(C, a.T - first);  // (may be <= 0 for the last waves)
+    const int span = static_cast<int>(id / a.H % a.n_spans);
+    const int64_t b = id / a.H / a.n_spans;
+    const int begin = span * a.span, end = min(begin + a.span, a.T);
 
-    const double x = lane < cnt ? log2_decay(a.g[b * a.g_sb + (first + lane) * a.g_st + h]) : 0.0;
-    const double sum = wave_prefix_f64(x);
-    if (lane < C) sg[w][lane] = split_log(sum);
-
-    f32x4_t acc[Sh::TRI];
-#pragma unroll
-    for (int i = 0; i < Sh::TRI; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int m = 0; m < G; ++m) {
-        const int64_t hq = static_cast<int64_t>(h) * G + m;
-        f32x4_t x1[Sh::TRI], x2[Sh::TRI];
-#pragma unroll
-        for (int i = 0; i < Sh::TRI; ++i) x1[i] = x2[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        for (int col = 8 * lg; col - 8 * lg < a.D; col += 32) {
-            auto rows = [&](const void* p, int64_t sb, int64_t st, int64_t sh, int64_t head, u32x4_t(&op)[MT][P]) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    Raw8<P> r;
-                    const int row = 16 * i + l16;
-                    if (row < cnt && col < a.D)
-                        r.load(static_cast<const typename Raw8<P>::E*>(p) + (b * sb + (first + row) * st + head * sh + col),
-                               a.D - col);
-                    else r.zero();
-                    r.planes(op[i]);
-                }
-            };
-            u32x4_t src[MT][P], dst[MT][P];
-            rows(a.k, a.k_sb, a.k_st, a.k_sh, h, src);
-            rows(a.q, a.q_sb, a.q_st, a.q_sh, hq, dst);
-#pragma unroll
-            for (int i = 0, n = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j <= i; ++j, ++n) x1[n] = mfma_planes<P, P>(src[j], dst[i], x1[n]);
-            rows(a.v, a.v_sb, a.v_st, a.v_sh, h, src);
-            rows(a.go, a.go_sb, a.go_st, a.go_sh, hq, dst);
-#pragma unroll
-            for (int i = 0, n = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j <= i; ++j, ++n) x2[n] = mfma_planes<P, P>(src[j], dst[i], x2[n]);
+    // the gradient at the span's first token
+    float around = 0.f;
+    {
+        const int64_t size = static_cast<int64_t>(a.D) * a.D;
+        const float *x = nullptr, *y = nullptr;
+        if (span > 0) {
+            x = a.ahead + ((b * a.n_spans + span) * a.H + h) * size;
+            y = a.back + ((b * a.n_spans + a.n_spans - span) * a.H + h) * size;
+        } else if (a.s0) {
+            x = a.s0 + (b * a.H + h) * size;
+            y = a.gs0 + (b * a.H + h) * size;  // (with the first token's decay already)
         }
+        if (x) {
+            float dot[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int64_t i = t; i < size; i += 1024)
 #pragma unroll
-        for (int i = 0; i < Sh::TRI; ++i) acc[i] += x1[i] * x2[i];
+                for (int j = 0; j < 4; ++j)
+                    if (i + 256 * j < size) dot[j] += x[i + 256 * j] * y[i + 256 * j];
+            const float sum = wave_sum_row3((dot[0] + dot[1]) + (dot[2] + dot[3]));
+            if (lane == 63) s_sum[w] = sum;
+            __syncthreads();
+            around = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+            if (span > 0) around *= exp2_f64(log2_decay(a.g[b * a.g_sb + begin * a.g_st + h]));
+        }
     }
-    __syncthreads();
+
+    float total = 0.f;
+    for (int base = begin; base < end; base += W * C) {
+        const int first = base + w * C, cnt = min(C, end - first);  // (may be <= 0 for the last waves)
+        const double x = lane < cnt ? log2_decay(a.g[b * a.g_sb + (first + lane) * a.g_st + h]) : 0.0;
+        // r from the last token to the first (lane l: row C - 1 - l), c from the first to the last
+        float r = 0.f, c = 0.f;
+        const int back = C - 1 - lane;
+        if (back >= 0 && back < cnt)
+            for (int y = 0; y < a.n_tiles; ++y)
+                for (int m = 0; m < G; ++m)
+                    r += a.r_part[(static_cast<int64_t>(y) * a.n_rows + b * a.T + first + back) * a.Hq + h * G + m];
+        if (lane < cnt)
+            for (int y = 0; y < a.n_tiles; ++y)
+                c += a.c_part[(static_cast<int64_t>(y) * a.n_rows + b * a.T + first + lane) * a.H + h];
+        __syncthreads();  // (the chunks before are done with LDS)
+        const double sum = wave_prefix_f64(x);
+        if (lane < C) sg[w][lane] = split_log(sum);
+
+        f32x4_t acc[Sh::TRI];
 #pragma unroll
-    for (int i = 0, n = 0; i < MT; ++i)
+        for (int i = 0; i < Sh::TRI; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int m = 0; m < G; ++m) {
+            const int64_t hq = static_cast<int64_t>(h) * G + m;
+            f32x4_t x1[Sh::TRI], x2[Sh::TRI];
 #pragma unroll
-        for (int j = 0; j <= i; ++j, ++n) {
-            const int row = 16 * i + l16;
-            const float2 gi = sg[w][row];
+            for (int i = 0; i < Sh::TRI; ++i) x1[i] = x2[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (int col = 8 * lg; col - 8 * lg < a.D; col += 32) {
+                auto rows = [&](const void* p, int64_t sb, int64_t st, int64_t sh, int64_t head, u32x4_t(&op)[MT][P]) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int col = 16 * j + 4 * lg + r;
-                sp[w][row][col] = col < row ? acc[n][r] * exp2_diff(gi, sg[w][col]) : 0.f;
+                    for (int i = 0; i < MT; ++i) {
+                        Raw8<P> v;
+                        const int row = 16 * i + l16;
+                        if (row < cnt && col < a.D)
+                            v.load(static_cast<const typename Raw8<P>::E*>(p) + (b * sb + (first + row) * st + head * sh + col),
+                                   a.D - col);
+                        else v.zero();
+                        v.planes(op[i]);
+                    }
+                };
+                u32x4_t src[MT][P], dst[MT][P];
+                rows(a.k, a.k_sb, a.k_st, a.k_sh, h, src);
+                rows(a.q, a.q_sb, a.q_st, a.q_sh, hq, dst);
+#pragma unroll
+                for (int i = 0, n = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j <= i; ++j, ++n) x1[n] = mfma_planes<P, P>(src[j], dst[i], x1[n]);
+                rows(a.v, a.v_sb, a.v_st, a.v_sh, h, src);
+                rows(a.go, a.go_sb, a.go_st, a.go_sh, hq, dst);
+#pragma unroll
+                for (int i = 0, n = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j <= i; ++j, ++n) x2[n] = mfma_planes<P, P>(src[j], dst[i], x2[n]);
+            }
+#pragma unroll
+            for (int i = 0; i < Sh::TRI; ++i) acc[i] += x1[i] * x2[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0, n = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j <= i; ++j, ++n) {
+                const int row = 16 * i + l16;
+                const float2 gi = sg[w][row];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int col = 16 * j + 4 * lg + k;
+                    sp[w][row][col] = col < row ? acc[n][k] * exp2_diff(gi, sg[w][col]) : 0.f;
+                }
+            }
+        r = wave_prefix_sum(r);
+        c = wave_prefix_sum(c);
+        if (lane < C) {
+            s_r[w][back] = r;      // the sum over tokens from `back` on
+            s_c[w][lane + 1] = c;  // the sum over tokens before lane + 1
+        }
+        if (lane == 0) s_c[w][0] = 0.f;
+        __syncthreads();
+        if (lane < C) {  // row by row: the sums over j < t
+            float run = 0.f;
+            for (int j = 0; j <= lane; ++j) {
+                const float p = sp[w][lane][j];
+                sp[w][lane][j] = run;
+                run += p;
             }
         }
-    // r from the last token to the first (lane l: row C - 1 - l), c from the first to the last
-    float r = 0.f, c = 0.f;
-    const int back = C - 1 - lane;
-    if (back >= 0 && back < cnt)
-        for (int x = 0; x < a.n_tiles; ++x)
-            for (int m = 0; m < G; ++m)
-                r += a.r_part[(static_cast<int64_t>(x) * a.n_rows + b * a.T + first + back) * a.Hq + h * G + m];
-    if (lane < cnt)
-        for (int x = 0; x < a.n_tiles; ++x)
-            c += a.c_part[(static_cast<int64_t>(x) * a.n_rows + b * a.T + first + lane) * a.H + h];
-    r = wave_prefix_sum(r);
-    c = wave_prefix_sum(c);
-    if (lane < C) {
-        s_r[w][back] = r;      // the sum over tokens from `back` on
-        s_c[w][lane + 1] = c;  // the sum over tokens before lane + 1
-    }
-    if (lane == 0) s_c[w][0] = 0.f;
-    __syncthreads();
-    if (lane < C) {  // row by row: the sums over j < t
-        float run = 0.f;
-        for (int j = 0; j <= lane; ++j) {
-            const float p = sp[w][lane][j];
-            sp[w][lane][j] = run;
-            run += p;
+        __syncthreads();
+        float dg = 0.f;
+        if (lane < C)
+            for (int i = lane; i < C; ++i) dg += sp[w][i][lane];
+        float here = around;  // at this wave's first token
+        for (int i = 0; i < w; ++i) here += s_c[i][C] - s_r[i][0];
+        for (int i = 0; i < W; ++i) around += s_c[i][C] - s_r[i][0];
+        if (lane < cnt) {
+            // (the chunk's first token: the gradient handed on, without taking r's sum out and in again)
+            dg = lane == 0 ? here : a.scale * dg + s_r[w][lane] + s_c[w][lane] + (here - s_r[w][0]);
+            if (a.gg) a.gg[(b * a.T + first + lane) * a.H + h] = dg;
+        } else {
+            dg = 0.f;
         }
-    }
-    __syncthreads();
-    float dg = 0.f;
-    if (lane < C)
-        for (int i = lane; i < C; ++i) dg += sp[w][i][lane];
-    float around = 0.f;
-    for (int x = 0; x < a.n_tiles; ++x) around += a.cross[(pair * a.n_keep + ks) * a.n_tiles + x];
-    for (int i = 0; i < w; ++i) around += s_c[i][C] - s_r[i][0];
-    if (lane < cnt) {
-        // (the chunk's first token: the gradient handed on, without taking r's sum out and in again)
-        dg = lane == 0 ? around : a.scale * dg + s_r[w][lane] + s_c[w][lane] + (around - s_r[w][0]);
-        if (a.gg) a.gg[(b * a.T + first + lane) * a.H + h] = dg;
-    } else {
-        dg = 0.f;
+        total += dg;
     }
     if (a.gg_part) {
-        const float total = wave_sum_row3(dg);
+        total = wave_sum_row3(total);
+        __syncthreads();
         if (lane == 63) s_sum[w] = total;
         __syncthreads();
-        if (t == 0) {
-            float s = 0.f;
-            for (int i = 0; i < W; ++i) s += s_sum[i];
-            a.gg_part[(b * a.n_keep + ks) * a.H + h] = s;
-        }
+        if (t == 0) a.gg_part[(b * a.n_spans + span) * a.H + h] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
     }
 }
 
 template <int P, int DK>
-hipError_t launch_pass(const DecayPass& a, int kind, hipStream_t st) {
-    const int groups = kind == kPassState ? a.HS : a.HO / a.n_dst;
-    const int64_t units = static_cast<int64_t>(a.n_slots_grid) * groups;
-    const dim3 grid(static_cast<unsigned>((units + 7) / 8 * 8 * a.n_tiles));
+hipError_t launch_pass(const DecayPasses& a, int kind, hipStream_t st) {
+    int64_t units = 0;
+    for (int i = 0; i < a.n; ++i) {
+        const DecayPass& x = a.pass[i];
+        units = std::max(units, static_cast<int64_t>(x.n_slots_grid) * (kind == kPassState ? x.HS : x.HO / x.n_dst));
+    }
+    const dim3 grid(static_cast<unsigned>((units + 7) / 8 * 8 * a.pass[0].n_tiles * a.n));
     switch (kind) {
         case kPassPlain: hipLaunchKernelGGL((decay_pass<P, DK, kPassPlain>), grid, dim3(256), 0, st, a); break;
-        case kPassGq: hipLaunchKernelGGL((decay_pass<P, DK, kPassGq>), grid, dim3(256), 0, st, a); break;
-        case kPassGk: hipLaunchKernelGGL((decay_pass<P, DK, kPassGk>), grid, dim3(256), 0, st, a); break;
+        case kPassPart: hipLaunchKernelGGL((decay_pass<P, DK, kPassPart>), grid, dim3(256), 0, st, a); break;
         default: hipLaunchKernelGGL((decay_pass<P, DK, kPassState>), grid, dim3(256), 0, st, a); break;
     }
     return hipGetLastError();
 }
 
 template <int P>
-hipError_t run_pass(const DecayPass& a, int kind, hipStream_t st) {
-    if (a.D <= 64) return launch_pass<P, 64>(a, kind, st);
-    if (a.D <= 128) return launch_pass<P, 128>(a, kind, st);
+hipError_t run_pass(const DecayPasses& a, int kind, hipStream_t st) {
+    const int D = a.pass[0].D;
+    if (D <= 64) return launch_pass<P, 64>(a, kind, st);
+    if (D <= 128) return launch_pass<P, 128>(a, kind, st);
     return launch_pass<P, 256>(a, kind, st);
 }
 
 template <int P>
 hipError_t run_gate_grad(const DecayGateGrad& a, hipStream_t st) {
-    const int64_t n = static_cast<int64_t>(a.B) * a.H * a.n_keep;
-    hipLaunchKernelGGL((decay_gate_grad<P>), dim3(static_cast<unsigned>(n)), dim3(P == 1 ? 256 : 512), 0, st, a);
+    const int64_t n = static_cast<int64_t>(a.B) * a.H * a.n_spans;
+    hipLaunchKernelGGL((decay_gate_grad<P>), dim3(static_cast<unsigned>(n)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

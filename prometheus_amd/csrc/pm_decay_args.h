@@ -6,7 +6,7 @@
 
 namespace pm {
 
-constexpr int kDecayKeep = 256;  // tokens between the states kept for the gates' gradient
+constexpr int kDecayGateSpan = 512;  // the longest span where the gates' gradient is wanted
 
 // Columns of the state that a workgroup keeps (pm_decay.h: DecayTile).
 constexpr int decay_cols(int D) { return D <= 64 ? 64 : 128; }
@@ -44,11 +44,14 @@ struct DecayPass {
     // for the gates' gradient
     const void* aux;    // q (gq's pass), k (gk's)
     int64_t x_sb, x_st, x_sh;
-    float* part;        // [tile][row][HO]
+    float* part;        // nullable; [tile][row][HO]: each token's product of aux with the state's part of O
     int64_t n_rows;
-    float* kept;        // [state][keep][tile] accumulators
-    float* cross;       // [state][keep][tile]
-    int keep, n_keep;   // chunks between kept states, and their number
+};
+
+// Up to three passes that run as one launch.
+struct DecayPasses {
+    DecayPass pass[3];
+    int n;
 };
 
 struct DecayGateGrad {
@@ -61,18 +64,21 @@ struct DecayGateGrad {
     int64_t g_sb, g_st;
     const float* r_part;
     const float* c_part;
-    const float* cross;
+    const float* ahead;   // nullable: the states before the spans, [slot][H] (slots in order of time)
+    const float* back;    // nullable: their gradients behind the spans, [slot][H], the last span's first
+    const float* s0;      // nullable: the first state
+    const float* gs0;     // its gradient, where s0 is given
     float* gg;       // nullable: (B, T, H)
-    float* gg_part;  // nullable: (B, n_keep, H)
+    float* gg_part;  // nullable: (B, n_spans, H)
     int64_t n_rows;
-    int B, T, Hq, H, D, n_tiles, n_keep;
+    int B, T, Hq, H, D, n_tiles, span, n_spans;
     float scale;
 };
 
-// kind: 0 outputs and state only, 1 gq's pass with its share of the gates' gradient, 2 gk's,
-// 3 each span's own share of the state (from zeros) but the last one's, to the next slot of span_state.
-hipError_t decay_pass_bf16(const DecayPass& a, int kind, hipStream_t st);
-hipError_t decay_pass_f32(const DecayPass& a, int kind, hipStream_t st);
+// kind: 0 outputs and states, 1 the same and `part`s, 2 each span's own share of the state (from zeros) but
+// the last one's, to the next slot of span_state.
+hipError_t decay_pass_bf16(const DecayPasses& a, int kind, hipStream_t st);
+hipError_t decay_pass_f32(const DecayPasses& a, int kind, hipStream_t st);
 hipError_t decay_gate_grad_bf16(const DecayGateGrad& a, hipStream_t st);
 hipError_t decay_gate_grad_f32(const DecayGateGrad& a, hipStream_t st);
 
