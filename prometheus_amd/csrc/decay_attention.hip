@@ -76,14 +76,18 @@ __global__ __launch_bounds__(1024) void assign_slots(const int32_t* cu, int n_se
     for (int j = sums[1023] + t; j < n_slots; j += 1024) table[j] = make_int2(-1, 0);
 }
 
-// States before the spans from each span's own share: S = e^G S + U, span after span, one thread per
-// element of a state.  The shares do not wait for each other: eight are asked for ahead.
+// States before the spans from each span's own share: S = e^G S + U, span after span, V elements of a
+// state to a thread (4 where a state's size allows it).  The shares do not wait for each other: sixteen
+// are asked for ahead.
+template <int V>
 __global__ __launch_bounds__(256) void scan_spans(DecayPasses passes, const int* first_slot) {
+    typedef float vec __attribute__((ext_vector_type(V)));
+    constexpr int AHEAD = 16;
     const DecayPass& a = passes.pass[blockIdx.z % passes.n];
     const int64_t pair = blockIdx.y + static_cast<int64_t>(blockIdx.z / passes.n) * 65535;
     if (pair >= static_cast<int64_t>(a.n_seqs) * a.HS) return;
     const int seq = static_cast<int>(pair / a.HS), h = static_cast<int>(pair % a.HS);
-    const int size = a.D * a.D, e = blockIdx.x * 256 + threadIdx.x;
+    const int size = a.D * a.D, e = (blockIdx.x * 256 + threadIdx.x) * V;
     if (e >= size) return;
     int len = a.T, slot = seq * a.n_spans;
     if (a.cu) {
@@ -91,7 +95,7 @@ __global__ __launch_bounds__(256) void scan_spans(DecayPasses passes, const int*
         slot = first_slot[seq];
     }
     const int n = min(max((len + a.span - 1) / a.span, 1), a.n_slots_grid - slot);
-    float S = 0.f;
+    vec S = {};
     if (a.s0) {
         int64_t from = seq;
         bool there = true;
@@ -99,27 +103,31 @@ __global__ __launch_bounds__(256) void scan_spans(DecayPasses passes, const int*
             from = a.slots[seq];
             there = from >= 0 && from < a.n_slots;
         }
-        if (there) S = a.s0[(from * a.HS + h) * size + e];
+        if (there) __builtin_memcpy(&S, a.s0 + (from * a.HS + h) * size + e, sizeof S);
     }
     float* u = a.span_state + (static_cast<int64_t>(slot) * a.HS + h) * size + e;
     const double* log = a.span_log + static_cast<int64_t>(slot) * a.HS + h;
     const int64_t step = static_cast<int64_t>(a.HS) * size;
-    if (n > 0) u[0] = S;
-    for (int i = 1; i < n; i += 8) {
-        float x[8], g[8];
+    if (n > 0) __builtin_memcpy(u, &S, sizeof S);
+    for (int i = 1; i < n; i += AHEAD) {
+        vec x[AHEAD];
+        float g[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j < n) x[j] = u[(i + j) * step], g[j] = exp2_f64(log[static_cast<int64_t>(i + j) * a.HS]);
+        for (int j = 0; j < AHEAD; ++j)
+            if (i + j < n) {
+                __builtin_memcpy(&x[j], u + (i + j) * step, sizeof S);
+                g[j] = exp2_f64(log[static_cast<int64_t>(i + j) * a.HS]);
+            }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < AHEAD; ++j)
             if (i + j < n) {
                 S = g[j] * S + x[j];
-                u[(i + j) * step] = S;
+                __builtin_memcpy(u + (i + j) * step, &S, sizeof S);
             }
     }
 }
 
-constexpr int kMinSpan = 128;
+constexpr int kMinSpan = 64;
 
 struct Plan {
     int n_tiles, n_dst, span, n_spans, n_slots;
@@ -254,9 +262,13 @@ hipError_t span_states(DecayPasses x, bool bf16, const int* first_slot, hipStrea
     if (hipError_t e = run_kind(x, bf16, 2, st); e != hipSuccess) return e;
     const DecayPass& a = x.pass[0];
     const int64_t pairs = static_cast<int64_t>(a.n_seqs) * a.HS;
-    const dim3 grid(static_cast<unsigned>((a.D * a.D + 255) / 256), static_cast<unsigned>(std::min<int64_t>(pairs, 65535)),
+    // (four elements a thread, where that leaves a workgroup for every CU: few states of a long sequence
+    // are bound by the loads in flight, 31 us against 40 for 4 heads' 128 spans of D 128)
+    const int V = a.D % 2 == 0 && pairs * x.n * a.D * a.D >= 256 * 1024 ? 4 : 1;
+    const dim3 grid(static_cast<unsigned>((a.D * a.D / V + 255) / 256), static_cast<unsigned>(std::min<int64_t>(pairs, 65535)),
                     static_cast<unsigned>((pairs + 65534) / 65535 * x.n));
-    hipLaunchKernelGGL(scan_spans, grid, dim3(256), 0, st, x, first_slot);
+    if (V == 4) hipLaunchKernelGGL(scan_spans<4>, grid, dim3(256), 0, st, x, first_slot);
+    else hipLaunchKernelGGL(scan_spans<1>, grid, dim3(256), 0, st, x, first_slot);
     return hipGetLastError();
 }
 
@@ -393,8 +405,10 @@ hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
 // again, 4 at a time.
 namespace {
 
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // at any address of a float
+
 template <int CG, typename E>
-__global__ __launch_bounds__(256) void decay_step(DecayAttnStepArgs a, int b0) {
+__global__ __launch_bounds__(256, 4) void decay_step(DecayAttnStepArgs a, int b0) {
     constexpr int RG = 256 / CG, GB = 4;
     __shared__ float sk[256], sq[GB][256], red[GB][4][4 * CG];
     const int h = blockIdx.x, b = b0 + blockIdx.y, t = threadIdx.x, cg = t % CG, rg = t / CG, lane = t & 63, w = t >> 6;
@@ -441,12 +455,12 @@ __global__ __launch_bounds__(256) void decay_step(DecayAttnStepArgs a, int b0) {
             for (int d = rg; d < D; d += RG) {
                 float* p = s + static_cast<int64_t>(d) * D + col;
                 f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-                if (left >= 4) __builtin_memcpy(&x, p, 16);
+                if (left >= 4) x = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(p));
                 else
                     for (int r = 0; r < left; ++r) x[r] = p[r];
                 if (m0 == 0) {
                     x = e * x + sk[d] * vv;
-                    if (left >= 4) __builtin_memcpy(p, &x, 16);
+                    if (left >= 4) __builtin_nontemporal_store(x, reinterpret_cast<f32x4_any*>(p));
                     else
                         for (int r = 0; r < left; ++r) p[r] = x[r];
                 }

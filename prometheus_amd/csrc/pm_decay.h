@@ -499,6 +499,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                 for (int x = 0; x < P; ++x) *reinterpret_cast<u32x4_t*>(sq + x * C * DK + row * DK + 8 * ch) = p[x];
             }
         lds_barrier();
+        if (!OUT) fetch(c_next, m_next);
         if (w == 0 && first_m) {
             sum_g(c + 1);
             fetch_g(c + 2);
@@ -760,7 +761,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                                     O[ct][i] = mfma32(__builtin_bit_cast(bf16x8_t, vo[kb][ct][p]),
                                                       __builtin_bit_cast(bf16x8_t, ao[i][x - p]), O[ct][i]);
             }
-        fetch(c_next, m_next);
+        if (OUT) fetch(c_next, m_next);
         // ---- outputs
         if (OUT && (dst || last_m)) {
             const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg), left = a.D - col;

@@ -339,7 +339,8 @@ def decay_attention_step(q, k, v, g, state, *, scale=1.0, out_dtype=None):
 def _step(state: int | None, slots, n_slots, qd, kd, vd, gd, g_sb, o, scale, stream):
     """One token on device tensors; ``state`` is the states' address."""
     batch, Hq, D = qd.shape
+    qs, ks, vs = qd.stride(), kd.stride(), vd.stride()
     _native.check(_native.lib().pm_decay_attention_step(
-        state, _k._ptr(slots), n_slots, qd.data_ptr(), kd.data_ptr(), vd.data_ptr(), gd.data_ptr(), o.data_ptr(), batch,
-        Hq, kd.shape[1], D, _strides(*qd.stride()[:2], *kd.stride()[:2], *vd.stride()[:2]), g_sb, _k._code(qd.dtype),
-        _k._code(o.dtype), scale, stream))
+        state, None if slots is None else slots.data_ptr(), n_slots, qd.data_ptr(), kd.data_ptr(), vd.data_ptr(),
+        gd.data_ptr(), o.data_ptr(), batch, Hq, kd.shape[1], D, _strides(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1]), g_sb,
+        _k._code(qd.dtype), _k._code(o.dtype), scale, stream))

@@ -94,6 +94,47 @@ def _dev(call, x, dtype):
     return call.dev(x, dtype)
 
 
+class _Quick:
+    """Stands for the ``_Call`` of tensors that are all on one GPU as the kernels take them."""
+
+    host_numpy = host_torch = False
+
+    def __init__(self, device):
+        self.device = device
+
+    dev = _k._Call.dev
+
+    @staticmethod
+    def out(t):
+        return t
+
+
+_CODES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16}
+_QUICK: dict = {}
+
+
+def _quick(shape, rows, weights):
+    """A ``_Quick`` where every one of the tensors ``rows`` has this shape, and every one of ``weights``
+    (or None) its last dimension's, all contiguous, fp32 or bf16 and on one GPU, so that no other check of
+    shapes, types or devices is left to do; None where that is not so."""
+    gpu = -1
+    for x in rows:
+        if not (isinstance(x, torch.Tensor) and x.shape == shape and x.dtype in _CODES and x.is_contiguous()):
+            return None
+        at = x.get_device()
+        if at < 0 or (gpu >= 0 and at != gpu):
+            return None
+        gpu = at
+    for w in weights:
+        if w is not None and not (isinstance(w, torch.Tensor) and w.dim() == 1 and w.shape[0] == shape[-1]
+                                  and w.dtype in _CODES and w.is_contiguous() and w.get_device() == gpu):
+            return None
+    call = _QUICK.get(gpu)
+    if call is None:
+        call = _QUICK[gpu] = _Quick(torch.device("cuda", gpu))
+    return call
+
+
 def _width(shape, *weights) -> int:
     if not shape or not 1 <= shape[-1] <= _native.NORM_MAX_ROW:
         raise _k.KernelError(f"rows must have 1 to {_native.NORM_MAX_ROW} elements; got shape {shape}")
@@ -108,17 +149,31 @@ def _check_eps(eps) -> None:
         raise _k.KernelError(f"eps must be >= 0, got {eps}")
 
 
+@functools.lru_cache(maxsize=64)
+def _one_stride(width):
+    return (ctypes.c_int64 * 4)(width, 0, width, 0)
+
+
 class _GatedPlan:
     """One call's device tensors and the arguments both directions share."""
 
     def __init__(self, x, gate, weight, activation, gate_first, eps, y_dtype, *more):
-        shape = _k._shape(x)
-        width = _width(shape, ("weight", weight))
-        if _k._shape(gate) != shape:
-            raise _k.KernelError(f"gate shape {_k._shape(gate)} != {shape}")
         if activation not in _ACTIVATIONS:
             raise _k.KernelError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
         _check_eps(eps)
+        shape = _k._shape(x)
+        call = _quick(shape, (x, gate), (weight,)) if shape and 0 < shape[-1] <= _native.NORM_MAX_ROW and not more else None
+        if call is not None:
+            self.call, self.x, self.gate, self.weight = call, x, gate, weight
+            self.rows, self.width = x.numel() // shape[-1], shape[-1]
+            self.y_dtype = x.dtype if y_dtype is None else _k._out_dtype(y_dtype)
+            self.shared = (self.rows, 1, self.width, _one_stride(self.width), _ACTIVATIONS[activation], int(gate_first),
+                           eps, _CODES[x.dtype], _CODES[gate.dtype], _CODES[self.y_dtype],
+                           0 if weight is None else _CODES[weight.dtype])
+            return
+        width = _width(shape, ("weight", weight))
+        if _k._shape(gate) != shape:
+            raise _k.KernelError(f"gate shape {_k._shape(gate)} != {shape}")
         self.call = call = _k._Call(x, gate, weight, *more)
         xt, zt, wt = _dtype(x), _dtype(gate), _dtype(weight)
         self.y_dtype = xt if y_dtype is None else _k._out_dtype(y_dtype)
@@ -143,9 +198,9 @@ def _gated_forward(x, gate, weight, activation, gate_first, eps, out_dtype):
     plan = _GatedPlan(x, gate, weight, activation, gate_first, eps, out_dtype)
     dev, ptr = plan.call.device, _k._ptr
     with _k._on(dev):
-        y = torch.empty(plan.x.shape, dtype=plan.y_dtype, device=dev)
-        _native.check(_native.lib().pm_gated_norm(ptr(plan.x), ptr(plan.gate), ptr(plan.weight), ptr(y), *plan.shared,
-                                                  _k._stream(dev)))
+        y = torch.empty_like(plan.x, dtype=plan.y_dtype, memory_format=torch.contiguous_format)
+        _native.check(_native.lib().pm_gated_norm(plan.x.data_ptr(), plan.gate.data_ptr(), ptr(plan.weight), y.data_ptr(),
+                                                  *plan.shared, _k._stream(dev)))
     return plan, y
 
 
@@ -260,13 +315,22 @@ class _ResidualPlan:
     """One call's device tensors and the arguments both directions share."""
 
     def __init__(self, x, residual, weight, post_weight, scale, eps, *more):
-        shape = _k._shape(x)
-        width = _width(shape, ("weight", weight), ("post_weight", post_weight))
-        if _k._shape(residual) != shape:
-            raise _k.KernelError(f"residual shape {_k._shape(residual)} != {shape}")
         if not math.isfinite(scale):
             raise _k.KernelError(f"scale must be finite, got {scale}")
         _check_eps(eps)
+        shape = _k._shape(x)
+        call = (_quick(shape, (x, residual), (weight, post_weight))
+                if shape and 0 < shape[-1] <= _native.NORM_MAX_ROW and not more else None)
+        if call is not None:
+            self.call, self.x, self.residual, self.weight, self.post_weight = call, x, residual, weight, post_weight
+            width = shape[-1]
+            self.shared = (x.numel() // width, width, width, width, scale, eps, _CODES[x.dtype], _CODES[residual.dtype],
+                           0 if weight is None else _CODES[weight.dtype],
+                           0 if post_weight is None else _CODES[post_weight.dtype])
+            return
+        width = _width(shape, ("weight", weight), ("post_weight", post_weight))
+        if _k._shape(residual) != shape:
+            raise _k.KernelError(f"residual shape {_k._shape(residual)} != {shape}")
         self.call = call = _k._Call(x, residual, weight, post_weight, *more)
         xt, rt, wt, pt = (_dtype(t) for t in (x, residual, weight, post_weight))
         xd, rd = _dev(call, x, xt), _dev(call, residual, rt)
@@ -293,10 +357,11 @@ def _residual_forward(x, residual, weight, post_weight, scale, eps):
     plan = _ResidualPlan(x, residual, weight, post_weight, scale, eps)
     dev, ptr = plan.call.device, _k._ptr
     with _k._on(dev):
-        y = torch.empty(plan.x.shape, dtype=plan.x.dtype, device=dev)
-        h = torch.empty(plan.x.shape, dtype=plan.residual.dtype, device=dev)
-        _native.check(_native.lib().pm_residual_norm(*(ptr(t) for t in plan.tensors()), ptr(y), ptr(h), *plan.shared,
-                                                     _k._stream(dev)))
+        y = torch.empty_like(plan.x, memory_format=torch.contiguous_format)
+        h = torch.empty_like(plan.residual, memory_format=torch.contiguous_format)
+        _native.check(_native.lib().pm_residual_norm(
+            plan.x.data_ptr(), plan.residual.data_ptr(), ptr(plan.weight), ptr(plan.post_weight), y.data_ptr(),
+            h.data_ptr(), *plan.shared, _k._stream(dev)))
     return plan, y, h
 
 

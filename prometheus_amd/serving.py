@@ -33,6 +33,7 @@ slots in the kernel, without gathering them first. ``DecayStateCache`` is the sa
 from __future__ import annotations
 
 import heapq
+import math
 
 import torch
 
@@ -369,22 +370,30 @@ class DecayStateCache(_SlotPool):
         self._check_cuda(q, k, v, g, slots)
         if slots.dim() != 1 or slots.dtype != torch.int32 or not slots.is_contiguous():
             raise ValueError("slots must be a contiguous int32 tensor of shape (B,)")
-        (batch,), _, heads, dim = decay._check(q, k, v, g, 3, scale)
-        if batch != slots.shape[0] or (heads, dim) != (self.heads, self.dim):
-            raise ValueError(f"k must be {(slots.shape[0], self.heads, self.dim)}, got {tuple(k.shape)}")
-        if q.dtype != k.dtype or q.dtype != v.dtype or q.dtype not in (torch.float32, torch.bfloat16):
+        qs, ks, dtype = q.shape, k.shape, q.dtype
+        heads, dim = self.heads, self.dim
+        if ks != (slots.shape[0], heads, dim):
+            raise ValueError(f"k must be {(slots.shape[0], heads, dim)}, got {tuple(ks)}")
+        if v.shape != ks or len(qs) != 3 or qs[0] != ks[0] or qs[1] < 1 or qs[1] % heads or qs[2] != dim or (
+                dim > _native.MAX_D):
+            decay._check(q, k, v, g, 3, scale)  # (which says what is wrong)
+        if g.shape != ks[:2] and g.shape != (heads,):
+            raise ValueError(f"g must be {tuple(ks[:2])} or {(heads,)}, got {tuple(g.shape)}")
+        if dtype != k.dtype or dtype != v.dtype or (dtype != torch.bfloat16 and dtype != torch.float32):
             raise ValueError("q, k, v must share one dtype, fp32 or bf16")
         if g.dtype != torch.float32:
             raise ValueError("g must be fp32")
+        if not math.isfinite(scale):
+            raise ValueError(f"scale must be finite, got {scale}")
         if dim > 1 and not q.stride(2) == k.stride(2) == v.stride(2) == 1:
             raise ValueError("q, k and v must have the elements of a head contiguous")
         if heads > 1 and g.stride(-1) != 1:
             raise ValueError("g must have contiguous heads")
         if out is None:
-            out = torch.empty(q.shape, dtype=decay._out_dtype(out_dtype, q.dtype), device=q.device)
-        elif (out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16) or not out.is_contiguous()
+            out = torch.empty(qs, dtype=dtype if out_dtype is None else kernels._out_dtype(out_dtype), device=q.device)
+        elif (out.shape != qs or out.dtype not in (torch.float32, torch.bfloat16) or not out.is_contiguous()
               or out.device != q.device):
-            raise ValueError(f"out must be contiguous fp32 or bf16 {tuple(q.shape)} on the pool's device")
+            raise ValueError(f"out must be contiguous fp32 or bf16 {tuple(qs)} on the pool's device")
         with kernels._on(q.device):
             decay._step(self._pool.data_ptr() + layer * self._pool.stride(0) * 4, slots, self.n_slots, q, k, v, g,
                         g.stride(0) if g.dim() == 2 else 0, out, scale, kernels._stream(q.device))
