@@ -11,7 +11,7 @@
 namespace pm {
 
 hipError_t decay_pass_bf16(const DecayPasses& a, int kind, hipStream_t st) { return run_pass<1>(a, kind, st); }
-hipError_t decay_gate_grad_bf16(const DecayGateGrad& a, hipStream_t st) { return run_gate_grad<1>(a, st); }
+hipError_t decay_near_bf16(const DecayNear& a, hipStream_t st) { return run_near<1>(a, st); }
 
 namespace {
 
@@ -23,6 +23,96 @@ __global__ __launch_bounds__(256) void gather_states(const float* pool, const in
     const float* from = pool + (there ? slot : 0) * size;
     float* out = to + blockIdx.y * size;
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) out[i] = there ? from[i] : 0.f;
+}
+
+// The gates' gradient (pm_decay.h) from near, r and c: a workgroup takes a span, each of its four waves a
+// chunk at a time.
+__global__ __launch_bounds__(256) void gate_grad(DecayGateGrad a) {
+    constexpr int W = 4;
+    __shared__ float s_r[W][64], s_c[W][65], s_sum[W];
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, C = a.chunk, G = a.Hq / a.H;
+    const int64_t id = blockIdx.x;
+    const int h = static_cast<int>(id % a.H);
+    const int span = static_cast<int>(id / a.H % a.n_spans);
+    const int64_t b = id / a.H / a.n_spans;
+    const int begin = span * a.span, end = min(begin + a.span, a.T);
+
+    // the gradient at the span's first token
+    float around = 0.f;
+    {
+        const int64_t size = static_cast<int64_t>(a.D) * a.D;
+        const float *x = nullptr, *y = nullptr;
+        if (span > 0) {
+            x = a.ahead + ((b * a.n_spans + span) * a.H + h) * size;
+            y = a.back + ((b * a.n_spans + a.n_spans - span) * a.H + h) * size;
+        } else if (a.s0) {
+            x = a.s0 + (b * a.H + h) * size;
+            y = a.gs0 + (b * a.H + h) * size;  // (with the first token's decay already)
+        }
+        if (x) {
+            f32x4_t dot[4] = {};
+            const int quads = static_cast<int>(size / 4);
+            auto quad = [&](int i, int j) {
+                f32x4_t u, v;
+                __builtin_memcpy(&u, x + 4 * i, 16);
+                __builtin_memcpy(&v, y + 4 * i, 16);
+                dot[j] += u * v;
+            };
+            int i = t;
+            for (; i + 768 < quads; i += 1024) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) quad(i + 256 * j, j);
+            }
+            for (; i < quads; i += 256) quad(i, 0);
+            if (t < size % 4) dot[0][0] += x[4 * quads + t] * y[4 * quads + t];
+            dot[0] = (dot[0] + dot[1]) + (dot[2] + dot[3]);
+            const float sum = wave_sum_row3((dot[0][0] + dot[0][1]) + (dot[0][2] + dot[0][3]));
+            if (lane == 63) s_sum[w] = sum;
+            __syncthreads();
+            around = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+            if (span > 0) around *= exp2_f64(log2_decay(a.g[b * a.g_sb + begin * a.g_st + h]));
+        }
+    }
+    float total = 0.f;
+    for (int base = begin; base < end; base += W * C) {
+        const int first = base + w * C, cnt = min(C, end - first);  // (may be <= 0 for the last waves)
+        // r from the last token to the first (lane l: row C - 1 - l), c from the first to the last
+        float r = 0.f, c = 0.f, near = 0.f;
+        const int back = C - 1 - lane;
+        const int64_t row = b * a.T + first;
+        if (lane < cnt) near = a.near[h * a.n_rows + row + lane];
+        for (int y = 0; y < a.n_tiles; ++y) {
+            if (back >= 0 && back < cnt)
+                for (int m = 0; m < G; ++m)
+                    r += a.r_part[(static_cast<int64_t>(y) * a.Hq + h * G + m) * a.n_rows + row + back];
+            if (lane < cnt) c += a.c_part[(static_cast<int64_t>(y) * a.H + h) * a.n_rows + row + lane];
+        }
+        r = wave_prefix_sum(r);
+        c = wave_prefix_sum(c);
+        __syncthreads();  // (the chunks before are done with LDS)
+        if (lane < C) {
+            s_r[w][back] = r;      // the sum over tokens from `back` on
+            s_c[w][lane + 1] = c;  // the sum over tokens before lane + 1
+        }
+        if (lane == 0) s_c[w][0] = 0.f;
+        __syncthreads();
+        float here = around, dg = 0.f;  // `here`: at this wave's first token
+        for (int i = 0; i < w; ++i) here += s_c[i][C] - s_r[i][0];
+        for (int i = 0; i < W; ++i) around += s_c[i][C] - s_r[i][0];
+        if (lane < cnt) {
+            // (the chunk's first token: the gradient handed on, without taking r's sum out and in again)
+            dg = lane == 0 ? here : near + s_r[w][lane] + s_c[w][lane] + (here - s_r[w][0]);
+            if (a.gg) a.gg[(row + lane) * a.H + h] = dg;
+        }
+        total += dg;
+    }
+    if (a.gg_part) {
+        total = wave_sum_row3(total);
+        __syncthreads();
+        if (lane == 63) s_sum[w] = total;
+        __syncthreads();
+        if (t == 0) a.gg_part[(b * a.n_spans + span) * a.H + h] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    }
 }
 
 // gg[h] = the sum of its n parts, in 64 bits, in an order that does not change
@@ -212,7 +302,7 @@ BwdPlan plan_bwd(int B, int T, int Hq, int H, int D, bool gates) {
 }
 
 struct BwdWs {
-    size_t ahead, back, ahead_log, back_log, gs0, r_part, c_part, gg_part, bytes;
+    size_t ahead, back, ahead_log, back_log, gs0, r_part, c_part, near, gg_part, bytes;
 };
 BwdWs bwd_ws(int B, int T, int Hq, int H, int D, bool gates) {
     const Plan p = plan_bwd(B, T, Hq, H, D, gates).k;
@@ -228,6 +318,7 @@ BwdWs bwd_ws(int B, int T, int Hq, int H, int D, bool gates) {
         w.gs0 = l.take(B * state);
         w.r_part = l.take(tiles * rows * Hq * 4);
         w.c_part = l.take(tiles * rows * H * 4);
+        w.near = l.take(rows * H * 4);
         w.gg_part = l.take(static_cast<size_t>(p.n_slots) * H * 4);
     }
     w.bytes = l.bytes;
@@ -374,20 +465,27 @@ hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
     if (!gates) return hipSuccess;
     const bool constant = a.g_sb == 0 && a.g_st == 0;
     if (a.T > 0) {
+        float* near = at<float>(a.workspace, w.near);
+        DecayNear n{};
+        n.q = q.p, n.q_sb = q.s[0], n.q_st = q.s[1], n.q_sh = q.s[2];
+        n.k = k.p, n.k_sb = k.s[0], n.k_st = k.s[1], n.k_sh = k.s[2];
+        n.v = v.p, n.v_sb = v.s[0], n.v_st = v.s[1], n.v_sh = v.s[2];
+        n.go = go.p, n.go_sb = go.s[0], n.go_st = go.s[1], n.go_sh = go.s[2];
+        n.g = a.g, n.g_sb = a.g_sb, n.g_st = a.g_st;
+        n.near = near, n.n_rows = static_cast<int64_t>(a.B) * a.T;
+        n.B = a.B, n.T = a.T, n.Hq = a.Hq, n.H = a.H, n.D = a.D, n.scale = a.scale;
+        if (hipError_t e = a.bf16 ? decay_near_bf16(n, st) : decay_near_f32(n, st); e != hipSuccess) return e;
         DecayGateGrad x{};
-        x.q = q.p, x.q_sb = q.s[0], x.q_st = q.s[1], x.q_sh = q.s[2];
-        x.k = k.p, x.k_sb = k.s[0], x.k_st = k.s[1], x.k_sh = k.s[2];
-        x.v = v.p, x.v_sb = v.s[0], x.v_st = v.s[1], x.v_sh = v.s[2];
-        x.go = go.p, x.go_sb = go.s[0], x.go_st = go.s[1], x.go_sh = go.s[2];
         x.g = a.g, x.g_sb = a.g_sb, x.g_st = a.g_st;
-        x.r_part = gq.part, x.c_part = gk.part;
+        x.r_part = gq.part, x.c_part = gk.part, x.near = near;
         x.ahead = gq.span_state, x.back = gk.span_state, x.s0 = a.s0, x.gs0 = gs0;
         x.gg = constant ? nullptr : a.gg, x.gg_part = constant ? at<float>(a.workspace, w.gg_part) : nullptr;
         x.n_rows = static_cast<int64_t>(a.B) * a.T;
         x.B = a.B, x.T = a.T, x.Hq = a.Hq, x.H = a.H, x.D = a.D;
-        x.n_tiles = p.k.n_tiles, x.span = p.k.span, x.n_spans = p.k.n_spans;
-        x.scale = a.scale;
-        if (hipError_t e = a.bf16 ? decay_gate_grad_bf16(x, st) : decay_gate_grad_f32(x, st); e != hipSuccess) return e;
+        x.n_tiles = p.k.n_tiles, x.span = p.k.span, x.n_spans = p.k.n_spans, x.chunk = a.bf16 ? 64 : 32;
+        const int64_t groups = static_cast<int64_t>(a.B) * a.H * p.k.n_spans;
+        hipLaunchKernelGGL(gate_grad, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, x);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     if (constant) {
         hipLaunchKernelGGL(sum_gate_parts, dim3(static_cast<unsigned>(a.H)), dim3(256), 0, st,

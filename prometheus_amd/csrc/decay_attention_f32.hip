@@ -5,6 +5,6 @@
 namespace pm {
 
 hipError_t decay_pass_f32(const DecayPasses& a, int kind, hipStream_t st) { return run_pass<3>(a, kind, st); }
-hipError_t decay_gate_grad_f32(const DecayGateGrad& a, hipStream_t st) { return run_gate_grad<3>(a, st); }
+hipError_t decay_near_f32(const DecayNear& a, hipStream_t st) { return run_near<3>(a, st); }
 
 }  // namespace pm

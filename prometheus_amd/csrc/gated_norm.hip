@@ -119,9 +119,7 @@ hipError_t launch_gated_norm(const GatedNormArgs& a, hipStream_t st) { return by
 
 hipError_t launch_gated_norm_bwd(const GatedNormArgs& a, hipStream_t st) {
     if (hipError_t e = by_types<true>(a, st); e != hipSuccess || !a.gw) return e;
-    hipLaunchKernelGGL(sum_row_parts, dim3(static_cast<unsigned>((a.C + 15) / 16)), dim3(1024), 0, st, a.part,
-                       RowParts{{a.gw, nullptr}}, static_cast<int>(gated_norm_groups(a.rows, a.C)), a.C);
-    return hipGetLastError();
+    return launch_row_parts(a.part, {{a.gw, nullptr}}, static_cast<int>(gated_norm_groups(a.rows, a.C)), a.C, st);
 }
 
 }  // namespace pm

@@ -796,7 +796,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
         if constexpr (AUX)
             if (a.part && (dst || first_m) && t < cnt) {
                 const int64_t tok = rows0 + (a.reverse ? first + cnt - 1 - t : first + t);
-                a.part[(static_cast<int64_t>(tile) * a.n_rows + tok) * a.HO + ho] =
+                a.part[(static_cast<int64_t>(tile) * a.HO + ho) * a.n_rows + tok] =
                     (s_part[0][t] + s_part[1][t]) + (s_part[2][t] + s_part[3][t]);
             }
         c = c_next, m = m_next;
@@ -841,104 +841,76 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
 // token, e^g <the state before it, the gradient of the state behind it>, which is handed on from chunk
 // to chunk: no sum is taken as a difference of others over more than a span's 512 tokens.
 //
-// A workgroup takes a span, each of its four waves a chunk at a time.
-template <int P>
-__global__ __launch_bounds__(256) void decay_gate_grad(DecayGateGrad a) {
+// This kernel has the pairs inside chunks, one wave a chunk, from all four tensors once more.  (With
+// q's rows as a fourth tile of gq's pass instead, whose registers are full, that pass took 146 us
+// longer at B4 T4096 H16 D128.)  WIDE: D is a multiple of 8, rows load without tests.
+template <int P, bool WIDE>
+__global__ __launch_bounds__(256, P == 1 ? 2 : 3) void decay_near(DecayNear a) {
     using Sh = DecayShape<P>;
+    using E = typename Raw8<P>::E;
     constexpr int C = Sh::C, MT = Sh::MT, W = 4;
     __shared__ float sp[W][C][C + 1];
     __shared__ float2 sg[W][C];
-    __shared__ float s_r[W][C], s_c[W][C + 1], s_sum[W];
     const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, lg = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int G = a.Hq / a.H;
+    const int G = a.Hq / a.H, n_blocks = (a.T + W * C - 1) / (W * C);
     const int64_t id = blockIdx.x;
     const int h = static_cast<int>(id % a.H);
-    const int span = static_cast<int>(id / a.H % a.n_spans);
-    const int64_t b = id / a.H / a.n_spans;
-    const int begin = span * a.span, end = min(begin + a.span, a.T);
+    const int64_t b = id / a.H / n_blocks;
+    const int first = (static_cast<int>(id / a.H % n_blocks) * W + w) * C;
+    const int cnt = min(C, a.T - first);  // (may be <= 0 for the last waves)
 
-    // the gradient at the span's first token
-    float around = 0.f;
-    {
-        const int64_t size = static_cast<int64_t>(a.D) * a.D;
-        const float *x = nullptr, *y = nullptr;
-        if (span > 0) {
-            x = a.ahead + ((b * a.n_spans + span) * a.H + h) * size;
-            y = a.back + ((b * a.n_spans + a.n_spans - span) * a.H + h) * size;
-        } else if (a.s0) {
-            x = a.s0 + (b * a.H + h) * size;
-            y = a.gs0 + (b * a.H + h) * size;  // (with the first token's decay already)
-        }
-        if (x) {
-            float dot[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int64_t i = t; i < size; i += 1024)
+    const double x = lane < cnt ? log2_decay(a.g[b * a.g_sb + (first + lane) * a.g_st + h]) : 0.0;
+    const double sum = wave_prefix_f64(x);
+    if (lane < C) sg[w][lane] = split_log(sum);
+    float near = 0.f;
+    for (int m = 0; m < G; ++m) {
+        const int64_t hq = static_cast<int64_t>(h) * G + m;
+        f32x4_t x1[Sh::TRI], x2[Sh::TRI];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i + 256 * j < size) dot[j] += x[i + 256 * j] * y[i + 256 * j];
-            const float sum = wave_sum_row3((dot[0] + dot[1]) + (dot[2] + dot[3]));
-            if (lane == 63) s_sum[w] = sum;
-            __syncthreads();
-            around = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-            if (span > 0) around *= exp2_f64(log2_decay(a.g[b * a.g_sb + begin * a.g_st + h]));
-        }
-    }
-
-    float total = 0.f;
-    for (int base = begin; base < end; base += W * C) {
-        const int first = base + w * C, cnt = min(C, end - first);  // (may be <= 0 for the last waves)
-        const double x = lane < cnt ? log2_decay(a.g[b * a.g_sb + (first + lane) * a.g_st + h]) : 0.0;
-        // r from the last token to the first (lane l: row C - 1 - l), c from the first to the last
-        float r = 0.f, c = 0.f;
-        const int back = C - 1 - lane;
-        if (back >= 0 && back < cnt)
-            for (int y = 0; y < a.n_tiles; ++y)
-                for (int m = 0; m < G; ++m)
-                    r += a.r_part[(static_cast<int64_t>(y) * a.n_rows + b * a.T + first + back) * a.Hq + h * G + m];
-        if (lane < cnt)
-            for (int y = 0; y < a.n_tiles; ++y)
-                c += a.c_part[(static_cast<int64_t>(y) * a.n_rows + b * a.T + first + lane) * a.H + h];
-        __syncthreads();  // (the chunks before are done with LDS)
-        const double sum = wave_prefix_f64(x);
-        if (lane < C) sg[w][lane] = split_log(sum);
-
-        f32x4_t acc[Sh::TRI];
-#pragma unroll
-        for (int i = 0; i < Sh::TRI; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        for (int m = 0; m < G; ++m) {
-            const int64_t hq = static_cast<int64_t>(h) * G + m;
-            f32x4_t x1[Sh::TRI], x2[Sh::TRI];
-#pragma unroll
-            for (int i = 0; i < Sh::TRI; ++i) x1[i] = x2[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            for (int col = 8 * lg; col - 8 * lg < a.D; col += 32) {
-                auto rows = [&](const void* p, int64_t sb, int64_t st, int64_t sh, int64_t head, u32x4_t(&op)[MT][P]) {
+        for (int i = 0; i < Sh::TRI; ++i) x1[i] = x2[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (cnt > 0) {
+            const E* kp = static_cast<const E*>(a.k) + b * a.k_sb + first * a.k_st + h * a.k_sh;
+            const E* vp = static_cast<const E*>(a.v) + b * a.v_sb + first * a.v_st + h * a.v_sh;
+            const E* qp = static_cast<const E*>(a.q) + b * a.q_sb + first * a.q_st + hq * a.q_sh;
+            const E* op = static_cast<const E*>(a.go) + b * a.go_sb + first * a.go_st + hq * a.go_sh;
+            for (int c0 = 0; c0 < a.D; c0 += 32) {
+                const int col = c0 + 8 * lg;
+                // (rows and columns that are there, cleared afterwards where they stand for others)
+                auto ask = [&](Raw8<P>(&r)[MT], const E* p, int64_t st) {
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        Raw8<P> v;
-                        const int row = 16 * i + l16;
-                        if (row < cnt && col < a.D)
-                            v.load(static_cast<const typename Raw8<P>::E*>(p) + (b * sb + (first + row) * st + head * sh + col),
-                                   a.D - col);
-                        else v.zero();
-                        v.planes(op[i]);
+                        const E* at = p + min(16 * i + l16, cnt - 1) * st;
+                        if constexpr (WIDE) r[i].load(at + min(col, a.D - 8));
+                        else r[i].load(at + col, max(a.D - col, 0));
                     }
                 };
+                auto ready = [&](Raw8<P>(&r)[MT], u32x4_t(&x)[MT][P]) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        if (16 * i + l16 >= cnt || col >= a.D) r[i].zero();
+                        r[i].planes(x[i]);
+                    }
+                };
+                Raw8<P> r1[MT], r2[MT], r3[MT], r4[MT];
+                ask(r1, kp, a.k_st);
+                ask(r2, qp, a.q_st);
+                ask(r3, vp, a.v_st);
+                ask(r4, op, a.go_st);
                 u32x4_t src[MT][P], dst[MT][P];
-                rows(a.k, a.k_sb, a.k_st, a.k_sh, h, src);
-                rows(a.q, a.q_sb, a.q_st, a.q_sh, hq, dst);
+                ready(r1, src);
+                ready(r2, dst);
 #pragma unroll
                 for (int i = 0, n = 0; i < MT; ++i)
 #pragma unroll
                     for (int j = 0; j <= i; ++j, ++n) x1[n] = mfma_planes<P, P>(src[j], dst[i], x1[n]);
-                rows(a.v, a.v_sb, a.v_st, a.v_sh, h, src);
-                rows(a.go, a.go_sb, a.go_st, a.go_sh, hq, dst);
+                ready(r3, src);
+                ready(r4, dst);
 #pragma unroll
                 for (int i = 0, n = 0; i < MT; ++i)
 #pragma unroll
                     for (int j = 0; j <= i; ++j, ++n) x2[n] = mfma_planes<P, P>(src[j], dst[i], x2[n]);
             }
-#pragma unroll
-            for (int i = 0; i < Sh::TRI; ++i) acc[i] += x1[i] * x2[i];
         }
         __syncthreads();
 #pragma unroll
@@ -950,48 +922,29 @@ __global__ __launch_bounds__(256) void decay_gate_grad(DecayGateGrad a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int col = 16 * j + 4 * lg + k;
-                    sp[w][row][col] = col < row ? acc[n][k] * exp2_diff(gi, sg[w][col]) : 0.f;
+                    sp[w][row][col] = col < row ? x1[n][k] * x2[n][k] * exp2_diff(gi, sg[w][col]) : 0.f;
                 }
             }
-        r = wave_prefix_sum(r);
-        c = wave_prefix_sum(c);
-        if (lane < C) {
-            s_r[w][back] = r;      // the sum over tokens from `back` on
-            s_c[w][lane + 1] = c;  // the sum over tokens before lane + 1
-        }
-        if (lane == 0) s_c[w][0] = 0.f;
         __syncthreads();
-        if (lane < C) {  // row by row: the sums over j < t
+        if (lane < C) {  // row by row: the sums over j < t, sixteen reads in flight
             float run = 0.f;
-            for (int j = 0; j <= lane; ++j) {
-                const float p = sp[w][lane][j];
-                sp[w][lane][j] = run;
-                run += p;
+            for (int j = 0; j < C; j += 16) {
+                float p[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) p[k] = sp[w][lane][j + k];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    sp[w][lane][j + k] = run;
+                    run += j + k < lane ? p[k] : 0.f;  // (above the diagonal there may be anything)
+                }
             }
         }
         __syncthreads();
-        float dg = 0.f;
         if (lane < C)
-            for (int i = lane; i < C; ++i) dg += sp[w][i][lane];
-        float here = around;  // at this wave's first token
-        for (int i = 0; i < w; ++i) here += s_c[i][C] - s_r[i][0];
-        for (int i = 0; i < W; ++i) around += s_c[i][C] - s_r[i][0];
-        if (lane < cnt) {
-            // (the chunk's first token: the gradient handed on, without taking r's sum out and in again)
-            dg = lane == 0 ? here : a.scale * dg + s_r[w][lane] + s_c[w][lane] + (here - s_r[w][0]);
-            if (a.gg) a.gg[(b * a.T + first + lane) * a.H + h] = dg;
-        } else {
-            dg = 0.f;
-        }
-        total += dg;
+#pragma unroll 16
+            for (int i = 0; i < C; ++i) near += i >= lane ? sp[w][i][lane] : 0.f;
     }
-    if (a.gg_part) {
-        total = wave_sum_row3(total);
-        __syncthreads();
-        if (lane == 63) s_sum[w] = total;
-        __syncthreads();
-        if (t == 0) a.gg_part[(b * a.n_spans + span) * a.H + h] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-    }
+    if (lane < cnt) a.near[h * a.n_rows + b * a.T + first + lane] = a.scale * near;
 }
 
 template <int P, int DK>
@@ -1019,9 +972,11 @@ hipError_t run_pass(const DecayPasses& a, int kind, hipStream_t st) {
 }
 
 template <int P>
-hipError_t run_gate_grad(const DecayGateGrad& a, hipStream_t st) {
-    const int64_t n = static_cast<int64_t>(a.B) * a.H * a.n_spans;
-    hipLaunchKernelGGL((decay_gate_grad<P>), dim3(static_cast<unsigned>(n)), dim3(256), 0, st, a);
+hipError_t run_near(const DecayNear& a, hipStream_t st) {
+    const int64_t n = static_cast<int64_t>(a.B) * a.H * ((a.T + 4 * DecayShape<P>::C - 1) / (4 * DecayShape<P>::C));
+    const dim3 grid(static_cast<unsigned>(n));
+    if (a.D % 8 == 0) hipLaunchKernelGGL((decay_near<P, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((decay_near<P, false>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

@@ -44,7 +44,7 @@ struct DecayPass {
     // for the gates' gradient
     const void* aux;    // q (gq's pass), k (gk's)
     int64_t x_sb, x_st, x_sh;
-    float* part;        // nullable; [tile][row][HO]: each token's product of aux with the state's part of O
+    float* part;        // nullable; [tile][HO][row]: each token's product of aux with the state's part of O
     int64_t n_rows;
 };
 
@@ -54,7 +54,8 @@ struct DecayPasses {
     int n;
 };
 
-struct DecayGateGrad {
+// The pairs inside chunks.
+struct DecayNear {
     const void* q;
     const void* k;
     const void* v;
@@ -62,24 +63,34 @@ struct DecayGateGrad {
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, go_sb, go_st, go_sh;
     const float* g;
     int64_t g_sb, g_st;
-    const float* r_part;
-    const float* c_part;
+    float* near;  // [H][row]
+    int64_t n_rows;
+    int B, T, Hq, H, D;
+    float scale;
+};
+
+// The gates' gradient from what the passes left.
+struct DecayGateGrad {
+    const float* g;
+    int64_t g_sb, g_st;
+    const float* r_part;  // [tile][Hq][row]
+    const float* c_part;  // [tile][H][row]
+    const float* near;    // [H][row]
     const float* ahead;   // nullable: the states before the spans, [slot][H] (slots in order of time)
     const float* back;    // nullable: their gradients behind the spans, [slot][H], the last span's first
     const float* s0;      // nullable: the first state
     const float* gs0;     // its gradient, where s0 is given
-    float* gg;       // nullable: (B, T, H)
-    float* gg_part;  // nullable: (B, n_spans, H)
+    float* gg;            // nullable: (B, T, H)
+    float* gg_part;       // nullable: (B, n_spans, H)
     int64_t n_rows;
-    int B, T, Hq, H, D, n_tiles, span, n_spans;
-    float scale;
+    int B, T, Hq, H, D, n_tiles, span, n_spans, chunk;
 };
 
 // kind: 0 outputs and states, 1 the same and `part`s, 2 each span's own share of the state (from zeros) but
 // the last one's, to the next slot of span_state.
 hipError_t decay_pass_bf16(const DecayPasses& a, int kind, hipStream_t st);
 hipError_t decay_pass_f32(const DecayPasses& a, int kind, hipStream_t st);
-hipError_t decay_gate_grad_bf16(const DecayGateGrad& a, hipStream_t st);
-hipError_t decay_gate_grad_f32(const DecayGateGrad& a, hipStream_t st);
+hipError_t decay_near_bf16(const DecayNear& a, hipStream_t st);
+hipError_t decay_near_f32(const DecayNear& a, hipStream_t st);
 
 }  // namespace pm

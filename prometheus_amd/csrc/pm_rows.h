@@ -114,31 +114,38 @@ __device__ __forceinline__ void store_part(const float (&g)[NV][8], float* lds, 
     }
 }
 
-// gw[c] = the sum over n parts, 64 threads for each of 16 columns, in an order that does not change; row
-// blockIdx.y is another weight's.
+// gw[c] = the sum over n parts, COLS columns to a workgroup and 1024 / COLS threads to each, in an order
+// that does not change; row blockIdx.y is another weight's.
 struct RowParts {
     float* gw[2];
 };
+template <int COLS>
 __global__ __launch_bounds__(1024) void sum_row_parts(const float* part, RowParts to, int n, int C) {
-    __shared__ float s[64][17];
-    const int col = blockIdx.x * 16 + threadIdx.x % 16, first = threadIdx.x / 16;
+    constexpr int ROWS = 1024 / COLS;
+    __shared__ float s[ROWS][COLS + 1];
+    const int c = threadIdx.x % COLS, col = blockIdx.x * COLS + c, first = threadIdx.x / COLS;
     float* gw = to.gw[blockIdx.y];
     if (!gw) return;
     const float* p = part + static_cast<int64_t>(blockIdx.y) * n * C;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};  // (four loads in flight)
+    float x[8] = {};  // (eight loads in flight)
     if (col < C)
-        for (int i = first; i < n; i += 256)
+        for (int i = first; i < n; i += 8 * ROWS)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (i + 64 * j < n) x[j] += p[static_cast<int64_t>(i + 64 * j) * C + col];
-    s[first][threadIdx.x % 16] = (x[0] + x[1]) + (x[2] + x[3]);
-    __syncthreads();
-    if (threadIdx.x < 16 && col < C) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) sum += s[i][threadIdx.x];
-        gw[col] = sum;
+            for (int j = 0; j < 8; ++j)
+                if (i + ROWS * j < n) x[j] += p[static_cast<int64_t>(i + ROWS * j) * C + col];
+    s[first][c] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    for (int m = ROWS / 2; m > 0; m /= 2) {
+        __syncthreads();
+        if (first < m) s[first][c] += s[first + m][c];
     }
+    if (first == 0 && col < C) gw[col] = s[0][c];
+}
+// Few columns are spread over more workgroups (C 128 of 2048 parts: 12 us with 16 columns each).
+inline hipError_t launch_row_parts(const float* part, RowParts to, int n, int C, hipStream_t st) {
+    const unsigned weights = to.gw[1] ? 2 : 1;
+    if (C < 1024) hipLaunchKernelGGL(sum_row_parts<4>, dim3((C + 3) / 4, weights), dim3(1024), 0, st, part, to, n, C);
+    else hipLaunchKernelGGL(sum_row_parts<16>, dim3((C + 15) / 16, weights), dim3(1024), 0, st, part, to, n, C);
+    return hipGetLastError();
 }
 
 // How wide rows are held: f.template operator()<L, NV>().

@@ -132,9 +132,7 @@ hipError_t launch_residual_norm(const ResidualNormArgs& a, hipStream_t st) { ret
 
 hipError_t launch_residual_norm_bwd(const ResidualNormArgs& a, hipStream_t st) {
     if (hipError_t e = by_types<true>(a, st); e != hipSuccess || !(a.gw || a.gwp)) return e;
-    hipLaunchKernelGGL(sum_row_parts, dim3(static_cast<unsigned>((a.C + 15) / 16), a.gwp ? 2 : 1), dim3(1024), 0, st, a.part,
-                       RowParts{{a.gw, a.gwp}}, static_cast<int>(residual_norm_groups(a.rows, a.C)), a.C);
-    return hipGetLastError();
+    return launch_row_parts(a.part, {{a.gw, a.gwp}}, static_cast<int>(residual_norm_groups(a.rows, a.C)), a.C, st);
 }
 
 }  // namespace pm
