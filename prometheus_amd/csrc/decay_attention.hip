@@ -224,18 +224,24 @@ struct Plan {
     bool split;
 };
 
-// How a pass is cut into workgroups: one per sequence, state and column tile, or, where that leaves
-// CUs without two, as many again along the sequence (spans of at least kMinSpan tokens; calls of up to 512
-// tokens stay whole, since the states' own pass costs as much as they take).  The query heads of a
-// group go one after another through one workgroup, which reads their keys once, where there is work
-// enough for every CU without them.
+// Workgroups of a pass that the card holds at once (registers and LDS: three to a CU up to D 64, two up
+// to 128, one beyond).
+int64_t resident(int D) { return D <= 64 ? 768 : D <= 128 ? 512 : 256; }
+
+// How a pass is cut into workgroups: one per sequence, state and column tile, or, where the card holds
+// more, as many again along the sequence (spans of at least kMinSpan tokens; calls of up to 512 tokens
+// stay whole, since the states' own pass costs as much as they take).  Of packed sequences, half a span
+// each is lost on average.  The query heads of a group go one after another through one workgroup, which
+// reads their keys once, where there is work enough for every CU without them.
 Plan plan(int n_seqs, int T, int HO, int HS, int D, bool packed) {
     Plan p{(D + decay_cols(D) - 1) / decay_cols(D), 1, max(T, 1), 1, n_seqs, false};
-    const int64_t tokens = packed ? T : static_cast<int64_t>(n_seqs) * T, want = 512;
+    const int64_t tokens = packed ? T : static_cast<int64_t>(n_seqs) * T, want = resident(D);
     if (HO > HS && tokens * HS * p.n_tiles >= want * 256) p.n_dst = HO / HS;
     const int64_t groups = static_cast<int64_t>(HO / p.n_dst) * p.n_tiles;
     if (T > 512 && n_seqs * groups < want) {
-        const int64_t span = std::max<int64_t>((tokens * groups + want - 1) / want, kMinSpan);
+        int64_t slots = (want + groups - 1) / groups;  // wanted
+        if (packed) slots = std::max<int64_t>(want / groups - (n_seqs + 1) / 2, (slots + 1) / 2);
+        const int64_t span = std::max<int64_t>((tokens + slots - 1) / slots, kMinSpan);
         const int64_t n = (T + span - 1) / span;
         p.span = static_cast<int>(((T + n - 1) / n + 63) / 64 * 64);
         p.n_spans = (T + p.span - 1) / p.span;
@@ -282,7 +288,7 @@ struct BwdPlan {
 BwdPlan plan_bwd(int B, int T, int Hq, int H, int D, bool gates) {
     BwdPlan p;
     p.k = Plan{(D + decay_cols(D) - 1) / decay_cols(D), 1, max(T, 1), 1, B, false};
-    const int64_t tokens = static_cast<int64_t>(B) * T, want = 512;
+    const int64_t tokens = static_cast<int64_t>(B) * T, want = resident(D);
     int n_dst = 1;
     if (Hq > H && tokens * H * p.k.n_tiles >= want * 256) n_dst = Hq / H;
     const int64_t groups = static_cast<int64_t>(Hq / n_dst + 2 * H) * p.k.n_tiles;

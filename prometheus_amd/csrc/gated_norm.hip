@@ -98,7 +98,7 @@ struct Launch {
     hipStream_t st;
     template <int L, int NV>
     hipError_t run() const {
-        const int64_t n = gated_norm_groups(a.rows, a.C);
+        const int64_t n = row_groups(a.rows, a.C, BWD);
         hipLaunchKernelGGL((gated_norm_kernel<M, L, NV, BWD>), dim3(static_cast<unsigned>(n)), dim3(threads_of(L)), 0, st, a);
         return hipGetLastError();
     }
@@ -113,7 +113,7 @@ hipError_t by_types(const GatedNormArgs& a, hipStream_t st) {
 
 }  // namespace
 
-int64_t gated_norm_groups(int64_t rows, int C) { return row_groups(rows, C); }
+int64_t gated_norm_groups(int64_t rows, int C) { return row_groups(rows, C, true); }
 
 hipError_t launch_gated_norm(const GatedNormArgs& a, hipStream_t st) { return by_types<false>(a, st); }
 

@@ -432,7 +432,7 @@ struct GatedNormArgs {
 };
 hipError_t launch_gated_norm(const GatedNormArgs& a, hipStream_t st);
 hipError_t launch_gated_norm_bwd(const GatedNormArgs& a, hipStream_t st);
-int64_t gated_norm_groups(int64_t rows, int C);
+int64_t gated_norm_groups(int64_t rows, int C);  // workgroups of the backward
 
 // The norm after a block, the sum with the residual and the norm before the next (residual_norm.hip).
 // Rows of x and the residual are x_st and r_st elements apart; all else is contiguous.
@@ -458,6 +458,6 @@ struct ResidualNormArgs {
 };
 hipError_t launch_residual_norm(const ResidualNormArgs& a, hipStream_t st);
 hipError_t launch_residual_norm_bwd(const ResidualNormArgs& a, hipStream_t st);
-int64_t residual_norm_groups(int64_t rows, int C);
+int64_t residual_norm_groups(int64_t rows, int C);  // workgroups of the backward
 
 }  // namespace pm

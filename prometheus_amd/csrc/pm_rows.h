@@ -162,10 +162,11 @@ hipError_t by_width(int C, F f) {
     if (C <= 8192) return f.template run<1024, 1>();
     return f.template run<1024, 2>();  // (C up to kMaxRow)
 }
-// Workgroups that walk through `rows` rows: as many as stay on the card together.
-inline int64_t row_groups(int64_t rows, int C) {
+// Workgroups that walk through `rows` rows: as many as stay on the card together (a backward has the
+// weights' gradients in registers too, and every workgroup more is another part to sum).
+inline int64_t row_groups(int64_t rows, int C, bool bwd) {
     const int L = C <= 32 ? 4 : C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 1024 ? 64 : C <= 2048 ? 256 : C <= 4096 ? 512 : 1024;
-    const int64_t per = threads_of(L) / L, n = (rows + per - 1) / per, most = 2048 * 256 / threads_of(L);
+    const int64_t per = threads_of(L) / L, n = (rows + per - 1) / per, most = (bwd ? 1024 : 2048) * 256 / threads_of(L);
     return n < most ? n : most;
 }
 

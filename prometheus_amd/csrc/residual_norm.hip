@@ -110,7 +110,7 @@ struct Launch {
     hipStream_t st;
     template <int L, int NV>
     hipError_t run() const {
-        const dim3 grid(static_cast<unsigned>(residual_norm_groups(a.rows, a.C)));
+        const dim3 grid(static_cast<unsigned>(row_groups(a.rows, a.C, BWD)));
         if (a.wp) hipLaunchKernelGGL((residual_norm_kernel<M, L, NV, BWD, true>), grid, dim3(threads_of(L)), 0, st, a);
         else hipLaunchKernelGGL((residual_norm_kernel<M, L, NV, BWD, false>), grid, dim3(threads_of(L)), 0, st, a);
         return hipGetLastError();
@@ -126,7 +126,7 @@ hipError_t by_types(const ResidualNormArgs& a, hipStream_t st) {
 
 }  // namespace
 
-int64_t residual_norm_groups(int64_t rows, int C) { return row_groups(rows, C); }
+int64_t residual_norm_groups(int64_t rows, int C) { return row_groups(rows, C, true); }
 
 hipError_t launch_residual_norm(const ResidualNormArgs& a, hipStream_t st) { return by_types<false>(a, st); }
 
