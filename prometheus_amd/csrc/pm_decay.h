@@ -14,12 +14,15 @@
 // first token's own is applied to the last state.  In a group of query heads that share a key head,
 // the first two run once per query head, the others sum over the group's heads inside a chunk.
 //
-// Products run on bf16 MFMA.  A value of more than 8 bits is a sum of bf16 planes (hi, next, ...),
-// a product of two such sums the products of their planes down to the last plane's size: bf16 inputs
-// are one plane and exact; A, S and the decayed V are two planes next to them (a relative error of
-// 2^-17 at most, against 2^-9 with one: fp32 states and the gates' gradients need it); fp32 inputs
-// and everything else next to them are three (2^-25).  On this card six such bf16 products take 6/16
-// of the time of the fp32 MFMA.
+// Products run on bf16 MFMA.  A value of more than 8 bits is a sum of bf16 planes (the value rounded, what
+// that leaves rounded, ...), a product of two such sums the products of their planes down to the last
+// plane's size.  bf16 inputs are one plane and exact; next to them
+//   the decayed V, which sums into states      three planes (2^-25 relative)
+//   the state and V in passes that leave parts of the gates' gradient, which is fp32: two (2^-17; three
+//     took 403 us where two take 307, at B4 T4096 H16 D128: the registers for them are not there)
+//   A and the state in what comes out in bf16   one (2^-9): half a step of its own type, once
+// fp32 inputs and everything next to them are three.  On this card six such bf16 products take 6/16 of
+// the time of the fp32 MFMA.
 //
 // Log-decays are summed in 64 bits, and kept as a multiple of 2^-10 and a rest, so that a
 // difference G_i - G_j has fp32's relative error also where both are large (behind a closed gate).
@@ -37,7 +40,7 @@ namespace {
 template <int P>
 struct DecayShape {
     static constexpr int C = P == 1 ? 64 : 32;   // tokens of a chunk (three planes of 64 would not fit LDS)
-    static constexpr int PC = P == 1 ? 2 : 3;    // planes of what sums into states and gates' gradients
+    static constexpr int PG = P == 1 ? 2 : 3;    // planes of what sums into the gates' gradient
     static constexpr int PA = P;                 // planes of what sums into outputs of q's type alone
     static constexpr int MT = C / 16;            // 16-token tiles
     static constexpr int TRI = MT * (MT + 1) / 2;  // lower 16x16 tiles of A
@@ -249,12 +252,13 @@ struct DecayTile {
 template <int P, int DK, int KIND>
 __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void decay_pass(DecayPasses passes) {
     using Sh = DecayShape<P>;
-    constexpr int C = Sh::C, PC = Sh::PC, PA = Sh::PA, MT = Sh::MT, KB = DK / 32, MD = DK / 16;
+    constexpr int C = Sh::C, PA = Sh::PA, MT = Sh::MT, KB = DK / 32, MD = DK / 16;
     constexpr int CT = DecayTile<DK>::CT, NT = DecayTile<DK>::NT;
     constexpr int UQ = C * DK / 2048, UV = C * NT / 2048;  // 8-element units per thread
     constexpr int RQ = 2048 / DK, RV = 2048 / NT;          // rows between a thread's units
     constexpr bool OUT = KIND != kPassState, AUX = KIND == kPassPart;
-    constexpr int PS = AUX ? PC : PA;  // planes of the state in the outputs' part
+    constexpr int PS = AUX ? Sh::PG : PA;  // planes of the state in the outputs' part
+    constexpr int PC = AUX ? Sh::PG : 3;   // planes of the decayed V, which sums into the state
     using E = typename std::conditional<P == 1, uint16_t, float>::type;
 
     __shared__ __attribute__((aligned(16))) uint16_t sq[OUT ? P * C * DK : 8];
