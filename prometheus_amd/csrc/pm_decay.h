@@ -242,7 +242,7 @@ __device__ __forceinline__ float exp2_f64(double x) {
 // The next chunk's rows are loaded into registers while this one's products run.
 
 // What a launch of decay_pass does besides its outputs.
-enum { kPassPlain = 0, kPassPart = 1, kPassState = 2 };
+enum { kPassPlain = 0, kPassPart = 1, kPassState = 2, kPassStateG = 3 };  // (G: for the gates' gradient)
 
 template <int DK>
 struct DecayTile {
@@ -250,15 +250,15 @@ struct DecayTile {
 };
 
 template <int P, int DK, int KIND>
-__global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void decay_pass(DecayPasses passes) {
+__global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void decay_pass(DecayPasses passes) {
     using Sh = DecayShape<P>;
     constexpr int C = Sh::C, PA = Sh::PA, MT = Sh::MT, KB = DK / 32, MD = DK / 16;
     constexpr int CT = DecayTile<DK>::CT, NT = DecayTile<DK>::NT;
     constexpr int UQ = C * DK / 2048, UV = C * NT / 2048;  // 8-element units per thread
     constexpr int RQ = 2048 / DK, RV = 2048 / NT;          // rows between a thread's units
-    constexpr bool OUT = KIND != kPassState, AUX = KIND == kPassPart;
+    constexpr bool OUT = KIND < kPassState, AUX = KIND == kPassPart;
     constexpr int PS = AUX ? Sh::PG : PA;  // planes of the state in the outputs' part
-    constexpr int PC = AUX ? Sh::PG : 3;   // planes of the decayed V, which sums into the state
+    constexpr int PC = AUX || KIND == kPassStateG ? Sh::PG : 3;  // planes of the decayed V, which sums into the state
     using E = typename std::conditional<P == 1, uint16_t, float>::type;
 
     __shared__ __attribute__((aligned(16))) uint16_t sq[OUT ? P * C * DK : 8];
@@ -956,12 +956,15 @@ hipError_t launch_pass(const DecayPasses& a, int kind, hipStream_t st) {
     int64_t units = 0;
     for (int i = 0; i < a.n; ++i) {
         const DecayPass& x = a.pass[i];
-        units = std::max(units, static_cast<int64_t>(x.n_slots_grid) * (kind == kPassState ? x.HS : x.HO / x.n_dst));
+        units = std::max(units, static_cast<int64_t>(x.n_slots_grid) * (kind >= kPassState ? x.HS : x.HO / x.n_dst));
     }
     const dim3 grid(static_cast<unsigned>((units + 7) / 8 * 8 * a.pass[0].n_tiles * a.n));
     switch (kind) {
         case kPassPlain: hipLaunchKernelGGL((decay_pass<P, DK, kPassPlain>), grid, dim3(256), 0, st, a); break;
         case kPassPart: hipLaunchKernelGGL((decay_pass<P, DK, kPassPart>), grid, dim3(256), 0, st, a); break;
+        case kPassStateG:
+            hipLaunchKernelGGL((decay_pass<P, DK, P == 1 ? kPassStateG : kPassState>), grid, dim3(256), 0, st, a);
+            break;
         default: hipLaunchKernelGGL((decay_pass<P, DK, kPassState>), grid, dim3(256), 0, st, a); break;
     }
     return hipGetLastError();
