@@ -80,7 +80,8 @@ __global__ __launch_bounds__(256) void gate_grad(DecayGateGrad a) {
         float r = 0.f, c = 0.f, near = 0.f;
         const int back = C - 1 - lane;
         const int64_t row = b * a.T + first;
-        if (lane < cnt) near = a.near[h * a.n_rows + row + lane];
+        if (lane < cnt)
+            for (int m = 0; m < G; ++m) near += a.near[(static_cast<int64_t>(h) * G + m) * a.n_rows + row + lane];
         for (int y = 0; y < a.n_tiles; ++y) {
             if (back >= 0 && back < cnt)
                 for (int m = 0; m < G; ++m)
@@ -324,7 +325,7 @@ BwdWs bwd_ws(int B, int T, int Hq, int H, int D, bool gates) {
         w.gs0 = l.take(B * state);
         w.r_part = l.take(tiles * rows * Hq * 4);
         w.c_part = l.take(tiles * rows * H * 4);
-        w.near = l.take(rows * H * 4);
+        w.near = l.take(rows * Hq * 4);
         w.gg_part = l.take(static_cast<size_t>(p.n_slots) * H * 4);
     }
     w.bytes = l.bytes;

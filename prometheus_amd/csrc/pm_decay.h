@@ -857,98 +857,95 @@ __global__ __launch_bounds__(256, P == 1 ? 2 : 3) void decay_near(DecayNear a) {
     __shared__ float2 sg[W][C];
     const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, lg = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int G = a.Hq / a.H, n_blocks = (a.T + W * C - 1) / (W * C);
+    const int n_blocks = (a.T + W * C - 1) / (W * C);
     const int64_t id = blockIdx.x;
-    const int h = static_cast<int>(id % a.H);
-    const int64_t b = id / a.H / n_blocks;
-    const int first = (static_cast<int>(id / a.H % n_blocks) * W + w) * C;
+    const int hq = static_cast<int>(id % a.Hq), h = hq / (a.Hq / a.H);
+    const int64_t b = id / a.Hq / n_blocks;
+    const int first = (static_cast<int>(id / a.Hq % n_blocks) * W + w) * C;
     const int cnt = min(C, a.T - first);  // (may be <= 0 for the last waves)
 
     const double x = lane < cnt ? log2_decay(a.g[b * a.g_sb + (first + lane) * a.g_st + h]) : 0.0;
     const double sum = wave_prefix_f64(x);
     if (lane < C) sg[w][lane] = split_log(sum);
-    float near = 0.f;
-    for (int m = 0; m < G; ++m) {
-        const int64_t hq = static_cast<int64_t>(h) * G + m;
-        f32x4_t x1[Sh::TRI], x2[Sh::TRI];
+    f32x4_t x1[Sh::TRI], x2[Sh::TRI];
 #pragma unroll
-        for (int i = 0; i < Sh::TRI; ++i) x1[i] = x2[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        if (cnt > 0) {
-            const E* kp = static_cast<const E*>(a.k) + b * a.k_sb + first * a.k_st + h * a.k_sh;
-            const E* vp = static_cast<const E*>(a.v) + b * a.v_sb + first * a.v_st + h * a.v_sh;
-            const E* qp = static_cast<const E*>(a.q) + b * a.q_sb + first * a.q_st + hq * a.q_sh;
-            const E* op = static_cast<const E*>(a.go) + b * a.go_sb + first * a.go_st + hq * a.go_sh;
-            for (int c0 = 0; c0 < a.D; c0 += 32) {
-                const int col = c0 + 8 * lg;
-                // (rows and columns that are there, cleared afterwards where they stand for others)
-                auto ask = [&](Raw8<P>(&r)[MT], const E* p, int64_t st) {
+    for (int i = 0; i < Sh::TRI; ++i) x1[i] = x2[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (cnt > 0) {
+        const E* kp = static_cast<const E*>(a.k) + b * a.k_sb + first * a.k_st + h * a.k_sh;
+        const E* vp = static_cast<const E*>(a.v) + b * a.v_sb + first * a.v_st + h * a.v_sh;
+        const E* qp = static_cast<const E*>(a.q) + b * a.q_sb + first * a.q_st + hq * a.q_sh;
+        const E* op = static_cast<const E*>(a.go) + b * a.go_sb + first * a.go_st + hq * a.go_sh;
+        for (int c0 = 0; c0 < a.D; c0 += 32) {
+            const int col = c0 + 8 * lg;
+            // (rows and columns that are there, cleared afterwards where they stand for others)
+            auto ask = [&](Raw8<P>(&r)[MT], const E* p, int64_t st) {
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        const E* at = p + min(16 * i + l16, cnt - 1) * st;
-                        if constexpr (WIDE) r[i].load(at + min(col, a.D - 8));
-                        else r[i].load(at + col, max(a.D - col, 0));
-                    }
-                };
-                auto ready = [&](Raw8<P>(&r)[MT], u32x4_t(&x)[MT][P]) {
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        if (16 * i + l16 >= cnt || col >= a.D) r[i].zero();
-                        r[i].planes(x[i]);
-                    }
-                };
-                Raw8<P> r1[MT], r2[MT], r3[MT], r4[MT];
-                ask(r1, kp, a.k_st);
-                ask(r2, qp, a.q_st);
-                ask(r3, vp, a.v_st);
-                ask(r4, op, a.go_st);
-                u32x4_t src[MT][P], dst[MT][P];
-                ready(r1, src);
-                ready(r2, dst);
-#pragma unroll
-                for (int i = 0, n = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j <= i; ++j, ++n) x1[n] = mfma_planes<P, P>(src[j], dst[i], x1[n]);
-                ready(r3, src);
-                ready(r4, dst);
-#pragma unroll
-                for (int i = 0, n = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j <= i; ++j, ++n) x2[n] = mfma_planes<P, P>(src[j], dst[i], x2[n]);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0, n = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j <= i; ++j, ++n) {
-                const int row = 16 * i + l16;
-                const float2 gi = sg[w][row];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int col = 16 * j + 4 * lg + k;
-                    sp[w][row][col] = col < row ? x1[n][k] * x2[n][k] * exp2_diff(gi, sg[w][col]) : 0.f;
+                for (int i = 0; i < MT; ++i) {
+                    const E* at = p + min(16 * i + l16, cnt - 1) * st;
+                    if constexpr (WIDE) r[i].load(at + min(col, a.D - 8));
+                    else r[i].load(at + col, max(a.D - col, 0));
                 }
-            }
-        __syncthreads();
-        if (lane < C) {  // row by row: the sums over j < t, sixteen reads in flight
-            float run = 0.f;
-            for (int j = 0; j < C; j += 16) {
-                float p[16];
+            };
+            auto ready = [&](Raw8<P>(&r)[MT], u32x4_t(&x)[MT][P]) {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) p[k] = sp[w][lane][j + k];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    sp[w][lane][j + k] = run;
-                    run += j + k < lane ? p[k] : 0.f;  // (above the diagonal there may be anything)
+                for (int i = 0; i < MT; ++i) {
+                    if (16 * i + l16 >= cnt || col >= a.D) r[i].zero();
+                    r[i].planes(x[i]);
                 }
-            }
+            };
+            Raw8<P> r1[MT], r2[MT], r3[MT], r4[MT];
+            ask(r1, kp, a.k_st);
+            ask(r2, qp, a.q_st);
+            ask(r3, vp, a.v_st);
+            ask(r4, op, a.go_st);
+            u32x4_t src[MT][P], dst[MT][P];
+            ready(r1, src);
+            ready(r2, dst);
+#pragma unroll
+            for (int i = 0, n = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j <= i; ++j, ++n) x1[n] = mfma_planes<P, P>(src[j], dst[i], x1[n]);
+            ready(r3, src);
+            ready(r4, dst);
+#pragma unroll
+            for (int i = 0, n = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j <= i; ++j, ++n) x2[n] = mfma_planes<P, P>(src[j], dst[i], x2[n]);
         }
-        __syncthreads();
-        if (lane < C)
-#pragma unroll 16
-            for (int i = 0; i < C; ++i) near += i >= lane ? sp[w][i][lane] : 0.f;
     }
-    if (lane < cnt) a.near[h * a.n_rows + b * a.T + first + lane] = a.scale * near;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0, n = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j <= i; ++j, ++n) {
+            const int row = 16 * i + l16;
+            const float2 gi = sg[w][row];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int col = 16 * j + 4 * lg + k;
+                sp[w][row][col] = col < row ? x1[n][k] * x2[n][k] * exp2_diff(gi, sg[w][col]) : 0.f;
+            }
+        }
+    __syncthreads();
+    if (lane < C) {  // row by row: the sums over j < t, sixteen reads in flight
+        float run = 0.f;
+        for (int j = 0; j < C; j += 16) {
+            float p[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) p[k] = sp[w][lane][j + k];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                sp[w][lane][j + k] = run;
+                run += j + k < lane ? p[k] : 0.f;  // (above the diagonal there may be anything)
+            }
+        }
+    }
+    __syncthreads();
+    float near = 0.f;
+    if (lane < C)
+#pragma unroll 16
+        for (int i = 0; i < C; ++i) near += i >= lane ? sp[w][i][lane] : 0.f;
+    if (lane < cnt) a.near[hq * a.n_rows + b * a.T + first + lane] = a.scale * near;
 }
 
 template <int P, int DK>
@@ -980,7 +977,7 @@ hipError_t run_pass(const DecayPasses& a, int kind, hipStream_t st) {
 
 template <int P>
 hipError_t run_near(const DecayNear& a, hipStream_t st) {
-    const int64_t n = static_cast<int64_t>(a.B) * a.H * ((a.T + 4 * DecayShape<P>::C - 1) / (4 * DecayShape<P>::C));
+    const int64_t n = static_cast<int64_t>(a.B) * a.Hq * ((a.T + 4 * DecayShape<P>::C - 1) / (4 * DecayShape<P>::C));
     const dim3 grid(static_cast<unsigned>(n));
     if (a.D % 8 == 0) hipLaunchKernelGGL((decay_near<P, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((decay_near<P, false>), grid, dim3(256), 0, st, a);

@@ -63,7 +63,7 @@ struct DecayNear {
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, go_sb, go_st, go_sh;
     const float* g;
     int64_t g_sb, g_st;
-    float* near;  // [H][row]
+    float* near;  // [Hq][row]
     int64_t n_rows;
     int B, T, Hq, H, D;
     float scale;
@@ -75,7 +75,7 @@ struct DecayGateGrad {
     int64_t g_sb, g_st;
     const float* r_part;  // [tile][Hq][row]
     const float* c_part;  // [tile][H][row]
-    const float* near;    // [H][row]
+    const float* near;    // [Hq][row]
     const float* ahead;   // nullable: the states before the spans, [slot][H] (slots in order of time)
     const float* back;    // nullable: their gradients behind the spans, [slot][H], the last span's first
     const float* s0;      // nullable: the first state
