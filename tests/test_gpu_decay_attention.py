@@ -78,6 +78,8 @@ SHAPES = [
     (1, 100, 2, 2, 200),
     (1, 70, 1, 1, 256),
     (1, 40, 1, 1, 1),
+    (1, 100, 2, 2, 100),
+    (2, 90, 2, 2, 12),
     (3, 1100, 2, 1, 64),  # several workgroups along the sequence
     (1, 1555, 4, 2, 128),
 ]
@@ -353,3 +355,202 @@ def test_a_missing_gradient():
     for a, b in zip(only, both):
         assert torch.equal(a, b)
     assert not only[0].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_heads_of_a_group_one_after_another(dtype):
+    """So much work that a workgroup takes all query heads of a group."""
+    x = inputs(64, 800, 8, 4, 16, dtype, seed=5)
+    gen = torch.Generator().manual_seed(6)
+    go, gs = torch.randn(x[0].shape, generator=gen).to(dtype), torch.randn(64, 4, 16, 16, generator=gen)
+    dev = [t.requires_grad_(True) for t in gpu(*x)]
+    o, s = kernels.decay_attention(*dev)
+    check_forward(*x, 1.0, o, s)
+    got = torch.autograd.grad((o, s), dev, (go.cuda(), gs.cuda()))
+    want = ref.decay_bwd(*x, go, gs)
+    size = ref.decay_bwd(*size_of(*x[:3]), x[3], x[4].abs(), go.abs(), gs.abs())
+    for i in range(3):
+        near(got[i], want[i], size[i], eps_out(dtype, 800))
+    near(got[3], want[3], size[3].amax(1, keepdim=True).expand_as(size[3]), 17 * eps_of(dtype, 800))
+    near(got[4], want[4], size[4], eps_of(dtype, 800))
+
+
+@pytest.mark.parametrize("T", [70, 700])
+def test_gradients_without_the_gates(T):
+    """Constant decays that are not learned: the same gradients of everything else."""
+    q, k, v, g, s0 = inputs(1, T, 2, 1, 64, BF16, gate="head")
+    go = torch.randn(q.shape, device="cuda").to(BF16)
+    grads = []
+    for learned in (True, False):
+        dev = gpu(q, k, v, g, s0)
+        leaves = [t for i, t in enumerate(dev) if learned or i != 3]
+        for t in leaves:
+            t.requires_grad_(True)
+        got = list(torch.autograd.grad(kernels.decay_attention(*dev)[0], leaves, go))
+        if learned:
+            del got[3]
+        grads.append(got)
+    want = ref.decay_bwd(q, k, v, g, s0, go.cpu(), None)
+    size = ref.decay_bwd(*size_of(q, k, v), g, s0.abs(), go.cpu().abs(), None)
+    for got in grads:
+        for i, j in enumerate((0, 1, 2, 4)):
+            near(got[i], want[j], size[j], eps_out(BF16, T) if j < 3 else eps_of(BF16, T))
+
+
+def test_the_first_state_alone_needs_no_gradient():
+    """The gates' gradient takes the first state's, also where nobody asks for that."""
+    q, k, v, g, s0 = inputs(1, 70, 2, 2, 64, BF16)
+    go = torch.randn(q.shape, device="cuda").to(BF16)
+    dev = gpu(q, k, v, g, s0)
+    dev[3].requires_grad_(True)
+    alone, = torch.autograd.grad(kernels.decay_attention(*dev)[0], dev[3:4], go)
+    dev[4].requires_grad_(True)
+    both = torch.autograd.grad(kernels.decay_attention(*dev)[0], dev[3:5], go)
+    assert torch.equal(alone, both[0])
+
+
+def test_an_fp32_output_of_bf16_inputs():
+    q, k, v, g, s0 = inputs(1, 80, 2, 2, 64, BF16)
+    dev = [t.requires_grad_(True) for t in gpu(q, k, v, g, s0)]
+    o, s = kernels.decay_attention(*dev, out_dtype=F32)
+    go = torch.randn(o.shape, device="cuda")
+    got = torch.autograd.grad(o, dev, go)
+    rounded = torch.autograd.grad(kernels.decay_attention(*dev)[0], dev, go.to(BF16))
+    assert all(torch.equal(a, b) for a, b in zip(got, rounded))
+
+
+def test_saved_tensors_may_come_back_elsewhere():
+    """Hooks that park what autograd keeps on the host, in another layout."""
+    q, k, v, g, s0 = inputs(1, 70, 4, 2, 64, BF16)
+
+    def grads(pack, unpack):
+        dev = [t.requires_grad_(True) for t in gpu(q, k, v, g, s0)]
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            o, s = kernels.decay_attention(*dev)
+        return torch.autograd.grad((o, s), dev, (torch.ones_like(o), torch.ones_like(s)))
+
+    want = grads(lambda t: t, lambda t: t)
+    for unpack in (lambda t: t, lambda t: t.cuda().transpose(0, -1).contiguous().transpose(0, -1)):
+        got = grads(lambda t: t.cpu(), unpack)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_not_differentiable_twice():
+    q, k, v, g, s0 = inputs(1, 8, 2, 2, 32, F32)
+    dev = [t.requires_grad_(True) for t in gpu(q, k, v, g, s0)]
+    o, _ = kernels.decay_attention(*dev)
+    gq, = torch.autograd.grad(o.sum(), dev[:1], create_graph=True)
+    with pytest.raises(RuntimeError):
+        gq.sum().backward()
+
+
+def test_a_backward_again():
+    q, k, v, g, s0 = inputs(1, 600, 2, 2, 64, BF16)
+    dev = [t.requires_grad_(True) for t in gpu(q, k, v, g, s0)]
+    o, _ = kernels.decay_attention(*dev)
+    go = torch.randn(o.shape, device="cuda").to(BF16)
+    first = torch.autograd.grad(o, dev, go, retain_graph=True)
+    again = torch.autograd.grad(o, dev, go)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("n", [300, 1500])
+def test_many_packed_sequences(n):
+    """More sequences than threads that count them, most short, some empty, one long."""
+    rng = np.random.default_rng(n)
+    lengths = rng.integers(0, 6, n)
+    lengths[n // 3] = 900
+    N, H, D = int(lengths.sum()), 1, 32
+    q, k, v, g, _ = inputs(1, N, 1, H, D, BF16, seed=n)
+    cu = torch.from_numpy(np.concatenate([[0], np.cumsum(lengths)])).cuda()
+    o, s = kernels.decay_attention_varlen(*gpu(q, k, v, g), cu)
+    kernels.check_varlen()
+    a = 0
+    for i, length in enumerate(lengths.tolist()):
+        if i % 37 == 0 or i == n // 3 or i == n - 1:
+            part = [x[:, a:a + length] for x in (q, k, v, g)]
+            if length:
+                check_forward(*part, None, 1.0, o[:, a:a + length], s[i:i + 1])
+            else:
+                assert not s[i].any()
+        a += length
+
+
+def test_malformed_offsets_are_reported():
+    q, k, v, g, _ = inputs(1, 40, 1, 1, 32, BF16)
+    dev = gpu(q, k, v, g)
+    kernels.check_varlen()
+    for bad in ([0, 50, 40], [0, 30, 20, 40], [-3, 40], [0, 39], [0, 2**33, 40]):
+        kernels.decay_attention_varlen(*dev, torch.tensor(bad, device="cuda"))
+        with pytest.raises(kernels.KernelError):
+            kernels.check_varlen()
+    kernels.decay_attention_varlen(*dev, torch.tensor([0, 40], device="cuda"))
+    kernels.check_varlen()
+    # so many overlapping spans that the slots for them run out
+    dev = gpu(*inputs(1, 2000, 1, 1, 32, BF16)[:4])
+    kernels.decay_attention_varlen(*dev, torch.tensor([0, 2000] * 9 + [2000], device="cuda"))
+    with pytest.raises(kernels.KernelError):
+        kernels.check_varlen()
+
+
+def test_steps_of_views_and_padding():
+    q, k, v, g, s0 = inputs(4, 1, 4, 2, 64, BF16)
+    wide = torch.cat([q, k, v], 2)[:, 0].cuda()
+    state = s0.cuda()
+    want = kernels.decay_attention_step(*(x[:, 0].cuda() for x in (q, k, v, g)), state)
+    again = s0.cuda()
+    gates = torch.cat([torch.zeros(4, 3), g[:, 0]], 1).cuda()[:, 3:]
+    got = kernels.decay_attention_step(*wide.split([4, 2, 2], 1), gates, again)
+    assert torch.equal(got, want) and torch.equal(again, state)
+    cache = serving.DecayStateCache(1, 4, 2, 64)
+    cache.pool[0] = s0.cuda()
+    slots = torch.tensor([2, -1, 0, 4], dtype=torch.int32, device="cuda")
+    out = torch.full((4, 4, 64), 7.0, device="cuda")
+    cache.decode(0, slots, *wide.split([4, 2, 2], 1), gates, out)
+    assert not out[1].any() and not out[3].any()
+    assert torch.equal(cache.pool[0, [1, 3]].cpu(), s0[[1, 3]])
+
+
+def test_serving_in_a_graph():
+    """A captured prefill and decode with slots and offsets that change between replays."""
+    H, D, n = 2, 64, 3
+    q, k, v, g, _ = inputs(1, 700, 4, H, D, BF16, s0=False)
+    dev = gpu(q, k, v, g)
+    now = [x[0, :n].contiguous() for x in dev]
+    slots = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 100, 600, 700], dtype=torch.int32, device="cuda")
+    cache, eager = serving.DecayStateCache(1, 5, H, D), serving.DecayStateCache(1, 5, H, D)
+    out = torch.empty_like(now[0])
+
+    def serve(c, out):
+        o = c.prefill(0, slots, *dev, cu)
+        return o, c.decode(0, slots, *now, out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        serve(cache, out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, _ = serve(cache, out)
+    for i, (s, c) in enumerate((([4, 1, 0], [0, 1, 2, 700]), ([2, 3, 1], [0, 0, 650, 700]), ([0, 9, 4], [0, 300, 500, 700]))):
+        slots.copy_(torch.tensor(s))
+        cu.copy_(torch.tensor(c))
+        eager.pool.copy_(cache.pool)
+        graph.replay()
+        want = serve(eager, torch.empty_like(out))
+        torch.cuda.synchronize()
+        assert torch.equal(o, want[0]) and torch.equal(out, want[1]) and torch.equal(cache.pool, eager.pool)
+
+
+def test_infinities_and_nan_stay_in_their_heads_and_rows():
+    q, k, v, g, s0 = inputs(2, 70, 2, 2, 64, BF16)
+    v[0, 10, 1] = float("inf")
+    q[1, 60, 0] = float("nan")
+    o, s = kernels.decay_attention(*gpu(q, k, v, g, s0))
+    assert torch.isfinite(o[0, :, 0]).all() and torch.isfinite(o[1, :, 1]).all() and torch.isfinite(s[1]).all()
+    assert torch.isfinite(s[0, 0]).all() and not torch.isfinite(o[0, 10:, 1]).any() and torch.isnan(o[1, 60, 0]).all()
+    near_ones = torch.ones(1, 5, 1, 32, device="cuda")
+    o, s = kernels.decay_attention(near_ones, near_ones, near_ones, torch.tensor([[float("nan")]] * 5, device="cuda")[None])
+    assert torch.isnan(o).all() and torch.isnan(s).all()

@@ -232,3 +232,54 @@ def test_graph_replays():
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_saved_tensors_may_come_back_elsewhere():
+    x, z, gy = (normal(4, 6, 96, seed=i).to(BF16) for i in range(3))
+    w = 1 + 0.1 * normal(96, seed=3)
+
+    def grads(pack, unpack):
+        dev = [t.cuda().requires_grad_(True) for t in (x, z, w)]
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = kernels.gated_norm(*dev)
+            out = kernels.residual_norm(y, dev[1], dev[2], post_weight=dev[2])
+        return torch.autograd.grad(out, dev, (gy.cuda(), gy.cuda()))
+
+    want = grads(lambda t: t, lambda t: t)
+    for unpack in (lambda t: t, lambda t: t.cuda().t().contiguous().t() if t.dim() == 2 else t.cuda()):
+        got = grads(lambda t: t.cpu(), unpack)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_gradients_of_what_is_asked_for():
+    x, z = (normal(5, 64, seed=i).cuda() for i in range(2))
+    w = (1 + 0.1 * normal(64, seed=3)).cuda().requires_grad_(True)
+    gw, = torch.autograd.grad(kernels.gated_norm(x, z, w).sum(), w)
+    gx, = torch.autograd.grad(kernels.gated_norm(x.requires_grad_(True), z, w.detach()).sum(), x)
+    assert gw.shape == (64,) and gx.shape == x.shape
+    y, h = kernels.residual_norm(x.detach(), z, w, post_weight=w)
+    g, = torch.autograd.grad(y.sum(), w)  # (one weight in both places: its gradients add)
+    a, b = (w.detach().clone().requires_grad_(True) for _ in range(2))
+    both = torch.autograd.grad(kernels.residual_norm(x.detach(), z, a, post_weight=b)[0].sum(), (a, b))
+    assert torch.allclose(g, both[0] + both[1], rtol=1e-6)
+
+
+def test_fp16_and_fp64_run_in_fp32():
+    x, z = normal(5, 64), normal(5, 64, seed=1)
+    want = kernels.gated_norm(x.cuda(), z.cuda())
+    d = [t.cuda().double().requires_grad_(True) for t in (x, z)]
+    y = kernels.gated_norm(*d)
+    assert y.dtype == F32 and torch.equal(y, want)
+    assert all(g.dtype == torch.float64 for g in torch.autograd.grad(y.sum(), d))
+
+
+@pytest.mark.parametrize("C", [128, 4096])
+def test_another_stream(C):
+    x, z = (normal(300, C, seed=i).cuda() for i in range(2))
+    want = kernels.residual_norm(x, z)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = kernels.residual_norm(x, z)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
