@@ -168,12 +168,12 @@ __global__ __launch_bounds__(1024) void assign_slots(const int32_t* cu, int n_se
 }
 
 // States before the spans from each span's own share: S = e^G S + U, span after span, V elements of a
-// state to a thread (4 where a state's size allows it).  The shares do not wait for each other: sixteen
-// are asked for ahead.
+// state to a thread (4 where a state's size allows it).  The shares do not wait for each other: 128
+// bytes a thread are asked for ahead.
 template <int V>
 __global__ __launch_bounds__(256) void scan_spans(DecayPasses passes, const int* first_slot) {
     typedef float vec __attribute__((ext_vector_type(V)));
-    constexpr int AHEAD = 16;
+    constexpr int AHEAD = V == 1 ? 32 : 8;
     const DecayPass& a = passes.pass[blockIdx.z % passes.n];
     const int64_t pair = blockIdx.y + static_cast<int64_t>(blockIdx.z / passes.n) * 65535;
     if (pair >= static_cast<int64_t>(a.n_seqs) * a.HS) return;
@@ -204,11 +204,11 @@ __global__ __launch_bounds__(256) void scan_spans(DecayPasses passes, const int*
         vec x[AHEAD];
         float g[AHEAD];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
-            if (i + j < n) {
-                __builtin_memcpy(&x[j], u + (i + j) * step, sizeof S);
-                g[j] = exp2_f64(log[static_cast<int64_t>(i + j) * a.HS]);
-            }
+        for (int j = 0; j < AHEAD; ++j) {  // (past the last: the last again; a branch would wait for each)
+            const int64_t from = min(i + j, n - 1);
+            __builtin_memcpy(&x[j], u + from * step, sizeof S);
+            g[j] = exp2_f64(log[from * a.HS]);
+        }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
             if (i + j < n) {

@@ -741,6 +741,10 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                                                                 S[ct][2 * d32 + h]);
             }
         }
+        // (the next step's loads: after the products that need every register, before the wait for the other
+        // waves; 153 us here, 158 before the state's products, 170 before all of them, 166 after A V, at B32
+        // T1024 H16 D128.  A states' pass has registers to spare and asks before its products.)
+        if (OUT) fetch(c_next, m_next);
         // (from here on nothing reads the chunk's rows or log-decays: the next ones may come in; A is
         // written again only after the barrier that follows them)
         lds_barrier();
@@ -766,7 +770,6 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                                     O[ct][i] = mfma32(__builtin_bit_cast(bf16x8_t, vo[kb][ct][p]),
                                                       __builtin_bit_cast(bf16x8_t, ao[i][x - p]), O[ct][i]);
             }
-        if (OUT) fetch(c_next, m_next);
         // ---- outputs
         if (OUT && (dst || last_m)) {
             const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg), left = a.D - col;
