@@ -229,17 +229,29 @@ struct Plan {
 // to 128, one beyond).
 int64_t resident(int D) { return D <= 64 ? 768 : D <= 128 ? 512 : 256; }
 
-// How a pass is cut into workgroups: one per sequence, state and column tile, or, where the card holds
-// more, as many again along the sequence (spans of at least kMinSpan tokens; calls of up to 512 tokens
-// stay whole, since the states' own pass costs as much as they take).  Of packed sequences, half a span
-// each is lost on average.  The query heads of a group go one after another through one workgroup, which
-// reads their keys once, where there is work enough for every CU without them.
-Plan plan(int n_seqs, int T, int HO, int HS, int D, bool packed) {
+// Whether spans along the sequence pay where there are ``groups`` workgroups without them: the card holds
+// ``more`` = resident / groups times as many, each span is walked through twice (the states' own pass costs
+// half of the outputs'), and the states are summed in a launch between.  With D 128 in us, spans against
+// whole sequences: bf16 forward of 16 heads, more = 8: 52 against 49 for 512 tokens, 61 against 91 for 1024;
+// more = 4: 61 against 51 and 80 against 93; more = 2.7: 213 against 195 for 2048; more = 32: 31 against 27
+// for 256 tokens, 33 against 37 for 384.  fp32 chunks are half as long and take longer: more = 8: 51 against
+// 60 for 256 tokens; more = 4: 93 against 115 for 512; more = 2.7: 253 against 236 for 1024.
+bool spans_pay(int64_t groups, int T, int D, bool bf16) {
+    const int64_t want = resident(D);
+    return want >= 3 * groups && T >= (bf16 ? 384 : 256) && T * want >= groups * (bf16 ? 4096 : 2048);
+}
+
+// How a pass is cut into workgroups: one per sequence, state and column tile, or, where that pays, as many
+// along the sequence as the card holds (spans of at least kMinSpan tokens).  How long packed sequences are
+// is not known here: they are cut wherever the card holds more, from 512 tokens on, and half a span of each
+// is lost on average.  The query heads of a group go one after another through one workgroup, which reads
+// their keys once, where there is work enough for every CU without them.
+Plan plan(int n_seqs, int T, int HO, int HS, int D, bool packed, bool bf16) {
     Plan p{(D + decay_cols(D) - 1) / decay_cols(D), 1, max(T, 1), 1, n_seqs, false};
     const int64_t tokens = packed ? T : static_cast<int64_t>(n_seqs) * T, want = resident(D);
     if (HO > HS && tokens * HS * p.n_tiles >= want * 256) p.n_dst = HO / HS;
     const int64_t groups = static_cast<int64_t>(HO / p.n_dst) * p.n_tiles;
-    if (T > 512 && n_seqs * groups < want) {
+    if (packed ? T > 512 && n_seqs * groups < want : spans_pay(n_seqs * groups, T, D, bf16)) {
         int64_t slots = (want + groups - 1) / groups;  // wanted
         if (packed) slots = std::max<int64_t>(want / groups - (n_seqs + 1) / 2, (slots + 1) / 2);
         const int64_t span = std::max<int64_t>((tokens + slots - 1) / slots, kMinSpan);
@@ -267,8 +279,7 @@ struct FwdWs {
 };
 // Whether several workgroups read a first state that another one of them may already have replaced.
 bool shares_states(const Plan& p, int HO, int HS) { return !p.split && HO / p.n_dst > HS; }
-FwdWs fwd_ws(int n_seqs, int T, int Hq, int H, int D, bool packed, bool in_place) {
-    const Plan p = plan(n_seqs, T, Hq, H, D, packed);
+FwdWs fwd_ws(const Plan& p, int n_seqs, int Hq, int H, int D, bool packed, bool in_place) {
     const size_t state = static_cast<size_t>(H) * D * D * 4;
     Layout l;
     FwdWs w{};
@@ -282,11 +293,11 @@ FwdWs fwd_ws(int n_seqs, int T, int Hq, int H, int D, bool packed, bool in_place
 }
 
 // The backward's passes: one cut for all three, which run as one launch.  Where the gates' gradient is
-// wanted, spans of at most kDecayGateSpan tokens.
+// wanted, spans of at most kDecayGateSpan tokens (kept in sequences up to that whole, unless spans pay).
 struct BwdPlan {
     Plan q, k;  // gq's pass, and gk's and gv's
 };
-BwdPlan plan_bwd(int B, int T, int Hq, int H, int D, bool gates) {
+BwdPlan plan_bwd(int B, int T, int Hq, int H, int D, bool gates, bool bf16) {
     BwdPlan p;
     p.k = Plan{(D + decay_cols(D) - 1) / decay_cols(D), 1, max(T, 1), 1, B, false};
     const int64_t tokens = static_cast<int64_t>(B) * T, want = resident(D);
@@ -294,9 +305,9 @@ BwdPlan plan_bwd(int B, int T, int Hq, int H, int D, bool gates) {
     if (Hq > H && tokens * H * p.k.n_tiles >= want * 256) n_dst = Hq / H;
     const int64_t groups = static_cast<int64_t>(Hq / n_dst + 2 * H) * p.k.n_tiles;
     int64_t span = p.k.span;
-    if (B * groups < want) span = std::max<int64_t>((tokens * groups + want - 1) / want, kMinSpan);
+    if (spans_pay(B * groups, T, D, bf16)) span = std::max<int64_t>((tokens * groups + want - 1) / want, kMinSpan);
     if (gates) span = std::min<int64_t>(span, kDecayGateSpan);
-    if (T > 512 && span < T) {
+    if (span < T) {
         const int64_t n = (T + span - 1) / span;
         p.k.span = static_cast<int>(((T + n - 1) / n + 63) / 64 * 64);
         p.k.n_spans = (T + p.k.span - 1) / p.k.span;
@@ -311,8 +322,7 @@ BwdPlan plan_bwd(int B, int T, int Hq, int H, int D, bool gates) {
 struct BwdWs {
     size_t ahead, back, ahead_log, back_log, gs0, r_part, c_part, near, gg_part, bytes;
 };
-BwdWs bwd_ws(int B, int T, int Hq, int H, int D, bool gates) {
-    const Plan p = plan_bwd(B, T, Hq, H, D, gates).k;
+BwdWs bwd_ws(const Plan& p, int B, int T, int Hq, int H, int D, bool gates) {
     const size_t state = static_cast<size_t>(H) * D * D * 4, rows = static_cast<size_t>(B) * T;
     const size_t slots = p.split ? p.n_slots : 0, tiles = p.n_tiles;
     Layout l;
@@ -373,20 +383,27 @@ hipError_t span_states(DecayPasses x, bool bf16, bool gates, const int* first_sl
 }  // namespace
 
 size_t decay_attn_ws_bytes(int n_seqs, int T, int Hq, int H, int D, bool packed, bool in_place) {
-    return fwd_ws(n_seqs, T, Hq, H, D, packed, in_place).bytes;
+    const Plan x = plan(n_seqs, T, Hq, H, D, packed, true), y = plan(n_seqs, T, Hq, H, D, packed, false);
+    return std::max(fwd_ws(x, n_seqs, Hq, H, D, packed, in_place).bytes,
+                    fwd_ws(y, n_seqs, Hq, H, D, packed, in_place).bytes);
 }
 size_t decay_attn_bwd_ws_bytes(int B, int T, int Hq, int H, int D, bool gates) {
-    return bwd_ws(B, T, Hq, H, D, gates).bytes;
+    const Plan x = plan_bwd(B, T, Hq, H, D, gates, true).k, y = plan_bwd(B, T, Hq, H, D, gates, false).k;
+    return std::max(bwd_ws(x, B, T, Hq, H, D, gates).bytes, bwd_ws(y, B, T, Hq, H, D, gates).bytes);
 }
 int64_t decay_attn_groups(int n_seqs, int T, int Hq, int H, int D, bool packed) {
-    const Plan p = plan(n_seqs, T, Hq, H, D, packed);
-    return (static_cast<int64_t>(p.n_slots) * (Hq / p.n_dst) + 7) / 8 * 8 * p.n_tiles;
+    int64_t most = 0;
+    for (bool bf16 : {false, true}) {
+        const Plan p = plan(n_seqs, T, Hq, H, D, packed, bf16);
+        most = std::max(most, (static_cast<int64_t>(p.n_slots) * (Hq / p.n_dst) + 7) / 8 * 8 * p.n_tiles);
+    }
+    return most;
 }
 
 hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st) {
     const bool packed = a.cu != nullptr, in_place = a.s0 && a.s0 == a.s_out;
-    const Plan p = plan(a.n_seqs, a.T, a.Hq, a.H, a.D, packed);
-    const FwdWs w = fwd_ws(a.n_seqs, a.T, a.Hq, a.H, a.D, packed, in_place);
+    const Plan p = plan(a.n_seqs, a.T, a.Hq, a.H, a.D, packed, a.bf16);
+    const FwdWs w = fwd_ws(p, a.n_seqs, a.Hq, a.H, a.D, packed, in_place);
     DecayPass x{};
     x.q = a.q, x.k = a.k, x.v = a.v;
     x.q_sb = a.strides[0], x.q_st = a.strides[1], x.q_sh = a.strides[2];
@@ -432,8 +449,8 @@ hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st) {
 
 hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
     const bool gates = a.gg != nullptr;
-    const BwdPlan p = plan_bwd(a.B, a.T, a.Hq, a.H, a.D, gates);
-    const BwdWs w = bwd_ws(a.B, a.T, a.Hq, a.H, a.D, gates);
+    const BwdPlan p = plan_bwd(a.B, a.T, a.Hq, a.H, a.D, gates, a.bf16);
+    const BwdWs w = bwd_ws(p.k, a.B, a.T, a.Hq, a.H, a.D, gates);
     struct Role {
         const void* p;
         const int64_t* s;

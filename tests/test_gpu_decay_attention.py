@@ -82,6 +82,8 @@ SHAPES = [
     (2, 90, 2, 2, 12),
     (3, 1100, 2, 1, 64),  # several workgroups along the sequence
     (1, 1555, 4, 2, 128),
+    (2, 450, 2, 2, 128),  # short, but few heads
+    (8, 700, 33, 33, 16),  # longer, but many
 ]
 
 
