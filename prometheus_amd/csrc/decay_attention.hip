@@ -293,7 +293,8 @@ FwdWs fwd_ws(const Plan& p, int n_seqs, int Hq, int H, int D, bool packed, bool 
 }
 
 // The backward's passes: one cut for all three, which run as one launch.  Where the gates' gradient is
-// wanted, spans of at most kDecayGateSpan tokens (kept in sequences up to that whole, unless spans pay).
+// wanted, spans of at most kDecayGateSpan tokens, also where they do not pay (B8 T4096 H16 D128 bf16: 918 us
+// against 890 for whole sequences, D 256: 2836 against 2060): its sums stay short.
 struct BwdPlan {
     Plan q, k;  // gq's pass, and gk's and gv's
 };
@@ -370,8 +371,8 @@ hipError_t span_states(DecayPasses x, bool bf16, bool gates, const int* first_sl
     if (hipError_t e = run_kind(x, bf16, gates ? 3 : 2, st); e != hipSuccess) return e;
     const DecayPass& a = x.pass[0];
     const int64_t pairs = static_cast<int64_t>(a.n_seqs) * a.HS;
-    // (four elements a thread, where that leaves a workgroup for every CU: few states of a long sequence
-    // are bound by the loads in flight, 31 us against 40 for 4 heads' 128 spans of D 128)
+    // (four elements a thread, where that leaves a workgroup for every CU: 64 heads' 8 spans of D 128 take
+    // 12 us, and 36 element by element; 4 heads' 128 spans, bound by the loads in flight, 25.5 and 24)
     const int V = a.D % 2 == 0 && pairs * x.n * a.D * a.D >= 256 * 1024 ? 4 : 1;
     const dim3 grid(static_cast<unsigned>((a.D * a.D / V + 255) / 256), static_cast<unsigned>(std::min<int64_t>(pairs, 65535)),
                     static_cast<unsigned>((pairs + 65534) / 65535 * x.n));
@@ -391,12 +392,18 @@ size_t decay_attn_bwd_ws_bytes(int B, int T, int Hq, int H, int D, bool gates) {
     const Plan x = plan_bwd(B, T, Hq, H, D, gates, true).k, y = plan_bwd(B, T, Hq, H, D, gates, false).k;
     return std::max(bwd_ws(x, B, T, Hq, H, D, gates).bytes, bwd_ws(y, B, T, Hq, H, D, gates).bytes);
 }
+// (as launch_pass has them; in the backward's launch every pass may have a workgroup per query head)
+int64_t pass_groups(const Plan& p, int Hq) {
+    return (static_cast<int64_t>(p.n_slots) * (Hq / p.n_dst) + 7) / 8 * 8 * p.n_tiles;
+}
 int64_t decay_attn_groups(int n_seqs, int T, int Hq, int H, int D, bool packed) {
+    return std::max(pass_groups(plan(n_seqs, T, Hq, H, D, packed, true), Hq),
+                    pass_groups(plan(n_seqs, T, Hq, H, D, packed, false), Hq));
+}
+int64_t decay_attn_bwd_groups(int B, int T, int Hq, int H, int D) {
     int64_t most = 0;
-    for (bool bf16 : {false, true}) {
-        const Plan p = plan(n_seqs, T, Hq, H, D, packed, bf16);
-        most = std::max(most, (static_cast<int64_t>(p.n_slots) * (Hq / p.n_dst) + 7) / 8 * 8 * p.n_tiles);
-    }
+    for (bool bf16 : {false, true})
+        for (bool gates : {false, true}) most = std::max(most, 3 * pass_groups(plan_bwd(B, T, Hq, H, D, gates, bf16).k, Hq));
     return most;
 }
 
@@ -524,7 +531,8 @@ hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
 // S = e^g S + k v^T in place, o = scale S^T q for the group's query heads: the state is read and
 // written once, 16 bytes a lane (K3's mapping), and everything else is small beside it.  CG column
 // groups of 4, 256 / CG row groups.  More than 4 query heads take the new state from the caches
-// again, 4 at a time.
+// again, 4 at a time.  256 tokens of 32 query and 8 key heads, D 128: 274 MB in 58 us, 4.7 TB/s (71 us
+// with loads and stores that stay in the caches; a copy of 2 GiB runs at 5.0 TB/s here).
 namespace {
 
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // at any address of a float

@@ -29,6 +29,7 @@ size_t size_of(int dtype) { return dtype == PM_DTYPE_BF16 ? 2 : 4; }
 constexpr int64_t kMaxElems = int64_t(1) << 40;
 constexpr int64_t kMaxStride = int64_t(1) << 40;
 
+constexpr int64_t kMaxGroups = (int64_t(1) << 24) - 1;  // workgroups of 256 that one launch can have
 constexpr int64_t kMaxTokenStride = int64_t(1) << 23;  // (64 tokens are reached with 32-bit offsets)
 
 int check_stride(const char* name, int64_t s) {
@@ -36,25 +37,33 @@ int check_stride(const char* name, int64_t s) {
     return 0;
 }
 
-bool decay_sizes_fit(int n, int T, int Hq, int H, int D) {
+// What a call of K14 launches.
+enum class Decay { kForward, kPacked, kBackward, kStep };
+
+bool decay_sizes_fit(Decay call, int n, int T, int Hq, int H, int D) {
     if (n < 0 || T < 0 || Hq < 1 || H < 1 || Hq % H || D < 1 || D > PM_DELTA_MAX_D) return false;
-    if (T > INT32_MAX - 1024 || static_cast<int64_t>(Hq) * D > kMaxTokenStride) return false;
-    const int64_t rows = static_cast<int64_t>(n) * std::max(T, 1);
-    return rows <= kMaxElems / (static_cast<int64_t>(Hq) * D) &&
-           static_cast<int64_t>(n) * H <= kMaxElems / (static_cast<int64_t>(D) * D) &&
-           pm::decay_attn_groups(n, T, Hq, H, D, false) <= INT32_MAX &&
-           pm::decay_attn_groups(n, T, Hq, H, D, true) <= INT32_MAX && static_cast<int64_t>(n) * H * (T / 256 + 1) <= INT32_MAX;
+    const int64_t width = static_cast<int64_t>(Hq) * D;
+    if (T > INT32_MAX - 1024 || width > kMaxTokenStride) return false;
+    const int64_t rows = (call == Decay::kPacked ? 1 : static_cast<int64_t>(n)) * std::max(T, 1);
+    if (rows > kMaxElems / width || static_cast<int64_t>(n) * H > kMaxElems / (static_cast<int64_t>(D) * D)) return false;
+    switch (call) {
+        case Decay::kStep: return true;
+        case Decay::kBackward:  // (the pairs inside chunks: a workgroup to 128 tokens at least)
+            return static_cast<int64_t>(n) * Hq * (T / 128 + 1) <= kMaxGroups &&
+                   pm::decay_attn_bwd_groups(n, T, Hq, H, D) <= kMaxGroups;
+        default: return pm::decay_attn_groups(n, T, Hq, H, D, call == Decay::kPacked) <= kMaxGroups;
+    }
 }
 
 // Sizes, types and strides that the calls of K14 share.
-int check_decay(int n, int T, int Hq, int H, int D, int dtype, int out_dtype, const int64_t* strides, int n_strides,
-                int64_t g_sb, int64_t g_st, float scale) {
+int check_decay(Decay call, int n, int T, int Hq, int H, int D, int dtype, int out_dtype, const int64_t* strides,
+                int n_strides, int64_t g_sb, int64_t g_st, float scale) {
     if (!known(dtype) || !known(out_dtype))
         return fail(PM_E_DTYPE, "types %d, %d: each must be PM_DTYPE_F32 or PM_DTYPE_BF16", dtype, out_dtype);
     if (n < 0 || T < 0) return fail(PM_E_SHAPE, "sizes must be >= 0 (got %d, %d)", n, T);
     if (Hq < 1 || H < 1 || Hq % H) return fail(PM_E_SHAPE, "Hq must be a multiple of H >= 1 (got %d, %d)", Hq, H);
     if (D < 1 || D > PM_DELTA_MAX_D) return fail(PM_E_SHAPE, "D must be in [1, %d] (got %d)", PM_DELTA_MAX_D, D);
-    if (!decay_sizes_fit(n, T, Hq, H, D)) return fail(PM_E_SHAPE, "problem too large");
+    if (!decay_sizes_fit(call, n, T, Hq, H, D)) return fail(PM_E_SHAPE, "problem too large");
     if (!strides) return fail(PM_E_NULL, "strides is NULL");
     for (int i = 0; i < n_strides; ++i)
         if (int rc = check_stride("a stride", strides[i])) return rc;
@@ -84,7 +93,7 @@ extern "C" {
 
 size_t pm_decay_attention_workspace_bytes(int n_seqs, int T, int Hq, int H, int D, int packed,
                                           int in_place) {
-    if (!decay_sizes_fit(n_seqs, T, Hq, H, D)) return 0;
+    if (!decay_sizes_fit(packed ? Decay::kPacked : Decay::kForward, n_seqs, T, Hq, H, D)) return 0;
     return pm::decay_attn_ws_bytes(n_seqs, T, Hq, H, D, packed != 0, in_place != 0);
 }
 
@@ -94,7 +103,8 @@ int pm_decay_attention(const void* q, const void* k, const void* v, const float*
                        int64_t g_st, int dtype, int out_dtype, float scale, void* workspace, size_t ws_bytes,
                        void* stream) {
     pm::clear_error();
-    if (int rc = check_decay(n_seqs, T, Hq, H, D, dtype, out_dtype, strides, 9, g_sb, g_st, scale)) return rc;
+    if (int rc = check_decay(cu_seqlens ? Decay::kPacked : Decay::kForward, n_seqs, T, Hq, H, D, dtype, out_dtype,
+                             strides, 9, g_sb, g_st, scale)) return rc;
     if (n_seqs == 0) return 0;
     if (slots && n_slots < 0) return fail(PM_E_SHAPE, "n_slots must be >= 0 (got %d)", n_slots);
     if (!s_out) return fail(PM_E_NULL, "s_out is NULL");
@@ -115,7 +125,7 @@ int pm_decay_attention(const void* q, const void* k, const void* v, const float*
 }
 
 size_t pm_decay_attention_bwd_workspace_bytes(int B, int T, int Hq, int H, int D, int gates) {
-    if (!decay_sizes_fit(B, T, Hq, H, D)) return 0;
+    if (!decay_sizes_fit(Decay::kBackward, B, T, Hq, H, D)) return 0;
     return pm::decay_attn_bwd_ws_bytes(B, T, Hq, H, D, gates != 0);
 }
 
@@ -124,7 +134,7 @@ int pm_decay_attention_bwd(const void* q, const void* k, const void* v, const fl
                            int H, int D, const int64_t* strides, int64_t g_sb, int64_t g_st, int dtype, float scale,
                            void* workspace, size_t ws_bytes, void* stream) {
     pm::clear_error();
-    if (int rc = check_decay(B, T, Hq, H, D, dtype, dtype, strides, 9, g_sb, g_st, scale)) return rc;
+    if (int rc = check_decay(Decay::kBackward, B, T, Hq, H, D, dtype, dtype, strides, 9, g_sb, g_st, scale)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (B == 0) {
         if (gg && g_sb == 0 && g_st == 0)
@@ -150,7 +160,7 @@ int pm_decay_attention_step(float* s_inout, const int32_t* slots, int n_slots, c
                             const void* v, const float* g, void* o, int B, int Hq, int H, int D, const int64_t* strides,
                             int64_t g_sb, int dtype, int out_dtype, float scale, void* stream) {
     pm::clear_error();
-    if (int rc = check_decay(B, 1, Hq, H, D, dtype, out_dtype, strides, 6, g_sb, 0, scale)) return rc;
+    if (int rc = check_decay(Decay::kStep, B, 1, Hq, H, D, dtype, out_dtype, strides, 6, g_sb, 0, scale)) return rc;
     if (B == 0) return 0;
     if (slots && n_slots < 0) return fail(PM_E_SHAPE, "n_slots must be >= 0 (got %d)", n_slots);
     if (!s_inout || !q || !k || !v || !g || !o) return fail(PM_E_NULL, "s_inout, q, k, v, g and o must be non-NULL");

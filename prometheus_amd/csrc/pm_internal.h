@@ -365,7 +365,9 @@ struct DecayAttnArgs {
 };
 hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st);
 size_t decay_attn_ws_bytes(int n_seqs, int T, int Hq, int H, int D, bool packed, bool in_place);
-int64_t decay_attn_groups(int n_seqs, int T, int Hq, int H, int D, bool packed);  // workgroups of its grid
+// the most workgroups of a launch
+int64_t decay_attn_groups(int n_seqs, int T, int Hq, int H, int D, bool packed);
+int64_t decay_attn_bwd_groups(int B, int T, int Hq, int H, int D);
 
 // Its gradients; go contiguous in q's type, gq, gk, gv contiguous in it; gg (B, T, H), or (H) where
 // both of g's strides are 0 (nullable: not wanted).

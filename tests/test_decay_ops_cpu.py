@@ -235,7 +235,7 @@ def test_decay_abi_refuses():
     assert fwd(n=0) == 0
     # sizes: none where one workgroup does a sequence, the states of spans otherwise, a table for packed calls
     size = L.pm_decay_attention_workspace_bytes
-    assert size(1, 512, 2, 2, 64, 0, 0) == 0 and size(1, 4096, 2, 2, 64, 0, 0) > 0 and size(3, 10, 2, 2, 64, 1, 0) > 0
+    assert size(1, 200, 2, 2, 64, 0, 0) == 0 and size(32, 2048, 16, 16, 64, 0, 0) == 0 and size(1, 4096, 2, 2, 64, 0, 0) > 0 and size(3, 10, 2, 2, 64, 1, 0) > 0
     assert size(2, 10, 4, 2, 64, 0, 1) == 2 * 2 * 64 * 64 * 4 and size(1, 4, 3, 2, 8, 0, 0) == 0
 
     def bwd(q=P, go=P, gq=P, gg=P, gs0=P, s0=None, B=1, T=4, strides=_i64(*[64, 16, 8] * 3), g_sb=8, g_st=2, dt=0, ws=None,
@@ -248,6 +248,11 @@ def test_decay_abi_refuses():
                      (dict(gs0=odd), E.E_ALIGN), (dict(), E.E_WORKSPACE)):
         assert bwd(**kw) == want, kw
     assert bwd(B=0) == 0
+    # more workgroups than one launch can have; many short packed sequences are not
+    wide = dict(strides=_i64(*[16, 8, 8] * 3), T=1, ws=P, nbytes=1 << 60)
+    assert fwd(n=1 << 23, q=odd, **wide) == E.E_SHAPE and fwd(n=1 << 22, q=odd, **wide) == E.E_ALIGN
+    assert bwd(B=1 << 22, q=odd, **wide) == E.E_SHAPE and bwd(B=1 << 21, q=odd, **wide) == E.E_ALIGN
+    assert size(20000, 1 << 20, 32, 32, 8, 1, 0) > 0 and size(1 << 23, 1 << 23, 2, 2, 8, 1, 0) == 0
     need = L.pm_decay_attention_bwd_workspace_bytes
     assert need(1, 100, 2, 2, 64, 0) == 0 and need(1, 100, 2, 2, 64, 1) > 0 and need(-1, 100, 2, 2, 64, 1) == 0
 
