@@ -198,6 +198,14 @@ __device__ __forceinline__ u32x4_t join(u32x2_t a, u32x2_t b) {
     return r;
 }
 
+// The same number, as one the compiler knows nothing of: what is computed from it is computed where it is
+// used, not ahead of the loop, where it would take a register (or scratch memory, whose loads wait for
+// the rows that are on their way).
+__device__ __forceinline__ int fresh(int x) {
+    __asm__ volatile("" : "+v"(x));
+    return x;
+}
+
 // ---- log-decays -------------------------------------------------------------------------------
 
 template <int CTRL, int ROW_MASK>
@@ -431,15 +439,14 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
         if (row >= cnt || col >= a.D) x.zero();
         else if (!tiny && col != at) x.drop(col - at);
     };
-    // wave 0 has the log-decays: chunk c's are loaded while chunk c - 2 runs, and summed while c - 1 does
-    float rg = 0.f;
-    auto fetch_g = [&](int c) {  // (loads a value that is there; sum_g takes it for what it is)
+    // wave 0 has the log-decays: chunk c's are loaded and summed while chunk c - 1 runs
+    auto load_g = [&](int c) {  // (a value that is there; sum_g takes it for what it is)
         int first, cnt;
         chunk_at(min(c, n_chunks - 1), first, cnt);
         const int tok = a.reverse ? first + cnt - t : first + t;  // (backwards: the token after)
-        rg = gp[(start + max(min(tok, len - 1), 0)) * a.g_st];
+        return gp[(start + max(min(tok, len - 1), 0)) * a.g_st];
     };
-    auto sum_g = [&](int c) {
+    auto sum_g = [&](int c, float rg) {
         int first, cnt;
         chunk_at(min(c, n_chunks - 1), first, cnt);
         const int buf = c & 1;
@@ -447,10 +454,11 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
         const double G = wave_prefix_f64(there ? log2_decay(rg) : 0.0);
         const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(G), 63),
                                              __builtin_amdgcn_readlane(__double2loint(G), 63));
-        if (t < C) {
-            sg[buf][t] = split_log(G);
-            s_into[buf][t] = exp2_f64(G) * a.into_scale;
-            s_out[buf][t] = exp2_f64(last - G) * a.out_scale;
+        const int i = fresh(t);
+        if (i < C) {
+            sg[buf][i] = split_log(G);
+            s_into[buf][i] = exp2_f64(G) * a.into_scale;
+            s_out[buf][i] = exp2_f64(last - G) * a.out_scale;
         }
         if (t == 0) s_total[buf] = last;
     };
@@ -458,11 +466,7 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
     f32x4_t O[CT][MT];
     double log_total = 0.0;
     fetch(0, 0);
-    if (w == 0 && n_chunks > 0) {
-        fetch_g(0);
-        sum_g(0);
-        fetch_g(1);
-    }
+    if (w == 0 && n_chunks > 0) sum_g(0, load_g(0));
     for (int c = 0, m = 0; c < n_chunks;) {
         const int buf = c & 1, m_next = m + 1 < n_m ? m + 1 : 0, c_next = m_next ? c : c + 1;
         const bool first_m = m == 0, last_m = m == n_m - 1, dst = n_dst > 1;
@@ -504,11 +508,8 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                 for (int x = 0; x < P; ++x) *reinterpret_cast<u32x4_t*>(sq + x * C * DK + row * DK + 8 * ch) = p[x];
             }
         lds_barrier();
+        const float rg = load_g(c + 1);  // (by every wave: a branch around it would wait; summed below)
         if (!OUT) fetch(c_next, m_next);
-        if (w == 0 && first_m) {
-            sum_g(c + 1);
-            fetch_g(c + 2);
-        }
 
         const double chunk_log = s_total[buf];
         // ---- A's tiles of the wave's 16 source tokens and, from the same rows of Q, the state's part of
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                     // (rows and columns that are not there: some that are, since their O is 0)
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        const uint32_t tok = token_of(min(16 * i + l16, cnt - 1), cnt);
+                        const uint32_t tok = token_of(min(16 * i + (fresh(t) & 15), cnt - 1), cnt);
                         __builtin_memcpy(aux[AUX ? i : 0],
                                          reinterpret_cast<const char*>(x_p) +
                                              (tok * static_cast<uint32_t>(a.x_st * sizeof(E)) +
@@ -577,14 +578,14 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                 }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    const float e = s_into[buf][16 * i + l16];
+                    const float e = s_into[buf][16 * i + (fresh(t) & 15)];
 #pragma unroll
                     for (int ct = 0; ct < CT; ++ct) O[ct][i] *= e;
                 }
                 if (parts && !x_wide)
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        const int row = 16 * i + l16, left = row < cnt ? a.D - x_col : 0;
+                        const int row = 16 * i + (fresh(t) & 15), left = row < cnt ? a.D - x_col : 0;
                         const E* x = x_p + token_of(min(row, cnt - 1), cnt) * a.x_st + x_col;
 #pragma unroll
                         for (int r = 0; r < XN; ++r) {
@@ -608,7 +609,7 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                         }
                         sum += __shfl_xor(sum, 16);
                         sum += __shfl_xor(sum, 32);
-                        if (lg == 0) s_part[AUX ? w : 0][AUX ? 16 * i + l16 : 0] = sum;
+                        if (lg == 0) s_part[AUX ? w : 0][AUX ? 16 * i + (fresh(t) & 15) : 0] = sum;
                     }
                 }
             }
@@ -641,7 +642,7 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 if (i < w) continue;  // (above the diagonal)
-                const float2 gi = sg[buf][16 * i + l16];
+                const float2 gi = sg[buf][16 * i + (fresh(t) & 15)];
                 f32x4_t x;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -653,12 +654,11 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                 const int blk = i < 2 ? i : 2 * i - 2 + (w >> 1);  // (qblk)
 #pragma unroll
                 for (int p = 0; p < PA; ++p)
-                    *reinterpret_cast<u32x2_t*>(sa + (p * Sh::BLK + blk) * 512 + lane * 8 + 4 * (w & 1)) = ap[p];
+                    *reinterpret_cast<u32x2_t*>(sa + (p * Sh::BLK + blk) * 512 + (fresh(t) & 63) * 8 + 4 * (w & 1)) = ap[p];
             }
         }
-        if (first_m) {
-            log_total += chunk_log;
-        }
+        if (OUT && w == 0 && first_m) sum_g(c + 1, rg);
+        if (first_m) log_total += chunk_log;
         const bool update = !dst || last_m;
         if (dst ? last_m : first_m) {
             const float e = exp2_f64(chunk_log);
@@ -745,6 +745,7 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
         // waves; 153 us here, 158 before the state's products, 170 before all of them, 166 after A V, at B32
         // T1024 H16 D128.  A states' pass has registers to spare and asks before its products.)
         if (OUT) fetch(c_next, m_next);
+        if (!OUT && w == 0 && first_m) sum_g(c + 1, rg);
         // (from here on nothing reads the chunk's rows or log-decays: the next ones may come in; A is
         // written again only after the barrier that follows them)
         lds_barrier();
@@ -775,7 +776,7 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
             const int col = n0 + (CT == 1 ? 16 * w + 4 * lg : 32 * w + 8 * lg), left = a.D - col;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const int row = 16 * i + l16;
+                const int row = 16 * i + (fresh(t) & 15);
                 if (row >= cnt || left <= 0) continue;
                 const int64_t at = ((rows0 + first + token_of(row, cnt)) * a.HO + ho) * a.D + col;
                 float v[4 * CT];
@@ -803,9 +804,10 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
         }
         if constexpr (AUX)
             if (a.part && (dst || first_m) && t < cnt) {
-                const int64_t tok = rows0 + (a.reverse ? first + cnt - 1 - t : first + t);
+                const int i = fresh(t);
+                const int64_t tok = rows0 + first + token_of(i, cnt);
                 a.part[(static_cast<int64_t>(tile) * a.HO + ho) * a.n_rows + tok] =
-                    (s_part[0][t] + s_part[1][t]) + (s_part[2][t] + s_part[3][t]);
+                    (s_part[0][i] + s_part[1][i]) + (s_part[2][i] + s_part[3][i]);
             }
         c = c_next, m = m_next;
     }
