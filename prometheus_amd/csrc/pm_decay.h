@@ -19,7 +19,7 @@
 // plane's size.  bf16 inputs are one plane and exact; next to them
 //   the decayed V, which sums into states      three planes (2^-25 relative)
 //   the state and V in passes that leave parts of the gates' gradient, which is fp32: two (2^-17; three
-//     took 403 us where two take 307, at B4 T4096 H16 D128: the registers for them are not there)
+//     take 346 us where two take 240, at B4 T4096 H16 D128: the registers for them are not there)
 //   A and the state in what comes out in bf16   one (2^-9): half a step of its own type, once
 // fp32 inputs and everything next to them are three.  On this card six such bf16 products take 6/16 of
 // the time of the fp32 MFMA.
@@ -200,7 +200,7 @@ __device__ __forceinline__ u32x4_t join(u32x2_t a, u32x2_t b) {
 
 // The same number, as one the compiler knows nothing of: what is computed from it is computed where it is
 // used, not ahead of the loop, where it would take a register (or scratch memory, whose loads wait for
-// the rows that are on their way).
+// the rows that are on their way: the backward's three passes at B4 T4096 H16 D128 took 302 us, 240 so).
 __device__ __forceinline__ int fresh(int x) {
     __asm__ volatile("" : "+v"(x));
     return x;
