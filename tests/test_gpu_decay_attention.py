@@ -556,3 +556,42 @@ def test_infinities_and_nan_stay_in_their_heads_and_rows():
     near_ones = torch.ones(1, 5, 1, 32, device="cuda")
     o, s = kernels.decay_attention(near_ones, near_ones, near_ones, torch.tensor([[float("nan")]] * 5, device="cuda")[None])
     assert torch.isnan(o).all() and torch.isnan(s).all()
+
+
+def test_offsets_past_32_bits():
+    B, H, D, half = 1, 128, 128, 65536
+    T = 2 * half + 1  # 2.1e9 elements a tensor
+    q, k, v, go = (torch.empty(B, T, H, D, dtype=BF16, device="cuda").normal_(std=0.1) for _ in range(4))
+    g = torch.full((B, T, H), -0.5, device="cuda")
+    (o, s), res = kernels.decay_attention_fwd(q, k, v, g)
+    gq, gk, gv, gg, _ = kernels.decay_attention_bwd(res, (go, None))
+    # the second half by itself, from nothing: what the first leaves is e^-0.5 of itself a token later, below
+    # 2^-180 of it after 256
+    tail = [x[:, half:] for x in (q, k, v, g)]
+    (o2, s2), res2 = kernels.decay_attention_fwd(*tail)
+    two = kernels.decay_attention_bwd(res2, (go[:, half:], None))
+    (sizes, s_size), res3 = kernels.decay_attention_fwd(*(x.abs() for x in tail[:3]), tail[3], out_dtype=F32)
+    size = kernels.decay_attention_bwd(res3, (go[:, half:].abs(), None))
+    # either is off by the file's bounds for sums that decay by e^-0.5 a token (256 terms of them count)
+    eps = 2 * eps_out(BF16, 256)
+    for got, want, m in ((o, o2, sizes), (gq, two[0], size[0]), (gk, two[1], size[1]), (gv, two[2], size[2])):
+        a, b, m = (x[:, 256 - T + half:] if x.shape[1] == T - half else x[:, half + 256:] for x in (got, want, m))
+        assert bool(((a.float() - b.float()).abs() <= eps * m.float() + 2.0**-7 * b.float().abs() + 1e-30).all())
+    assert bool(((s - s2).abs() <= 2 * eps_of(BF16, 256) * s_size + 1e-30).all())
+    largest = size[3].abs().amax(1, keepdim=True)
+    assert bool(((gg[:, half + 256:] - two[3][:, 256:]).abs() <= 2 * 17 * eps_of(BF16, 512) * largest).all())
+
+
+def test_slots_past_32_bits():
+    H, D, n = 32, 256, 1100  # 2.3e9 elements of states
+    cache = serving.DecayStateCache(1, n, H, D)
+    small = serving.DecayStateCache(1, 2, H, D)
+    x = [torch.randn(1, 1100, H, D, device="cuda").to(BF16) * 0.1 for _ in range(3)]
+    g = -torch.rand(1, 1100, H, device="cuda")
+    with torch.no_grad():
+        for T in (1100, 60):  # (in spans and whole)
+            part = [t[:, :T] for t in x]
+            assert torch.equal(cache.prefill(0, [n - 1], *part, g[:, :T]), small.prefill(0, [1], *part, g[:, :T]))
+        one = [t[:, 0] for t in x]
+        far, near_ = (torch.tensor([i], dtype=torch.int32, device="cuda") for i in (n - 1, 1))
+        assert torch.equal(cache.decode(0, far, *one, g[:, 0]), small.decode(0, near_, *one, g[:, 0]))

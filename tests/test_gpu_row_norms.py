@@ -283,3 +283,19 @@ def test_another_stream(C):
         got = kernels.residual_norm(x, z)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_offsets_past_32_bits():
+    rows, C = (1 << 19) + 3, 4100  # 2.1e9 elements a tensor
+    x, z, gy, gh = (torch.empty(rows, C, dtype=torch.bfloat16, device="cuda").normal_() for _ in range(4))
+    last = slice(rows - 5, rows)
+    y, res = kernels.gated_norm_fwd(x, z)
+    want, res2 = kernels.gated_norm_fwd(x[last], z[last])
+    assert torch.equal(y[last], want)
+    for a, b in zip(kernels.gated_norm_bwd(res, gy)[:2], kernels.gated_norm_bwd(res2, gy[last])):
+        assert torch.equal(a[last], b)
+    (y, h), res = kernels.residual_norm_fwd(x, z)
+    (want_y, want_h), res2 = kernels.residual_norm_fwd(x[last], z[last])
+    assert torch.equal(y[last], want_y) and torch.equal(h[last], want_h)
+    for a, b in zip(kernels.residual_norm_bwd(res, (gy, gh))[:2], kernels.residual_norm_bwd(res2, (gy[last], gh[last]))):
+        assert torch.equal(a[last], b)
