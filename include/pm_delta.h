@@ -578,8 +578,8 @@ size_t pm_norm_rotate_bwd_workspace_bytes(int B, int T, int Hq, int Hk, int D);
  * D in [1, 256].  States and sums are fp32; products run on bf16 MFMA.  fp32
  * inputs and what is computed from them are factors in three bf16 parts (2^-24
  * relative).  bf16 inputs are factors as they are; the state and the products
- * q . k next to them are bf16 factors of o (2^-9 of each term, whatever o's
- * type), and states sum factors in three parts (2^-24).  A log-decay below -138
+ * q . k next to them are factors of o in two parts (2^-17 of each term), and
+ * states sum factors in three parts (2^-24).  A log-decay below -138
  * counts as closed and one above 138 as infinite; an infinity may come out as
  * NaN, and either reaches the other tokens of its chunk of 64 (fp32 inputs: 32).
  * workspace: pm_decay_attention_workspace_bytes (packed: cu_seqlens is given,
@@ -599,9 +599,8 @@ size_t pm_decay_attention_workspace_bytes(int n_seqs, int T, int Hq, int H, int 
  * (fp32, NULL for zeros).  gq, gk, gv contiguous in dtype; gs0 (B, H, D, D) fp32,
  * NULL: not wanted; gg fp32: (B, T, H), or (H), summed over all tokens in an order that does not
  * change, where both of g's strides are 0; NULL: not wanted.  Every output is
- * written in full; none may overlap an input.  With bf16 inputs gq, gk and gv take
- * bf16 factors as o does; gg, and gs0 where gg is wanted, factors in two bf16
- * parts (2^-17).  workspace:
+ * written in full; none may overlap an input.  With bf16 inputs gq, gk, gv and gg,
+ * and gs0 where gg is wanted, take factors in two bf16 parts (2^-17).  workspace:
  * pm_decay_attention_bwd_workspace_bytes (gates: gg is wanted).
  */
 int pm_decay_attention_bwd(const void* q, const void* k, const void* v, const float* g, const float* s0,

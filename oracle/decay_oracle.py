@@ -108,3 +108,59 @@ def gradients(f, inputs, grads):
     there = [x for x in leaves if x is not None]
     got = iter(torch.autograd.grad(loss, there, allow_unused=True))
     return [None if x is None else next(got) for x in leaves]
+
+
+def planes(x, n):
+    """x as the sum of its first n bf16 parts: the value rounded, what that leaves rounded, and so on."""
+    rest, out = x.to(F64), torch.zeros_like(x, dtype=F64)
+    for _ in range(n):
+        part = rest.float().bfloat16().to(F64)
+        out, rest = out + part, rest - part
+    return out
+
+
+def chunked(q, k, v, g, s0=None, scale=1.0, chunk=64, inputs=None, factors=None, decayed=None):
+    """``decay`` in chunks, in 64 bits but for the factors of its products, which are sums of so many bf16
+    parts (None: as they are): of the inputs, of the state and of A = e^{G_i - G_j} q_i . k_j in what
+    comes out, and of the decayed V that enters the state."""
+    def cut(x, n):
+        return x if n is None else planes(x, n)
+
+    (B, T, Hq, D), H = q.shape, k.shape[2]
+    q, k, v = (cut(x.to(F64), inputs) for x in (q, k, v))
+    g = _per_token(g, q, H)
+    s = torch.zeros(B, H, D, D, dtype=F64) if s0 is None else s0.to(F64).clone()
+    o = torch.empty(q.shape, dtype=F64)
+    for a in range(0, T, chunk):
+        z = min(a + chunk, T)
+        G = torch.cumsum(g[:, a:z], 1).transpose(1, 2)  # B, H, C
+        qc, kc, vc = (x[:, a:z].transpose(1, 2) for x in (q, k, v))
+        qc = qc.unflatten(1, (H, Hq // H))  # B, H, group, C, D
+        lower = torch.ones(z - a, z - a, dtype=torch.bool).tril()
+        pair = torch.exp(torch.where(lower, G[..., :, None] - G[..., None, :], float("-inf")))
+        A = cut(scale * (qc @ kc[:, :, None].transpose(-1, -2)) * pair[:, :, None], factors)
+        into = scale * torch.exp(G)[:, :, None, :, None] * (qc @ cut(s, factors)[:, :, None])
+        o[:, a:z] = (into + A @ vc[:, :, None]).flatten(1, 2).transpose(1, 2)
+        s = torch.exp(G[..., -1])[..., None, None] * s + kc.transpose(-1, -2) @ cut(
+            vc * torch.exp(G[..., -1:] - G)[..., None], decayed)
+    return o, s
+
+
+def _squares(*xs):
+    return [None if x is None else x.to(F64) ** 2 for x in xs]
+
+
+def spread(q, k, v, g, s0=None, scale=1.0):
+    """The root of the sum of squares of the terms of o and of the state: what independent errors of the
+    terms, relative to each, come to."""
+    return [x.sqrt() for x in decay(*_squares(q, k, v), 2 * g.to(F64), *_squares(s0), scale**2)]
+
+
+def spread_bwd(q, k, v, g, s0, go, gs, scale=1.0):
+    """The same of the gradients (per token, also where g is one constant a head)."""
+    g = _per_token(g, q, k.shape[2])
+    return [x.sqrt() for x in decay_bwd(*_squares(q, k, v), 2 * g, *_squares(s0, go, gs), scale**2)]
+
+
+def rms(x):
+    return x.to(F64).square().mean().sqrt().item()

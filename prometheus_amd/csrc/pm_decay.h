@@ -18,9 +18,10 @@
 // that leaves rounded, ...), a product of two such sums the products of their planes down to the last
 // plane's size.  bf16 inputs are one plane and exact; next to them
 //   the decayed V, which sums into states      three planes (2^-25 relative)
-//   the state and V in passes that leave parts of the gates' gradient, which is fp32: two (2^-17; three
-//     take 346 us where two take 240, at B4 T4096 H16 D128: the registers for them are not there)
-//   A and the state in what comes out in bf16   one (2^-9): half a step of its own type, once
+//   A and the state in what comes out          two (2^-17).  What comes out in bf16 is then as if it were
+//     rounded once, and in fp32 nearly so; one part (2^-8 of each term) took 128 us where two take 135 at
+//     B4 T4096 H16 D128, forward, and 536 for 556 with the backward, and was 1.4 times one rounding off
+//   the decayed V in passes that leave parts of the gates' gradient   two (2^-17)
 // fp32 inputs and everything next to them are three.  On this card six such bf16 products take 6/16 of
 // the time of the fp32 MFMA.
 //
@@ -40,8 +41,7 @@ namespace {
 template <int P>
 struct DecayShape {
     static constexpr int C = P == 1 ? 64 : 32;   // tokens of a chunk (three planes of 64 would not fit LDS)
-    static constexpr int PG = P == 1 ? 2 : 3;    // planes of what sums into the gates' gradient
-    static constexpr int PA = P;                 // planes of what sums into outputs of q's type alone
+    static constexpr int PA = P == 1 ? 2 : 3;    // planes of A, and of the state as a factor
     static constexpr int MT = C / 16;            // 16-token tiles
     static constexpr int TRI = MT * (MT + 1) / 2;  // lower 16x16 tiles of A
     static constexpr int BLK = P == 1 ? 6 : 2;   // packed operand blocks of A (qblk)
@@ -265,8 +265,7 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
     constexpr int UQ = C * DK / 2048, UV = C * NT / 2048;  // 8-element units per thread
     constexpr int RQ = 2048 / DK, RV = 2048 / NT;          // rows between a thread's units
     constexpr bool OUT = KIND < kPassState, AUX = KIND == kPassPart;
-    constexpr int PS = AUX ? Sh::PG : PA;  // planes of the state in the outputs' part
-    constexpr int PC = AUX || KIND == kPassStateG ? Sh::PG : 3;  // planes of the decayed V, which sums into the state
+    constexpr int PC = AUX || KIND == kPassStateG ? PA : 3;  // planes of the decayed V, which sums into the state
     using E = typename std::conditional<P == 1, uint16_t, float>::type;
 
     __shared__ __attribute__((aligned(16))) uint16_t sq[OUT ? P * C * DK : 8];
@@ -542,7 +541,7 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                     for (int i = 0; i < MT; ++i) O[ct][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
-                    u32x4_t so[CT][PS], qo[MT][P], ko[P];
+                    u32x4_t so[CT][PA], qo[MT][P], ko[P];
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -553,7 +552,7 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                     for (int ct = 0; ct < CT; ++ct) {
                         const f32x4_t s0 = S[ct][2 * kb], s1 = S[ct][2 * kb + 1];
                         const float s8[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
-                        split8<PS>(s8, so[ct]);
+                        split8<PA>(s8, so[ct]);
                     }
 #pragma unroll
                     for (int x = P - 1; x >= 0; --x)
@@ -565,10 +564,10 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
                                     A[i] = mfma32(__builtin_bit_cast(bf16x8_t, ko[x - p]),
                                                   __builtin_bit_cast(bf16x8_t, qo[i][p]), A[i]);
 #pragma unroll
-                    for (int x = PS - 1; x >= 0; --x)  // (the small products first, all tiles of one before the next)
+                    for (int x = PA - 1; x >= 0; --x)  // (the small products first, all tiles of one before the next)
 #pragma unroll
                         for (int p = 0; p < P; ++p)
-                            if (x - p >= 0 && (x < PA || parts))
+                            if (x - p >= 0)
 #pragma unroll
                                 for (int ct = 0; ct < CT; ++ct)
 #pragma unroll

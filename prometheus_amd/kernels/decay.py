@@ -218,10 +218,10 @@ def decay_attention(q, k, v, g, state=None, *, scale=1.0, out_dtype=None):
     ``(o, next_state)``: o shaped like q, in bf16 for bf16 q, k and v and in fp32 otherwise unless
     ``out_dtype`` says so, next_state (batch, H, D, D) fp32.
 
-    fp32 inputs have fp32 accuracy. bf16 inputs enter the products as they are; of o and of their
-    gradients the state and the products ``q k`` are bf16 factors (2^-9 of each term, also where
-    ``out_dtype`` is fp32), the next state's sums keep 2^-24 and the decays' gradient 2^-17. A log-decay below -138 counts as closed. An infinity may come out as NaN, and either reaches the
-    other tokens of its chunk of 64 (fp32: 32) beside those it reaches token by token.
+    fp32 inputs have fp32 accuracy. bf16 inputs enter the products as they are; o and the gradients
+    keep 2^-17 of each term before they are rounded to their type, the next state's sums 2^-24. A
+    log-decay below -138 counts as closed. An infinity may come out as NaN, and either reaches the other
+    tokens of its chunk of 64 (fp32: 32) beside those it reaches token by token.
 
     Differentiable: when autograd records and a torch input requires grad, the backward is
     ``decay_attention_bwd``.
