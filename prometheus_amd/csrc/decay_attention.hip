@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void gate_grad(DecayGateGrad a) {
     const int h = static_cast<int>(id % a.H);
     const int span = static_cast<int>(id / a.H % a.n_spans);
     const int64_t b = id / a.H / a.n_spans;
-    const int begin = span * a.span, end = min(begin + a.span, a.T);
+    const int begin = span * a.span, end = span_end(begin, a.span, a.T);
 
     // the gradient at the span's first token
     float around = 0.f;
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(1024) void assign_slots(const int32_t* cu, int n_se
     const int t = threadIdx.x, per = (n_seqs + 1023) / 1024, i0 = min(t * per, n_seqs), i1 = min(i0 + per, n_seqs);
     auto spans = [&](int i) {
         const int z0 = min(max(cu[i], 0), T), z1 = min(max(cu[i + 1], 0), T);
-        return max((z1 - z0 + span - 1) / span, 1);
+        return spans_of(z1 - z0, span);
     };
     int n = 0, bits = 0;
     for (int i = i0; i < i1; ++i) {
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256) void scan_spans(DecayPasses passes, const int*
         len = max(min(max(a.cu[seq + 1], 0), a.T) - min(max(a.cu[seq], 0), a.T), 0);
         slot = first_slot[seq];
     }
-    const int n = min(max((len + a.span - 1) / a.span, 1), a.n_slots_grid - slot);
+    const int n = min(spans_of(len, a.span), a.n_slots_grid - slot);
     vec S = {};
     if (a.s0) {
         int64_t from = seq;
@@ -257,7 +257,7 @@ Plan plan(int n_seqs, int T, int HO, int HS, int D, bool packed, bool bf16) {
         const int64_t span = std::max<int64_t>((tokens + slots - 1) / slots, kMinSpan);
         const int64_t n = (T + span - 1) / span;
         p.span = static_cast<int>(((T + n - 1) / n + 63) / 64 * 64);
-        p.n_spans = (T + p.span - 1) / p.span;
+        p.n_spans = spans_of(T, p.span);
         p.n_slots = packed ? T / p.span + n_seqs : n_seqs * p.n_spans;
         p.split = p.n_spans > 1;
     }
@@ -311,7 +311,7 @@ BwdPlan plan_bwd(int B, int T, int Hq, int H, int D, bool gates, bool bf16) {
     if (span < T) {
         const int64_t n = (T + span - 1) / span;
         p.k.span = static_cast<int>(((T + n - 1) / n + 63) / 64 * 64);
-        p.k.n_spans = (T + p.k.span - 1) / p.k.span;
+        p.k.n_spans = spans_of(T, p.k.span);
         p.k.n_slots = B * p.k.n_spans;
         p.k.split = p.k.n_spans > 1;
     }

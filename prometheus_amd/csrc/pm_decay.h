@@ -312,12 +312,12 @@ __global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void d
         qp += seq * a.q_sb, kp += seq * a.k_sb, vp += seq * a.v_sb, gp += seq * a.g_sb, xp += seq * a.x_sb;
         rows0 = static_cast<int64_t>(seq) * a.T;
     }
-    const int n_spans = max((len + a.span - 1) / a.span, 1);
+    const int n_spans = spans_of(len, a.span);
     // (the last span's share is not wanted; where malformed offsets overlap, a next slot may be missing)
     if (!OUT && (order + 1 >= n_spans || slot_id + 1 >= a.n_slots_grid)) return;
     const int my_span = a.reverse ? n_spans - 1 - order : order;
     const int c_begin = my_span * a.span;  // first token, relative to the sequence
-    const int c_end = min(c_begin + a.span, len);
+    const int c_end = span_end(c_begin, a.span, len);
     const int n_chunks = (c_end - c_begin + C - 1) / C;
     const int64_t state_pair = static_cast<int64_t>(seq) * a.HS + hs;
 

@@ -11,6 +11,13 @@ constexpr int kDecayGateSpan = 512;  // the longest span where the gates' gradie
 // Columns of the state that a workgroup keeps (pm_decay.h: DecayTile).
 constexpr int decay_cols(int D) { return D <= 64 ? 64 : 128; }
 
+// Spans of a sequence, one at least.  (No sum with the span's length: both may be near 2^31.)
+__host__ __device__ inline int spans_of(int len, int span) { return len > 0 ? 1 + (len - 1) / span : 1; }
+// The last token of the span that begins at `begin` < len, plus one.
+__host__ __device__ inline int span_end(int begin, int span, int len) {
+    return span < len - begin ? begin + span : len;
+}
+
 // One pass over n_seqs sequences (roles as in pm_decay.h).  Strides are in elements; the elements of
 // a head are contiguous.  HO heads of Q and O, HK of K and V, HS = min(HO, HK) states.
 struct DecayPass {

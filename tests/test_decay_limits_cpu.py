@@ -1,0 +1,32 @@
+"""CPU tests of decay attention and the norms around it at the edges of their sizes: what they plan or
+refuse there, before any device work."""
+
+from __future__ import annotations
+
+import pytest
+
+from prometheus_amd import _native
+
+MOST = 2**31 - 1 - 1024  # tokens of a sequence
+
+
+@pytest.mark.parametrize("H", [1, 8])
+def test_workspaces_of_very_many_tokens(H):
+    """A sequence of many tokens is cut into spans, whose states the workspace holds, up to the last length
+    that a call takes (sums of a length and a span's pass 2^31 from about 2.13e9 on)."""
+    L = _native.lib()
+    sizes = [
+        lambda T: L.pm_decay_attention_workspace_bytes(1, T, H, H, 1, 0, 0),
+        lambda T: L.pm_decay_attention_workspace_bytes(1, T, H, H, 1, 1, 0),
+        lambda T: L.pm_decay_attention_workspace_bytes(3, T, H, H, 1, 1, 1),
+    ]
+    if H == 1:  # (more heads would take more workgroups than a launch of the backward has)
+        sizes.append(lambda T: L.pm_decay_attention_bwd_workspace_bytes(1, T, H, H, 1, 0))
+    lengths = (2_000_000_000, 2_131_000_000, 2_144_000_000, 2_145_500_000, MOST)
+    for i, size in enumerate(sizes):
+        got = [size(T) for T in lengths]
+        # (a state and its log-decay are 12 bytes; the card holds 768 workgroups, three of them to a span of
+        # the backward)
+        assert min(got) >= 12 * 250, (i, got)
+        assert max(got) <= 1.5 * min(got), (i, got)  # (as many spans as the card holds)
+        assert size(MOST + 1) == 0
