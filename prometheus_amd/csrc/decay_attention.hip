@@ -365,10 +365,10 @@ DecayPass turned(DecayPass x) {
 }
 
 // The states before the spans of each pass, from each span's own share.
-hipError_t span_states(DecayPasses x, bool bf16, bool gates, const int* first_slot, hipStream_t st) {
+hipError_t span_states(DecayPasses x, bool bf16, const int* first_slot, hipStream_t st) {
     for (int i = 0; i < x.n; ++i)  // (the way round that stores a state's rows in 16-byte pieces)
         if (x.pass[i].u_row != 1) x.pass[i] = turned(x.pass[i]);
-    if (hipError_t e = run_kind(x, bf16, gates ? 3 : 2, st); e != hipSuccess) return e;
+    if (hipError_t e = run_kind(x, bf16, 2, st); e != hipSuccess) return e;
     const DecayPass& a = x.pass[0];
     const int64_t pairs = static_cast<int64_t>(a.n_seqs) * a.HS;
     // (four elements a thread, where that leaves a workgroup for every CU: 64 heads' 8 spans of D 128 take
@@ -449,7 +449,7 @@ hipError_t launch_decay_attn(const DecayAttnArgs& a, hipStream_t st) {
     if (p.split) {
         x.span_state = at<float>(a.workspace, w.span_state);
         x.span_log = at<double>(a.workspace, w.span_log);
-        if (hipError_t e = span_states({{x}, 1}, a.bf16, false, first_slot, st); e != hipSuccess) return e;
+        if (hipError_t e = span_states({{x}, 1}, a.bf16, first_slot, st); e != hipSuccess) return e;
     }
     return run_kind({{x}, 1}, a.bf16, 0, st);
 }
@@ -491,7 +491,7 @@ hipError_t launch_decay_attn_bwd(const DecayAttnBwdArgs& a, hipStream_t st) {
     const DecayPass gv = pass(k, q, go, k, a.H, a.Hq, p.k, true, false, a.gs, gs0, a.gv, false);
     const DecayPass gk = pass(v, go, q, k, a.H, a.Hq, p.k, true, true, a.gs, nullptr, a.gk, true);
     if (p.k.split)  // (gk's and gv's states are the same, one transposed)
-        if (hipError_t e = span_states({{gq, gk}, 2}, a.bf16, gates, nullptr, st); e != hipSuccess) return e;
+        if (hipError_t e = span_states({{gq, gk}, 2}, a.bf16, nullptr, st); e != hipSuccess) return e;
     if (hipError_t e = run_kind({{gq, gv, gk}, 3}, a.bf16, gates ? 1 : 0, st); e != hipSuccess) return e;
     if (!gates) return hipSuccess;
     const bool constant = a.g_sb == 0 && a.g_st == 0;

@@ -17,11 +17,11 @@
 // Products run on bf16 MFMA.  A value of more than 8 bits is a sum of bf16 planes (the value rounded, what
 // that leaves rounded, ...), a product of two such sums the products of their planes down to the last
 // plane's size.  bf16 inputs are one plane and exact; next to them
-//   the decayed V, which sums into states      three planes (2^-25 relative)
+//   the decayed V, which sums into states      three planes (2^-25 relative; two, 2^-17, in the backward's
+//     passes alone took 556 us where three take 580, with the forward)
 //   A and the state in what comes out          two (2^-17).  What comes out in bf16 is then as if it were
 //     rounded once, and in fp32 nearly so; one part (2^-8 of each term) took 128 us where two take 135 at
 //     B4 T4096 H16 D128, forward, and 536 for 556 with the backward, and was 1.4 times one rounding off
-//   the decayed V in passes that leave parts of the gates' gradient   two (2^-17)
 // fp32 inputs and everything next to them are three.  On this card six such bf16 products take 6/16 of
 // the time of the fp32 MFMA.
 //
@@ -250,7 +250,7 @@ __device__ __forceinline__ float exp2_f64(double x) {
 // The next chunk's rows are loaded into registers while this one's products run.
 
 // What a launch of decay_pass does besides its outputs.
-enum { kPassPlain = 0, kPassPart = 1, kPassState = 2, kPassStateG = 3 };  // (G: for the gates' gradient)
+enum { kPassPlain = 0, kPassPart = 1, kPassState = 2 };
 
 template <int DK>
 struct DecayTile {
@@ -258,14 +258,14 @@ struct DecayTile {
 };
 
 template <int P, int DK, int KIND>
-__global__ __launch_bounds__(256, KIND >= kPassState || DK < 256 ? 2 : 1) void decay_pass(DecayPasses passes) {
+__global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void decay_pass(DecayPasses passes) {
     using Sh = DecayShape<P>;
     constexpr int C = Sh::C, PA = Sh::PA, MT = Sh::MT, KB = DK / 32, MD = DK / 16;
     constexpr int CT = DecayTile<DK>::CT, NT = DecayTile<DK>::NT;
     constexpr int UQ = C * DK / 2048, UV = C * NT / 2048;  // 8-element units per thread
     constexpr int RQ = 2048 / DK, RV = 2048 / NT;          // rows between a thread's units
-    constexpr bool OUT = KIND < kPassState, AUX = KIND == kPassPart;
-    constexpr int PC = AUX || KIND == kPassStateG ? PA : 3;  // planes of the decayed V, which sums into the state
+    constexpr bool OUT = KIND != kPassState, AUX = KIND == kPassPart;
+    constexpr int PC = 3;  // planes of the decayed V, which sums into the state
     using E = typename std::conditional<P == 1, uint16_t, float>::type;
 
     __shared__ __attribute__((aligned(16))) uint16_t sq[OUT ? P * C * DK : 8];
@@ -958,15 +958,12 @@ hipError_t launch_pass(const DecayPasses& a, int kind, hipStream_t st) {
     int64_t units = 0;
     for (int i = 0; i < a.n; ++i) {
         const DecayPass& x = a.pass[i];
-        units = std::max(units, static_cast<int64_t>(x.n_slots_grid) * (kind >= kPassState ? x.HS : x.HO / x.n_dst));
+        units = std::max(units, static_cast<int64_t>(x.n_slots_grid) * (kind == kPassState ? x.HS : x.HO / x.n_dst));
     }
     const dim3 grid(static_cast<unsigned>((units + 7) / 8 * 8 * a.pass[0].n_tiles * a.n));
     switch (kind) {
         case kPassPlain: hipLaunchKernelGGL((decay_pass<P, DK, kPassPlain>), grid, dim3(256), 0, st, a); break;
         case kPassPart: hipLaunchKernelGGL((decay_pass<P, DK, kPassPart>), grid, dim3(256), 0, st, a); break;
-        case kPassStateG:
-            hipLaunchKernelGGL((decay_pass<P, DK, P == 1 ? kPassStateG : kPassState>), grid, dim3(256), 0, st, a);
-            break;
         default: hipLaunchKernelGGL((decay_pass<P, DK, kPassState>), grid, dim3(256), 0, st, a); break;
     }
     return hipGetLastError();

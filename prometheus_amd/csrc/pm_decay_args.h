@@ -94,7 +94,7 @@ struct DecayGateGrad {
 };
 
 // kind: 0 outputs and states, 1 the same and `part`s, 2 each span's own share of the state (from zeros) but
-// the last one's, to the next slot of span_state, 3 the same in as many planes as 1.
+// the last one's, to the next slot of span_state.
 hipError_t decay_pass_bf16(const DecayPasses& a, int kind, hipStream_t st);
 hipError_t decay_pass_f32(const DecayPasses& a, int kind, hipStream_t st);
 hipError_t decay_near_bf16(const DecayNear& a, hipStream_t st);

@@ -219,8 +219,8 @@ def decay_attention(q, k, v, g, state=None, *, scale=1.0, out_dtype=None):
     ``out_dtype`` says so, next_state (batch, H, D, D) fp32.
 
     fp32 inputs have fp32 accuracy. bf16 inputs enter the products as they are; o and the gradients
-    keep 2^-17 of each term before they are rounded to their type, the next state's sums 2^-24. A
-    log-decay below -138 counts as closed. An infinity may come out as NaN, and either reaches the other
+    keep 2^-17 of each term before they are rounded to their type, the states and the first state's
+    gradient 2^-24. A log-decay below -138 counts as closed. An infinity may come out as NaN, and either reaches the other
     tokens of its chunk of 64 (fp32: 32) beside those it reaches token by token.
 
     Differentiable: when autograd records and a torch input requires grad, the backward is
@@ -242,7 +242,7 @@ def decay_attention_fwd(q, k, v, g, state=None, *, scale=1.0, out_dtype=None):
 def decay_attention_bwd(residual: _DecayResidual, grads):
     """Backward of the VJP pair: ``grads = (go, gs)``, dL/do (batch, seq, Hq, D) and dL/dnext_state
     (batch, H, D, D), either may be None. Returns ``(gq, gk, gv, gg, gstate)``: gq, gk and gv in q's
-    type, gg shaped like g and gstate in fp32. With bf16 q, k and v an fp32 go is rounded to bf16
+    type, gg shaped like g and gstate in fp32, each as accurate whichever are wanted. With bf16 q, k and v an fp32 go is rounded to bf16
     first: it is a factor of products, as they are. What heads or tokens share is summed in an order
     that does not change."""
     go, gs = grads

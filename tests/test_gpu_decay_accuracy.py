@@ -41,3 +41,18 @@ def test_gradients_of_the_inputs(B, T, Hq, H, D, dtype):
     for i in range(3):
         assert got[i].dtype == dtype
         acc.check(got[i], want[i], spread[i], acc.of_factors(dtype, T, Hq // H, D))
+
+
+@pytest.mark.parametrize("B,T,Hq,H,D", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("gates", [True, False])
+def test_gradient_of_the_first_state(B, T, Hq, H, D, dtype, gates):
+    """As near whether the decays' gradient is taken with it or not."""
+    q, k, v, g, s0, go, gs = acc.inputs(B, T, Hq, H, D, dtype, seed=T)
+    dev = gpu(q, k, v, g, s0)
+    for x in (dev if gates else dev[:3] + dev[4:]):
+        x.requires_grad_(True)
+    o, s = kernels.decay_attention(*dev, scale=0.7)
+    (got,) = torch.autograd.grad((o, s), dev[4], gpu(go, gs))
+    want, spread = ref.decay_bwd(q, k, v, g, s0, go, gs, 0.7), ref.spread_bwd(q, k, v, g, s0, go, gs, 0.7)
+    acc.check(got, want[4], spread[4], acc.of_sums(T, Hq // H, D))
