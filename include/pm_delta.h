@@ -580,8 +580,8 @@ size_t pm_norm_rotate_bwd_workspace_bytes(int B, int T, int Hq, int Hk, int D);
  * relative).  bf16 inputs are factors as they are; the state and the products
  * q . k next to them are factors of o in two parts (2^-17 of each term), and
  * states sum factors in three parts (2^-24).  A log-decay below -138
- * counts as closed and one above 138 as infinite; an infinity may come out as
- * NaN, and either reaches the other tokens of its chunk of 64 (fp32 inputs: 32).
+ * counts as closed and one above 138 as infinite; infinities and NaN reach what
+ * they reach token by token, an infinity possibly as NaN.
  * workspace: pm_decay_attention_workspace_bytes (packed: cu_seqlens is given,
  * in_place: s0 is s_out and not NULL; 0 where none is needed).
  */
@@ -600,7 +600,8 @@ size_t pm_decay_attention_workspace_bytes(int n_seqs, int T, int Hq, int H, int 
  * NULL: not wanted; gg fp32: (B, T, H), or (H), summed over all tokens in an order that does not
  * change, where both of g's strides are 0; NULL: not wanted.  Every output is
  * written in full; none may overlap an input.  With bf16 inputs gq, gk, gv and gg
- * take factors in two bf16 parts (2^-17), gs0 in three.  workspace:
+ * take factors in two bf16 parts (2^-17), gs0 in three.  Infinities and NaN in q
+ * and go reach gg of up to 512 tokens behind theirs too.  workspace:
  * pm_decay_attention_bwd_workspace_bytes (gates: gg is wanted).
  */
 int pm_decay_attention_bwd(const void* q, const void* k, const void* v, const float* g, const float* s0,

@@ -198,6 +198,12 @@ __device__ __forceinline__ u32x4_t join(u32x2_t a, u32x2_t b) {
     return r;
 }
 
+// The larger halves of two pairs, as unsigned numbers.
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+
 // The same number, as one the compiler knows nothing of: what is computed from it is computed where it is
 // used, not ahead of the loop, where it would take a register (or scratch memory, whose loads wait for
 // the rows that are on their way: the backward's three passes at B4 T4096 H16 D128 took 302 us, 240 so).
@@ -738,6 +744,47 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                                     S[ct][2 * d32 + h] = mfma32(__builtin_bit_cast(bf16x8_t, ko[h][p]),
                                                                 __builtin_bit_cast(bf16x8_t, wo[ct][x - p]),
                                                                 S[ct][2 * d32 + h]);
+            }
+        }
+        // ---- infinities and NaN of V stay out of A V, where A's zeros would carry them to tokens before theirs:
+        // zeros go in their place, and from its first such token on a column comes out as NaN.  (No cost but
+        // for the test; without its weight in the compiler's favour 24 us of the training step's 568 went
+        // into registers that the branch takes.)
+        if (OUT) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int kb = 0; kb < MT / 2; ++kb)
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) most = max_halves(most, vo[kb][ct][0][x] & 0x7fff7fffu);
+            if (__builtin_expect(__any((most & 0xffffu) >= 0x7f80u || most >= 0x7f800000u), 0)) {
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    int from = C;  // the first such token of the lane's column
+                    const int tok = 4 * (fresh(t) >> 4 & 3);
+#pragma unroll
+                    for (int kb = MT / 2 - 1; kb >= 0; --kb)
+#pragma unroll
+                        for (int x = 3; x >= 0; --x) {
+                            const uint32_t v = vo[kb][ct][0][x] & 0x7fff7fffu;
+                            const bool hi = v >= 0x7f800000u, lo = (v & 0xffffu) >= 0x7f80u;
+                            from = hi ? tok + (32 * kb + 8 * (x / 2) * 2 + 2 * (x % 2) + 1) : from;
+                            from = lo ? tok + (32 * kb + 8 * (x / 2) * 2 + 2 * (x % 2)) : from;
+                            const uint32_t keep = (hi ? 0u : 0xffff0000u) | (lo ? 0u : 0xffffu);
+#pragma unroll
+                            for (int p = 0; p < P; ++p) vo[kb][ct][p][x] &= keep;
+                        }
+                    from = min(from, __shfl_xor(from, 16));
+                    from = min(from, __shfl_xor(from, 32));
+                    const int row = fresh(t) & 15;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int x = __shfl(from, tok + r) - row;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) O[ct][i][r] = 16 * i >= x ? __builtin_nanf("") : O[ct][i][r];
+                    }
+                }
             }
         }
         // (the next step's loads: after the products that need every register, before the wait for the other
