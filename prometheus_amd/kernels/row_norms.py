@@ -58,6 +58,8 @@ def _dtype(x) -> torch.dtype:
 def _even(shape, strides):
     """The stride between consecutive ones of the elements that ``shape`` and ``strides`` enumerate,
     or None where they are not evenly spaced."""
+    if 0 in shape:
+        return 0
     step, reach = None, 0
     for size, stride in zip(reversed(shape), reversed(strides)):
         if size == 1:
@@ -76,6 +78,8 @@ def _rows_of(shape, x_strides, z_strides):
     has to be copied: rows evenly spaced, or evenly spaced groups of the last dimension but one."""
     lead = shape[:-1]
     rows = math.prod(lead)
+    if rows == 0:
+        return 0, 1, (ctypes.c_int64 * 4)(0, 0, 0, 0)
     both = (x_strides[:-1], z_strides[:-1])
     whole = [_even(lead, s) for s in both]
     if None not in whole:

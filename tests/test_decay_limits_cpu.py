@@ -4,8 +4,10 @@ refuse there, before any device work."""
 from __future__ import annotations
 
 import pytest
+import torch
 
 from prometheus_amd import _native
+from prometheus_amd.kernels import row_norms
 
 MOST = 2**31 - 1 - 1024  # tokens of a sequence
 
@@ -30,3 +32,17 @@ def test_workspaces_of_very_many_tokens(H):
         assert min(got) >= 12 * 250, (i, got)
         assert max(got) <= 1.5 * min(got), (i, got)  # (as many spans as the card holds)
         assert size(MOST + 1) == 0
+
+
+EMPTY = [(0, 16), (2, 0, 16), (0, 5, 16), (2, 0, 4, 16), (3, 0, 2, 5, 8), (2, 3, 0, 16), (0, 0, 8)]
+
+
+@pytest.mark.parametrize("shape", EMPTY)
+def test_no_rows_are_evenly_spaced(shape):
+    """Wherever the dimension without elements stands, for contiguous tensors and for views."""
+    x = torch.zeros(shape)
+    wide = torch.zeros(*shape[:-1], shape[-1] + 3)[..., 1:shape[-1] + 1]
+    for a in (x, wide):
+        rows, inner, strides = row_norms._rows_of(shape, a.stride(), x.stride())
+        assert rows == 0 and inner == 1 and len(strides) == 4
+        assert row_norms._even(shape[:-1], a.stride()[:-1]) is not None

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from prometheus_amd import kernels
+from tests.test_decay_limits_cpu import EMPTY
 
 pytestmark = pytest.mark.gpu
 MOST = 2**31 - 1 - 1024  # tokens of a sequence
@@ -30,3 +31,29 @@ def test_as_many_tokens_as_a_call_takes(cu):
     low, high = o.aminmax()
     assert low.item() == high.item() == 2.0
     assert (s - 2.0).abs().max().item() < 1e-5
+
+
+@pytest.mark.parametrize("shape", EMPTY)
+@pytest.mark.parametrize("kind", ["gpu", "view", "fp16", "cpu", "numpy"])
+def test_norms_of_no_rows(shape, kind):
+    """Both directions, through autograd and without, where the fast path of contiguous tensors is not taken."""
+    x, w = torch.zeros(shape), torch.ones(shape[-1])
+    if kind != "cpu" and kind != "numpy":
+        x, w = x.cuda(), w.cuda()
+    if kind == "view":
+        x = torch.zeros(*shape[:-1], shape[-1] + 3, device="cuda")[..., 1:shape[-1] + 1]
+    if kind == "fp16":
+        x = x.half()
+    if kind == "numpy":
+        x, w = x.numpy(), w.numpy()
+    y, res = kernels.gated_norm_fwd(x, x, w)
+    gx, gz, gw = kernels.gated_norm_bwd(res, y)
+    assert y.shape == gx.shape == gz.shape == shape and gw.shape == w.shape and not gw.any()
+    (y, h), res = kernels.residual_norm_fwd(x, x, w, post_weight=w)
+    gx, gr, gw, gwp = kernels.residual_norm_bwd(res, (y, h))
+    assert y.shape == h.shape == gx.shape == gr.shape == shape and not gw.any() and not gwp.any()
+    if kind != "numpy":
+        leaves = [x.clone().requires_grad_(True), x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        for f in (kernels.gated_norm, lambda *a: kernels.residual_norm(*a)[0]):
+            grads = torch.autograd.grad(f(*leaves).sum(), leaves)
+            assert grads[0].shape == shape and not grads[2].any()
