@@ -74,6 +74,8 @@ def _check(q, k, v, g, rank, scale) -> tuple:
         raise _k.KernelError(f"q, k and v must be {names}, k and v alike and q alike but for its heads; "
                              f"got {qs}, {ks} and {vs}")
     lead, Hq, H, D = qs[:-2], qs[-2], ks[-2], qs[-1]
+    if max(qs) >= 2**31:  # (the library's sizes are 32-bit ones: a larger one would come to another there)
+        raise _k.KernelError(f"problem too large: {qs}")
     if H < 1 or Hq < 1 or Hq % H:
         raise _k.KernelError(f"q's heads must be a multiple of k's; got {Hq} and {H}")
     if not 1 <= D <= _native.MAX_D:

@@ -85,7 +85,7 @@ def _rows_of(shape, x_strides, z_strides):
     if None not in whole:
         return rows, 1, (ctypes.c_int64 * 4)(whole[0], 0, whole[1], 0)
     outer = [_even(lead[:-1], s[:-1]) for s in both]
-    if None in outer:
+    if None in outer or lead[-1] >= 2**31:  # (the library counts a group's rows in 32 bits)
         return None
     return rows, lead[-1], (ctypes.c_int64 * 4)(outer[0], both[0][-1], outer[1], both[1][-1])
 

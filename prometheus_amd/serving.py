@@ -375,7 +375,7 @@ class DecayStateCache(_SlotPool):
         if ks != (slots.shape[0], heads, dim):
             raise ValueError(f"k must be {(slots.shape[0], heads, dim)}, got {tuple(ks)}")
         if v.shape != ks or len(qs) != 3 or qs[0] != ks[0] or qs[1] < 1 or qs[1] % heads or qs[2] != dim or (
-                dim > _native.MAX_D):
+                dim > _native.MAX_D) or max(qs) >= 2**31:
             decay._check(q, k, v, g, 3, scale)  # (which says what is wrong)
         if g.shape != ks[:2] and g.shape != (heads,):
             raise ValueError(f"g must be {tuple(ks[:2])} or {(heads,)}, got {tuple(g.shape)}")

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from prometheus_amd import _native
+from prometheus_amd import _native, kernels, serving
 from prometheus_amd.kernels import row_norms
 
 MOST = 2**31 - 1 - 1024  # tokens of a sequence
@@ -46,3 +46,26 @@ def test_no_rows_are_evenly_spaced(shape):
         rows, inner, strides = row_norms._rows_of(shape, a.stride(), x.stride())
         assert rows == 0 and inner == 1 and len(strides) == 4
         assert row_norms._even(shape[:-1], a.stride()[:-1]) is not None
+
+
+@pytest.mark.parametrize("sizes", [(1, 2**32 + 5, 2, 2), (2**32 + 2, 1, 2, 2), (1, 3, 2**32 + 2, 2)])
+def test_sizes_past_32_bits_are_refused(sizes):
+    """A view may have them without memory; the library's own sizes are 32-bit ones."""
+    B, T, Hq, H = sizes
+    q, k = torch.zeros(1, 1, 1, 1).expand(B, T, Hq, 1), torch.zeros(1, 1, 1, 1).expand(B, T, H, 1)
+    g = torch.zeros(H)
+    calls = [lambda: kernels.decay_attention(q, k, k, g), lambda: kernels.decay_attention_fwd(q, k, k, g),
+             lambda: serving.DecayStateCache(1, 2, H, 1, device="cpu").prefill(0, [0], q, k, k, g)]
+    if max(B, Hq) >= 2**31:
+        calls.append(lambda: kernels.decay_attention_step(q[:, 0], k[:, 0], k[:, 0], g,
+                                                          torch.zeros(1).expand(B, H, 1, 1)))
+    for f in calls:
+        with pytest.raises(kernels.KernelError, match="too large"):
+            f()
+
+
+def test_rows_of_more_than_32_bits_are_copied():
+    shape = (2, 2**31, 8)
+    assert row_norms._rows_of(shape, (2**40, 16, 1), (2**34, 8, 1)) is None
+    rows, inner, strides = row_norms._rows_of(shape, (2**35, 16, 1), (2**34, 8, 1))
+    assert (rows, inner, list(strides)) == (2**32, 1, [16, 0, 8, 0])
