@@ -22,9 +22,11 @@ namespace {
 struct Act {
     float a, slope;
 };
+// With e = e^-|z|: s = 1 / (1 + e) or e / (1 + e), and its slope s (1 - s) = e / (1 + e)^2, which keeps its
+// digits where the gate is wide open (1 - s has lost them at z = 16).
 __device__ __forceinline__ Act act_of(float z, bool silu) {
-    const float s = __builtin_amdgcn_rcpf(1.f + exp2_hw(z * -1.44269504f));
-    const float d = s * (1.f - s);
+    const float e = exp2_hw(fabsf(z) * -1.44269504f), r = __builtin_amdgcn_rcpf(1.f + e);
+    const float s = z < 0.f ? e * r : r, d = e * r * r;
     return silu ? Act{z * s, s + z * d} : Act{s, d};
 }
 
