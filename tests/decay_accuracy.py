@@ -8,7 +8,7 @@ chunk of 32 tokens, the same way in all terms: T / 32 of that. A factor in three
 most 2^-24 (five of them at most, and the products left out: 8 in all), one in two parts by 2^-17
 (half a step of the second part, which is at most 2^-8 of the value and itself off by 2^-9 of that).
 The decays' gradients hand what they sum over up to 16 chunks on from chunk to chunk, each chunk's own
-sums once in and once out: sqrt(33) of the largest one's, 6.
+sums once in and once out: sqrt(33) of one's, 6.
 What comes out in bf16 is rounded once: the exact value's own rounding error, and 2% for the values that
 another rounding falls upon.
 """
@@ -56,3 +56,24 @@ def inputs(B, T, Hq, H, D, dtype, s0=True, seed=0, low=-0.3, zeros=False):
         g = torch.where(torch.rand(B, T, H, generator=gen) < 1 / 3, 0.0, g)
     go, gs = normal(B, T, Hq, D).to(dtype), normal(B, H, D, D)
     return q, k, v, g, normal(B, H, D, D) if s0 else None, go, gs
+
+
+def bound_gates(spread, dtype, T, G, D):
+    """What the rms of the decays' gradient's error may be. What a chunk's tokens add to it or take from it
+    are parts of the gradient at the chunk's first token and behind its last, next to bf16 inputs with one
+    factor, the state, in two parts; where a span begins it is a product of two states, whose sums' errors
+    are handed to all of its tokens."""
+    eps = of_sums(T, G, D)
+    largest = spread.amax(1, keepdim=True).expand_as(spread)
+    return 6 * (eps * ref.rms(largest) + (2.0**-17 * ref.rms(spread) if dtype == BF16 else 0.0))
+
+
+def check_gates(got, want, spread, dtype, T, G, D):
+    assert got.shape == want.shape and got.dtype == F32
+    off, most = ref.rms(got.detach().cpu().double() - want), bound_gates(spread, dtype, T, G, D)
+    assert off <= most, (off, most)
+
+
+def slow(B, T, Hq, H, D, dtype, seed=0):
+    """Inputs whose states live through the whole sequence: rates of 0 to 0.002 a token."""
+    return inputs(B, T, Hq, H, D, dtype, seed=seed, low=-2e-3, zeros=True)

@@ -60,3 +60,45 @@ def test_spreads_are_of_the_terms():
     last = ((gs[0, 0].double() * k[0, 4, 0, :, None].double())**2).sum(0)
     last += ((q[0, 4, 0, :, None].double() * go[0, 4, 0].double() * k[0, 4, 0, :, None].double())**2).sum(0)
     assert torch.allclose(gv[0, 4, 0], last.sqrt())
+
+
+@pytest.mark.parametrize("dtype", [acc.BF16, acc.F32])
+def test_what_spans_hand_on_is_seen(dtype):
+    """Slow decays: a span that does not start from the state before it, or whose gradients miss what comes
+    from before it, is far outside of the bounds."""
+    T, at = 1100, 576
+    x = acc.slow(1, T, 2, 1, 16, dtype)
+    q, k, v, g, s0, go, gs = x
+    want, spread = ref.decay(q, k, v, g, s0), ref.spread(q, k, v, g, s0)
+    lost = [t[:, at:] for t in (q, k, v, g)]
+    o, s = ref.decay(*lost)
+    for got, e, m, eps in ((o, want[0][:, at:], spread[0][:, at:], acc.of_factors(dtype, T, 2, 16)),
+                           (s, want[1], spread[1], acc.of_sums(T, 1, 16))):
+        assert ref.rms(got - e) > 1000 * acc.bound(e, m, acc.F32, eps)
+    grads, sizes = ref.decay_bwd(*x[:5], go, gs), ref.spread_bwd(*x)
+    got = ref.decay_bwd(*lost, None, go[:, at:], gs)
+    most = acc.bound(grads[0][:, at:], sizes[0][:, at:], acc.F32, acc.of_factors(dtype, T, 2, 16))
+    assert ref.rms(got[0] - grads[0][:, at:]) > 100 * most
+    assert ref.rms(got[3] - grads[3][:, at:]) > 100 * acc.bound_gates(sizes[3], dtype, T, 2, 16)
+
+
+def test_a_lost_part_of_the_decays_gradient_is_seen():
+    """The state as one bf16 part in what sums into it (dL/dg_t = <gradient of the state, e^g state before>)."""
+    B, T, Hq, H, D = 1, 200, 2, 2, 64
+    x = acc.inputs(B, T, Hq, H, D, acc.BF16)
+    want, spread = ref.decay_bwd(*x)[3], ref.spread_bwd(*x)[3]
+    most = acc.bound_gates(spread, acc.BF16, T, 1, D)
+    q, k, v, g, s0, go, gs = x
+    # a token's r: q_t . (e^{G} S go_t) from the state at its chunk's start, with that state in parts
+    off = {}
+    for parts in (1, 2):
+        total = 0.0
+        for a in range(64, T, 64):
+            z = min(a + 64, T)
+            state = ref.decay(q[:, :a], k[:, :a], v[:, :a], g[:, :a], s0)[1]
+            G = torch.exp(torch.cumsum(g[:, a:z].double(), 1))
+            r = G * torch.einsum("bthd,bhde,bthe->bth", q[:, a:z].double(), ref.planes(state, parts) - state,
+                                 go[:, a:z].double())
+            total += r.square().sum().item()  # (an error of the gradient at each token that r is summed to)
+        off[parts] = (total / want.numel()) ** 0.5
+    assert off[2] < most < off[1]

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import decay_oracle as ref
-from prometheus_amd import kernels
+from prometheus_amd import kernels, serving
 from tests import decay_accuracy as acc
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +56,54 @@ def test_gradient_of_the_first_state(B, T, Hq, H, D, dtype, gates):
     (got,) = torch.autograd.grad((o, s), dev[4], gpu(go, gs))
     want, spread = ref.decay_bwd(q, k, v, g, s0, go, gs, 0.7), ref.spread_bwd(q, k, v, g, s0, go, gs, 0.7)
     acc.check(got, want[4], spread[4], acc.of_sums(T, Hq // H, D))
+
+
+@pytest.mark.parametrize("B,T,Hq,H,D", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradient_of_the_decays(B, T, Hq, H, D, dtype):
+    x = acc.inputs(B, T, Hq, H, D, dtype, seed=T)
+    _, res = kernels.decay_attention_fwd(*gpu(*x[:5]), scale=0.7)
+    gg = kernels.decay_attention_bwd(res, gpu(*x[5:]))[3]
+    want, spread = ref.decay_bwd(*x, 0.7)[3], ref.spread_bwd(*x, 0.7)[3]
+    acc.check_gates(gg, want, spread, dtype, T, Hq // H, D)
+
+
+@pytest.mark.parametrize("B,T,Hq,H,D", [(1, 1100, 4, 2, 64), (2, 1300, 2, 1, 128), (1, 900, 2, 2, 33)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_slow_decays_through_many_spans(B, T, Hq, H, D, dtype):
+    """States that live through the whole sequence, from a state and with a gradient of the last one."""
+    x = acc.slow(B, T, Hq, H, D, dtype)
+    (o, s), res = kernels.decay_attention_fwd(*gpu(*x[:5]), scale=0.7)
+    got = kernels.decay_attention_bwd(res, gpu(*x[5:]))
+    want, spread = ref.decay(*x[:5], 0.7), ref.spread(*x[:5], 0.7)
+    acc.check(o, want[0], spread[0], acc.of_factors(dtype, T, Hq // H, D))
+    acc.check(s, want[1], spread[1], acc.of_sums(T, 1, D))
+    want, spread = ref.decay_bwd(*x, 0.7), ref.spread_bwd(*x, 0.7)
+    for i in range(3):
+        acc.check(got[i], want[i], spread[i], acc.of_factors(dtype, T, Hq // H, D))
+    acc.check_gates(got[3], want[3], spread[3], dtype, T, Hq // H, D)
+    acc.check(got[4], want[4], spread[4], acc.of_sums(T, Hq // H, D))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Hq,H", [(2, 2), (4, 2)])
+def test_slow_decays_of_packed_prompts_in_slots(dtype, Hq, H):
+    """Sequences of several spans each, into a cache's slots and on from there."""
+    D, lengths = 64, [1500, 0, 700, 3]
+    q, k, v, g, *_ = acc.slow(1, sum(lengths), Hq, H, D, dtype)
+    cache = serving.DecayStateCache(1, 6, H, D)
+    s0 = torch.randn(4, H, D, D, generator=torch.Generator().manual_seed(1))
+    slots = torch.tensor([3, 5, 0, 2], device="cuda")
+    cache.pool[0, slots] = s0.cuda()
+    cu = torch.tensor([0, *lengths]).cumsum(0).cuda()
+    o = cache.prefill(0, slots, *gpu(q, k, v, g), cu)
+    cache.check_slots()
+    kernels.check_varlen()
+    a = 0
+    for i, n in enumerate(lengths):
+        part = [t[:, a:a + n] for t in (q, k, v, g)]
+        want, spread = ref.decay(*part, s0[i:i + 1]), ref.spread(*part, s0[i:i + 1])
+        if n:
+            acc.check(o[:, a:a + n], want[0], spread[0], acc.of_factors(dtype, n, Hq // H, D))
+        acc.check(cache.pool[0, slots[i]][None], want[1], spread[1], acc.of_sums(n, 1, D))
+        a += n
