@@ -231,14 +231,25 @@ int64_t resident(int D) { return D <= 64 ? 768 : D <= 128 ? 512 : 256; }
 
 // Whether spans along the sequence pay where there are ``groups`` workgroups without them: the card holds
 // ``more`` = resident / groups times as many, each span is walked through twice (the states' own pass costs
-// half of the outputs'), and the states are summed in a launch between.  With D 128 in us, spans against
-// whole sequences: bf16 forward of 16 heads, more = 8: 52 against 49 for 512 tokens, 61 against 91 for 1024;
-// more = 4: 61 against 51 and 80 against 93; more = 2.7: 213 against 195 for 2048; more = 32: 31 against 27
-// for 256 tokens, 33 against 37 for 384.  fp32 chunks are half as long and take longer: more = 8: 51 against
-// 60 for 256 tokens; more = 4: 93 against 115 for 512; more = 2.7: 253 against 236 for 1024.
+// half of the outputs'), and the states are summed in a launch between.  Whole sequences against spans in us,
+// forward, by D, heads (one sequence) and tokens:
+//   bf16  D 64   16: 20, 23 (256)  28, 23 (384)     128: 37, 31 (512)    256: 71, 63 (1024)  512: 356, 461 (4096)
+//         D 96  128: 67, 59 (512)  96, 72 (768)     256: 480, 438 (4096)
+//         D 128   1: 29, 31 (256)  40, 32 (384)      64: 54, 53 (512)  75, 58 (768)
+//               128: 76, 76 (768)  98, 86 (1024)    256: 197, 219 (2048)  380, 401 (4096)
+//         D 192  32: 97, 73 (512)                    64: 185, 169 (1024)
+//         D 256  32: 80, 75 (512)  113, 88 (768)     64: 149, 149 (1024)  283, 250 (2048)
+//   fp32  D 64  256: 53, 53 (384)  69, 63 (512)
+//         D 128  64: 58, 49 (256)  128: 83, 83 (384)  110, 92 (512)  256: 817, 889 (4096)
+//         D 256  32: 93, 81 (256)   64: 174, 171 (512)  253, 229 (768)
+// D 65 to 128 need three times as many, and longer sequences in bf16 (two workgroups already share a CU;
+// D 96 alone would rather be cut earlier), the others twice as many.  Over 1536 such calls of D 32 to 256,
+// forward and backward, the rule's choice takes 0.4% more than the better one in the mean, 41% at most, and
+// nowhere 5% more than one rule for all, measured at D 128 (which takes 1.1%, 57% at most).
 bool spans_pay(int64_t groups, int T, int D, bool bf16) {
-    const int64_t want = resident(D);
-    return want >= 3 * groups && T >= (bf16 ? 384 : 256) && T * want >= groups * (bf16 ? 4096 : 2048);
+    const bool two = D > 64 && D <= 128;
+    const int64_t want = resident(D), tokens = bf16 ? (two ? 4096 : 2800) : 1280;
+    return want >= (two ? 3 : 2) * groups && T >= (bf16 ? 384 : 256) && T * want >= groups * tokens;
 }
 
 // How a pass is cut into workgroups: one per sequence, state and column tile, or, where that pays, as many

@@ -69,3 +69,18 @@ def test_rows_of_more_than_32_bits_are_copied():
     assert row_norms._rows_of(shape, (2**40, 16, 1), (2**34, 8, 1)) is None
     rows, inner, strides = row_norms._rows_of(shape, (2**35, 16, 1), (2**34, 8, 1))
     assert (rows, inner, list(strides)) == (2**32, 1, [16, 0, 8, 0])
+
+
+def test_spans_by_the_head_dimension():
+    """Sequences are cut (and the workspace holds the states between) where the card holds twice as many
+    workgroups, between D 65 and 128 three times as many, and only then."""
+    L = _native.lib()
+
+    def states(T, H, D):
+        return L.pm_decay_attention_workspace_bytes(1, T, H, H, D, 0, 0) // (4 * H * D * D)
+
+    for D, resident, tiles, more in ((16, 768, 1, 2), (64, 768, 1, 2), (65, 512, 1, 3), (128, 512, 1, 3), (129, 256, 2, 2),
+                                     (256, 256, 2, 2)):
+        H = resident // (more * tiles)
+        assert states(4096, H, D) >= 2 and states(4096, H + 1, D) == 0, D
+        assert states(200, 1, D) == 0 and states(400, 1, D) >= 2

@@ -107,3 +107,16 @@ def test_slow_decays_of_packed_prompts_in_slots(dtype, Hq, H):
             acc.check(o[:, a:a + n], want[0], spread[0], acc.of_factors(dtype, n, Hq // H, D))
         acc.check(cache.pool[0, slots[i]][None], want[1], spread[1], acc.of_sums(n, 1, D))
         a += n
+
+
+@pytest.mark.parametrize("H,D,T", [(300, 24, 700), (60, 130, 500)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_many_heads_in_spans(H, D, T, dtype):
+    """Where the card holds just twice as many workgroups as there are heads."""
+    x = acc.slow(1, T, H, H, D, dtype)
+    o, s = kernels.decay_attention(*gpu(*x[:5]))
+    some = [0, H // 2, H - 1]
+    part = [t[:, :, some] for t in x[:4]]
+    want, spread = ref.decay(*part, x[4][:, some]), ref.spread(*part, x[4][:, some])
+    acc.check(o[:, :, some], want[0], spread[0], acc.of_factors(dtype, T, 1, D))
+    acc.check(s[:, some], want[1], spread[1], acc.of_sums(T, 1, D))
