@@ -246,7 +246,7 @@ def decay_attention_bwd(residual: _DecayResidual, grads):
     """Backward of the VJP pair: ``grads = (go, gs)``, dL/do (batch, seq, Hq, D) and dL/dnext_state
     (batch, H, D, D), either may be None. Returns ``(gq, gk, gv, gg, gstate)``: gq, gk and gv in q's
     type, gg shaped like g and gstate in fp32, each as accurate whichever are wanted. With bf16 q, k and v an fp32 go is rounded to bf16
-    first: it is a factor of products, as they are. What heads or tokens share is summed in an order
+    first: it is a factor of products, as they are (fp32 q, k and v keep it). What heads or tokens share is summed in an order
     that does not change."""
     go, gs = grads
     r = residual
