@@ -19,6 +19,8 @@
 // plane's size.  bf16 inputs are one plane and exact; next to them
 //   the decayed V, which sums into states      three planes (2^-25 relative; two, 2^-17, in the backward's
 //     passes alone took 556 us where three take 580, with the forward)
+//   the state in passes that leave parts of the gates' gradient, which is fp32    three (two: 580 for 599 us,
+//     and the gradient 3.0e-6 off in the 2-norm where it is 3.7e-7)
 //   A and the state in what comes out          two (2^-17).  What comes out in bf16 is then as if it were
 //     rounded once, and in fp32 nearly so; one part (2^-8 of each term) took 128 us where two take 135 at
 //     B4 T4096 H16 D128, forward, and 536 for 556 with the backward, and was 1.4 times one rounding off
@@ -41,7 +43,7 @@ namespace {
 template <int P>
 struct DecayShape {
     static constexpr int C = P == 1 ? 64 : 32;   // tokens of a chunk (three planes of 64 would not fit LDS)
-    static constexpr int PA = P == 1 ? 2 : 3;    // planes of A, and of the state as a factor
+    static constexpr int PA = P == 1 ? 2 : 3;    // planes of A, and of the state in what comes out
     static constexpr int MT = C / 16;            // 16-token tiles
     static constexpr int TRI = MT * (MT + 1) / 2;  // lower 16x16 tiles of A
     static constexpr int BLK = P == 1 ? 6 : 2;   // packed operand blocks of A (qblk)
@@ -271,6 +273,8 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
     constexpr int UQ = C * DK / 2048, UV = C * NT / 2048;  // 8-element units per thread
     constexpr int RQ = 2048 / DK, RV = 2048 / NT;          // rows between a thread's units
     constexpr bool OUT = KIND != kPassState, AUX = KIND == kPassPart;
+    constexpr int PS = AUX ? 3 : PA;  // planes of the state as a factor
+    constexpr int CS = AUX ? 1 : CT;  // column tiles whose planes are held at once (three of both spill 32 registers)
     constexpr int PC = 3;  // planes of the decayed V, which sums into the state
     using E = typename std::conditional<P == 1, uint16_t, float>::type;
 
@@ -547,19 +551,22 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                     for (int i = 0; i < MT; ++i) O[ct][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
-                    u32x4_t so[CT][PA], qo[MT][P], ko[P];
+                    u32x4_t so[CS][PS], qo[MT][P], ko[P];
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
                         for (int p = 0; p < P; ++p) qo[i][p] = op_row<DK>(sq + p * C * DK, 16 * i + l16, kb, lg);
 #pragma unroll
                     for (int p = 0; p < P; ++p) ko[p] = op_row<DK>(sk + p * C * DK, 16 * (w % MT) + l16, kb, lg);
+                    auto split_state = [&](int c0) {
 #pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        const f32x4_t s0 = S[ct][2 * kb], s1 = S[ct][2 * kb + 1];
-                        const float s8[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
-                        split8<PA>(s8, so[ct]);
-                    }
+                        for (int ct = 0; ct < CS; ++ct) {
+                            const f32x4_t s0 = S[c0 + ct][2 * kb], s1 = S[c0 + ct][2 * kb + 1];
+                            const float s8[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
+                            split8<PS>(s8, so[ct]);
+                        }
+                    };
+                    if (!AUX) split_state(0);
 #pragma unroll
                     for (int x = P - 1; x >= 0; --x)
 #pragma unroll
@@ -570,16 +577,20 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
                                     A[i] = mfma32(__builtin_bit_cast(bf16x8_t, ko[x - p]),
                                                   __builtin_bit_cast(bf16x8_t, qo[i][p]), A[i]);
 #pragma unroll
-                    for (int x = PA - 1; x >= 0; --x)  // (the small products first, all tiles of one before the next)
+                    for (int c0 = 0; c0 < CT; c0 += CS) {
+                        if (AUX) split_state(c0);
 #pragma unroll
-                        for (int p = 0; p < P; ++p)
-                            if (x - p >= 0)
+                        for (int x = PS - 1; x >= 0; --x)  // (the small products first, all tiles of one before the next)
 #pragma unroll
-                                for (int ct = 0; ct < CT; ++ct)
+                            for (int p = 0; p < P; ++p)
+                                if (x - p >= 0)
 #pragma unroll
-                                    for (int i = 0; i < MT; ++i)
-                                        O[ct][i] = mfma32(__builtin_bit_cast(bf16x8_t, so[ct][x - p]),
-                                                          __builtin_bit_cast(bf16x8_t, qo[i][p]), O[ct][i]);
+                                    for (int ct = 0; ct < CS; ++ct)
+#pragma unroll
+                                        for (int i = 0; i < MT; ++i)
+                                            O[c0 + ct][i] = mfma32(__builtin_bit_cast(bf16x8_t, so[ct][x - p]),
+                                                                   __builtin_bit_cast(bf16x8_t, qo[i][p]), O[c0 + ct][i]);
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {

@@ -221,8 +221,8 @@ def decay_attention(q, k, v, g, state=None, *, scale=1.0, out_dtype=None):
     ``out_dtype`` says so, next_state (batch, H, D, D) fp32.
 
     fp32 inputs have fp32 accuracy. bf16 inputs enter the products as they are; o and the gradients
-    keep 2^-17 of each term before they are rounded to their type, the states and the first state's
-    gradient 2^-24. A log-decay below -138 counts as closed. Infinities and NaN reach what they reach
+    of q, k and v keep 2^-17 of each term before they are rounded to their type, the states, the decays'
+    and the first state's gradient 2^-24. A log-decay below -138 counts as closed. Infinities and NaN reach what they reach
     token by token (an infinity may come out as NaN), in the decays' gradient up to 512 tokens more
     behind theirs.
 

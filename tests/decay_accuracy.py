@@ -58,19 +58,17 @@ def inputs(B, T, Hq, H, D, dtype, s0=True, seed=0, low=-0.3, zeros=False):
     return q, k, v, g, normal(B, H, D, D) if s0 else None, go, gs
 
 
-def bound_gates(spread, dtype, T, G, D):
+def bound_gates(spread, T, G, D):
     """What the rms of the decays' gradient's error may be. What a chunk's tokens add to it or take from it
-    are parts of the gradient at the chunk's first token and behind its last, next to bf16 inputs with one
-    factor, the state, in two parts; where a span begins it is a product of two states, whose sums' errors
-    are handed to all of its tokens."""
-    eps = of_sums(T, G, D)
-    largest = spread.amax(1, keepdim=True).expand_as(spread)
-    return 6 * (eps * ref.rms(largest) + (2.0**-17 * ref.rms(spread) if dtype == BF16 else 0.0))
+    are parts of the gradient at the chunk's first token and behind its last; where a span begins it is a
+    product of two states, whose sums' errors are handed to all of its tokens. (Factors are in three parts,
+    for bf16 inputs too.)"""
+    return 6 * of_sums(T, G, D) * ref.rms(spread.amax(1, keepdim=True).expand_as(spread))
 
 
-def check_gates(got, want, spread, dtype, T, G, D):
+def check_gates(got, want, spread, T, G, D):
     assert got.shape == want.shape and got.dtype == F32
-    off, most = ref.rms(got.detach().cpu().double() - want), bound_gates(spread, dtype, T, G, D)
+    off, most = ref.rms(got.detach().cpu().double() - want), bound_gates(spread, T, G, D)
     assert off <= most, (off, most)
 
 

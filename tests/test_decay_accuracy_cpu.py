@@ -79,7 +79,7 @@ def test_what_spans_hand_on_is_seen(dtype):
     got = ref.decay_bwd(*lost, None, go[:, at:], gs)
     most = acc.bound(grads[0][:, at:], sizes[0][:, at:], acc.F32, acc.of_factors(dtype, T, 2, 16))
     assert ref.rms(got[0] - grads[0][:, at:]) > 100 * most
-    assert ref.rms(got[3] - grads[3][:, at:]) > 100 * acc.bound_gates(sizes[3], dtype, T, 2, 16)
+    assert ref.rms(got[3] - grads[3][:, at:]) > 100 * acc.bound_gates(sizes[3], T, 2, 16)
 
 
 def test_a_lost_part_of_the_decays_gradient_is_seen():
@@ -87,7 +87,7 @@ def test_a_lost_part_of_the_decays_gradient_is_seen():
     B, T, Hq, H, D = 1, 200, 2, 2, 64
     x = acc.inputs(B, T, Hq, H, D, acc.BF16)
     want, spread = ref.decay_bwd(*x)[3], ref.spread_bwd(*x)[3]
-    most = acc.bound_gates(spread, acc.BF16, T, 1, D)
+    most = acc.bound_gates(spread, T, 1, D)
     q, k, v, g, s0, go, gs = x
     # a token's r: q_t . (e^{G} S go_t) from the state at its chunk's start, with that state in parts
     off = {}
