@@ -304,8 +304,8 @@ FwdWs fwd_ws(const Plan& p, int n_seqs, int Hq, int H, int D, bool packed, bool 
 }
 
 // The backward's passes: one cut for all three, which run as one launch.  Where the gates' gradient is
-// wanted, spans of at most kDecayGateSpan tokens, also where they do not pay (B8 T4096 H16 bf16, D 64: 391 us
-// against 470 for whole sequences, D 128: 776 against 683, D 256: 2870 against 2098): its sums stay short.
+// wanted, spans of at most kDecayGateSpan tokens, also where they do not pay (B8 T4096 H16 bf16, D 128: 898 us
+// against 811 for whole sequences, D 256: 3405 against 2509): its sums stay short.
 struct BwdPlan {
     Plan q, k;  // gq's pass, and gk's and gv's
 };

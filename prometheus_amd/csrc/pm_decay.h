@@ -208,7 +208,7 @@ __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
 
 // The same number, as one the compiler knows nothing of: what is computed from it is computed where it is
 // used, not ahead of the loop, where it would take a register (or scratch memory, whose loads wait for
-// the rows that are on their way: the backward's three passes at B4 T4096 H16 D128 took 302 us, 240 so).
+// the rows that are on their way: the backward of B4 T4096 H16 D128 takes 549 us without, 467 so).
 __device__ __forceinline__ int fresh(int x) {
     __asm__ volatile("" : "+v"(x));
     return x;
@@ -254,7 +254,8 @@ __device__ __forceinline__ float exp2_f64(double x) {
 // K and V, or their Q), NT = 64 CT columns of the state: wave w keeps 16 CT of them for all DK rows in
 // accumulators, 16 CT columns of O for the chunk, and a quarter of A's tiles, which the waves exchange
 // through LDS.  Two column tiles a wave (DK >= 128) halve the LDS reads of Q and K^T per product, which
-// bound the kernel with one (B4 T4096 H16 D128: 118 us with one, LDS at 220 KB a chunk and 64 columns).
+// bound the kernel with one (forward of B4 T4096 H16 D128: 156 us with one, LDS at 220 KB a chunk and 64
+// columns, 135 with two).
 // The next chunk's rows are loaded into registers while this one's products run.
 
 // What a launch of decay_pass does besides its outputs.
@@ -799,7 +800,7 @@ __global__ __launch_bounds__(256, KIND == kPassState || DK < 256 ? 2 : 1) void d
             }
         }
         // (the next step's loads: after the products that need every register, before the wait for the other
-        // waves; 153 us here, 158 before the state's products, 170 before all of them, 166 after A V, at B32
+        // waves; 179 us here, 184 before the state's products, 186 before all of them, 182 after A V, at B32
         // T1024 H16 D128.  A states' pass has registers to spare and asks before its products.)
         if (OUT) fetch(c_next, m_next);
         if (!OUT && w == 0 && first_m) sum_g(c + 1, rg);
