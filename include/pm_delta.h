@@ -599,9 +599,9 @@ size_t pm_decay_attention_workspace_bytes(int n_seqs, int T, int Hq, int H, int 
  * (fp32, NULL for zeros).  gq, gk, gv contiguous in dtype; gs0 (B, H, D, D) fp32,
  * NULL: not wanted; gg fp32: (B, T, H), or (H), summed over all tokens in an order that does not
  * change, where both of g's strides are 0; NULL: not wanted.  Every output is
- * written in full; none may overlap an input.  With bf16 inputs gq, gk and gv
- * take factors in two bf16 parts (2^-17), gg and gs0 in three.  Infinities and NaN in q
- * and go reach gg of up to 512 tokens behind theirs too.  workspace:
+ * written in full; none may overlap an input.  With bf16 inputs gq, gk and gv take
+ * factors in two bf16 parts (2^-17), gg and gs0 in three.  Infinities and NaN in q and
+ * go reach gg of up to 512 tokens behind theirs too.  workspace:
  * pm_decay_attention_bwd_workspace_bytes (gates: gg is wanted).
  */
 int pm_decay_attention_bwd(const void* q, const void* k, const void* v, const float* g, const float* s0,

@@ -221,10 +221,10 @@ def decay_attention(q, k, v, g, state=None, *, scale=1.0, out_dtype=None):
     ``out_dtype`` says so, next_state (batch, H, D, D) fp32.
 
     fp32 inputs have fp32 accuracy. bf16 inputs enter the products as they are; o and the gradients
-    of q, k and v keep 2^-17 of each term before they are rounded to their type, the states, the decays'
-    and the first state's gradient 2^-24. A log-decay below -138 counts as closed. Infinities and NaN reach what they reach
-    token by token (an infinity may come out as NaN), in the decays' gradient up to 512 tokens more
-    behind theirs.
+    of q, k and v keep 2^-17 of each term before they are rounded to their type, the states and the
+    gradients of the decays and of the first state 2^-24. A log-decay below -138 counts as closed.
+    Infinities and NaN reach what they reach token by token (an infinity may come out as NaN), in the
+    decays' gradient up to 512 tokens more behind theirs.
 
     Differentiable: when autograd records and a torch input requires grad, the backward is
     ``decay_attention_bwd``.
@@ -245,9 +245,9 @@ def decay_attention_fwd(q, k, v, g, state=None, *, scale=1.0, out_dtype=None):
 def decay_attention_bwd(residual: _DecayResidual, grads):
     """Backward of the VJP pair: ``grads = (go, gs)``, dL/do (batch, seq, Hq, D) and dL/dnext_state
     (batch, H, D, D), either may be None. Returns ``(gq, gk, gv, gg, gstate)``: gq, gk and gv in q's
-    type, gg shaped like g and gstate in fp32, each as accurate whichever are wanted. With bf16 q, k and v an fp32 go is rounded to bf16
-    first: it is a factor of products, as they are (fp32 q, k and v keep it). What heads or tokens share is summed in an order
-    that does not change."""
+    type, gg shaped like g and gstate in fp32, each as accurate whichever are wanted. With bf16 q, k and
+    v an fp32 go is rounded to bf16 first: it is a factor of products, as they are (fp32 q, k and v keep
+    it). What heads or tokens share is summed in an order that does not change."""
     go, gs = grads
     r = residual
     lead, Hq, H, D = _check(r.q, r.k, r.v, r.g, 4, r.scale)

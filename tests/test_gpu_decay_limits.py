@@ -57,3 +57,22 @@ def test_norms_of_no_rows(shape, kind):
         for f in (kernels.gated_norm, lambda *a: kernels.residual_norm(*a)[0]):
             grads = torch.autograd.grad(f(*leaves).sum(), leaves)
             assert grads[0].shape == shape and not grads[2].any()
+
+
+def test_gradients_of_as_many_tokens_as_a_call_takes():
+    """The same from both ends: gq is 2 - 2^-t after t more tokens, gk and gv before as many, and every token
+    adds the decayed state before it times the gradient behind it, 2 of them, to the one decay's gradient."""
+    x = torch.ones(1, 1, 1, 1, dtype=torch.bfloat16, device="cuda").expand(1, MOST, 1, 1)
+    g = torch.full((1,), -math.log(2.0), device="cuda")
+    _, res = kernels.decay_attention_fwd(x, x, x, g)
+    gq, gk, gv, gg, gs = kernels.decay_attention_bwd(res, (x, None))
+    want = [2.0 - 2.0**-t for t in range(8)]
+    for grad, ends in ((gq, slice(0, 64)), (gk, slice(MOST - 64, MOST)), (gv, slice(MOST - 64, MOST))):
+        grad = grad.flatten()
+        part = grad[ends] if ends.start == 0 else grad[ends].flip(0)
+        assert part[:8].tolist() == want and bool((part[8:] >= want[-1]).all())
+        grad[ends] = 2.0
+        low, high = grad.aminmax()
+        assert low.item() == high.item() == 2.0
+    assert gg.item() == pytest.approx(2.0 * MOST, rel=1e-6)
+    assert gs.item() == pytest.approx(1.0, rel=1e-6)
