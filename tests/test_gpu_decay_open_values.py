@@ -95,3 +95,54 @@ def test_gradients(dtype, token):
         want = ref.decay_bwd(q, k, v, g, s0, go, gs)
         for i in (0, 1, 2, 4):
             assert torch.equal(got[i].cpu().isfinite(), want[i].isfinite()), (which, i)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,D", [(100000, 16), (70000, 128), (200, 64)])
+def test_other_values_keep_their_bits(dtype, T, D):
+    """Groups of query heads, one after another in a workgroup where there is work enough: a NaN in v changes
+    its own column from its token on, one in k its group's gq from there on, one in q its key head's gk up to
+    there, and no other bit."""
+    Hq, H, token, column = 4, 2, T // 2 + 5, 9
+    gen = torch.Generator(device="cuda").manual_seed(T)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=gen, device="cuda")
+
+    q, k, v = normal(1, T, Hq, D).to(dtype), (normal(1, T, H, D) / D**0.5).to(dtype), normal(1, T, H, D).to(dtype)
+    g, s0, go = -0.3 * torch.rand(1, T, H, generator=gen, device="cuda"), normal(1, H, D, D), normal(1, T, Hq, D).to(dtype)
+
+    def run(q, k, v):
+        (o, s), res = kernels.decay_attention_fwd(q, k, v, g, s0)
+        gq, gk, gv, _, _ = kernels.decay_attention_bwd(res, (go, None))
+        return {"o": o, "s": s, "gq": gq, "gk": gk, "gv": gv}
+
+    def with_nan(x, head):
+        x = x.clone()
+        x[0, token, head, column] = NAN
+        return x
+
+    def same(name, got, open_values):
+        """The same bits, but for the values of ``open_values``, which are not finite."""
+        want = clean[name].clone()
+        assert not got[name][open_values].isfinite().any(), name
+        want[open_values] = got[name][open_values] = 0.0
+        assert torch.equal(got[name], want), name
+
+    def mask(name, *index):
+        m = torch.zeros_like(clean[name], dtype=torch.bool)
+        m[(0, *index)] = True
+        return m
+
+    clean = run(q, k, v)
+    later, earlier, whole = slice(token, T), slice(0, token + 1), slice(None)
+    got = run(q, k, with_nan(v, 1))
+    same("o", got, mask("o", later, slice(2, 4), column))
+    same("s", got, mask("s", 1, whole, column))
+    same("gv", got, mask("gv", slice(0, 0)))
+    same("gk", got, mask("gk", slice(token, token + 1), 1))
+    got = run(q, with_nan(k, 1), v)
+    same("gq", got, mask("gq", later, slice(2, 4), column))
+    got = run(with_nan(q, 3), k, v)
+    same("gk", got, mask("gk", earlier, 1, column))
+    same("gq", got, mask("gq", slice(0, 0)))
